@@ -743,6 +743,48 @@ int mi355_rms_norm_bwd(const void* dy, const void* x, const void* weight, const 
                        int dtype, void* dx, void* dweight, void* workspace, int64_t rows,
                        int64_t D, void* stream);
 
+/*
+ * Rotary positions of the queries and keys (the `rotary` entry of the reference's kernel registry,
+ * llmtuner/kernel/ops/rotary.py), in one launch for both.
+ *   a = positions[t] * inv_freq[i];  c = attention_factor cos a;  s = attention_factor sin a
+ *   u' = u c - v s,  v' = v c + u s   over the pairs (i, i + pairs) of a head, or (2i, 2i + 1) where `interleaved`
+ * Elements from 2 * pairs on are copied.  `transpose` turns the other way, which is the backward pass.
+ * Angles are formed in fp64 and reduced there, the rest is fp32 with one rounding to `dtype` (fp32 or bf16).
+ * q is (T, H, D) and k (T, G, D) with the given strides in elements, the elements of a head next to each
+ * other; the results are dense.  2 <= D <= 512, 2 * pairs <= D.  positions: int32, or int64 where positions_i64.
+ * Operands need be aligned to their element only (16-byte pieces where sizes, strides and bases allow).
+ */
+int mi355_rotary(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                 int64_t k_token_stride, int64_t k_head_stride, int dtype, const void* positions,
+                 int positions_i64, const float* inv_freq, int64_t pairs, float attention_factor,
+                 int interleaved, int transpose, void* q_out, void* k_out, int64_t T, int64_t H,
+                 int64_t G, int64_t D, void* stream);
+
+/*
+ * The RMS norm of every query and key head (weights (D), shared by the heads) and the rotation above, in one pass:
+ *   y = rotate((x r) w),  r = 1/sqrt(mean_d x^2 + epsilon)
+ * Backward, with g = the gradient turned back, gw = g w, xh = x r (r is formed again from x):
+ *   dx = r (gw - xh mean_d(gw xh)),   dweight[d] = sum over tokens and heads of g xh (fixed order, no atomics)
+ * dq_out and dk_out are dense; dq, dk, dq_weight, dk_weight may be NULL to skip them.  workspace (for the weights'
+ * gradients): mi355_qk_norm_rotary_bwd_workspace_bytes(D) bytes.
+ */
+int mi355_qk_norm_rotary_fwd(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                             const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                             const void* q_weight, const void* k_weight, int dtype,
+                             const void* positions, int positions_i64, const float* inv_freq,
+                             int64_t pairs, float attention_factor, int interleaved, float epsilon,
+                             void* q_out, void* k_out, int64_t T, int64_t H, int64_t G, int64_t D,
+                             void* stream);
+int64_t mi355_qk_norm_rotary_bwd_workspace_bytes(int64_t D);
+int mi355_qk_norm_rotary_bwd(const void* dq_out, const void* dk_out, const void* q,
+                             int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                             int64_t k_token_stride, int64_t k_head_stride, const void* q_weight,
+                             const void* k_weight, int dtype, const void* positions,
+                             int positions_i64, const float* inv_freq, int64_t pairs,
+                             float attention_factor, int interleaved, float epsilon, void* dq,
+                             void* dk, void* dq_weight, void* dk_weight, void* workspace, int64_t T,
+                             int64_t H, int64_t G, int64_t D, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

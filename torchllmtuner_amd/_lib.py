@@ -42,6 +42,13 @@ SIGNATURES = {
     "mi355_rms_norm_fwd": (I, [P, P, I, P, P, L, L, F, P]),
     "mi355_rms_norm_bwd_workspace_bytes": (L, [L, L]),
     "mi355_rms_norm_bwd": (I, [P, P, P, P, I, P, P, P, L, L, P]),
+    "mi355_rotary": (I, [P, L, L, P, L, L, I, P, I, P, L, F, I, I, P, P, L, L, L, L, P]),
+    "mi355_qk_norm_rotary_fwd": (I, [P, L, L, P, L, L, P, P, I, P, I, P, L, F, I, F, P, P, L, L, L, L, P]),
+    "mi355_qk_norm_rotary_bwd_workspace_bytes": (L, [L]),
+    "mi355_qk_norm_rotary_bwd": (
+        I,
+        [P, P, P, L, L, P, L, L, P, P, I, P, I, P, L, F, I, F, P, P, P, P, P, L, L, L, L, P],
+    ),
     "mi355_permute_plan_workspace_bytes": (L, [L, L, L]),
     "mi355_permute_plan": (I, [P, L, L, L, L, L, L, L, P, P, P, P, P, P, L, P, P, P, L, P, P]),
     "mi355_segments_from_counts": (I, [P, L, L, L, P, P, P, P, P, L, P]),

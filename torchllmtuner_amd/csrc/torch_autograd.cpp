@@ -377,6 +377,97 @@ std::tuple<Tensor, Tensor> rms_norm_autograd(const Tensor& x, const Tensor& weig
   return {r[0], r[1]};
 }
 
+// ---- rotary positions: linear in q and k, so the backward is the operator itself, turned the other way ------------
+using RotarySig = std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const Tensor&, bool, double, bool);
+
+struct Rotary : public torch::autograd::Function<Rotary> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& positions, const Tensor& inv_freq,
+                               bool interleaved, double factor, bool transpose) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    static auto op = typed_op<RotarySig>("mi355_moe::rotary");
+    auto r = op.call(q, k, positions, inv_freq, interleaved, factor, transpose);
+    ctx->save_for_backward({positions, inv_freq});
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["factor"] = factor;
+    ctx->saved_data["transpose"] = transpose;
+    return {std::get<0>(r), std::get<1>(r)};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list out(7);
+    const bool n0 = ctx->needs_input_grad(0), n1 = ctx->needs_input_grad(1);
+    if (!(n0 || n1)) return out;
+    const auto s = ctx->get_saved_variables();
+    // (gradients are materialised here: one launch serves both, and a result nobody differentiated counts as zeros)
+    static auto op = typed_op<RotarySig>("mi355_moe::rotary");
+    auto r = op.call(grads[0], grads[1], s[0], s[1], ctx->saved_data["interleaved"].toBool(), ctx->saved_data["factor"].toDouble(),
+                     !ctx->saved_data["transpose"].toBool());
+    out[0] = keep(std::get<0>(r), n0);
+    out[1] = keep(std::get<1>(r), n1);
+    return out;
+  }
+};
+
+std::tuple<Tensor, Tensor> rotary_autograd(const Tensor& q, const Tensor& k, const Tensor& positions, const Tensor& inv_freq,
+                                           bool interleaved, double factor, bool transpose) {
+  if (!torch::autograd::compute_requires_grad(q, k)) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    static auto op = typed_op<RotarySig>("mi355_moe::rotary");
+    return op.call(q, k, positions, inv_freq, interleaved, factor, transpose);
+  }
+  auto r = Rotary::apply(q, k, positions, inv_freq, interleaved, factor, transpose);
+  return {r[0], r[1]};
+}
+
+// ---- norms of the query and key heads with the rotation -------------------------------------------------
+using QkNormFwdSig = std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                                                const Tensor&, double, bool, double);
+using QkNormBwdSig = std::tuple<Tensor, Tensor, Tensor, Tensor>(const OptTensor&, const OptTensor&, const Tensor&, const Tensor&,
+                                                                const Tensor&, const Tensor&, const Tensor&, const Tensor&, double,
+                                                                bool, double, bool, bool);
+
+struct QkNormRotary : public torch::autograd::Function<QkNormRotary> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& qw, const Tensor& kw,
+                               const Tensor& positions, const Tensor& inv_freq, double eps, bool interleaved, double factor) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    static auto op = typed_op<QkNormFwdSig>("mi355_moe::qk_norm_rotary_fwd");
+    auto r = op.call(q, k, qw, kw, positions, inv_freq, eps, interleaved, factor);
+    ctx->save_for_backward({q, k, qw, kw, positions, inv_freq});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["factor"] = factor;
+    ctx->set_materialize_grads(false);
+    return {std::get<0>(r), std::get<1>(r)};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list out(9);
+    bool need[4];
+    for (int i = 0; i < 4; ++i) need[i] = ctx->needs_input_grad(i) && grads[i % 2].defined();
+    const bool dx = need[0] || need[1], dw = need[2] || need[3];
+    if (!(dx || dw)) return out;
+    const auto s = ctx->get_saved_variables();
+    static auto op = typed_op<QkNormBwdSig>("mi355_moe::qk_norm_rotary_bwd");
+    auto r = op.call(opt(grads[0]), opt(grads[1]), s[0], s[1], s[2], s[3], s[4], s[5], ctx->saved_data["eps"].toDouble(),
+                     ctx->saved_data["interleaved"].toBool(), ctx->saved_data["factor"].toDouble(), dx, dw);
+    out[0] = keep(std::get<0>(r), need[0]);
+    out[1] = keep(std::get<1>(r), need[1]);
+    out[2] = keep(std::get<2>(r), need[2]);
+    out[3] = keep(std::get<3>(r), need[3]);
+    return out;
+  }
+};
+
+std::tuple<Tensor, Tensor> qk_norm_rotary_autograd(const Tensor& q, const Tensor& k, const Tensor& qw, const Tensor& kw,
+                                                   const Tensor& positions, const Tensor& inv_freq, double eps, bool interleaved,
+                                                   double factor) {
+  if (!torch::autograd::compute_requires_grad(q, k, qw, kw)) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    static auto op = typed_op<QkNormFwdSig>("mi355_moe::qk_norm_rotary_fwd");
+    return op.call(q, k, qw, kw, positions, inv_freq, eps, interleaved, factor);
+  }
+  auto r = QkNormRotary::apply(q, k, qw, kw, positions, inv_freq, eps, interleaved, factor);
+  return {r[0], r[1]};
+}
+
 // ---- load-balance loss: out = (loss, f_E...); the gradient flows into the scores -------------------
 using BalanceFwdSig = Tensor(const Tensor&, const Tensor&, const OptTensor&);
 using BalanceBwdSig = Tensor(const Tensor&, const Tensor&, const OptTensor&, const Tensor&);
@@ -530,6 +621,8 @@ TORCH_LIBRARY_IMPL(mi355_moe, Autograd, m) {
   m.impl("router_select_fwd", router_select_autograd);
   m.impl("router_select_cutoff_fwd", router_select_cutoff_autograd);
   m.impl("rms_norm_fwd", rms_norm_autograd);
+  m.impl("rotary", rotary_autograd);
+  m.impl("qk_norm_rotary_fwd", qk_norm_rotary_autograd);
   m.impl("balance_loss_fwd", balance_loss_autograd);
   m.impl("permute_rows_fwd", permute_rows_autograd);
   m.impl("combine_fwd", combine_autograd);

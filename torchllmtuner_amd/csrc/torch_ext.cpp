@@ -187,6 +187,109 @@ std::tuple<Tensor, Tensor> rms_norm_bwd(const Tensor& dy_, const Tensor& x_, con
   return {dx, dw};
 }
 
+// (..., heads, size) as the kernels that take strides read it: tokens flattened, a head's elements next to each
+// other.  A view of that shape (the queries within a fused projection) is read where it lies, anything else is copied.
+struct Heads {
+  Tensor t;
+  int64_t tokens, heads, size, token_stride, head_stride;
+  explicit Heads(const Tensor& x) {
+    TORCH_CHECK_VALUE(x.dim() >= 3, "queries and keys are (..., heads, size), got ", x.sizes());
+    t = x.dim() == 3 ? x : x.flatten(0, x.dim() - 3);
+    if (t.size(2) > 1 && t.stride(2) != 1) t = t.contiguous();
+    tokens = t.size(0), heads = t.size(1), size = t.size(2);
+    token_stride = tokens > 1 ? t.stride(0) : 0;  // (the stride of a single token or head says nothing)
+    head_stride = heads > 1 ? t.stride(1) : 0;
+  }
+};
+// ... and as the operators that take dense heads only do, in the wanted type
+Tensor heads_like(const OptTensor& grad, const Tensor& like) {
+  if (!grad.has_value() || !grad->defined()) return at::zeros(like.sizes(), like.options());
+  return dense(grad->scalar_type() == like.scalar_type() ? *grad : grad->to(like.scalar_type()));
+}
+
+void check_heads(const Heads& q, const Heads& k, const Tensor& positions, const Tensor& inv_freq) {
+  TORCH_CHECK_TYPE(q.t.scalar_type() == k.t.scalar_type(), "queries (", q.t.scalar_type(), ") and keys (", k.t.scalar_type(),
+                   ") must share a dtype");
+  TORCH_CHECK_VALUE(q.tokens == k.tokens && q.size == k.size, "queries ", q.t.sizes(), " and keys ", k.t.sizes(),
+                    " must agree in tokens and head size");
+  TORCH_CHECK_VALUE(positions.numel() == q.tokens, "got ", positions.numel(), " positions for ", q.tokens, " tokens");
+  TORCH_CHECK_VALUE(k.t.device() == q.t.device() && positions.device() == q.t.device() && inv_freq.device() == q.t.device(),
+                    "queries, keys, positions and inv_freq must share a device");
+}
+void check_weights(const Heads& q, const Tensor& qw, const Tensor& kw) {
+  TORCH_CHECK_TYPE(qw.scalar_type() == q.t.scalar_type() && kw.scalar_type() == q.t.scalar_type(),
+                   "norm weights must have the queries' dtype");
+  TORCH_CHECK_VALUE(qw.numel() == q.size && kw.numel() == q.size, "norm weights must have the head's ", q.size, " elements");
+  TORCH_CHECK_VALUE(qw.device() == q.t.device() && kw.device() == q.t.device(), "norm weights must be on the queries' device");
+}
+
+struct Positions {
+  Tensor t;
+  int wide;
+  explicit Positions(const Tensor& p) : t(p.contiguous()), wide(p.scalar_type() == at::kLong) {
+    TORCH_CHECK_TYPE(wide || p.scalar_type() == at::kInt, "positions must be int32 or int64, got ", p.scalar_type());
+  }
+};
+
+std::tuple<Tensor, Tensor> rotary(const Tensor& q_, const Tensor& k_, const Tensor& positions_, const Tensor& inv_freq_,
+                                  bool interleaved, double factor, bool transpose) {
+  Launch L(q_);
+  const Heads q(q_), k(k_);
+  const Positions positions(positions_);
+  const Tensor inv_freq = cf(inv_freq_);
+  check_heads(q, k, positions.t, inv_freq);
+  Tensor q_out = at::empty(q_.sizes(), q_.options()), k_out = at::empty(k_.sizes(), k_.options());
+  check(mi355_rotary(ptr(q.t), q.token_stride, q.head_stride, ptr(k.t), k.token_stride, k.head_stride, dtype_code(q.t),
+                     ptr(positions.t), positions.wide, fptr(inv_freq), inv_freq.numel(), (float)factor, interleaved, transpose,
+                     ptr(q_out), ptr(k_out), q.tokens, q.heads, k.heads, q.size, L.stream),
+        "rotary");
+  return {q_out, k_out};
+}
+
+std::tuple<Tensor, Tensor> qk_norm_rotary_fwd(const Tensor& q_, const Tensor& k_, const Tensor& qw_, const Tensor& kw_,
+                                              const Tensor& positions_, const Tensor& inv_freq_, double eps, bool interleaved,
+                                              double factor) {
+  Launch L(q_);
+  const Heads q(q_), k(k_);
+  const Tensor qw = qw_.contiguous(), kw = kw_.contiguous(), inv_freq = cf(inv_freq_);
+  const Positions positions(positions_);
+  check_heads(q, k, positions.t, inv_freq);
+  check_weights(q, qw, kw);
+  Tensor q_out = at::empty(q_.sizes(), q_.options()), k_out = at::empty(k_.sizes(), k_.options());
+  check(mi355_qk_norm_rotary_fwd(ptr(q.t), q.token_stride, q.head_stride, ptr(k.t), k.token_stride, k.head_stride, ptr(qw), ptr(kw),
+                                 dtype_code(q.t), ptr(positions.t), positions.wide, fptr(inv_freq), inv_freq.numel(), (float)factor,
+                                 interleaved, (float)eps, ptr(q_out), ptr(k_out), q.tokens, q.heads, k.heads, q.size, L.stream),
+        "qk_norm_rotary_fwd");
+  return {q_out, k_out};
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> qk_norm_rotary_bwd(const OptTensor& dq_out_, const OptTensor& dk_out_, const Tensor& q_,
+                                                              const Tensor& k_, const Tensor& qw_, const Tensor& kw_,
+                                                              const Tensor& positions_, const Tensor& inv_freq_, double eps,
+                                                              bool interleaved, double factor, bool need_dx, bool need_dw) {
+  Launch L(q_);
+  const Heads q(q_), k(k_);
+  const Tensor dq_out = heads_like(dq_out_, q_), dk_out = heads_like(dk_out_, k_);
+  const Tensor qw = qw_.contiguous(), kw = kw_.contiguous(), inv_freq = cf(inv_freq_);
+  const Positions positions(positions_);
+  check_heads(q, k, positions.t, inv_freq);
+  check_weights(q, qw, kw);
+  TORCH_CHECK_VALUE(dq_out.sizes() == q_.sizes() && dk_out.sizes() == k_.sizes(), "gradients must have the results' shapes");
+  Tensor dq = need_dx ? at::empty(q_.sizes(), q_.options()) : none_like(q_);
+  Tensor dk = need_dx ? at::empty(k_.sizes(), k_.options()) : none_like(k_);
+  Tensor dqw = need_dw ? at::empty(qw_.sizes(), qw_.options()) : none_like(qw_);
+  Tensor dkw = need_dw ? at::empty(kw_.sizes(), kw_.options()) : none_like(kw_);
+  Tensor ws;
+  if (need_dw) ws = bytes(mi355_qk_norm_rotary_bwd_workspace_bytes(q.size), q_);
+  check(mi355_qk_norm_rotary_bwd(ptr(dq_out), ptr(dk_out), ptr(q.t), q.token_stride, q.head_stride, ptr(k.t), k.token_stride,
+                                 k.head_stride, ptr(qw), ptr(kw), dtype_code(q.t), ptr(positions.t), positions.wide, fptr(inv_freq),
+                                 inv_freq.numel(), (float)factor, interleaved, (float)eps, need_dx ? ptr(dq) : nullptr,
+                                 need_dx ? ptr(dk) : nullptr, need_dw ? ptr(dqw) : nullptr, need_dw ? ptr(dkw) : nullptr, ptr(ws),
+                                 q.tokens, q.heads, k.heads, q.size, L.stream),
+        "qk_norm_rotary_bwd");
+  return {dq, dk, dqw, dkw};
+}
+
 Tensor balance_loss_fwd(const Tensor& scores_, const Tensor& map_, const OptTensor& pad_) {
   Launch L(scores_);
   TORCH_CHECK_TYPE(scores_.scalar_type() == at::kFloat, "router scores must be float32");
@@ -613,6 +716,16 @@ TORCH_LIBRARY(mi355_moe, m) {
   m.def("rms_norm_fwd(Tensor x, Tensor weight, float epsilon) -> (Tensor, Tensor)");
   m.def(
       "rms_norm_bwd(Tensor dy, Tensor x, Tensor weight, Tensor rstd, bool need_dx, bool need_dw) -> (Tensor, Tensor)");
+  m.def(
+      "rotary(Tensor q, Tensor k, Tensor positions, Tensor inv_freq, bool interleaved, float attention_factor, "
+      "bool transpose) -> (Tensor, Tensor)");
+  m.def(
+      "qk_norm_rotary_fwd(Tensor q, Tensor k, Tensor q_weight, Tensor k_weight, Tensor positions, Tensor inv_freq, "
+      "float epsilon, bool interleaved, float attention_factor) -> (Tensor, Tensor)");
+  m.def(
+      "qk_norm_rotary_bwd(Tensor? dq_out, Tensor? dk_out, Tensor q, Tensor k, Tensor q_weight, Tensor k_weight, "
+      "Tensor positions, Tensor inv_freq, float epsilon, bool interleaved, float attention_factor, bool need_dx, "
+      "bool need_dw) -> (Tensor, Tensor, Tensor, Tensor)");
   m.def("balance_loss_fwd(Tensor scores, Tensor routing_map, Tensor? padding_mask) -> Tensor");
   m.def("balance_loss_bwd(Tensor scores, Tensor f, Tensor? padding_mask, Tensor grad_loss) -> Tensor");
   m.def(
@@ -677,6 +790,9 @@ TORCH_LIBRARY_IMPL(mi355_moe, CUDA, m) {
   m.impl("quantile_estimate", quantile_estimate);
   m.impl("rms_norm_fwd", rms_norm_fwd);
   m.impl("rms_norm_bwd", rms_norm_bwd);
+  m.impl("rotary", rotary);
+  m.impl("qk_norm_rotary_fwd", qk_norm_rotary_fwd);
+  m.impl("qk_norm_rotary_bwd", qk_norm_rotary_bwd);
   m.impl("balance_loss_fwd", balance_loss_fwd);
   m.impl("balance_loss_bwd", balance_loss_bwd);
   m.impl("permute_plan", permute_plan);

@@ -191,12 +191,60 @@ def rms_norm(hidden_states: torch.Tensor, weight: torch.Tensor, epsilon: float, 
     return dispatch_kernel("rms_norm", hidden_states, weight, epsilon)
 
 
+def _no_torch_math(name: str) -> None:
+    raise NotImplementedError(
+        f"{name}: no torch-math backend in this package; the HIP kernel is the only implementation")
+
+
+@register_kernel("rotary", "cuda")
+def rotary_mi355(query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *,
+                 interleaved: bool = False, attention_factor: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rotary positions of queries ``(..., H, D)`` and keys ``(..., G, D)`` on the GPU, both in one launch
+    (``ops.rotary``; frequencies, scaled ones for long contexts among them, from ``ops.rotary_frequencies``)."""
+    return ops.rotary(query, key, positions, inv_freq, interleaved=interleaved, attention_factor=attention_factor)
+
+
+def rotary(query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *,
+           interleaved: bool = False, attention_factor: float = 1.0,
+           use_eager: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    """The rotary operator, dispatched on the queries' device.  Frequencies and positions come as they are, not as
+    tables of sines: the angles are formed in the kernel, in fp64."""
+    if use_eager:
+        _no_torch_math("rotary")
+    return dispatch_kernel("rotary", query, key, positions, inv_freq, interleaved=interleaved,
+                           attention_factor=attention_factor)
+
+
+@register_kernel("qk_norm_rotary", "cuda")
+def qk_norm_rotary_mi355(query: torch.Tensor, key: torch.Tensor, query_weight: torch.Tensor, key_weight: torch.Tensor,
+                         positions: torch.Tensor, inv_freq: torch.Tensor, epsilon: float, *,
+                         interleaved: bool = False,
+                         attention_factor: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
+    """The RMS norm of every query and key head followed by ``rotary``, in one pass (``ops.qk_norm_rotary``)."""
+    return ops.qk_norm_rotary(query, key, query_weight, key_weight, positions, inv_freq, epsilon,
+                              interleaved=interleaved, attention_factor=attention_factor)
+
+
+def qk_norm_rotary(query: torch.Tensor, key: torch.Tensor, query_weight: torch.Tensor, key_weight: torch.Tensor,
+                   positions: torch.Tensor, inv_freq: torch.Tensor, epsilon: float, *, interleaved: bool = False,
+                   attention_factor: float = 1.0, use_eager: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    """``rotary(rms_norm(query, query_weight), rms_norm(key, key_weight))`` per head, dispatched on the queries' device."""
+    if use_eager:
+        _no_torch_math("qk_norm_rotary")
+    return dispatch_kernel("qk_norm_rotary", query, key, query_weight, key_weight, positions, inv_freq, epsilon,
+                           interleaved=interleaved, attention_factor=attention_factor)
+
+
 __all__ = [
     "dispatch_kernel",
     "get_kernel",
     "moe_token_permute",
     "moe_token_permute_mi355",
+    "qk_norm_rotary",
+    "qk_norm_rotary_mi355",
     "register_kernel",
     "rms_norm",
     "rms_norm_mi355",
+    "rotary",
+    "rotary_mi355",
 ]

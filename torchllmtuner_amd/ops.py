@@ -16,6 +16,7 @@ pre-allocated buffers) go straight to the C ABI through ``ctypes``.
 from __future__ import annotations
 
 import atexit
+import math
 import time
 from dataclasses import dataclass
 
@@ -167,6 +168,23 @@ def _(x, weight, epsilon):
 @_fake("rms_norm_bwd")
 def _(dy, x, weight, rstd, need_dx, need_dw):
     return (torch.empty_like(x) if need_dx else _e0(x)), (torch.empty_like(weight) if need_dw else _e0(weight))
+
+
+@_fake("rotary")
+def _(q, k, positions, inv_freq, interleaved, attention_factor, transpose):
+    return q.new_empty(q.shape), k.new_empty(k.shape)
+
+
+@_fake("qk_norm_rotary_fwd")
+def _(q, k, q_weight, k_weight, positions, inv_freq, epsilon, interleaved, attention_factor):
+    return q.new_empty(q.shape), k.new_empty(k.shape)
+
+
+@_fake("qk_norm_rotary_bwd")
+def _(dq_out, dk_out, q, k, q_weight, k_weight, positions, inv_freq, epsilon, interleaved, attention_factor, need_dx,
+      need_dw):
+    return (*(t.new_empty(t.shape) if need_dx else _e0(t) for t in (q, k)),
+            *(t.new_empty(t.shape) if need_dw else _e0(t) for t in (q_weight, k_weight)))
 
 
 @_fake("balance_loss_fwd")
@@ -395,6 +413,108 @@ def rms_norm_bwd(dy, x, weight, rstd, need_dx=True, need_dw=True):
     _dev(dy, x, weight, rstd)
     dx, dw = _O.rms_norm_bwd(dy, x, weight, rstd, bool(need_dx), bool(need_dw))
     return _opt(dx, need_dx), _opt(dw, need_dw)
+
+
+# ====================================================================== rotary positions
+def rotary_frequencies(rotary_dim, base=10000.0, *, scaling=None, factor=1.0, original_context=None, beta_fast=32.0,
+                       beta_slow=1.0, low_freq_factor=1.0, high_freq_factor=4.0, device=None):
+    """``(inv_freq, attention_factor)`` for ``rotary`` and ``qk_norm_rotary``: an fp32 tensor of
+    ``rotary_dim / 2`` frequencies ``base ** (-2 i / rotary_dim)``, formed in fp64, and the factor on the
+    rotated elements.  ``scaling`` stretches them for contexts ``factor`` times as long:
+
+    ``"linear"``  every frequency over ``factor`` (positions interpolated);
+    ``"ntk"``     the base times ``factor ** (rotary_dim / (rotary_dim - 2))``: the slowest pair is
+                  interpolated in full, the fastest not at all;
+    ``"yarn"``    pairs of more than ``beta_fast`` turns over ``original_context`` positions as they are, of fewer than
+                  ``beta_slow`` interpolated, a linear ramp over the pairs between; the attention factor is ``0.1 ln(factor) + 1``;
+    ``"llama3"``  wavelengths below ``original_context / high_freq_factor`` as they are, above
+                  ``original_context / low_freq_factor`` interpolated, between them a blend linear in the frequency.
+    """
+    R = int(rotary_dim)
+    if R < 2 or R % 2:
+        raise ValueError(f"rotary_dim must be a positive even number, got {rotary_dim}")
+    if not (math.isfinite(base) and base > 1.0):
+        raise ValueError(f"rotary base must be finite and above 1, got {base}")
+    if scaling not in (None, "linear", "ntk", "yarn", "llama3"):
+        raise ValueError(f"Unknown rotary scaling {scaling!r}")
+    if not (math.isfinite(factor) and factor >= 1.0):
+        raise ValueError(f"rotary scaling factor must be finite and at least 1, got {factor}")
+    if scaling in ("yarn", "llama3") and not (original_context and original_context > 0):
+        raise ValueError(f"rotary scaling {scaling!r} needs original_context")
+    if scaling == "yarn" and not beta_fast > beta_slow > 0:
+        raise ValueError("rotary scaling 'yarn' needs beta_fast > beta_slow > 0")
+    if scaling == "llama3" and not high_freq_factor > low_freq_factor > 0:
+        raise ValueError("rotary scaling 'llama3' needs high_freq_factor > low_freq_factor > 0")
+    if scaling == "ntk" and R > 2:
+        base = base * factor ** (R / (R - 2))
+    freq = torch.tensor([base ** (-2.0 * i / R) for i in range(R // 2)], dtype=torch.float64)
+    attention_factor = 1.0
+    if scaling == "linear" or (scaling == "ntk" and R == 2):
+        freq = freq / factor
+    elif scaling == "yarn":
+        def pair_of(turns):  # the (fractional) pair that makes so many turns over the original context
+            return R * math.log(original_context / (turns * 2.0 * math.pi)) / (2.0 * math.log(base))
+
+        low, high = max(math.floor(pair_of(beta_fast)), 0), min(math.ceil(pair_of(beta_slow)), R - 1)
+        ramp = ((torch.arange(R // 2, dtype=torch.float64) - low) / max(high - low, 1e-3)).clamp(0.0, 1.0)
+        freq = freq * (1.0 - ramp) + freq / factor * ramp
+        attention_factor = 0.1 * math.log(factor) + 1.0
+    elif scaling == "llama3":
+        turns = original_context * freq / (2.0 * math.pi)
+        kept = ((turns - low_freq_factor) / (high_freq_factor - low_freq_factor)).clamp(0.0, 1.0)
+        freq = freq * kept + freq / factor * (1.0 - kept)
+    return freq.float().to(device=device), attention_factor
+
+
+def _check_rotary(what, q, k, positions, inv_freq, attention_factor):
+    _dev(q, k, positions, inv_freq)
+    if q.ndim < 3 or k.ndim != q.ndim or q.shape[:-2] != k.shape[:-2] or q.shape[-1] != k.shape[-1]:
+        raise ValueError(f"{what}: queries {tuple(q.shape)} and keys {tuple(k.shape)} must be (..., heads, size) "
+                         "and agree in all but the heads")
+    if q.dtype != k.dtype:
+        raise TypeError(f"{what}: queries ({q.dtype}) and keys ({k.dtype}) must share a dtype")
+    _dt(q, fp64=False)
+    if not 2 <= q.shape[-1] <= 512 or q.shape[-2] < 1 or k.shape[-2] < 1:
+        raise ValueError(f"{what}: heads must have 2 to 512 elements, got {tuple(q.shape)} and {tuple(k.shape)}")
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"{what}: positions must be int32 or int64, got {positions.dtype}")
+    if positions.shape != q.shape[:-2]:
+        raise ValueError(f"{what}: positions {tuple(positions.shape)} must match the tokens {tuple(q.shape[:-2])}")
+    if inv_freq.dtype != torch.float32 or inv_freq.ndim != 1:
+        raise TypeError(f"{what}: inv_freq must be a 1-D float32 tensor")
+    if inv_freq.requires_grad:
+        raise ValueError(f"{what}: there is no gradient for inv_freq")
+    if not 1 <= inv_freq.shape[0] <= q.shape[-1] // 2:
+        raise ValueError(f"{what}: {inv_freq.shape[0]} frequencies turn {2 * inv_freq.shape[0]} elements of heads of {q.shape[-1]}")
+    if not math.isfinite(attention_factor):
+        raise ValueError(f"{what}: the attention factor must be finite")
+
+
+def rotary(q, k, positions, inv_freq, *, interleaved=False, attention_factor=1.0):
+    """Queries ``(..., H, D)`` and keys ``(..., G, D)`` with their first ``2 len(inv_freq)`` elements turned by
+    ``positions * inv_freq``: pairs ``(i, i + len(inv_freq))``, or ``(2 i, 2 i + 1)`` where ``interleaved``; the turned
+    elements are scaled by ``attention_factor``, the others copied.  ``positions`` has the tokens' shape ``(...)``.
+    Heads may be views into a fused projection (their elements next to each other): they are read where they lie; the
+    results are new dense tensors.  Differentiable in both (the same kernel, turned back)."""
+    _check_rotary("rotary", q, k, positions, inv_freq, attention_factor)
+    return _O.rotary(q, k, positions, inv_freq, bool(interleaved), float(attention_factor), False)
+
+
+def qk_norm_rotary(q, k, q_weight, k_weight, positions, inv_freq, epsilon, *, interleaved=False, attention_factor=1.0):
+    """``rotary(rms_norm(q, q_weight), rms_norm(k, k_weight))`` over the heads' elements in one pass, rounded once.
+    Weights are ``(D,)`` in the dtype of the heads.  Differentiable in the heads and the weights; the
+    backward keeps nothing but the inputs."""
+    _check_rotary("qk_norm_rotary", q, k, positions, inv_freq, attention_factor)
+    _dev(q, q_weight, k_weight)
+    for w in (q_weight, k_weight):
+        if w.dtype != q.dtype:
+            raise TypeError(f"qk_norm_rotary: heads ({q.dtype}) and norm weights ({w.dtype}) must share a dtype")
+        if w.shape != (q.shape[-1],):
+            raise ValueError(f"qk_norm_rotary: norm weights must be ({q.shape[-1]},), got {tuple(w.shape)}")
+    if not math.isfinite(epsilon) or epsilon < 0:
+        raise ValueError("qk_norm_rotary: epsilon must be finite and nonnegative")
+    return _O.qk_norm_rotary_fwd(q, k, q_weight, k_weight, positions, inv_freq, float(epsilon), bool(interleaved),
+                                 float(attention_factor))
 
 
 def _as_bool(m):
