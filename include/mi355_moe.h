@@ -785,6 +785,39 @@ int mi355_qk_norm_rotary_bwd(const void* dq_out, const void* dk_out, const void*
                              void* dk, void* dq_weight, void* dk_weight, void* workspace, int64_t T,
                              int64_t H, int64_t G, int64_t D, void* stream);
 
+/*
+ * Causal attention over packed sequences with grouped heads (the `varlen_attention` entry of the reference's kernel
+ * registry, llmtuner/kernel/ops/varlen_attention.py).  Query head h of row r in sequence [start, end), key head g = h / (H / G):
+ *   out[r][h] = sum_{start <= j <= r} softmax_j(scale q[r][h] . k[j][g]) v[j][g]
+ * cu_seqlens (sequences + 1, int32, ascending): where the sequences begin and the last one ends.  It stays on the device: no size depends on
+ * it.  Rows in no sequence (behind the last entry) get zeros, and have zero gradients.  Entries out of order or out of
+ * range give meaningless rows but never an access outside the tensors.
+ * q (T, H, D), k and v (T, G, D) with the given strides in elements, a head's elements next to each other; out dense.
+ * fp32 or bf16, 1 <= D <= 256, H a multiple of G, scale finite and positive, T < 2^30.  Scores, weights' statistics
+ * and sums are fp32; with bf16 storage the weights are rounded to bf16 for the second product where matrix kernels serve the call.
+ * lse: optional (H, T) fp32, log2 of each row's sum of exp(scale q.k), +inf for rows in no sequence; the backward reads it.
+ */
+int mi355_varlen_attention_fwd(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                               const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                               const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                               int dtype, const int32_t* cu_seqlens, int64_t sequences, float scale,
+                               void* out, float* lse, int64_t T, int64_t H, int64_t G, int64_t D,
+                               void* stream);
+
+/*
+ * Its backward; dout and out (the forward's) dense, so are dq, dk and dv.  Scores are formed again.  No atomics: dk and dv of a key
+ * head are sums over its query heads in a fixed order, by way of fp32 parts in the workspace where few key heads would
+ * leave the card idle.  workspace: mi355_varlen_attention_bwd_workspace_bytes(T, H, G, D) bytes.
+ */
+int64_t mi355_varlen_attention_bwd_workspace_bytes(int64_t T, int64_t H, int64_t G, int64_t D);
+int mi355_varlen_attention_bwd(const void* dout, const void* q, int64_t q_token_stride,
+                               int64_t q_head_stride, const void* k, int64_t k_token_stride,
+                               int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                               int64_t v_head_stride, const void* out, const float* lse, int dtype,
+                               const int32_t* cu_seqlens, int64_t sequences, float scale, void* dq,
+                               void* dk, void* dv, void* workspace, int64_t T, int64_t H, int64_t G,
+                               int64_t D, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,453 @@
+"""Causal attention over packed sequences against the formulas in fp64, element by element within derived bounds.
+
+Arithmetic is fp32 (u = 2^-24, half a step) on the stored inputs; with bf16 storage the weights p and the ds of the backward may
+be rounded to bf16 in front of their products and results are rounded to bf16 (half a step h = 2^-8 of the value).  With n visible
+keys, in natural units:
+
+* a score is a sum of D products: off by D u |scale| sum |q k|; its scaling, the row maximum and lse by 4 u of their sizes.  E = the
+  largest of that over a row's keys.
+* a weight: exp of it, over a sum of n such: off by e = 2 E + (2 n + 32) u of the weight; from lse (backward) 4 u |lse| more.
+* a result: sum p |v| (e + h + n u).
+* dp off by D u sum |do v|; delta = do . o by sum |do| (h |o| + the result's bound) of the stored, rounded o, and D u sum |do o|.
+* a weight below 2^-126, the least normal number of fp32, may come out as zero: exp2 has no others.  TINY = 2^-126 of absolute error
+  a weight, which a ds takes times |dp| + |delta|, and the products' results and the stored ones once more each.
+* ds = p (dp - delta): p ((|dp| + |delta|) (e + h + 4 u) + both errors), then sums of N terms add N u of their sizes.
+"""
+
+import math
+
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+from torchllmtuner_amd import _lib, kernel_registry, ops
+
+DEV = "cuda:0"
+U = 2.0**-24
+TINY = 2.0**-126
+BF, F32 = torch.bfloat16, torch.float32
+HALF_STEP = {BF: 2.0**-8, F32: 2.0**-24}
+gpu = pytest.mark.gpu
+
+
+def reference(q, k, v, dout, cu, scale, dtype):
+    """fp64 values and bounds of out, dq, dk, dv (before the storage rounding), on the CPU."""
+    q, k, v, dout = (t.detach().cpu().double() for t in (q, k, v, dout))
+    T, H, D = q.shape
+    group = H // k.shape[1]
+    h = 2.0**-8 if dtype == BF else 0.0
+    store = HALF_STEP[dtype]
+    val = [torch.zeros_like(t) for t in (q, q, k, v)]
+    off = [torch.zeros_like(t) for t in (q, q, k, v)]
+    for a, b in zip(cu, cu[1:]):
+        n = b - a
+        if n <= 0:
+            continue
+        seen = torch.ones(n, n, dtype=torch.bool).tril()
+        for head in range(H):
+            g = head // group
+            Q, K, V, G = q[a:b, head], k[a:b, g], v[a:b, g], dout[a:b, head]
+            s = (Q @ K.T * scale).masked_fill(~seen, -math.inf)
+            size = scale * (Q.abs() @ K.abs().T)
+            lse = torch.logsumexp(s, 1, keepdim=True)
+            p = torch.exp(s - lse)
+            E = ((D + 4) * U * size).masked_fill(~seen, 0).amax(1, keepdim=True)
+            e = 2 * E + (2 * n + 32) * U
+            out = p @ V
+            dout_bound = (p * (e + h + n * U) + TINY) @ V.abs()
+            val[0][a:b, head], off[0][a:b, head] = out, dout_bound
+            e = e + 4 * U * lse.abs()
+            N = n * group
+            val[3][a:b, g] += p.T @ G
+            off[3][a:b, g] += (p * (e + h + N * U) + TINY * seen).T @ G.abs()
+            dp, delta = G @ V.T, (G * out).sum(1, keepdim=True)
+            e_delta = (G.abs() * (store * (out.abs() + dout_bound) + dout_bound)).sum(1, keepdim=True)
+            e_delta = e_delta + D * U * (G.abs() * out.abs()).sum(1, keepdim=True)
+            e_dp = D * U * (G.abs() @ V.abs().T)
+            ds = p * (dp - delta)
+            e_ds = TINY * seen * (1 + dp.abs() + delta.abs()) + p * ((dp.abs() + delta.abs() + e_dp + e_delta) * (e + h + 4 * U) + e_dp + e_delta) * (1 + h)
+            val[1][a:b, head] = scale * (ds @ K)
+            off[1][a:b, head] = scale * ((e_ds + (n + 4) * U * ds.abs()) @ K.abs())
+            val[2][a:b, g] += scale * (ds.T @ Q)
+            off[2][a:b, g] += scale * ((e_ds + (N + 4) * U * ds.abs()).T @ Q.abs())
+    return val, off
+
+
+def inputs(T, H, G, D, dtype, seed, fused=False, size=1.0):
+    gen = torch.Generator().manual_seed(seed)
+    rows = (size * torch.randn(T, H + 2 * G, D, generator=gen)).to(dtype).to(DEV)
+    dout = torch.randn(T, H, D, generator=gen).to(dtype).to(DEV)
+    q, k, v = rows[:, :H], rows[:, H:H + G], rows[:, H + G:]
+    if not fused:
+        q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+    return [t.detach().requires_grad_() for t in (q, k, v)], dout
+
+
+def bounds_of(lengths, behind=0):
+    cu = [0]
+    for n in lengths:
+        cu.append(cu[-1] + n)
+    return cu, cu[-1] + behind
+
+
+def check(got, val, off, dtype, names=("out", "dq", "dk", "dv")):
+    for x, want, bound, name in zip(got, val, off, names):
+        x = x.detach().cpu().double()
+        assert not x.isnan().any(), name
+        over = (x - want).abs() - bound - HALF_STEP[dtype] * (want.abs() + bound) - 256 * TINY
+        worst = over.flatten().argmax().item()
+        assert over.max() <= 0, (f"{name}: {over.max():.3g} beyond the bound, {x.flatten()[worst]:.6g} for "
+                                 f"{want.flatten()[worst]:.6g}, element {worst} of {tuple(x.shape)}")
+
+
+def step(leaves, dout, cu, scale=None):
+    out = kernel_registry.varlen_attention(*leaves, cu, scale=scale)
+    return [out.detach(), *torch.autograd.grad(out, leaves, dout)]
+
+
+# (lengths, rows behind, heads, key heads, head size)
+CASES = [
+    ([1], 0, 1, 1, 64),
+    ([1, 1, 1], 2, 4, 2, 128),
+    ([0, 2, 0, 0, 5, 0], 0, 2, 1, 32),
+    ([33], 0, 3, 3, 128),
+    ([64], 0, 2, 1, 64),
+    ([65, 63], 0, 2, 2, 128),
+    ([127, 1, 129], 3, 4, 1, 128),
+    ([300], 0, 8, 2, 64),
+    ([31, 200, 7, 90], 17, 5, 1, 96),
+    ([130, 0, 260], 1, 2, 1, 80),
+    ([97, 100], 0, 6, 3, 112),
+    ([75, 50], 0, 2, 2, 8),
+    ([40, 85], 5, 2, 1, 160),
+    ([70, 66], 0, 2, 1, 192),
+    ([140], 9, 2, 2, 256),
+    ([30, 70], 0, 3, 1, 33),
+    ([45], 2, 2, 1, 1),
+    ([90, 20], 0, 1, 1, 127),
+    ([3] * 60, 4, 2, 2, 64),
+    ([513], 0, 4, 4, 128),
+    ([400, 380], 0, 2, 1, 128),
+]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("lengths,behind,H,G,D", CASES)
+def test_attention_matches_the_formula_in_both_directions(lengths, behind, H, G, D, dtype):
+    cu, T = bounds_of(lengths, behind)
+    print(f"varlen_attention {lengths}+{behind} heads {H}/{G} of {D} {dtype}", flush=True)
+    leaves, dout = inputs(T, H, G, D, dtype, seed=T + D, fused=T % 2 == 0)
+    got = step(leaves, dout, torch.tensor(cu, dtype=torch.int32, device=DEV))
+    for x, like in zip(got, (leaves[0], *leaves)):
+        assert x.shape == like.shape and x.dtype == dtype and x.is_contiguous()
+    val, off = reference(*leaves, dout, cu, D**-0.5, dtype)
+    check(got, val, off, dtype)
+    if behind:  # rows in no sequence: zeros, not merely small
+        assert not any(x[cu[-1]:].any() for x in got)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("size,scale", [(1.0, 0.01), (4.0, None), (12.0, 0.5)])
+def test_attention_over_flat_and_peaked_scores(size, scale, dtype):
+    cu, T = bounds_of([150, 60])
+    print(f"varlen_attention size {size} scale {scale} {dtype}", flush=True)
+    leaves, dout = inputs(T, 4, 2, 64, dtype, seed=3, size=size)
+    got = step(leaves, dout, torch.tensor(cu, dtype=torch.int32, device=DEV), scale)
+    check(got, *reference(*leaves, dout, cu, scale or 64**-0.5, dtype), dtype)
+
+
+@gpu
+def test_gradients_match_differences():
+    """Along a direction, against central differences of the formula in fp64 (step 1e-5: fp64 noise and the third derivative
+    below 1e-8 of the sum's size); the kernel's share is bounded element by element as above."""
+    cu, T = bounds_of([37, 22], 2)
+    leaves, dout = inputs(T, 4, 2, 24, F32, seed=8)
+    got = step(leaves, dout, torch.tensor(cu, dtype=torch.int32, device=DEV))[1:]
+    gen = torch.Generator().manual_seed(9)
+    way = [torch.randn(t.shape, generator=gen, dtype=torch.float64) for t in leaves]
+    base = [t.detach().cpu().double() for t in leaves]
+
+    def value(t):
+        q, k, v = (b + t * d for b, d in zip(base, way))
+        total = 0.0
+        for a, b in zip(cu, cu[1:]):
+            seen = torch.ones(b - a, b - a, dtype=torch.bool).tril()
+            for h in range(4):
+                s = (q[a:b, h] @ k[a:b, h // 2].T * 24**-0.5).masked_fill(~seen, -math.inf)
+                total = total + ((s.softmax(1) @ v[a:b, h // 2]) * dout[a:b, h].cpu().double()).sum()
+        return total
+
+    along = sum((g.cpu().double() * d).sum() for g, d in zip(got, way))
+    _, off = reference(*leaves, dout, cu, 24**-0.5, F32)
+    bound = sum(((o + U * g.cpu().double().abs()) * d.abs()).sum() for o, g, d in zip(off[1:], got, way))
+    assert abs(along - (value(1e-5) - value(-1e-5)) / 2e-5) < bound + 1e-6
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("D", [64, 128, 40, 160])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_values_in_masked_places_reach_no_row(value, D, dtype):
+    """A sequence whose inputs are spoilt, and the rows behind the last sequence, leave the others' results as they were bit for bit; in a
+    sequence, what comes before a spoilt row is its own, too."""
+    cu, T = bounds_of([20, 30, 90], 6)
+    print(f"varlen_attention with {value} {D} {dtype}", flush=True)
+    leaves, dout = inputs(T, 4, 2, D, dtype, seed=12)
+    at = torch.tensor(cu, dtype=torch.int32, device=DEV)
+    want = step(leaves, dout, at)
+    val, off = reference(*leaves, dout, cu, D**-0.5, dtype)
+    for which in range(4):
+        spoilt = [t.detach().clone() for t in (*leaves, dout)]
+        spoilt[which][33, 0, :3] = value  # in the second sequence
+        spoilt[which][cu[-1]:] = value    # in none
+        got = step([t.requires_grad_() for t in spoilt[:3]], spoilt[3], at)
+        clean = torch.ones(T, dtype=torch.bool)
+        clean[20:50] = False
+        for x, y in zip(got, want):
+            x, y = x[clean], y[clean]
+            assert x.isfinite().all()
+            torch.testing.assert_close(x, y, rtol=2**-5, atol=2**-5)
+        # (formed again key by key where a tile was spoilt: within the same bounds, though not of the same bits)
+        check([x[clean.to(DEV)] for x in got], [w[clean] for w in val], [o[clean] for o in off], dtype)
+        assert not any(x[cu[-1]:].any() for x in got)
+        # causality within the spoilt sequence: results above the row are as they were, gradients of keys behind it too
+        above, below = slice(20, 33), slice(34, 50)
+        check([got[0][above]], [val[0][above]], [off[0][above]], dtype)
+        if which in (0, 3):
+            check([x[below] for x in got], [w[below] for w in val], [o[below] for o in off], dtype)
+            assert got[0 if which == 0 else 1][33, 0].isnan().any()
+        else:
+            check([got[1][above]], [val[1][above]], [off[1][above]], dtype)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_layouts_give_the_same_bits(dtype):
+    T, H, G, D = 150, 6, 2, 64
+    cu = torch.tensor([0, 70, 149], dtype=torch.int32, device=DEV)
+    leaves, dout = inputs(T, H, G, D, dtype, seed=2)
+    want = step(leaves, dout, cu)
+
+    def same(other, g=dout):
+        return all(torch.equal(a, b) for a, b in zip(step([t.detach().requires_grad_() for t in other], g, cu), want))
+
+    fused = torch.cat(leaves, 1).detach()
+    assert same([fused[:, :H], fused[:, H:H + G], fused[:, H + G:]])
+    assert same([t.detach().transpose(0, 1).contiguous().transpose(0, 1) for t in leaves])  # heads in front
+    assert same([t.detach().repeat_interleave(2, -1)[..., ::2] for t in leaves])            # every other element
+    assert same(leaves, dout.repeat_interleave(2, 0)[::2])
+    off = []
+    for t in leaves:
+        flat = torch.empty(t.numel() + 1, dtype=dtype, device=DEV)
+        flat[1:] = t.detach().flatten()
+        off.append(flat[1:].view(t.shape))
+    for a, b in zip(step([t.requires_grad_() for t in off], dout, cu), want):
+        torch.testing.assert_close(a, b, rtol=2**-6, atol=2**-6)
+    # one key head for all, by a stride of zero: its gradient is the sum
+    one = [leaves[0], *(t.detach()[:, :1] for t in leaves[1:])]
+    a = step([t.detach().requires_grad_() for t in one], dout, cu)
+    wide = [one[0].detach().requires_grad_(), *(t.expand(T, 3, D).detach().requires_grad_() for t in one[1:])]
+    b = step(wide, dout, cu)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    for x, y in zip(a[2:], b[2:]):  # (three sums rounded to the storage type, then added)
+        torch.testing.assert_close(x.double(), y.double().sum(1, keepdim=True), rtol=2**-6, atol=2**-4 if dtype == BF else 2**-18)
+
+
+@gpu
+def test_streams_and_graphs_over_other_lengths_give_the_same_bits():
+    T, H, G, D = 200, 4, 2, 128
+    leaves, dout = inputs(T, H, G, D, BF, seed=4)
+    lengths = [[0, 120, 190], [0, 3, 200], [0, 0, 64], [0, 200, 200], [0, 77, 78]]
+    cus = [torch.tensor(c, dtype=torch.int32, device=DEV) for c in lengths]
+    want = [step(leaves, dout, c) for c in cus]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step(leaves, dout, cus[0])
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, want[0]))
+    # a captured step, replayed over other lengths, with eager work between the replays; two graphs alive at once
+    fresh = [t.detach().clone().requires_grad_() for t in leaves]
+    graphs = []
+    for _ in range(2):
+        cu = cus[0].clone()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(fresh, dout, cu)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            captured = step(fresh, dout, cu)
+        graphs.append((graph, cu, captured))
+    for i in range(len(cus)):
+        for j, (graph, cu, captured) in enumerate(graphs):
+            cu.copy_(cus[(i + j) % len(cus)])
+            graph.replay()
+        torch.cuda.synchronize()
+        eager = step(leaves, dout, cus[i])
+        assert all(torch.equal(a, b) for a, b in zip(eager, want[i]))
+        for j, (graph, cu, captured) in enumerate(graphs):
+            assert all(torch.equal(a, b) for a, b in zip(captured, want[(i + j) % len(cus)])), (i, j)
+
+
+@gpu
+def test_bounds_out_of_order_stay_inside_the_tensors():
+    """Entries that no caller should pass: results mean nothing, but every look-up stays inside (the sequence of a row always contains
+    it) and rows keep to what a call with sound bounds writes."""
+    T = 130
+    leaves, dout = inputs(T, 2, 1, 64, BF, seed=6)
+    for cu in ([0, 100, 50, 130], [5, 60], [-7, 40, 1000], [0, 2**31 - 1], [90, 90, 3], [7]):
+        print(f"varlen_attention bounds {cu}", flush=True)
+        got = step(leaves, dout, torch.tensor(cu, dtype=torch.int32, device=DEV))
+        assert all(x.isfinite().all() for x in got)
+    got = step(leaves, dout, torch.tensor([5, 60], dtype=torch.int32, device=DEV))
+    assert not any(x[:5].any() or x[60:].any() for x in got)  # rows in front of the first sequence are in none
+
+
+@gpu
+def test_no_tokens_and_only_some_gradients():
+    cu = torch.zeros(3, dtype=torch.int32, device=DEV)
+    leaves, dout = inputs(0, 4, 2, 64, BF, seed=1)
+    assert [x.shape for x in step(leaves, dout, cu)] == [(0, 4, 64), (0, 4, 64), (0, 2, 64), (0, 2, 64)]
+    cu = torch.tensor([0, 50], dtype=torch.int32, device=DEV)
+    leaves, dout = inputs(50, 4, 2, 64, BF, seed=1)
+    want = step(leaves, dout, cu)
+    for i in range(3):
+        part = [t if j == i else t.detach() for j, t in enumerate(leaves)]
+        out = ops.varlen_attention(*part, cu)
+        assert torch.equal(torch.autograd.grad(out, part[i], dout)[0], want[1 + i])
+    with torch.no_grad():
+        assert torch.equal(ops.varlen_attention(*leaves, cu), want[0])
+    # a gradient in another dtype, as autocast hands it on
+    assert torch.equal(torch.ops.mi355_moe.varlen_attention_bwd(
+        dout.float(), *(t.detach() for t in leaves), *torch.ops.mi355_moe.varlen_attention_fwd(
+            *(t.detach() for t in leaves), cu, 64**-0.5), cu, 64**-0.5)[0], want[1])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_the_attention_half_of_a_layer(dtype):
+    """Norms and rotation, then attention, over packed sequences whose positions start over: against the same in fp64 with
+    autograd.  The kernels' own bounds hold by themselves; here the chain's, by relative L2: bf16 rounds q and k, then p, out, ds and
+    the gradients, each by at most 2^-8 of the value (rms half that), some eight roundings on the longest way; fp32 in the same way
+    2^-24 times a few hundred additions."""
+    H, G, D, eps = 8, 2, 64, 1e-6
+    cu, T = bounds_of([100, 28, 60], 3)
+    print(f"norm, rotation, attention {dtype}", flush=True)
+    leaves, dout = inputs(T, H, G, D, dtype, seed=41, fused=True)
+    gen = torch.Generator().manual_seed(42)
+    w = [(1 + 0.1 * torch.randn(D, generator=gen)).to(dtype).to(DEV).requires_grad_() for _ in range(2)]
+    inv_freq, factor = ops.rotary_frequencies(D, 1e4, scaling="yarn", factor=4.0, original_context=64, device=DEV)
+    positions = torch.cat([torch.arange(b - a) for a, b in zip(cu, [*cu[1:], T])]).to(DEV)
+    at = torch.tensor(cu, dtype=torch.int32, device=DEV)
+    turned = kernel_registry.qk_norm_rotary(leaves[0], leaves[1], *w, positions, inv_freq, eps, attention_factor=factor)
+    out = kernel_registry.varlen_attention(*turned, leaves[2], at)
+    got = [out, *torch.autograd.grad(out, [*leaves, *w], dout)]
+
+    exact = [t.detach().cpu().double().requires_grad_() for t in (*leaves, *w)]
+    angle = positions.cpu().double()[:, None] * inv_freq.cpu().double()
+    c, s = factor * angle.cos()[:, None], factor * angle.sin()[:, None]
+    qk = []
+    for x, wi in zip(exact[:2], exact[3:]):
+        y = x / (x.pow(2).mean(-1, keepdim=True) + eps).sqrt() * wi
+        u, v = y.chunk(2, -1)
+        qk.append(torch.cat([u * c - v * s, v * c + u * s], -1))
+    rows = []
+    for a, b in zip(cu, cu[1:]):
+        seen = torch.ones(b - a, b - a, dtype=torch.bool).tril()
+        heads = [((qk[0][a:b, h] @ qk[1][a:b, h // 4].T * D**-0.5).masked_fill(~seen, -math.inf).softmax(1)
+                  @ exact[2][a:b, h // 4]) for h in range(H)]
+        rows.append(torch.stack(heads, 1))
+    rows.append(torch.zeros(T - cu[-1], H, D, dtype=torch.float64))
+    want = torch.cat(rows)
+    want = [want, *torch.autograd.grad(want, exact, dout.cpu().double())]
+    for x, y in zip(got, want):
+        err = (x.detach().cpu().double() - y.detach()).norm() / y.detach().norm()
+        assert err < (8 * 2.0**-8 if dtype == BF else 300 * 2.0**-24), err
+
+
+# ---- without a GPU ---------------------------------------------------------------------------------
+
+
+def test_operator_is_registered_for_the_gpu_only():
+    assert kernel_registry.get_kernel("varlen_attention", "cuda") is kernel_registry.varlen_attention_mi355
+    assert set(kernel_registry._KERNEL_REGISTRY["varlen_attention"]) == {"cuda"}
+    q, cu = torch.ones(2, 1, 4), torch.tensor([0, 2], dtype=torch.int32)
+    with pytest.raises(KeyError, match="not available"):
+        kernel_registry.varlen_attention(q, q, q, cu)
+    with pytest.raises(NotImplementedError, match="no torch-math backend"):
+        kernel_registry.varlen_attention(q, q, q, cu, use_eager=True)
+    with pytest.raises(RuntimeError, match="no CPU implementation"):
+        ops.varlen_attention(q, q, q, cu)
+
+
+def test_operator_refuses_what_does_not_fit_and_propagates_shapes():
+    with FakeTensorMode():
+        def t(*shape, dtype=BF):
+            return torch.empty(shape, dtype=dtype, device="cuda")
+
+        q, k, cu = t(10, 8, 64), t(10, 2, 64), t(3, dtype=torch.int32)
+
+        def refused(error, message, **change):
+            a = dict(q=q, k=k, v=k, cu_seqlens=cu, scale=None)
+            a.update(change)
+            with pytest.raises(error, match=message):
+                ops.varlen_attention(**a)
+
+        refused(ValueError, "agree in tokens and size", k=t(9, 2, 64))
+        refused(ValueError, "agree in tokens and size", v=t(10, 2, 32))
+        refused(ValueError, "agree in tokens and size", v=t(10, 1, 64))
+        refused(ValueError, "agree in tokens and size", q=t(1, 10, 8, 64))
+        refused(ValueError, "agree in tokens and size", q=t(10, 8, 32))
+        refused(TypeError, "share a dtype", v=k.float())
+        refused(TypeError, "float32 and bfloat16", q=q.half(), k=k.half(), v=k.half())
+        refused(TypeError, "float32 and bfloat16", q=q.double(), k=k.double(), v=k.double())
+        refused(ValueError, "no multiple", q=t(10, 5, 64))
+        refused(ValueError, "no multiple", k=t(10, 0, 64), v=t(10, 0, 64))
+        refused(ValueError, "1 to 256", q=t(10, 8, 257), k=t(10, 2, 257), v=t(10, 2, 257))
+        refused(ValueError, "cu_seqlens", cu_seqlens=t(3, dtype=torch.int64))
+        refused(ValueError, "cu_seqlens", cu_seqlens=t(0, dtype=torch.int32))
+        refused(ValueError, "cu_seqlens", cu_seqlens=t(1, 3, dtype=torch.int32))
+        for scale in (0.0, -1.0, math.inf, math.nan):
+            refused(ValueError, "finite and positive", scale=scale)
+        q.requires_grad_()
+        out = ops.varlen_attention(q, k, k, cu)
+        assert out.shape == q.shape and out.dtype == BF and out.requires_grad
+        out, lse = torch.ops.mi355_moe.varlen_attention_fwd(q.detach(), k, k, cu, 0.1)
+        assert lse.shape == (8, 10) and lse.dtype == F32
+        assert [x.shape for x in torch.ops.mi355_moe.varlen_attention_bwd(out, q.detach(), k, k, out, lse, cu, 0.1)] == [
+            q.shape, k.shape, k.shape]
+
+
+def test_c_entry_points_refuse_before_any_launch():
+    lib, p = _lib.load(), 0x1000  # (never dereferenced)
+
+    def forward(T=4, H=4, G=2, D=64, dtype=1, scale=0.1, cu=p, sequences=1):
+        return lib.mi355_varlen_attention_fwd(p, H * D, D, p, G * D, D, p, G * D, D, dtype, cu, sequences, scale, p, p, T, H, G, D, None)
+
+    def backward(T=4, H=4, G=2, D=64, workspace=p):
+        return lib.mi355_varlen_attention_bwd(p, p, H * D, D, p, G * D, D, p, G * D, D, p, p, 1, p, 1, 0.1, p, p, p, workspace, T, H, G,
+                                              D, None)
+
+    def text(rc, needle):
+        assert rc == -1 and needle in lib.mi355_moe_last_error(), (rc, lib.mi355_moe_last_error())
+
+    text(forward(dtype=2), b"neither fp32 nor bf16")
+    text(forward(D=257), b"head size 257")
+    text(forward(D=0), b"head size 0")
+    text(forward(H=3), b"no multiple")
+    text(forward(T=1 << 30), b"bad shape")
+    text(forward(T=-1), b"bad shape")
+    text(forward(sequences=-1), b"bad shape")
+    text(forward(scale=0.0), b"finite and positive")
+    text(forward(scale=math.nan), b"finite and positive")
+    text(forward(cu=None), b"null pointer")
+    assert forward(T=0) == 0
+    text(backward(H=3), b"no multiple")
+    text(backward(workspace=None), b"null pointer")
+    text(backward(workspace=p + 8), b"16-byte")
+    assert backward(T=0) == 0
+    assert lib.mi355_varlen_attention_bwd_workspace_bytes(100, 4, 2, 64) >= 4 * 4 * 100
+    assert lib.mi355_varlen_attention_bwd_workspace_bytes(0, 4, 2, 64) == 0

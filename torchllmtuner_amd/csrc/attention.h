@@ -1,0 +1,181 @@
+// What the attention kernels share: their arguments, the sequence of a row, and the careful row-by-row forms for what a
+// value that is not finite has spoilt.
+//
+// Causal attention over sequences packed one behind another, for query head h on key head h / (H / G):
+//   s_rj = q_r . k_j,   p_rj = exp2(c s_rj - lse_r) for start(r) <= j <= r,   o_r = sum_j p_rj v_j
+// with c = scale log2(e) and lse_r = log2 sum_j exp2(c s_rj); and backward, with delta_r = do_r . o_r,
+//   ds_rj = p_rj (do_r . v_j - delta_r) scale,
+//   dq_r = sum_j ds_rj k_j,   dk_j = sum_h,r ds_rj q_r,   dv_j = sum_h,r p_rj do_r.
+//
+// Tiles are runs of rows of the packed tensors, whatever sequences they cut through: a tile of many short sequences is
+// then as full as one of a long one, and the grid follows from the sizes alone, without reading cu_seqlens back.  Every row looks
+// up its own sequence; the look-up's answer holds start <= row < end whatever the array holds, so no index leaves the tensors.
+//
+// Rows whose mask leaves nothing (in no sequence) get zeros.  A matrix product cannot leave out an element:
+// 0 x NaN, of a value in a masked place of the same tile, is NaN in the sum.  Such a sum shows at the end
+// as NaN, and only then the row is formed again by the functions here, key by key, without the masked ones.  Where no input is
+// NaN or infinite that costs one comparison an element of the result.
+#pragma once
+#include "bf16_tiles.h"
+#include "common.h"
+
+namespace mi355 {
+
+struct AttnArgs {
+  const void *q, *k, *v;  // (T, H, D), (T, G, D), (T, G, D); elements of a head contiguous
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head;  // strides, in elements
+  void* out;              // (T, H, D) dense
+  float* lse;             // (H, T), log2
+  // backward
+  const void *o, *dout;   // (T, H, D) dense
+  float* delta;           // (H, T)
+  void *dq, *dk, *dv;     // dense; (splits > 1: dk_part, dv_part instead of dk, dv)
+  float *dk_part, *dv_part;  // [splits][T][G][D] fp32
+  const int32_t* cu;      // [sequences + 1]
+  int sequences;
+  int T, H, G, D, group;  // group = H / G
+  int splits;             // parts that a key head's group of query heads is cut into for dk and dv
+  float scale, c;         // c = scale log2(e)
+};
+
+constexpr float kNegInf = -INFINITY;
+
+// The sequence [start, end) that a row lies in, or start = end = 0.  The entries on both sides of the answer have been compared with the
+// row, so start <= row < end however the array is ordered; clamped to the rows there are.
+__device__ __forceinline__ void sequence_of(const int32_t* cu, int sequences, int T, int row, int& start, int& end) {
+  int a = 0, b = sequences + 1;  // entries below a are <= row, entries from b on are > row
+  while (a < b) {
+    const int mid = (a + b) >> 1;
+    if (cu[mid] <= row) a = mid + 1;
+    else b = mid;
+  }
+  start = end = 0;
+  if (a == 0 || a > sequences || row >= T) return;
+  start = max(cu[a - 1], 0);
+  end = min(cu[a], T);
+}
+
+__device__ __forceinline__ float exp2_f32(float x) { return __builtin_amdgcn_exp2f(x); }
+
+template <typename T>
+__device__ __forceinline__ const T* row_at(const void* base, int64_t token, int64_t head, int64_t t, int64_t h) {
+  return static_cast<const T*>(base) + t * token + h * head;
+}
+
+// ---- one row by one wave: lanes over keys (or queries) for the products, over the head's elements for the sums -------------------
+constexpr int kHeadMax = 256;          // elements of a head
+constexpr int kLaneCols = kHeadMax / 64;
+
+// sum_d a[d] b[d], a wave's lanes each with rows of their own
+template <typename T>
+__device__ float careful_dot(const T* a, const T* b, int D) {
+  float s = 0.0f;
+  for (int d = 0; d < D; ++d) s = fmaf(load_as_f32<T>(a + d), load_as_f32<T>(b + d), s);
+  return s;
+}
+
+template <typename T>
+__device__ __forceinline__ void careful_forward_row(const AttnArgs& p, int h, int row, int start) {
+  const int lane = threadIdx.x & 63;
+  const T* q = row_at<T>(p.q, p.q_token, p.q_head, row, h);
+  float acc[kLaneCols] = {}, m = kNegInf, l = 0.0f;
+  for (int j0 = start; j0 <= row; j0 += kWave) {
+    const int j = j0 + lane;
+    const float s = j <= row ? careful_dot<T>(q, row_at<T>(p.k, p.k_token, p.k_head, j, h / p.group), p.D) : kNegInf;
+    const float top = fmaxf(m, wave_max(s)), ref = top == kNegInf ? 0.0f : top * p.c;
+    const float w = j <= row ? exp2_f32(fmaf(s, p.c, -ref)) : 0.0f, keep = m == kNegInf ? 0.0f : exp2_f32(m * p.c - ref);
+    l = l * keep + wave_sum(w);
+#pragma unroll
+    for (int i = 0; i < kLaneCols; ++i) acc[i] *= keep;
+    for (int n = 0; n < kWave && j0 + n <= row; ++n) {
+      const float wn = __shfl(w, n, kWave);
+      const T* v = row_at<T>(p.v, p.v_token, p.v_head, j0 + n, h / p.group);
+#pragma unroll
+      for (int i = 0; i < kLaneCols; ++i)
+        if (lane + 64 * i < p.D) acc[i] = fmaf(wn, load_as_f32<T>(v + lane + 64 * i), acc[i]);
+    }
+    m = top;
+  }
+  T* out = static_cast<T*>(p.out) + (static_cast<int64_t>(row) * p.H + h) * p.D;
+#pragma unroll
+  for (int i = 0; i < kLaneCols; ++i)
+    if (lane + 64 * i < p.D) store_from_f32<T>(out + lane + 64 * i, acc[i] / l);
+}
+
+template <typename T>
+__device__ __forceinline__ void careful_dq_row(const AttnArgs& p, int h, int row, int start, float lse, float delta) {
+  const int lane = threadIdx.x & 63;
+  const T* q = row_at<T>(p.q, p.q_token, p.q_head, row, h);
+  const T* dout = static_cast<const T*>(p.dout) + (static_cast<int64_t>(row) * p.H + h) * p.D;
+  float acc[kLaneCols] = {};
+  for (int j0 = start; j0 <= row; j0 += kWave) {
+    const int j = j0 + lane;
+    float ds = 0.0f;
+    if (j <= row) {
+      const float w = exp2_f32(fmaf(careful_dot<T>(q, row_at<T>(p.k, p.k_token, p.k_head, j, h / p.group), p.D), p.c, -lse));
+      ds = w * (careful_dot<T>(dout, row_at<T>(p.v, p.v_token, p.v_head, j, h / p.group), p.D) - delta);
+    }
+    for (int n = 0; n < kWave && j0 + n <= row; ++n) {
+      const float dn = __shfl(ds, n, kWave);
+      const T* k = row_at<T>(p.k, p.k_token, p.k_head, j0 + n, h / p.group);
+#pragma unroll
+      for (int i = 0; i < kLaneCols; ++i)
+        if (lane + 64 * i < p.D) acc[i] = fmaf(dn, load_as_f32<T>(k + lane + 64 * i), acc[i]);
+    }
+  }
+  T* dq = static_cast<T*>(p.dq) + (static_cast<int64_t>(row) * p.H + h) * p.D;
+#pragma unroll
+  for (int i = 0; i < kLaneCols; ++i)
+    if (lane + 64 * i < p.D) store_from_f32<T>(dq + lane + 64 * i, acc[i] * p.scale);
+}
+
+// dk and dv of one key over the query heads [h0, h1), into the part `split` where there are parts
+template <typename T>
+__device__ __forceinline__ void careful_dkv_row(const AttnArgs& p, int g, int key, int end, int h0, int h1, int split) {
+  const int lane = threadIdx.x & 63;
+  const T* k = row_at<T>(p.k, p.k_token, p.k_head, key, g);
+  const T* v = row_at<T>(p.v, p.v_token, p.v_head, key, g);
+  float dk[kLaneCols] = {}, dv[kLaneCols] = {};
+  for (int h = h0; h < h1; ++h) {
+    for (int r0 = key; r0 < end; r0 += kWave) {
+      const int r = r0 + lane;
+      float w = 0.0f, ds = 0.0f;
+      if (r < end) {
+        const T* dout = static_cast<const T*>(p.dout) + (static_cast<int64_t>(r) * p.H + h) * p.D;
+        const int64_t at = static_cast<int64_t>(h) * p.T + r;
+        w = exp2_f32(fmaf(careful_dot<T>(row_at<T>(p.q, p.q_token, p.q_head, r, h), k, p.D), p.c, -p.lse[at]));
+        ds = w * (careful_dot<T>(dout, v, p.D) - p.delta[at]);
+      }
+      for (int n = 0; n < kWave && r0 + n < end; ++n) {
+        const float wn = __shfl(w, n, kWave), dn = __shfl(ds, n, kWave);
+        const T* q = row_at<T>(p.q, p.q_token, p.q_head, r0 + n, h);
+        const T* dout = static_cast<const T*>(p.dout) + (static_cast<int64_t>(r0 + n) * p.H + h) * p.D;
+#pragma unroll
+        for (int i = 0; i < kLaneCols; ++i)
+          if (lane + 64 * i < p.D) {
+            dv[i] = fmaf(wn, load_as_f32<T>(dout + lane + 64 * i), dv[i]);
+            dk[i] = fmaf(dn, load_as_f32<T>(q + lane + 64 * i), dk[i]);
+          }
+      }
+    }
+  }
+  const int64_t at = (static_cast<int64_t>(key) * p.G + g) * p.D, part = static_cast<int64_t>(split) * p.T * p.G * p.D + at;
+#pragma unroll
+  for (int i = 0; i < kLaneCols; ++i) {
+    const int d = lane + 64 * i;
+    if (d >= p.D) continue;
+    if (p.splits > 1) {
+      p.dk_part[part + d] = dk[i] * p.scale;
+      p.dv_part[part + d] = dv[i];
+    } else {
+      store_from_f32<T>(static_cast<T*>(p.dk) + at + d, dk[i] * p.scale);
+      store_from_f32<T>(static_cast<T*>(p.dv) + at + d, dv[i]);
+    }
+  }
+}
+
+// ---- launches, by file --------------------------------------------------------------------------------
+void attention_any_forward(const AttnArgs& p, int dtype, hipStream_t s);
+void attention_any_backward(const AttnArgs& p, int dtype, hipStream_t s);
+
+}  // namespace mi355

@@ -1,0 +1,561 @@
+// Causal attention over packed sequences (attention.h has the formulas), for every head size up to 256, fp32 and bf16
+// storage, on v_mfma_f32_16x16x4_f32: fp32 products throughout.  And the entry points, which choose between this and the
+// bf16 matrix kernels.
+//
+// v_mfma_f32_16x16x4_f32 takes one element a lane of each operand (row or column lane % 16, k = lane / 16) and yields four
+// (column lane % 16, rows 4 (lane / 16) + i).  Products are formed turned so that one's result is the next one's operand as it lies:
+//   forward, dq:  s^T = K Q^T (columns: the wave's 16 queries) is the right operand of o^T += V^T p^T and dq^T += K^T ds^T,
+//   dk, dv:       s = Q K^T (columns: the wave's 16 keys) that of dv^T += dO^T p and dk^T += Q^T ds.
+// Keys 4 g + i of a block then meet in step i from lane group g; the contraction over a head's elements takes them in the order
+// 4 g + i of each 16 too, so that a lane reads 16 bytes of a row for four steps.
+//
+// Rows of the other operand pass through LDS in tiles of 32 a wave column, at a pitch of 4 floats beyond the head: the row reads
+// (16 rows, 16 bytes) and the column reads (four rows 4 apart, 16 floats) both meet every bank once.  Bound by the fp32 matrix
+// rate, 256 flops a cycle and CU; a wave's softmax is a twentieth of its products.
+//
+// A workgroup is four waves: QW groups of 16 rows by KW parts of the other axis, each with its own running
+// maximum and sum, joined through LDS at the end.  Four parts where the rows alone would not fill the card.
+#include <algorithm>
+#include <cmath>
+
+#include "attention.h"
+
+namespace mi355 {
+namespace {
+
+template <typename T>
+__device__ __forceinline__ float4 four_at(const T* p, int n, bool vec) {  // the first n of p[0..3], zeros behind them
+  if (vec) {
+    if constexpr (sizeof(T) == 4) return *reinterpret_cast<const float4*>(p);
+    const u32x2 q = *reinterpret_cast<const u32x2*>(p);
+    return make_float4(__uint_as_float(q[0] << 16), __uint_as_float(q[0] & 0xffff0000u), __uint_as_float(q[1] << 16),
+                       __uint_as_float(q[1] & 0xffff0000u));
+  }
+  float4 v = make_float4(0, 0, 0, 0);
+  if (n > 0) v.x = load_as_f32<T>(p);
+  if (n > 1) v.y = load_as_f32<T>(p + 1);
+  if (n > 2) v.z = load_as_f32<T>(p + 2);
+  if (n > 3) v.w = load_as_f32<T>(p + 3);
+  return v;
+}
+
+// rows [row0, row0 + ROWS) of a head into LDS as fp32, zeros behind row T and behind the head's elements
+template <typename T, int DP, int ROWS>
+__device__ __forceinline__ void fill_tile(float* tile, const T* base, int64_t token, int row0, int T_, int D, bool vec) {
+  constexpr int P = DP + 4, QUADS = DP / 4;
+  for (int i = threadIdx.x; i < ROWS * QUADS; i += 256) {
+    const int r = i / QUADS, d = (i % QUADS) * 4;
+    float4 v = make_float4(0, 0, 0, 0);
+    if (row0 + r < T_ && d < D) v = four_at<T>(base + static_cast<int64_t>(row0 + r) * token + d, D - d, vec && d + 4 <= D);
+    *reinterpret_cast<float4*>(tile + r * P + d) = v;
+  }
+}
+
+// a wave's 16 rows as an operand over the head's elements: lane's row lane % 16, elements 16 j + 4 (lane / 16) + i
+template <typename T, int DP>
+__device__ __forceinline__ void own_rows(float (&x)[DP / 4], const T* base, int64_t token, int row, bool on, int D, bool vec, int lane) {
+#pragma unroll
+  for (int j = 0; j < DP / 16; ++j) {
+    const int d = 16 * j + 4 * (lane >> 4);
+    float4 v = make_float4(0, 0, 0, 0);
+    if (on && d < D) v = four_at<T>(base + static_cast<int64_t>(row) * token + d, D - d, vec && d + 4 <= D);
+    x[4 * j] = v.x, x[4 * j + 1] = v.y, x[4 * j + 2] = v.z, x[4 * j + 3] = v.w;
+  }
+}
+
+// 16 rows of a tile times the wave's own rows, over the head's elements
+template <int DP>
+__device__ __forceinline__ f32x4 rows_product(const float* tile, const float (&x)[DP / 4], int lane) {
+  constexpr int P = DP + 4;
+  f32x4 s = {0, 0, 0, 0};
+  const float* a = tile + (lane & 15) * P + 4 * (lane >> 4);
+#pragma unroll
+  for (int j = 0; j < DP / 16; ++j) {
+    const float4 v = *reinterpret_cast<const float4*>(a + 16 * j);
+    s = __builtin_amdgcn_mfma_f32_16x16x4f32(v.x, x[4 * j], s, 0, 0, 0);
+    s = __builtin_amdgcn_mfma_f32_16x16x4f32(v.y, x[4 * j + 1], s, 0, 0, 0);
+    s = __builtin_amdgcn_mfma_f32_16x16x4f32(v.z, x[4 * j + 2], s, 0, 0, 0);
+    s = __builtin_amdgcn_mfma_f32_16x16x4f32(v.w, x[4 * j + 3], s, 0, 0, 0);
+  }
+  return s;
+}
+
+// acc^T (head's elements x the wave's 16) += tile^T w, over 16 rows of a tile
+template <int DP>
+__device__ __forceinline__ void columns_product(f32x4 (&acc)[DP / 16], const float* tile, const f32x4& w, int lane) {
+  constexpr int P = DP + 4;
+  const float* a = tile + 4 * (lane >> 4) * P + (lane & 15);
+#pragma unroll
+  for (int n = 0; n < DP / 16; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i * P + 16 * n], w[i], acc[n], 0, 0, 0);
+}
+
+// over the four lane groups that hold a column
+__device__ __forceinline__ float column_max(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16, kWave));
+  return fmaxf(v, __shfl_xor(v, 32, kWave));
+}
+__device__ __forceinline__ float column_sum(float v) {
+  v += __shfl_xor(v, 16, kWave);
+  return v + __shfl_xor(v, 32, kWave);
+}
+__device__ __forceinline__ int wave_min_i(int v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, kWave));
+  return __builtin_amdgcn_readfirstlane(v);
+}
+__device__ __forceinline__ int wave_max_i(int v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o, kWave));
+  return __builtin_amdgcn_readfirstlane(v);
+}
+
+constexpr int kStep = 32;  // rows of the other axis that a wave takes at a time
+
+template <int DP, int KW>
+constexpr size_t kAnyLds = sizeof(float) * (KW * kStep * 2 * (DP + 4) + 128);
+
+struct Range {
+  int lo, hi;
+};
+// the range of the workgroup from those of its waves
+__device__ __forceinline__ Range group_range(int lo, int hi, int* red) {
+  const int wave = threadIdx.x >> 6;
+  if ((threadIdx.x & 63) == 0) red[2 * wave] = lo, red[2 * wave + 1] = hi;
+  __syncthreads();
+  Range r = {min(min(red[0], red[2]), min(red[4], red[6])), max(max(red[1], red[3]), max(red[5], red[7]))};
+  __syncthreads();
+  r.lo = __builtin_amdgcn_readfirstlane(r.lo);
+  r.hi = __builtin_amdgcn_readfirstlane(r.hi);
+  return r;
+}
+
+// the last tiles first: the later rows of a long sequence have the most keys, and what starts last should be short
+__device__ __forceinline__ int tile_from_the_end(int tiles) { return tiles - 1 - static_cast<int>(blockIdx.x); }
+
+template <typename T, int DP, int KW>
+__global__ __launch_bounds__(256) void any_forward_kernel(const AttnArgs p, int tiles, int vec) {
+  constexpr int QW = 4 / KW, P = DP + 4, NB = DP / 16;
+  extern __shared__ __attribute__((aligned(16))) float lds[];
+  float *kt = lds, *vt = lds + KW * kStep * P, *stats = lds + 2 * KW * kStep * P;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int qw = wave / KW, kw = wave % KW, h = blockIdx.y, g = h / p.group;
+  const int row0 = tile_from_the_end(tiles) * 16 * QW, row = row0 + 16 * qw + (lane & 15);
+  int start, end;
+  sequence_of(p.cu, p.sequences, p.T, row, start, end);
+  const bool on = start < end;
+  const int lo = wave_min_i(on ? start : p.T), hi = wave_max_i(on ? row + 1 : 0);
+  const Range all = group_range(lo, hi, reinterpret_cast<int*>(stats));
+  float q[DP / 4];
+  own_rows<T, DP>(q, static_cast<const T*>(p.q) + h * p.q_head, p.q_token, row, on, p.D, vec, lane);
+  f32x4 o[NB];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) o[n] = f32x4{0, 0, 0, 0};
+  float m = kNegInf, l = 0.0f;
+  for (int k0 = all.lo; k0 < all.hi; k0 += KW * kStep) {
+    __syncthreads();
+    fill_tile<T, DP, KW * kStep>(kt, static_cast<const T*>(p.k) + g * p.k_head, p.k_token, k0, p.T, p.D, vec);
+    fill_tile<T, DP, KW * kStep>(vt, static_cast<const T*>(p.v) + g * p.v_head, p.v_token, k0, p.T, p.D, vec);
+    __syncthreads();
+    const int kb = k0 + kw * kStep;
+    if (kb >= hi || kb + kStep <= lo) continue;
+    f32x4 s[2];
+    float top = m;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      s[b] = rows_product<DP>(kt + (kw * kStep + 16 * b) * P, q, lane);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = kb + 16 * b + 4 * (lane >> 4) + i;
+        s[b][i] = on && key >= start && key <= row ? s[b][i] : kNegInf;
+        top = fmaxf(top, s[b][i]);
+      }
+    }
+    top = column_max(top);
+    const float ref = top == kNegInf ? 0.0f : top * p.c;  // (nothing seen yet: every weight is 0, not NaN)
+    const float keep = m == kNegInf ? 0.0f : exp2_f32(m * p.c - ref);
+    float sum = 0.0f;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s[b][i] = exp2_f32(fmaf(s[b][i], p.c, -ref));
+        sum += s[b][i];
+      }
+    l = l * keep + sum;  // the lane group's share; the four are added at the end
+    m = top;
+#pragma unroll
+    for (int n = 0; n < NB; ++n) o[n] *= keep;
+    columns_product<DP>(o, vt + (kw * kStep) * P, s[0], lane);
+    columns_product<DP>(o, vt + (kw * kStep + 16) * P, s[1], lane);
+  }
+  l = column_sum(l);
+  // join the parts: [wave][16 rows][DP] of sums, [wave][16] of maxima and sums
+  __syncthreads();
+  float *sums = lds, *tops = stats, *lens = stats + 64;
+  static_assert(64 * (DP + 4) <= 2 * KW * kStep * P, "the waves' sums fit in the tiles");
+#pragma unroll
+  for (int n = 0; n < NB; ++n)
+    *reinterpret_cast<f32x4*>(sums + (wave * 16 + (lane & 15)) * P + 16 * n + 4 * (lane >> 4)) = o[n];
+  if (lane < 16) tops[wave * 16 + lane] = m, lens[wave * 16 + lane] = l;
+  __syncthreads();
+  // a wave writes the rows that it and its parts share: 16 / KW of them
+  for (int i = 0; i < 16 / KW; ++i) {
+    const int mine = kw * (16 / KW) + i, r = row0 + 16 * qw + mine;
+    if (r >= p.T) break;
+    int first, last;
+    sequence_of(p.cu, p.sequences, p.T, r, first, last);
+    float w[KW], best = kNegInf, len = 0.0f;
+#pragma unroll
+    for (int part = 0; part < KW; ++part) best = fmaxf(best, tops[(qw * KW + part) * 16 + mine]);
+    const float ref = best == kNegInf ? 0.0f : best * p.c;
+#pragma unroll
+    for (int part = 0; part < KW; ++part) {
+      const float t = tops[(qw * KW + part) * 16 + mine];
+      w[part] = t == kNegInf ? 0.0f : exp2_f32(t * p.c - ref);
+      len += w[part] * lens[(qw * KW + part) * 16 + mine];
+      // a part without a finite score: 0 as above, unless its own sum is NaN already
+      if (t == kNegInf && lens[(qw * KW + part) * 16 + mine] != 0.0f) len = NAN;
+    }
+    bool spoilt = false;
+    T* out = static_cast<T*>(p.out) + (static_cast<int64_t>(r) * p.H + h) * p.D;
+    for (int d = lane; d < p.D; d += kWave) {
+      float v = 0.0f;
+#pragma unroll
+      for (int part = 0; part < KW; ++part) v += w[part] * sums[((qw * KW + part) * 16 + mine) * P + d];
+      v /= len;
+      spoilt |= v != v;
+      store_from_f32<T>(out + d, first < last ? v : 0.0f);
+    }
+    if (lane == 0 && p.lse) p.lse[static_cast<int64_t>(h) * p.T + r] = first < last ? ref + log2f(len) : INFINITY;
+    if (first < last && __any(spoilt)) careful_forward_row<T>(p, h, r, first);
+  }
+}
+
+// dq, and delta for the kernel behind this one
+template <typename T, int DP, int KW>
+__global__ __launch_bounds__(256) void any_dq_kernel(const AttnArgs p, int tiles, int vec) {
+  constexpr int QW = 4 / KW, P = DP + 4, NB = DP / 16;
+  extern __shared__ __attribute__((aligned(16))) float lds[];
+  float *kt = lds, *vt = lds + KW * kStep * P, *stats = lds + 2 * KW * kStep * P;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int qw = wave / KW, kw = wave % KW, h = blockIdx.y, g = h / p.group;
+  const int row0 = tile_from_the_end(tiles) * 16 * QW, row = row0 + 16 * qw + (lane & 15);
+  int start, end;
+  sequence_of(p.cu, p.sequences, p.T, row, start, end);
+  const bool on = start < end;
+  const int lo = wave_min_i(on ? start : p.T), hi = wave_max_i(on ? row + 1 : 0);
+  const Range all = group_range(lo, hi, reinterpret_cast<int*>(stats));
+  float q[DP / 4], dout[DP / 4];
+  const int64_t dense = static_cast<int64_t>(p.H) * p.D;
+  own_rows<T, DP>(q, static_cast<const T*>(p.q) + h * p.q_head, p.q_token, row, on, p.D, vec, lane);
+  own_rows<T, DP>(dout, static_cast<const T*>(p.dout) + h * p.D, dense, row, on, p.D, vec, lane);
+  float delta = 0.0f;
+  {
+    float o[DP / 4];
+    own_rows<T, DP>(o, static_cast<const T*>(p.o) + h * p.D, dense, row, on, p.D, vec, lane);
+#pragma unroll
+    for (int i = 0; i < DP / 4; ++i) delta = fmaf(o[i], dout[i], delta);
+  }
+  delta = column_sum(delta);
+  const float lse = on ? p.lse[static_cast<int64_t>(h) * p.T + row] : INFINITY;
+  if (kw == 0 && lane < 16 && row < p.T) p.delta[static_cast<int64_t>(h) * p.T + row] = on ? delta : 0.0f;
+  f32x4 dq[NB];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) dq[n] = f32x4{0, 0, 0, 0};
+  for (int k0 = all.lo; k0 < all.hi; k0 += KW * kStep) {
+    __syncthreads();
+    fill_tile<T, DP, KW * kStep>(kt, static_cast<const T*>(p.k) + g * p.k_head, p.k_token, k0, p.T, p.D, vec);
+    fill_tile<T, DP, KW * kStep>(vt, static_cast<const T*>(p.v) + g * p.v_head, p.v_token, k0, p.T, p.D, vec);
+    __syncthreads();
+    const int kb = k0 + kw * kStep;
+    if (kb >= hi || kb + kStep <= lo) continue;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const float* kb_t = kt + (kw * kStep + 16 * b) * P;
+      const f32x4 s = rows_product<DP>(kb_t, q, lane);
+      const f32x4 dp = rows_product<DP>(vt + (kw * kStep + 16 * b) * P, dout, lane);
+      f32x4 ds;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = kb + 16 * b + 4 * (lane >> 4) + i;
+        const bool seen = on && key >= start && key <= row;
+        ds[i] = seen ? exp2_f32(fmaf(s[i], p.c, -lse)) * (dp[i] - delta) : 0.0f;
+      }
+      columns_product<DP>(dq, kb_t, ds, lane);
+    }
+  }
+  __syncthreads();
+  float *sums = lds, *lses = stats, *deltas = stats + 64;
+#pragma unroll
+  for (int n = 0; n < NB; ++n)
+    *reinterpret_cast<f32x4*>(sums + (wave * 16 + (lane & 15)) * P + 16 * n + 4 * (lane >> 4)) = dq[n];
+  if (lane < 16) lses[wave * 16 + lane] = lse, deltas[wave * 16 + lane] = delta;
+  __syncthreads();
+  for (int i = 0; i < 16 / KW; ++i) {
+    const int mine = kw * (16 / KW) + i, r = row0 + 16 * qw + mine;
+    if (r >= p.T) break;
+    int first, last;
+    sequence_of(p.cu, p.sequences, p.T, r, first, last);
+    bool spoilt = false;
+    T* out = static_cast<T*>(p.dq) + (static_cast<int64_t>(r) * p.H + h) * p.D;
+    for (int d = lane; d < p.D; d += kWave) {
+      float v = 0.0f;
+#pragma unroll
+      for (int part = 0; part < KW; ++part) v += sums[((qw * KW + part) * 16 + mine) * P + d];
+      spoilt |= v != v;
+      store_from_f32<T>(out + d, first < last ? v * p.scale : 0.0f);
+    }
+    if (first < last && __any(spoilt)) careful_dq_row<T>(p, h, r, first, lses[(qw * KW) * 16 + mine], deltas[(qw * KW) * 16 + mine]);
+  }
+}
+
+// dk and dv: a wave's 16 keys against the query heads of their group, or a part of them
+template <typename T, int DP, int KW>
+__global__ __launch_bounds__(256) void any_dkv_kernel(const AttnArgs p, int vec) {
+  constexpr int QW = 4 / KW, P = DP + 4, NB = DP / 16;
+  extern __shared__ __attribute__((aligned(16))) float lds[];
+  float *qt = lds, *dt = lds + KW * kStep * P, *stats = lds + 2 * KW * kStep * P;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int qw = wave / KW, kw = wave % KW;
+  const int g = blockIdx.y / p.splits, split = blockIdx.y % p.splits;
+  const int heads = (p.group + p.splits - 1) / p.splits, h0 = g * p.group + split * heads, h1 = min(h0 + heads, (g + 1) * p.group);
+  const int key0 = blockIdx.x * 16 * QW, key = key0 + 16 * qw + (lane & 15);
+  int start, end;
+  sequence_of(p.cu, p.sequences, p.T, key, start, end);
+  const bool on = start < end;
+  const int lo = wave_min_i(on ? key : p.T), hi = wave_max_i(on ? end : 0);
+  const Range all = group_range(lo, hi, reinterpret_cast<int*>(stats));
+  float k[DP / 4], v[DP / 4];
+  own_rows<T, DP>(k, static_cast<const T*>(p.k) + g * p.k_head, p.k_token, key, on, p.D, vec, lane);
+  own_rows<T, DP>(v, static_cast<const T*>(p.v) + g * p.v_head, p.v_token, key, on, p.D, vec, lane);
+  f32x4 dk[NB], dv[NB];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) dk[n] = dv[n] = f32x4{0, 0, 0, 0};
+  const int64_t dense = static_cast<int64_t>(p.H) * p.D;
+  for (int h = h0; h < h1; ++h) {
+    const float *lse = p.lse + static_cast<int64_t>(h) * p.T, *delta = p.delta + static_cast<int64_t>(h) * p.T;
+    for (int r0 = all.lo; r0 < all.hi; r0 += KW * kStep) {
+      __syncthreads();
+      fill_tile<T, DP, KW * kStep>(qt, static_cast<const T*>(p.q) + h * p.q_head, p.q_token, r0, p.T, p.D, vec);
+      fill_tile<T, DP, KW * kStep>(dt, static_cast<const T*>(p.dout) + h * p.D, dense, r0, p.T, p.D, vec);
+      __syncthreads();
+      const int rb = r0 + kw * kStep;
+      if (rb >= hi || rb + kStep <= lo) continue;
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const float *q_t = qt + (kw * kStep + 16 * b) * P, *d_t = dt + (kw * kStep + 16 * b) * P;
+        const f32x4 s = rows_product<DP>(q_t, k, lane);
+        const f32x4 dp = rows_product<DP>(d_t, v, lane);
+        f32x4 w, ds;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = rb + 16 * b + 4 * (lane >> 4) + i;
+          const bool seen = on && r >= key && r < end;
+          w[i] = seen ? exp2_f32(fmaf(s[i], p.c, -lse[min(r, p.T - 1)])) : 0.0f;
+          ds[i] = seen ? w[i] * (dp[i] - delta[min(r, p.T - 1)]) : 0.0f;
+        }
+        columns_product<DP>(dv, d_t, w, lane);
+        columns_product<DP>(dk, q_t, ds, lane);
+      }
+    }
+  }
+  const int64_t part0 = static_cast<int64_t>(split) * p.T * p.G * p.D;
+  bool spoilt[16 / KW];
+#pragma unroll
+  for (int i = 0; i < 16 / KW; ++i) spoilt[i] = false;
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+      *reinterpret_cast<f32x4*>(lds + (wave * 16 + (lane & 15)) * P + 16 * n + 4 * (lane >> 4)) = which ? dk[n] : dv[n];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 16 / KW; ++i) {
+      const int mine = kw * (16 / KW) + i, r = key0 + 16 * qw + mine;
+      if (r >= p.T) continue;
+      int first, last;
+      sequence_of(p.cu, p.sequences, p.T, r, first, last);
+      const int64_t at = (static_cast<int64_t>(r) * p.G + g) * p.D;
+      bool bad = false;
+      for (int d = lane; d < p.D; d += kWave) {
+        float x = 0.0f;
+#pragma unroll
+        for (int part = 0; part < KW; ++part) x += lds[((qw * KW + part) * 16 + mine) * P + d];
+        bad |= x != x;
+        x = first < last ? (which ? x * p.scale : x) : 0.0f;
+        if (p.splits > 1) (which ? p.dk_part : p.dv_part)[part0 + at + d] = x;
+        else store_from_f32<T>(static_cast<T*>(which ? p.dk : p.dv) + at + d, x);
+      }
+      spoilt[i] |= first < last && __any(bad);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 16 / KW; ++i)
+    if (spoilt[i]) {
+      const int r = key0 + 16 * qw + kw * (16 / KW) + i;
+      int first, last;
+      sequence_of(p.cu, p.sequences, p.T, r, first, last);
+      careful_dkv_row<T>(p, g, r, last, h0, h1, split);
+    }
+}
+
+// dk and dv from their parts, added in order
+template <typename T>
+__global__ __launch_bounds__(256) void join_parts_kernel(const float* __restrict__ dk_part, const float* __restrict__ dv_part,
+                                                         T* __restrict__ dk, T* __restrict__ dv, int splits, int64_t n) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= n) return;
+  const float* part = blockIdx.y ? dv_part : dk_part;
+  float v = 0.0f;
+  for (int s = 0; s < splits; ++s) v += part[s * n + i];
+  store_from_f32<T>((blockIdx.y ? dv : dk) + i, v);
+}
+
+template <typename Fn>
+void with_head(int D, Fn f) {
+  if (D <= 64) f(std::integral_constant<int, 64>{});
+  else if (D <= 96) f(std::integral_constant<int, 96>{});
+  else if (D <= 128) f(std::integral_constant<int, 128>{});
+  else if (D <= 192) f(std::integral_constant<int, 192>{});
+  else f(std::integral_constant<int, 256>{});
+}
+
+bool in_fours(const AttnArgs& p, int item, bool backward) {
+  uintptr_t bits = reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v);
+  if (backward) bits |= reinterpret_cast<uintptr_t>(p.o) | reinterpret_cast<uintptr_t>(p.dout);
+  return bits % (4 * item) == 0 && (p.q_token | p.q_head | p.k_token | p.k_head | p.v_token | p.v_head | p.D) % 4 == 0;
+}
+
+template <typename K>
+void allow_lds(K kernel, size_t bytes, PerDeviceOnce& once) {
+  if (bytes <= 65536 || !once.needed()) return;
+  (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  once.done();
+}
+
+}  // namespace
+
+template <typename T, int DP, int KW>
+void any_forward(const AttnArgs& p, int vec, hipStream_t s) {
+  static PerDeviceOnce once;
+  allow_lds(any_forward_kernel<T, DP, KW>, kAnyLds<DP, KW>, once);
+  const int rows = 64 / KW, tiles = (p.T + rows - 1) / rows;
+  hipLaunchKernelGGL((any_forward_kernel<T, DP, KW>), dim3(tiles, p.H), dim3(256), (kAnyLds<DP, KW>), s, p, tiles, vec);
+}
+
+void attention_any_forward(const AttnArgs& p, int dtype, hipStream_t s) {
+  auto run = [&](auto tag) {
+    using T = decltype(tag);
+    const int vec = in_fours(p, sizeof(T), false);
+    with_head(p.D, [&](auto d) { any_forward<T, decltype(d)::value, 2>(p, vec, s); });
+  };
+  if (dtype == MI355_F32) run(float{});
+  else run(uint16_t{});
+}
+
+template <typename T, int DP, int KW>
+void any_backward(const AttnArgs& p, int vec, hipStream_t s) {
+  static PerDeviceOnce once_q, once_kv;
+  allow_lds(any_dq_kernel<T, DP, KW>, kAnyLds<DP, KW>, once_q);
+  allow_lds(any_dkv_kernel<T, DP, KW>, kAnyLds<DP, KW>, once_kv);
+  const int rows = 64 / KW, tiles = (p.T + rows - 1) / rows;
+  hipLaunchKernelGGL((any_dq_kernel<T, DP, KW>), dim3(tiles, p.H), dim3(256), (kAnyLds<DP, KW>), s, p, tiles, vec);
+  hipLaunchKernelGGL((any_dkv_kernel<T, DP, KW>), dim3(tiles, p.G * p.splits), dim3(256), (kAnyLds<DP, KW>), s, p, vec);
+  if (p.splits > 1) {
+    const int64_t n = static_cast<int64_t>(p.T) * p.G * p.D;
+    hipLaunchKernelGGL(join_parts_kernel<T>, dim3((unsigned)((n + 255) / 256), 2), dim3(256), 0, s, p.dk_part, p.dv_part,
+                       static_cast<T*>(p.dk), static_cast<T*>(p.dv), p.splits, n);
+  }
+}
+
+void attention_any_backward(const AttnArgs& p, int dtype, hipStream_t s) {
+  auto run = [&](auto tag) {
+    using T = decltype(tag);
+    const int vec = in_fours(p, sizeof(T), true);
+    with_head(p.D, [&](auto d) { any_backward<T, decltype(d)::value, 2>(p, vec, s); });
+  };
+  if (dtype == MI355_F32) run(float{});
+  else run(uint16_t{});
+}
+
+}  // namespace mi355
+
+using namespace mi355;
+
+namespace {
+
+int check_attention(const char* what, int dtype, int64_t sequences, int64_t T, int64_t H, int64_t G, int64_t D, float scale) {
+  MI355_REQUIRE(dtype == MI355_F32 || dtype == MI355_BF16, "%s: dtype %d is neither fp32 nor bf16", what, dtype);
+  MI355_REQUIRE(T >= 0 && T < (1ll << 30) && sequences >= 0 && sequences < (1ll << 30), "%s: bad shape tokens=%lld sequences=%lld", what,
+                (long long)T, (long long)sequences);
+  MI355_REQUIRE(H >= 1 && G >= 1 && H <= 65535 && H % G == 0, "%s: %lld query heads are no multiple of %lld key heads", what,
+                (long long)H, (long long)G);
+  MI355_REQUIRE(D >= 1 && D <= kHeadMax, "%s: head size %lld is not within 1 to %d", what, (long long)D, kHeadMax);
+  MI355_REQUIRE(std::isfinite(scale) && scale > 0.0f, "%s: the scale must be finite and positive", what);
+  return MI355_OK;
+}
+
+// Parts of a key head's group of query heads: as many as it takes for dk and dv to fill the card
+int head_parts(int64_t T, int64_t H, int64_t G) {
+  const int64_t group = H / G, tiles = (T + 63) / 64 * G;
+  int64_t parts = std::min<int64_t>(group, (1024 + tiles - 1) / std::max<int64_t>(tiles, 1));
+  const int64_t heads = (group + parts - 1) / parts;
+  return (int)((group + heads - 1) / heads);
+}
+
+AttnArgs attention_args(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token, int64_t k_head, const void* v,
+                        int64_t v_token, int64_t v_head, const int32_t* cu, int64_t sequences, float scale, int64_t T, int64_t H,
+                        int64_t G, int64_t D) {
+  AttnArgs p = {};
+  p.q = q, p.k = k, p.v = v;
+  p.q_token = q_token, p.q_head = q_head, p.k_token = k_token, p.k_head = k_head, p.v_token = v_token, p.v_head = v_head;
+  p.cu = cu, p.sequences = (int)sequences;
+  p.T = (int)T, p.H = (int)H, p.G = (int)G, p.D = (int)D, p.group = (int)(H / G);
+  p.scale = scale, p.c = (float)(scale * 1.4426950408889634);
+  return p;
+}
+
+}  // namespace
+
+extern "C" int mi355_varlen_attention_fwd(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                                          int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                                          int64_t v_head_stride, int dtype, const int32_t* cu_seqlens, int64_t sequences, float scale,
+                                          void* out, float* lse, int64_t T, int64_t H, int64_t G, int64_t D, void* stream) {
+  if (int rc = check_attention("varlen_attention_fwd", dtype, sequences, T, H, G, D, scale)) return rc;
+  if (T == 0) return MI355_OK;
+  MI355_REQUIRE(q && k && v && cu_seqlens && out, "varlen_attention_fwd: null pointer");
+  AttnArgs p = attention_args(q, q_token_stride, q_head_stride, k, k_token_stride, k_head_stride, v, v_token_stride, v_head_stride,
+                              cu_seqlens, sequences, scale, T, H, G, D);
+  p.out = out, p.lse = lse;
+  attention_any_forward(p, dtype, as_stream(stream));
+  return check_launch("varlen_attention_fwd");
+}
+
+extern "C" int64_t mi355_varlen_attention_bwd_workspace_bytes(int64_t T, int64_t H, int64_t G, int64_t D) {
+  if (T < 1 || H < 1 || G < 1 || H % G || D < 1) return 0;
+  const int64_t parts = head_parts(T, H, G);
+  return 4 * ((H * T + 3) / 4 * 4 + (parts > 1 ? 2 * parts * T * G * D : 0));
+}
+
+extern "C" int mi355_varlen_attention_bwd(const void* dout, const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                                          int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                                          int64_t v_head_stride, const void* out, const float* lse, int dtype,
+                                          const int32_t* cu_seqlens, int64_t sequences, float scale, void* dq, void* dk, void* dv,
+                                          void* workspace, int64_t T, int64_t H, int64_t G, int64_t D, void* stream) {
+  if (int rc = check_attention("varlen_attention_bwd", dtype, sequences, T, H, G, D, scale)) return rc;
+  if (T == 0) return MI355_OK;
+  MI355_REQUIRE(dout && q && k && v && out && lse && cu_seqlens && dq && dk && dv && workspace, "varlen_attention_bwd: null pointer");
+  MI355_REQUIRE(aligned16(workspace), "varlen_attention_bwd: the workspace must start on a 16-byte boundary");
+  AttnArgs p = attention_args(q, q_token_stride, q_head_stride, k, k_token_stride, k_head_stride, v, v_token_stride, v_head_stride,
+                              cu_seqlens, sequences, scale, T, H, G, D);
+  p.o = out, p.dout = dout, p.lse = const_cast<float*>(lse), p.dq = dq, p.dk = dk, p.dv = dv;
+  p.splits = head_parts(T, H, G);
+  p.delta = static_cast<float*>(workspace);
+  p.dk_part = p.delta + (H * T + 3) / 4 * 4;
+  p.dv_part = p.dk_part + static_cast<int64_t>(p.splits) * T * G * D;
+  attention_any_backward(p, dtype, as_stream(stream));
+  return check_launch("varlen_attention_bwd");
+}

@@ -468,6 +468,46 @@ std::tuple<Tensor, Tensor> qk_norm_rotary_autograd(const Tensor& q, const Tensor
   return {r[0], r[1]};
 }
 
+// ---- causal attention over packed sequences: the row statistics carry no gradient -----------------------
+using AttentionFwdSig = std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const Tensor&, double);
+using AttentionBwdSig = std::tuple<Tensor, Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                                                           const Tensor&, const Tensor&, double);
+
+struct VarlenAttention : public torch::autograd::Function<VarlenAttention> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu, double scale) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    static auto op = typed_op<AttentionFwdSig>("mi355_moe::varlen_attention_fwd");
+    auto r = op.call(q, k, v, cu, scale);
+    ctx->save_for_backward({q, k, v, std::get<0>(r), std::get<1>(r), cu});
+    ctx->saved_data["scale"] = scale;
+    ctx->mark_non_differentiable({std::get<1>(r)});
+    ctx->set_materialize_grads(false);
+    return {std::get<0>(r), std::get<1>(r)};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list out(5);
+    const bool n0 = ctx->needs_input_grad(0), n1 = ctx->needs_input_grad(1), n2 = ctx->needs_input_grad(2);
+    if (!grads[0].defined() || !(n0 || n1 || n2)) return out;
+    const auto s = ctx->get_saved_variables();
+    static auto op = typed_op<AttentionBwdSig>("mi355_moe::varlen_attention_bwd");
+    auto r = op.call(grads[0], s[0], s[1], s[2], s[3], s[4], s[5], ctx->saved_data["scale"].toDouble());
+    out[0] = keep(std::get<0>(r), n0);
+    out[1] = keep(std::get<1>(r), n1);
+    out[2] = keep(std::get<2>(r), n2);
+    return out;
+  }
+};
+
+std::tuple<Tensor, Tensor> varlen_attention_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu, double scale) {
+  if (!torch::autograd::compute_requires_grad(q, k, v)) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    static auto op = typed_op<AttentionFwdSig>("mi355_moe::varlen_attention_fwd");
+    return op.call(q, k, v, cu, scale);
+  }
+  auto r = VarlenAttention::apply(q, k, v, cu, scale);
+  return {r[0], r[1]};
+}
+
 // ---- load-balance loss: out = (loss, f_E...); the gradient flows into the scores -------------------
 using BalanceFwdSig = Tensor(const Tensor&, const Tensor&, const OptTensor&);
 using BalanceBwdSig = Tensor(const Tensor&, const Tensor&, const OptTensor&, const Tensor&);
@@ -623,6 +663,7 @@ TORCH_LIBRARY_IMPL(mi355_moe, Autograd, m) {
   m.impl("rms_norm_fwd", rms_norm_autograd);
   m.impl("rotary", rotary_autograd);
   m.impl("qk_norm_rotary_fwd", qk_norm_rotary_autograd);
+  m.impl("varlen_attention_fwd", varlen_attention_autograd);
   m.impl("balance_loss_fwd", balance_loss_autograd);
   m.impl("permute_rows_fwd", permute_rows_autograd);
   m.impl("combine_fwd", combine_autograd);

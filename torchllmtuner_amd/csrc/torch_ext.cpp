@@ -290,6 +290,48 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> qk_norm_rotary_bwd(const OptTensor& d
   return {dq, dk, dqw, dkw};
 }
 
+void check_attention(const Heads& q, const Heads& k, const Heads& v, const Tensor& cu) {
+  TORCH_CHECK_TYPE(q.t.scalar_type() == k.t.scalar_type() && q.t.scalar_type() == v.t.scalar_type(), "queries, keys and values must share a dtype");
+  TORCH_CHECK_VALUE(k.t.sizes() == v.t.sizes() && q.tokens == k.tokens && q.size == k.size, "queries ", q.t.sizes(), ", keys ",
+                    k.t.sizes(), " and values ", v.t.sizes(), " must agree in tokens and head size");
+  TORCH_CHECK_TYPE(cu.scalar_type() == at::kInt, "cu_seqlens must be int32, got ", cu.scalar_type());
+  TORCH_CHECK_VALUE(cu.dim() == 1 && cu.numel() >= 1, "cu_seqlens must be 1-D with at least one entry");
+  TORCH_CHECK_VALUE(k.t.device() == q.t.device() && v.t.device() == q.t.device() && cu.device() == q.t.device(),
+                    "queries, keys, values and cu_seqlens must share a device");
+}
+
+std::tuple<Tensor, Tensor> varlen_attention_fwd(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& cu_, double scale) {
+  Launch L(q_);
+  const Heads q(q_), k(k_), v(v_);
+  check_attention(q, k, v, cu_);
+  const Tensor cu = cu_.contiguous();
+  Tensor out = at::empty(q_.sizes(), q_.options()), lse = at::empty({q.heads, q.tokens}, q_.options().dtype(at::kFloat));
+  check(mi355_varlen_attention_fwd(ptr(q.t), q.token_stride, q.head_stride, ptr(k.t), k.token_stride, k.head_stride, ptr(v.t),
+                                   v.token_stride, v.head_stride, dtype_code(q.t), iptr(cu), cu.numel() - 1, (float)scale, ptr(out),
+                                   static_cast<float*>(ptr(lse)), q.tokens, q.heads, k.heads, q.size, L.stream),
+        "varlen_attention_fwd");
+  return {out, lse};
+}
+
+std::tuple<Tensor, Tensor, Tensor> varlen_attention_bwd(const Tensor& dout_, const Tensor& q_, const Tensor& k_, const Tensor& v_,
+                                                        const Tensor& out_, const Tensor& lse_, const Tensor& cu_, double scale) {
+  Launch L(q_);
+  const Heads q(q_), k(k_), v(v_);
+  check_attention(q, k, v, cu_);
+  const Tensor dout = heads_like(dout_, q_), out = dense(out_), lse = dense(lse_), cu = cu_.contiguous();
+  TORCH_CHECK_VALUE(dout.sizes() == q_.sizes() && out.sizes() == q_.sizes() && out.scalar_type() == q_.scalar_type() &&
+                        lse.numel() == q.heads * q.tokens && lse.scalar_type() == at::kFloat,
+                    "the gradient, the result and its statistics do not fit the queries");
+  Tensor dq = at::empty(q_.sizes(), q_.options()), dk = at::empty(k_.sizes(), k_.options()), dv = at::empty(v_.sizes(), v_.options());
+  const Tensor ws = bytes(mi355_varlen_attention_bwd_workspace_bytes(q.tokens, q.heads, k.heads, q.size), q_);
+  check(mi355_varlen_attention_bwd(ptr(dout), ptr(q.t), q.token_stride, q.head_stride, ptr(k.t), k.token_stride, k.head_stride,
+                                   ptr(v.t), v.token_stride, v.head_stride, ptr(out), fptr(lse), dtype_code(q.t), iptr(cu),
+                                   cu.numel() - 1, (float)scale, ptr(dq), ptr(dk), ptr(dv), ptr(ws), q.tokens, q.heads, k.heads,
+                                   q.size, L.stream),
+        "varlen_attention_bwd");
+  return {dq, dk, dv};
+}
+
 Tensor balance_loss_fwd(const Tensor& scores_, const Tensor& map_, const OptTensor& pad_) {
   Launch L(scores_);
   TORCH_CHECK_TYPE(scores_.scalar_type() == at::kFloat, "router scores must be float32");
@@ -726,6 +768,10 @@ TORCH_LIBRARY(mi355_moe, m) {
       "qk_norm_rotary_bwd(Tensor? dq_out, Tensor? dk_out, Tensor q, Tensor k, Tensor q_weight, Tensor k_weight, "
       "Tensor positions, Tensor inv_freq, float epsilon, bool interleaved, float attention_factor, bool need_dx, "
       "bool need_dw) -> (Tensor, Tensor, Tensor, Tensor)");
+  m.def("varlen_attention_fwd(Tensor q, Tensor k, Tensor v, Tensor cu_seqlens, float scale) -> (Tensor, Tensor)");
+  m.def(
+      "varlen_attention_bwd(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor out, Tensor lse, Tensor cu_seqlens, "
+      "float scale) -> (Tensor, Tensor, Tensor)");
   m.def("balance_loss_fwd(Tensor scores, Tensor routing_map, Tensor? padding_mask) -> Tensor");
   m.def("balance_loss_bwd(Tensor scores, Tensor f, Tensor? padding_mask, Tensor grad_loss) -> Tensor");
   m.def(
@@ -793,6 +839,8 @@ TORCH_LIBRARY_IMPL(mi355_moe, CUDA, m) {
   m.impl("rotary", rotary);
   m.impl("qk_norm_rotary_fwd", qk_norm_rotary_fwd);
   m.impl("qk_norm_rotary_bwd", qk_norm_rotary_bwd);
+  m.impl("varlen_attention_fwd", varlen_attention_fwd);
+  m.impl("varlen_attention_bwd", varlen_attention_bwd);
   m.impl("balance_loss_fwd", balance_loss_fwd);
   m.impl("balance_loss_bwd", balance_loss_bwd);
   m.impl("permute_plan", permute_plan);

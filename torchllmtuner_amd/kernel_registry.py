@@ -235,6 +235,22 @@ def qk_norm_rotary(query: torch.Tensor, key: torch.Tensor, query_weight: torch.T
                            interleaved=interleaved, attention_factor=attention_factor)
 
 
+@register_kernel("varlen_attention", "cuda")
+def varlen_attention_mi355(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, cu_seqlens: torch.Tensor, *,
+                           scale: float | None = None) -> torch.Tensor:
+    """Causal attention over sequences packed along the tokens, with grouped heads, on the GPU (``ops.varlen_attention``)."""
+    return ops.varlen_attention(query, key, value, cu_seqlens, scale=scale)
+
+
+def varlen_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, cu_seqlens: torch.Tensor, *,
+                     scale: float | None = None, use_eager: bool = False) -> torch.Tensor:
+    """Causal attention of queries ``(T, H, D)`` over keys and values ``(T, G, D)`` within the sequences that
+    ``cu_seqlens`` bounds, dispatched on the queries' device."""
+    if use_eager:
+        _no_torch_math("varlen_attention")
+    return dispatch_kernel("varlen_attention", query, key, value, cu_seqlens, scale=scale)
+
+
 __all__ = [
     "dispatch_kernel",
     "get_kernel",
@@ -247,4 +263,6 @@ __all__ = [
     "rms_norm_mi355",
     "rotary",
     "rotary_mi355",
+    "varlen_attention",
+    "varlen_attention_mi355",
 ]

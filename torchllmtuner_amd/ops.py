@@ -187,6 +187,16 @@ def _(dq_out, dk_out, q, k, q_weight, k_weight, positions, inv_freq, epsilon, in
             *(t.new_empty(t.shape) if need_dw else _e0(t) for t in (q_weight, k_weight)))
 
 
+@_fake("varlen_attention_fwd")
+def _(q, k, v, cu_seqlens, scale):
+    return q.new_empty(q.shape), q.new_empty((q.shape[1], q.shape[0]), dtype=torch.float32)
+
+
+@_fake("varlen_attention_bwd")
+def _(dout, q, k, v, out, lse, cu_seqlens, scale):
+    return tuple(t.new_empty(t.shape) for t in (q, k, v))
+
+
 @_fake("balance_loss_fwd")
 def _(scores, routing_map, padding_mask):
     return scores.new_empty((1 + scores.shape[1],))
@@ -515,6 +525,36 @@ def qk_norm_rotary(q, k, q_weight, k_weight, positions, inv_freq, epsilon, *, in
         raise ValueError("qk_norm_rotary: epsilon must be finite and nonnegative")
     return _O.qk_norm_rotary_fwd(q, k, q_weight, k_weight, positions, inv_freq, float(epsilon), bool(interleaved),
                                  float(attention_factor))
+
+
+# ====================================================================== attention
+def varlen_attention(q, k, v, cu_seqlens, *, scale=None):
+    """Causal attention over packed sequences: queries ``(T, H, D)``, keys and values ``(T, G, D)`` with ``H`` a
+    multiple of ``G`` (query head ``h`` reads key head ``h // (H // G)``), ``1 <= D <= 256``, fp32 or bf16.
+    ``cu_seqlens`` (int32, ascending, on the device) holds where each sequence begins and where the last one ends, as
+    ``[0, n_0, n_0 + n_1, ...]``; sequences may be empty.  A row sees the rows of its own sequence up to itself; rows behind the last
+    sequence get zeros and have zero gradients.  ``scale`` defaults to ``D ** -0.5``.  Views into a fused projection are read
+    where they lie.  Nothing is read back from the device: a call can be captured, and replayed over other
+    lengths.  Differentiable in queries, keys and values; bit-identical from run to run."""
+    _dev(q, k, v, cu_seqlens)
+    if q.ndim != 3 or k.ndim != 3 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
+        raise ValueError(f"varlen_attention: queries {tuple(q.shape)}, keys {tuple(k.shape)} and values {tuple(v.shape)} "
+                         "must be (tokens, heads, size) and agree in tokens and size")
+    if not q.dtype == k.dtype == v.dtype:
+        raise TypeError(f"varlen_attention: queries ({q.dtype}), keys ({k.dtype}) and values ({v.dtype}) must share a dtype")
+    _dt(q, fp64=False)
+    if k.shape[1] < 1 or q.shape[1] < 1 or q.shape[1] % k.shape[1]:
+        raise ValueError(f"varlen_attention: {q.shape[1]} query heads are no multiple of {k.shape[1]} key heads")
+    if not 1 <= q.shape[2] <= 256:
+        raise ValueError(f"varlen_attention: heads must have 1 to 256 elements, got {q.shape[2]}")
+    if cu_seqlens.dtype != torch.int32 or cu_seqlens.ndim != 1 or cu_seqlens.shape[0] < 1:
+        raise ValueError("varlen_attention: cu_seqlens must be a 1-D int32 tensor with at least one entry, got "
+                         f"{cu_seqlens.dtype} {tuple(cu_seqlens.shape)}")
+    if scale is None:
+        scale = q.shape[2] ** -0.5
+    if not (math.isfinite(scale) and scale > 0):
+        raise ValueError(f"varlen_attention: the scale must be finite and positive, got {scale}")
+    return _O.varlen_attention_fwd(q, k, v, cu_seqlens, float(scale))[0]
 
 
 def _as_bool(m):
