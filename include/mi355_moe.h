@@ -795,17 +795,19 @@ int mi355_qk_norm_rotary_bwd(const void* dq_out, const void* dk_out, const void*
  * q (T, H, D), k and v (T, G, D) with the given strides in elements, a head's elements next to each other; out dense.
  * fp32 or bf16, 1 <= D <= 256, H a multiple of G, scale finite and positive, T < 2^30.  Scores, weights' statistics
  * and sums are fp32; with bf16 storage the weights are rounded to bf16 for the second product where matrix kernels serve the call.
+ * out_rest: optional, bf16 only, dense like out: what rounding took from it, rounded itself; with it the backward's out . dout is as good as
+ * out in fp32 (from the rounded out alone, the gradients of short rows come out twice as far from the formula).
  * lse: optional (H, T) fp32, log2 of each row's sum of exp(scale q.k), +inf for rows in no sequence; the backward reads it.
  */
 int mi355_varlen_attention_fwd(const void* q, int64_t q_token_stride, int64_t q_head_stride,
                                const void* k, int64_t k_token_stride, int64_t k_head_stride,
                                const void* v, int64_t v_token_stride, int64_t v_head_stride,
                                int dtype, const int32_t* cu_seqlens, int64_t sequences, float scale,
-                               void* out, float* lse, int64_t T, int64_t H, int64_t G, int64_t D,
-                               void* stream);
+                               void* out, void* out_rest, float* lse, int64_t T, int64_t H,
+                               int64_t G, int64_t D, void* stream);
 
 /*
- * Its backward; dout and out (the forward's) dense, so are dq, dk and dv.  Scores are formed again.  No atomics: dk and dv of a key
+ * Its backward; dout, out and out_rest (the forward's; out_rest may be NULL) dense, so are dq, dk and dv.  Scores are formed again.  No atomics: dk and dv of a key
  * head are sums over its query heads in a fixed order, by way of fp32 parts in the workspace where few key heads would
  * leave the card idle.  workspace: mi355_varlen_attention_bwd_workspace_bytes(T, H, G, D) bytes.
  */
@@ -813,8 +815,8 @@ int64_t mi355_varlen_attention_bwd_workspace_bytes(int64_t T, int64_t H, int64_t
 int mi355_varlen_attention_bwd(const void* dout, const void* q, int64_t q_token_stride,
                                int64_t q_head_stride, const void* k, int64_t k_token_stride,
                                int64_t k_head_stride, const void* v, int64_t v_token_stride,
-                               int64_t v_head_stride, const void* out, const float* lse, int dtype,
-                               const int32_t* cu_seqlens, int64_t sequences, float scale, void* dq,
+                               int64_t v_head_stride, const void* out, const void* out_rest,
+                               const float* lse, int dtype, const int32_t* cu_seqlens, int64_t sequences, float scale, void* dq,
                                void* dk, void* dv, void* workspace, int64_t T, int64_t H, int64_t G,
                                int64_t D, void* stream);
 

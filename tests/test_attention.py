@@ -8,7 +8,8 @@ keys, in natural units:
   largest of that over a row's keys.
 * a weight: exp of it, over a sum of n such: off by e = 2 E + (2 n + 32) u of the weight; from lse (backward) 4 u |lse| more.
 * a result: sum p |v| (e + h + n u).
-* dp off by D u sum |do v|; delta = do . o by sum |do| (h |o| + the result's bound) of the stored, rounded o, and D u sum |do o|.
+* dp off by D u sum |do v|; delta = do . o by sum |do| (r |o| + the result's bound), of o as stored: fp32, r = u; bf16 and
+  what its rounding took, in bf16 as well, r = h^2; and 2 D u sum |do o|.
 * a weight below 2^-126, the least normal number of fp32, may come out as zero: exp2 has no others.  TINY = 2^-126 of absolute error
   a weight, which a ds takes times |dp| + |delta|, and the products' results and the stored ones once more each.
 * ds = p (dp - delta): p ((|dp| + |delta|) (e + h + 4 u) + both errors), then sums of N terms add N u of their sizes.
@@ -61,8 +62,9 @@ def reference(q, k, v, dout, cu, scale, dtype):
             val[3][a:b, g] += p.T @ G
             off[3][a:b, g] += (p * (e + h + N * U) + TINY * seen).T @ G.abs()
             dp, delta = G @ V.T, (G * out).sum(1, keepdim=True)
-            e_delta = (G.abs() * (store * (out.abs() + dout_bound) + dout_bound)).sum(1, keepdim=True)
-            e_delta = e_delta + D * U * (G.abs() * out.abs()).sum(1, keepdim=True)
+            kept = store if dtype == F32 else store * store
+            e_delta = (G.abs() * (kept * (out.abs() + dout_bound) + dout_bound)).sum(1, keepdim=True)
+            e_delta = e_delta + 2 * D * U * (G.abs() * out.abs()).sum(1, keepdim=True)
             e_dp = D * U * (G.abs() @ V.abs().T)
             ds = p * (dp - delta)
             e_ds = TINY * seen * (1 + dp.abs() + delta.abs()) + p * ((dp.abs() + delta.abs() + e_dp + e_delta) * (e + h + 4 * U) + e_dp + e_delta) * (1 + h)
@@ -323,7 +325,7 @@ def test_no_tokens_and_only_some_gradients():
     # a gradient in another dtype, as autocast hands it on
     assert torch.equal(torch.ops.mi355_moe.varlen_attention_bwd(
         dout.float(), *(t.detach() for t in leaves), *torch.ops.mi355_moe.varlen_attention_fwd(
-            *(t.detach() for t in leaves), cu, 64**-0.5), cu, 64**-0.5)[0], want[1])
+            *(t.detach() for t in leaves), cu, 64**-0.5, True), cu, 64**-0.5)[0], want[1])
 
 
 @gpu
@@ -415,9 +417,10 @@ def test_operator_refuses_what_does_not_fit_and_propagates_shapes():
         q.requires_grad_()
         out = ops.varlen_attention(q, k, k, cu)
         assert out.shape == q.shape and out.dtype == BF and out.requires_grad
-        out, lse = torch.ops.mi355_moe.varlen_attention_fwd(q.detach(), k, k, cu, 0.1)
-        assert lse.shape == (8, 10) and lse.dtype == F32
-        assert [x.shape for x in torch.ops.mi355_moe.varlen_attention_bwd(out, q.detach(), k, k, out, lse, cu, 0.1)] == [
+        out, lse, rest = torch.ops.mi355_moe.varlen_attention_fwd(q.detach(), k, k, cu, 0.1, True)
+        assert lse.shape == (8, 10) and lse.dtype == F32 and rest.shape == q.shape
+        assert torch.ops.mi355_moe.varlen_attention_fwd(q.detach(), k, k, cu, 0.1, False)[2].shape == (0,)
+        assert [x.shape for x in torch.ops.mi355_moe.varlen_attention_bwd(out, q.detach(), k, k, out, lse, rest, cu, 0.1)] == [
             q.shape, k.shape, k.shape]
 
 
@@ -425,11 +428,11 @@ def test_c_entry_points_refuse_before_any_launch():
     lib, p = _lib.load(), 0x1000  # (never dereferenced)
 
     def forward(T=4, H=4, G=2, D=64, dtype=1, scale=0.1, cu=p, sequences=1):
-        return lib.mi355_varlen_attention_fwd(p, H * D, D, p, G * D, D, p, G * D, D, dtype, cu, sequences, scale, p, p, T, H, G, D, None)
+        return lib.mi355_varlen_attention_fwd(p, H * D, D, p, G * D, D, p, G * D, D, dtype, cu, sequences, scale, p, p, p, T, H, G, D, None)
 
     def backward(T=4, H=4, G=2, D=64, workspace=p):
-        return lib.mi355_varlen_attention_bwd(p, p, H * D, D, p, G * D, D, p, G * D, D, p, p, 1, p, 1, 0.1, p, p, p, workspace, T, H, G,
-                                              D, None)
+        return lib.mi355_varlen_attention_bwd(p, p, H * D, D, p, G * D, D, p, G * D, D, p, p, p, 1, p, 1, 0.1, p, p, p, workspace, T, H,
+                                              G, D, None)
 
     def text(rc, needle):
         assert rc == -1 and needle in lib.mi355_moe_last_error(), (rc, lib.mi355_moe_last_error())

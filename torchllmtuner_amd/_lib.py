@@ -49,11 +49,11 @@ SIGNATURES = {
         I,
         [P, P, P, L, L, P, L, L, P, P, I, P, I, P, L, F, I, F, P, P, P, P, P, L, L, L, L, P],
     ),
-    "mi355_varlen_attention_fwd": (I, [P, L, L, P, L, L, P, L, L, I, P, L, F, P, P, L, L, L, L, P]),
+    "mi355_varlen_attention_fwd": (I, [P, L, L, P, L, L, P, L, L, I, P, L, F, P, P, P, L, L, L, L, P]),
     "mi355_varlen_attention_bwd_workspace_bytes": (L, [L, L, L, L]),
     "mi355_varlen_attention_bwd": (
         I,
-        [P, P, L, L, P, L, L, P, L, L, P, P, I, P, L, F, P, P, P, P, L, L, L, L, P],
+        [P, P, L, L, P, L, L, P, L, L, P, P, P, I, P, L, F, P, P, P, P, L, L, L, L, P],
     ),
     "mi355_permute_plan_workspace_bytes": (L, [L, L, L]),
     "mi355_permute_plan": (I, [P, L, L, L, L, L, L, L, P, P, P, P, P, P, L, P, P, P, L, P, P]),

@@ -26,6 +26,7 @@ struct AttnArgs {
   int64_t q_token, q_head, k_token, k_head, v_token, v_head;  // strides, in elements
   void* out;              // (T, H, D) dense
   float* lse;             // (H, T), log2
+  void* rest;             // (T, H, D) dense, bf16 only: what rounding took from out (written forward, read backward); null: not kept
   // backward
   const void *o, *dout;   // (T, H, D) dense
   float* delta;           // (H, T)
@@ -62,6 +63,15 @@ __device__ __forceinline__ const T* row_at(const void* base, int64_t token, int6
   return static_cast<const T*>(base) + t * token + h * head;
 }
 
+// an element of the forward's result, and what its rounding took
+template <typename T>
+__device__ __forceinline__ void store_result(const AttnArgs& p, int64_t at, float v) {
+  T* out = static_cast<T*>(p.out) + at;
+  store_from_f32<T>(out, v);
+  if constexpr (sizeof(T) == 2)
+    if (p.rest) static_cast<uint16_t*>(p.rest)[at] = f32_to_bf16(v - round_bf16(v));
+}
+
 // ---- one row by one wave: lanes over keys (or queries) for the products, over the head's elements for the sums -------------------
 constexpr int kHeadMax = 256;          // elements of a head
 constexpr int kLaneCols = kHeadMax / 64;
@@ -96,10 +106,10 @@ __device__ __forceinline__ void careful_forward_row(const AttnArgs& p, int h, in
     }
     m = top;
   }
-  T* out = static_cast<T*>(p.out) + (static_cast<int64_t>(row) * p.H + h) * p.D;
+  const int64_t dense = (static_cast<int64_t>(row) * p.H + h) * p.D;
 #pragma unroll
   for (int i = 0; i < kLaneCols; ++i)
-    if (lane + 64 * i < p.D) store_from_f32<T>(out + lane + 64 * i, acc[i] / l);
+    if (lane + 64 * i < p.D) store_result<T>(p, dense + lane + 64 * i, acc[i] / l);
 }
 
 template <typename T>
@@ -177,5 +187,8 @@ __device__ __forceinline__ void careful_dkv_row(const AttnArgs& p, int g, int ke
 // ---- launches, by file --------------------------------------------------------------------------------
 void attention_any_forward(const AttnArgs& p, int dtype, hipStream_t s);
 void attention_any_backward(const AttnArgs& p, int dtype, hipStream_t s);
+bool attention_bf16_covers(const AttnArgs& p);
+void attention_bf16_forward(const AttnArgs& p, hipStream_t s);
+void attention_bf16_backward(const AttnArgs& p, hipStream_t s);
 
 }  // namespace mi355

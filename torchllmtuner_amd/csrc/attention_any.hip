@@ -219,14 +219,14 @@ __global__ __launch_bounds__(256) void any_forward_kernel(const AttnArgs p, int 
       if (t == kNegInf && lens[(qw * KW + part) * 16 + mine] != 0.0f) len = NAN;
     }
     bool spoilt = false;
-    T* out = static_cast<T*>(p.out) + (static_cast<int64_t>(r) * p.H + h) * p.D;
+    const int64_t dense = (static_cast<int64_t>(r) * p.H + h) * p.D;
     for (int d = lane; d < p.D; d += kWave) {
       float v = 0.0f;
 #pragma unroll
       for (int part = 0; part < KW; ++part) v += w[part] * sums[((qw * KW + part) * 16 + mine) * P + d];
       v /= len;
       spoilt |= v != v;
-      store_from_f32<T>(out + d, first < last ? v : 0.0f);
+      store_result<T>(p, dense + d, first < last ? v : 0.0f);
     }
     if (lane == 0 && p.lse) p.lse[static_cast<int64_t>(h) * p.T + r] = first < last ? ref + log2f(len) : INFINITY;
     if (first < last && __any(spoilt)) careful_forward_row<T>(p, h, r, first);
@@ -254,9 +254,13 @@ __global__ __launch_bounds__(256) void any_dq_kernel(const AttnArgs p, int tiles
   float delta = 0.0f;
   {
     float o[DP / 4];
-    own_rows<T, DP>(o, static_cast<const T*>(p.o) + h * p.D, dense, row, on, p.D, vec, lane);
+    auto dot = [&](const void* base) {
+      own_rows<T, DP>(o, static_cast<const T*>(base) + h * p.D, dense, row, on, p.D, vec, lane);
 #pragma unroll
-    for (int i = 0; i < DP / 4; ++i) delta = fmaf(o[i], dout[i], delta);
+      for (int i = 0; i < DP / 4; ++i) delta = fmaf(o[i], dout[i], delta);
+    };
+    dot(p.o);
+    if (p.rest) dot(p.rest);
   }
   delta = column_sum(delta);
   const float lse = on ? p.lse[static_cast<int64_t>(h) * p.T + row] : INFINITY;
@@ -425,7 +429,7 @@ void with_head(int D, Fn f) {
 
 bool in_fours(const AttnArgs& p, int item, bool backward) {
   uintptr_t bits = reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v);
-  if (backward) bits |= reinterpret_cast<uintptr_t>(p.o) | reinterpret_cast<uintptr_t>(p.dout);
+  if (backward) bits |= reinterpret_cast<uintptr_t>(p.o) | reinterpret_cast<uintptr_t>(p.rest) | reinterpret_cast<uintptr_t>(p.dout);
   return bits % (4 * item) == 0 && (p.q_token | p.q_head | p.k_token | p.k_head | p.v_token | p.v_head | p.D) % 4 == 0;
 }
 
@@ -464,11 +468,14 @@ void any_backward(const AttnArgs& p, int vec, hipStream_t s) {
   const int rows = 64 / KW, tiles = (p.T + rows - 1) / rows;
   hipLaunchKernelGGL((any_dq_kernel<T, DP, KW>), dim3(tiles, p.H), dim3(256), (kAnyLds<DP, KW>), s, p, tiles, vec);
   hipLaunchKernelGGL((any_dkv_kernel<T, DP, KW>), dim3(tiles, p.G * p.splits), dim3(256), (kAnyLds<DP, KW>), s, p, vec);
-  if (p.splits > 1) {
-    const int64_t n = static_cast<int64_t>(p.T) * p.G * p.D;
-    hipLaunchKernelGGL(join_parts_kernel<T>, dim3((unsigned)((n + 255) / 256), 2), dim3(256), 0, s, p.dk_part, p.dv_part,
-                       static_cast<T*>(p.dk), static_cast<T*>(p.dv), p.splits, n);
-  }
+}
+
+template <typename T>
+void join_parts(const AttnArgs& p, hipStream_t s) {
+  if (p.splits <= 1) return;
+  const int64_t n = static_cast<int64_t>(p.T) * p.G * p.D;
+  hipLaunchKernelGGL(join_parts_kernel<T>, dim3((unsigned)((n + 255) / 256), 2), dim3(256), 0, s, p.dk_part, p.dv_part,
+                     static_cast<T*>(p.dk), static_cast<T*>(p.dv), p.splits, n);
 }
 
 void attention_any_backward(const AttnArgs& p, int dtype, hipStream_t s) {
@@ -523,14 +530,16 @@ AttnArgs attention_args(const void* q, int64_t q_token, int64_t q_head, const vo
 extern "C" int mi355_varlen_attention_fwd(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
                                           int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
                                           int64_t v_head_stride, int dtype, const int32_t* cu_seqlens, int64_t sequences, float scale,
-                                          void* out, float* lse, int64_t T, int64_t H, int64_t G, int64_t D, void* stream) {
+                                          void* out, void* out_rest, float* lse, int64_t T, int64_t H, int64_t G, int64_t D,
+                                          void* stream) {
   if (int rc = check_attention("varlen_attention_fwd", dtype, sequences, T, H, G, D, scale)) return rc;
   if (T == 0) return MI355_OK;
   MI355_REQUIRE(q && k && v && cu_seqlens && out, "varlen_attention_fwd: null pointer");
   AttnArgs p = attention_args(q, q_token_stride, q_head_stride, k, k_token_stride, k_head_stride, v, v_token_stride, v_head_stride,
                               cu_seqlens, sequences, scale, T, H, G, D);
-  p.out = out, p.lse = lse;
-  attention_any_forward(p, dtype, as_stream(stream));
+  p.out = out, p.lse = lse, p.rest = dtype == MI355_BF16 ? out_rest : nullptr;
+  if (dtype == MI355_BF16 && attention_bf16_covers(p)) attention_bf16_forward(p, as_stream(stream));
+  else attention_any_forward(p, dtype, as_stream(stream));
   return check_launch("varlen_attention_fwd");
 }
 
@@ -542,8 +551,8 @@ extern "C" int64_t mi355_varlen_attention_bwd_workspace_bytes(int64_t T, int64_t
 
 extern "C" int mi355_varlen_attention_bwd(const void* dout, const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
                                           int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
-                                          int64_t v_head_stride, const void* out, const float* lse, int dtype,
-                                          const int32_t* cu_seqlens, int64_t sequences, float scale, void* dq, void* dk, void* dv,
+                                          int64_t v_head_stride, const void* out, const void* out_rest, const float* lse,
+                                          int dtype, const int32_t* cu_seqlens, int64_t sequences, float scale, void* dq, void* dk, void* dv,
                                           void* workspace, int64_t T, int64_t H, int64_t G, int64_t D, void* stream) {
   if (int rc = check_attention("varlen_attention_bwd", dtype, sequences, T, H, G, D, scale)) return rc;
   if (T == 0) return MI355_OK;
@@ -551,11 +560,15 @@ extern "C" int mi355_varlen_attention_bwd(const void* dout, const void* q, int64
   MI355_REQUIRE(aligned16(workspace), "varlen_attention_bwd: the workspace must start on a 16-byte boundary");
   AttnArgs p = attention_args(q, q_token_stride, q_head_stride, k, k_token_stride, k_head_stride, v, v_token_stride, v_head_stride,
                               cu_seqlens, sequences, scale, T, H, G, D);
-  p.o = out, p.dout = dout, p.lse = const_cast<float*>(lse), p.dq = dq, p.dk = dk, p.dv = dv;
+  p.o = out, p.rest = dtype == MI355_BF16 ? const_cast<void*>(out_rest) : nullptr;
+  p.dout = dout, p.lse = const_cast<float*>(lse), p.dq = dq, p.dk = dk, p.dv = dv;
   p.splits = head_parts(T, H, G);
   p.delta = static_cast<float*>(workspace);
   p.dk_part = p.delta + (H * T + 3) / 4 * 4;
   p.dv_part = p.dk_part + static_cast<int64_t>(p.splits) * T * G * D;
-  attention_any_backward(p, dtype, as_stream(stream));
+  if (dtype == MI355_BF16 && attention_bf16_covers(p)) attention_bf16_backward(p, as_stream(stream));
+  else attention_any_backward(p, dtype, as_stream(stream));
+  if (dtype == MI355_F32) join_parts<float>(p, as_stream(stream));
+  else join_parts<uint16_t>(p, as_stream(stream));
   return check_launch("varlen_attention_bwd");
 }

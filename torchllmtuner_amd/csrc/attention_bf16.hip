@@ -1,0 +1,612 @@
+// Causal attention over packed sequences (attention.h has the formulas) on v_mfma_f32_32x32x16_bf16: bf16 storage, head sizes in whole
+// 16-byte pieces up to 128, fp32 sums and statistics.
+//
+// The matrix instruction takes per lane 8 elements of a row (column) lane % 32 at k = 8 (lane / 32) .. + 7 and yields 16 fp32 of column
+// lane % 32, rows 8 (i / 4) + 4 (lane / 32) + i % 4.  Products are formed turned so that a result is the next product's right operand where
+// it lies, without a trip through LDS: the forward and dq form s^T = K Q^T, a column a query, so a query's weights lie in its two
+// lanes (lane and lane + 32), its maximum and sum are in-lane reductions and one exchange, and o^T += V^T p^T takes
+// the weights as they are, rounded to bf16; dk and dv form s = Q K^T, a column a key, for dv^T += dO^T p and dk^T += Q^T ds.
+// The keys of 16 then meet in the order in which the result holds them, 4 h + {0..3} and 8 + 4 h + {0..3} for lane half h, which
+// only says which rows the left operand's transposing LDS reads fetch.
+//
+// A wave holds 32 rows (queries, or keys), a workgroup four waves.  The other axis passes through LDS in tiles of 64 rows, requested
+// straight into LDS a tile ahead, two buffers, one barrier a tile.  A row's 16-byte pieces are swizzled by a key of its
+// number that spreads both the row reads (16 rows, one piece) and the transposing reads (4 rows, 64 bytes) over all banks.
+#include <algorithm>
+
+#include "attention.h"
+
+namespace mi355 {
+namespace {
+
+constexpr int kTile = 64;     // rows of the other axis a tile
+constexpr int kRows = 32;     // rows a wave
+constexpr uint32_t kFarOff = 1u << 30;  // an offset past every buffer: reads zeros
+
+template <int DP>
+__device__ __forceinline__ int swizzle(int r) {  // (of the low four bits of r)
+  return DP == 64 ? (((r >> 1) & 1) << 2) | ((r >> 2) & 3) : ((r & 3) << 2) | ((r >> 2) & 3);
+}
+
+// LDS byte offsets of a lane's reads of a tile
+template <int DP>
+struct Reads {
+  uint32_t row[DP / 16];        // 8 elements of row lane % 32 (+ 32 b), step kk
+  uint32_t turned[DP / 32][2];  // elements 32 n + lane % 32 of rows 4 h + {0..3} and 8 + 4 h + {0..3} (+ 16 kk)
+  __device__ __forceinline__ void find(int lane) {
+    const int h = lane >> 5, r = lane & 31;
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk) row[kk] = r * DP * 2 + (((2 * kk + h) ^ swizzle<DP>(r)) << 4);
+    const int i = lane & 15, side = (lane >> 4) & 1;
+#pragma unroll
+    for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int t = 8 * half + 4 * h + (i >> 2), c = 4 * n + 2 * side + ((i & 3) >> 1);
+        turned[n][half] = t * DP * 2 + ((c ^ swizzle<DP>(t)) << 4) + 8 * (i & 1);
+      }
+  }
+};
+
+__device__ __forceinline__ bf16x8 read_row(uint32_t at) { return lds_read16(at); }
+__device__ __forceinline__ bf16x8 read_turned(uint32_t at_lo, uint32_t at_hi) {
+  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<s16x4>(at_lo));
+  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<s16x4>(at_hi));
+  const s16x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  return __builtin_bit_cast(bf16x8, v);
+}
+
+// Requests of a workgroup's four waves for a tile of a head's rows, 1 KiB each: a wave's j-th brings rows of its own
+template <int DP>
+struct Requests {
+  static constexpr int EACH = kTile * DP * 2 / 4096;  // a wave's requests a tile
+  static constexpr int ROWS = 1024 / (DP * 2);        // rows a request
+  uint64_t base;
+  int64_t row_bytes;
+  uint32_t voff[EACH];
+  int T, D;
+  __device__ __forceinline__ void find(const void* p, int64_t token, int T_, int D_, int lane, int wave) {
+    base = reinterpret_cast<uint64_t>(p);
+    row_bytes = token * 2;
+    T = T_, D = D_;
+    constexpr int CPR = DP / 8;
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+      const int r = ROWS * (4 * j + wave) + lane / CPR, c = (lane % CPR) ^ swizzle<DP>(r);
+      voff[j] = c * 8 < D_ ? static_cast<uint32_t>(r * row_bytes) + c * 16 : kFarOff;
+    }
+  }
+  // rows [row0, row0 + 64) to LDS at `lds`; zeros for rows from T on
+  __device__ __forceinline__ void request(int row0, uint32_t lds, int wave) const {
+    const int64_t left = static_cast<int64_t>(T - 1 - row0) * row_bytes + D * 2;
+    const uint32_t bytes = left < 0 ? 0 : left < kFarOff ? static_cast<uint32_t>(left) : kFarOff;
+    const uint64_t at = base + static_cast<int64_t>(row0) * row_bytes;
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) lds_load16_within(at, bytes, voff[j], lds + (4 * j + wave) * 1024);
+  }
+};
+
+// a wave's own 32 rows as right operand: 8 elements of row lane % 32 a step, zeros where `on` is not set
+template <int DP>
+__device__ __forceinline__ void own_rows(bf16x8 (&x)[DP / 16], const uint16_t* row, bool on, int D, int lane) {
+#pragma unroll
+  for (int kk = 0; kk < DP / 16; ++kk) {
+    const int d = 16 * kk + 8 * (lane >> 5);
+    u32x4 v = {0, 0, 0, 0};
+    if (on && d < D) v = *reinterpret_cast<const u32x4*>(row + d);
+    x[kk] = __builtin_bit_cast(bf16x8, v);
+  }
+}
+
+__device__ __forceinline__ f32x16 mfma(const bf16x8& a, const bf16x8& b, const f32x16& c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 zeros() {
+  f32x16 z;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) z[i] = 0.0f;
+  return z;
+}
+
+// the value of the other lane half, both in one
+__device__ __forceinline__ float halves_max(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float halves_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ int least(int v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, kWave));
+  return __builtin_amdgcn_readfirstlane(v);
+}
+__device__ __forceinline__ int most(int v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o, kWave));
+  return __builtin_amdgcn_readfirstlane(v);
+}
+
+// rows 16 kk + ... of a 32 x 32 result as the right operand of the next product
+__device__ __forceinline__ bf16x8 operand_of(const f32x16& s, int kk) {
+  u32x4 v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = pack_bf16x2(s[8 * kk + 2 * i], s[8 * kk + 2 * i + 1]);
+  return __builtin_bit_cast(bf16x8, v);
+}
+
+// elements 32 n + 8 (2 a + h) .. + 7 of the lane's row from a turned result's block: lane half h's pieces of 4 exchanged for whole ones of 8
+__device__ __forceinline__ void eight_of(const f32x16& o, int a, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(o[8 * a + i]), __float_as_uint(o[8 * a + 4 + i]), false, false);
+    v[i] = __uint_as_float(r[0]);
+    v[4 + i] = __uint_as_float(r[1]);
+  }
+}
+__device__ __forceinline__ u32x4 pack8(const float (&v)[8]) {
+  return u32x4{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
+}
+
+struct Place {
+  int head, tile;
+};
+// Workgroup b runs on XCD b % 8.  Heads that share keys go to one XCD, whose L2 then holds them once; the last tiles, which see the most
+// keys, start first, so that what starts last is short.
+__device__ __forceinline__ Place place_of(int block, int heads, int tiles) {
+  Place w;
+  if (heads % 8 == 0) {
+    const int each = heads / 8, j = block >> 3;
+    w.head = (block & 7) * each + j % each;
+    w.tile = tiles - 1 - j / each;
+  } else {
+    w.head = block % heads;
+    w.tile = tiles - 1 - block / heads;
+  }
+  return w;
+}
+
+// the workgroup's range over the other axis and the wave's, from every lane's row's
+struct Ranges {
+  int lo, hi, first, last;  // workgroup: [lo, hi), wave: [first, last)
+  __device__ __forceinline__ void find(int lane_lo, int lane_hi, int* red, int wave) {
+    first = least(lane_lo);
+    last = most(lane_hi);
+    if ((threadIdx.x & 63) == 0) red[2 * wave] = first, red[2 * wave + 1] = last;
+    __syncthreads();
+    lo = __builtin_amdgcn_readfirstlane(min(min(red[0], red[2]), min(red[4], red[6])));
+    hi = __builtin_amdgcn_readfirstlane(max(max(red[1], red[3]), max(red[5], red[7])));
+    __syncthreads();
+  }
+};
+
+constexpr float kGrowth = 8.0f;  // a row's weights stay below 2^8 of its reference: the reference follows its maximum in such steps
+
+template <int DP>
+__global__ __launch_bounds__(256, 2) void bf16_forward_kernel(const AttnArgs p, int tiles) {
+  constexpr int KK = DP / 16, NB = DP / 32;
+  constexpr uint32_t TILE_BYTES = kTile * DP * 2;
+  extern __shared__ __attribute__((aligned(16))) uint16_t smem[];
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_cptr)smem));
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+  const Place at = place_of(blockIdx.x, p.H, tiles);
+  const int h = at.head, g = h / p.group;
+  const int row0 = at.tile * 4 * kRows + wave * kRows, row = row0 + (lane & 31);
+  int start, end;
+  sequence_of(p.cu, p.sequences, p.T, row, start, end);
+  const bool on = start < end;
+  Ranges range;
+  range.find(on ? start : p.T, on ? row + 1 : 0, reinterpret_cast<int*>(smem), wave);
+  const int latest = most(on ? start : p.T);  // keys from here to the wave's first row are seen by all its rows
+  Reads<DP> reads;
+  reads.find(lane);
+  Requests<DP> keys, values;
+  keys.find(static_cast<const uint16_t*>(p.k) + g * p.k_head, p.k_token, p.T, p.D, lane, wave);
+  values.find(static_cast<const uint16_t*>(p.v) + g * p.v_head, p.v_token, p.T, p.D, lane, wave);
+  auto request = [&](int k0, uint32_t buffer) {
+    keys.request(k0, lds0 + buffer * 2 * TILE_BYTES, wave);
+    values.request(k0, lds0 + buffer * 2 * TILE_BYTES + TILE_BYTES, wave);
+  };
+  if (range.lo < range.hi) request(range.lo, 0);
+  bf16x8 q[KK];
+  own_rows<DP>(q, row_at<uint16_t>(p.q, p.q_token, p.q_head, min(row, p.T - 1), h), on, p.D, lane);
+  f32x16 o[NB];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) o[n] = zeros();
+  float m = kNegInf, ref = 0.0f, l = 0.0f;
+  const float c = p.c, growth = kGrowth / p.c;
+  uint32_t buffer = 0;
+  for (int k0 = range.lo; k0 < range.hi; k0 += kTile, buffer ^= 1) {
+    lds_wait<0>();
+    lds_sync<63>();  // everyone's requests of this tile have landed, and everyone has read the other buffer
+    if (k0 + kTile < range.hi) request(k0 + kTile, buffer ^ 1);
+    if (k0 >= range.last || k0 + kTile <= range.first) continue;
+    const uint32_t kt = lds0 + buffer * 2 * TILE_BYTES, vt = kt + TILE_BYTES;
+    f32x16 s[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      s[b] = zeros();
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) s[b] = mfma(read_row(kt + reads.row[kk] + b * 32 * DP * 2), q[kk], s[b]);
+    }
+    if (k0 + kTile - 1 > row0 || k0 < latest) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int key = k0 + 32 * b + 8 * (i >> 2) + 4 * half + (i & 3);
+          s[b][i] = on && key >= start && key <= row ? s[b][i] : kNegInf;
+        }
+    }
+    float top = kNegInf;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
+    top = halves_max(top);
+    if (__any(top > m + growth)) {
+      const float next = fmaxf(m, top), next_ref = next == kNegInf ? 0.0f : next * c;  // (nothing seen yet: weights of 0, not NaN)
+      const float keep = m == kNegInf ? 0.0f : exp2_f32(ref - next_ref);
+      l *= keep;
+#pragma unroll
+      for (int n = 0; n < NB; ++n) o[n] *= keep;
+      m = next;
+      ref = next_ref;
+    }
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[b][i] = exp2_f32(fmaf(s[b][i], c, -ref));
+        l += s[b][i];
+      }
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) {
+        const bf16x8 w = operand_of(s[b], kk);
+        const uint32_t rows = vt + (2 * b + kk) * 16 * DP * 2;
+#pragma unroll
+        for (int n = 0; n < NB; ++n) o[n] = mfma(read_turned(rows + reads.turned[n][0], rows + reads.turned[n][1]), w, o[n]);
+      }
+    }
+  }
+  l = halves_sum(l);
+  const float inverse = 1.0f / l;
+  bool spoilt = false;
+#pragma unroll
+  for (int n = 0; n < NB; ++n)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      o[n][i] = on ? o[n][i] * inverse : 0.0f;
+      spoilt |= o[n][i] != o[n][i];
+    }
+  if (row < p.T) {
+    const int64_t dense = (static_cast<int64_t>(row) * p.H + h) * p.D;
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
+        float v[8];
+        eight_of(o[n], a, v);
+        const int d = 32 * n + 16 * a + 8 * half;
+        if (d >= p.D) continue;
+        const u32x4 packed = pack8(v);
+        *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p.out) + dense + d) = packed;
+        if (p.rest) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] -= __uint_as_float(i & 1 ? packed[i / 2] & 0xffff0000u : packed[i / 2] << 16);
+          *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p.rest) + dense + d) = pack8(v);
+        }
+      }
+    if (half == 0 && p.lse) p.lse[static_cast<int64_t>(h) * p.T + row] = on ? ref + log2f(l) : INFINITY;
+  }
+  uint64_t again = __ballot(spoilt && row < p.T);
+  again = (again | again >> 32) & 0xffffffffu;
+  if (again) lds_wait<0>();
+  for (; again; again &= again - 1) {
+    const int i = __builtin_ctzll(again);
+    careful_forward_row<uint16_t>(p, h, row0 + i, __builtin_amdgcn_readlane(start, i));
+  }
+}
+
+// dq, and delta for the kernel behind this one
+template <int DP>
+__global__ __launch_bounds__(256, 2) void bf16_dq_kernel(const AttnArgs p, int tiles) {
+  constexpr int KK = DP / 16, NB = DP / 32;
+  constexpr uint32_t TILE_BYTES = kTile * DP * 2;
+  extern __shared__ __attribute__((aligned(16))) uint16_t smem[];
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_cptr)smem));
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+  const Place at = place_of(blockIdx.x, p.H, tiles);
+  const int h = at.head, g = h / p.group;
+  const int row0 = at.tile * 4 * kRows + wave * kRows, row = row0 + (lane & 31);
+  int start, end;
+  sequence_of(p.cu, p.sequences, p.T, row, start, end);
+  const bool on = start < end;
+  Ranges range;
+  range.find(on ? start : p.T, on ? row + 1 : 0, reinterpret_cast<int*>(smem), wave);
+  const int latest = most(on ? start : p.T);
+  Reads<DP> reads;
+  reads.find(lane);
+  Requests<DP> keys, values;
+  keys.find(static_cast<const uint16_t*>(p.k) + g * p.k_head, p.k_token, p.T, p.D, lane, wave);
+  values.find(static_cast<const uint16_t*>(p.v) + g * p.v_head, p.v_token, p.T, p.D, lane, wave);
+  auto request = [&](int k0, uint32_t buffer) {
+    keys.request(k0, lds0 + buffer * 2 * TILE_BYTES, wave);
+    values.request(k0, lds0 + buffer * 2 * TILE_BYTES + TILE_BYTES, wave);
+  };
+  if (range.lo < range.hi) request(range.lo, 0);
+  const int here = min(row, p.T - 1);
+  const int64_t dense = (static_cast<int64_t>(here) * p.H + h) * p.D;
+  bf16x8 q[KK], dout[KK];
+  own_rows<DP>(q, row_at<uint16_t>(p.q, p.q_token, p.q_head, here, h), on, p.D, lane);
+  own_rows<DP>(dout, static_cast<const uint16_t*>(p.dout) + dense, on, p.D, lane);
+  float delta = 0.0f;
+  {
+    auto dot = [&](const void* base) {
+      bf16x8 x[KK];
+      own_rows<DP>(x, static_cast<const uint16_t*>(base) + dense, on, p.D, lane);
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) delta = fmaf(static_cast<float>(x[kk][i]), static_cast<float>(dout[kk][i]), delta);
+    };
+    dot(p.o);
+    if (p.rest) dot(p.rest);
+  }
+  delta = halves_sum(delta);
+  const float lse = on ? p.lse[static_cast<int64_t>(h) * p.T + row] : INFINITY;
+  if (half == 0 && row < p.T) p.delta[static_cast<int64_t>(h) * p.T + row] = on ? delta : 0.0f;
+  f32x16 dq[NB];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) dq[n] = zeros();
+  const float c = p.c;
+  uint32_t buffer = 0;
+  for (int k0 = range.lo; k0 < range.hi; k0 += kTile, buffer ^= 1) {
+    lds_wait<0>();
+    lds_sync<63>();
+    if (k0 + kTile < range.hi) request(k0 + kTile, buffer ^ 1);
+    if (k0 >= range.last || k0 + kTile <= range.first) continue;
+    const uint32_t kt = lds0 + buffer * 2 * TILE_BYTES, vt = kt + TILE_BYTES;
+    const bool masked = k0 + kTile - 1 > row0 || k0 < latest;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      f32x16 s = zeros(), ds = zeros();
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) s = mfma(read_row(kt + reads.row[kk] + b * 32 * DP * 2), q[kk], s);
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) ds = mfma(read_row(vt + reads.row[kk] + b * 32 * DP * 2), dout[kk], ds);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) ds[i] = exp2_f32(fmaf(s[i], c, -lse)) * (ds[i] - delta);
+      if (masked) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int key = k0 + 32 * b + 8 * (i >> 2) + 4 * half + (i & 3);
+          ds[i] = on && key >= start && key <= row ? ds[i] : 0.0f;
+        }
+      }
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) {
+        const bf16x8 w = operand_of(ds, kk);
+        const uint32_t rows = kt + (2 * b + kk) * 16 * DP * 2;
+#pragma unroll
+        for (int n = 0; n < NB; ++n) dq[n] = mfma(read_turned(rows + reads.turned[n][0], rows + reads.turned[n][1]), w, dq[n]);
+      }
+    }
+  }
+  bool spoilt = false;
+#pragma unroll
+  for (int n = 0; n < NB; ++n)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      dq[n][i] = on ? dq[n][i] * p.scale : 0.0f;
+      spoilt |= dq[n][i] != dq[n][i];
+    }
+  if (row < p.T) {
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
+        float v[8];
+        eight_of(dq[n], a, v);
+        const int d = 32 * n + 16 * a + 8 * half;
+        if (d < p.D) *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p.dq) + dense + d) = pack8(v);
+      }
+  }
+  uint64_t again = __ballot(spoilt && row < p.T);
+  again = (again | again >> 32) & 0xffffffffu;
+  if (again) lds_wait<0>();
+  for (; again; again &= again - 1) {
+    const int i = __builtin_ctzll(again);
+    careful_dq_row<uint16_t>(p, h, row0 + i, __builtin_amdgcn_readlane(start, i),
+                             __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lse), i)),
+                             __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(delta), i)));
+  }
+}
+
+// dk and dv: a wave's 32 keys against the query heads of their group, or a part of them
+template <int DP>
+__global__ __launch_bounds__(256, 1) void bf16_dkv_kernel(const AttnArgs p, int tiles) {
+  constexpr int KK = DP / 16, NB = DP / 32;
+  constexpr uint32_t TILE_BYTES = kTile * DP * 2, STAGE = 2 * TILE_BYTES + 512;  // queries, gradients, lse, delta
+  extern __shared__ __attribute__((aligned(16))) uint16_t smem[];
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_cptr)smem));
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+  const Place at = place_of(blockIdx.x, p.G * p.splits, tiles);
+  const int g = at.head / p.splits, split = at.head % p.splits;
+  const int heads = (p.group + p.splits - 1) / p.splits, h0 = g * p.group + split * heads, h1 = min(h0 + heads, (g + 1) * p.group);
+  const int key0 = (tiles - 1 - at.tile) * 4 * kRows + wave * kRows, key = key0 + (lane & 31);  // the first keys are seen by the most rows
+  int start, end;
+  sequence_of(p.cu, p.sequences, p.T, key, start, end);
+  const bool on = start < end;
+  Ranges range;
+  range.find(on ? key : p.T, on ? end : 0, reinterpret_cast<int*>(smem), wave);
+  const int earliest = least(on ? end : 0);  // rows from the wave's last key to here see all its keys
+  Reads<DP> reads;
+  reads.find(lane);
+  const int here = min(key, p.T - 1);
+  bf16x8 k[KK], v[KK];
+  own_rows<DP>(k, row_at<uint16_t>(p.k, p.k_token, p.k_head, here, g), on, p.D, lane);
+  own_rows<DP>(v, row_at<uint16_t>(p.v, p.v_token, p.v_head, here, g), on, p.D, lane);
+  f32x16 dk[NB], dv[NB];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) dk[n] = zeros(), dv[n] = zeros();
+  const float c = p.c;
+  Requests<DP> queries, grads;
+  queries.find(p.q, p.q_token, p.T, p.D, lane, wave);
+  grads.find(p.dout, static_cast<int64_t>(p.H) * p.D, p.T, p.D, lane, wave);
+  const int steps = range.lo < range.hi ? (range.hi - range.lo + kTile - 1) / kTile : 0;
+  auto request = [&](int h, int r0, uint32_t buffer) {
+    const uint32_t to = lds0 + buffer * STAGE;
+    queries.base = reinterpret_cast<uint64_t>(static_cast<const uint16_t*>(p.q) + h * p.q_head);
+    grads.base = reinterpret_cast<uint64_t>(static_cast<const uint16_t*>(p.dout) + h * p.D);
+    queries.request(r0, to, wave);
+    grads.request(r0, to + TILE_BYTES, wave);
+    if (wave < 2) {  // lse and delta of the tile's 64 rows, one wave each
+      const float* from = (wave ? p.delta : p.lse) + static_cast<int64_t>(h) * p.T;
+      lds_load4_within(reinterpret_cast<uint64_t>(from + r0), static_cast<uint32_t>(min(p.T - r0, kTile)) * 4, lane * 4,
+                       to + 2 * TILE_BYTES + wave * 256);
+    }
+  };
+  uint32_t buffer = 0;
+  if (steps) request(h0, range.lo, 0);
+  for (int h = h0; h < h1 && steps; ++h)
+    for (int t = 0; t < steps; ++t, buffer ^= 1) {
+      const int r0 = range.lo + t * kTile;
+      lds_wait<0>();
+      lds_sync<63>();
+      if (t + 1 < steps) request(h, r0 + kTile, buffer ^ 1);
+      else if (h + 1 < h1) request(h + 1, range.lo, buffer ^ 1);
+      if (r0 >= range.last || r0 + kTile <= range.first) continue;
+      const uint32_t qt = lds0 + buffer * STAGE, dt = qt + TILE_BYTES, stats = dt + TILE_BYTES;
+      const bool masked = r0 < key0 + kRows - 1 || r0 + kTile > earliest;
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        f32x16 s = zeros(), ds = zeros();
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) s = mfma(read_row(qt + reads.row[kk] + b * 32 * DP * 2), k[kk], s);
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) ds = mfma(read_row(dt + reads.row[kk] + b * 32 * DP * 2), v[kk], ds);
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+          const f32x4 lse = *lds_at<const f32x4>(stats + (32 * b + 8 * a + 4 * half) * 4);
+          const f32x4 delta = *lds_at<const f32x4>(stats + 256 + (32 * b + 8 * a + 4 * half) * 4);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            s[4 * a + i] = exp2_f32(fmaf(s[4 * a + i], c, -lse[i]));
+            ds[4 * a + i] = s[4 * a + i] * (ds[4 * a + i] - delta[i]);
+          }
+        }
+        if (masked) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int r = r0 + 32 * b + 8 * (i >> 2) + 4 * half + (i & 3);
+            const bool seen = on && r >= key && r < end;
+            s[i] = seen ? s[i] : 0.0f;
+            ds[i] = seen ? ds[i] : 0.0f;
+          }
+        }
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+          const bf16x8 w = operand_of(s, kk), dw = operand_of(ds, kk);
+          const uint32_t rows = (2 * b + kk) * 16 * DP * 2;
+#pragma unroll
+          for (int n = 0; n < NB; ++n)
+            dv[n] = mfma(read_turned(dt + rows + reads.turned[n][0], dt + rows + reads.turned[n][1]), w, dv[n]);
+#pragma unroll
+          for (int n = 0; n < NB; ++n)
+            dk[n] = mfma(read_turned(qt + rows + reads.turned[n][0], qt + rows + reads.turned[n][1]), dw, dk[n]);
+        }
+      }
+    }
+  bool spoilt = false;
+#pragma unroll
+  for (int n = 0; n < NB; ++n)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      dk[n][i] = on ? dk[n][i] * p.scale : 0.0f;
+      dv[n][i] = on ? dv[n][i] : 0.0f;
+      spoilt |= dk[n][i] != dk[n][i] || dv[n][i] != dv[n][i];
+    }
+  if (key < p.T) {
+    const int64_t dense = (static_cast<int64_t>(key) * p.G + g) * p.D, part = static_cast<int64_t>(split) * p.T * p.G * p.D + dense;
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+          float x[8];
+          eight_of(which ? dk[n] : dv[n], a, x);
+          const int d = 32 * n + 16 * a + 8 * half;
+          if (d >= p.D) continue;
+          if (p.splits > 1) {
+            f32x4* to = reinterpret_cast<f32x4*>((which ? p.dk_part : p.dv_part) + part + d);
+            to[0] = f32x4{x[0], x[1], x[2], x[3]};
+            to[1] = f32x4{x[4], x[5], x[6], x[7]};
+          } else {
+            *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(which ? p.dk : p.dv) + dense + d) = pack8(x);
+          }
+        }
+  }
+  uint64_t again = __ballot(spoilt && key < p.T);
+  again = (again | again >> 32) & 0xffffffffu;
+  if (again) lds_wait<0>();
+  for (; again; again &= again - 1) {
+    const int i = __builtin_ctzll(again);
+    careful_dkv_row<uint16_t>(p, g, key0 + i, __builtin_amdgcn_readlane(end, i), h0, h1, split);
+  }
+}
+
+template <int DP>
+constexpr uint32_t kForwardLds = 4 * kTile * DP * 2;
+template <int DP>
+constexpr uint32_t kDkvLds = 4 * kTile * DP * 2 + 1024;
+
+template <typename K>
+void allow(K kernel, size_t bytes, PerDeviceOnce& once) {
+  if (bytes <= 65536 || !once.needed()) return;
+  (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  once.done();
+}
+
+template <int DP>
+void forward(const AttnArgs& p, hipStream_t s) {
+  const int tiles = (p.T + 4 * kRows - 1) / (4 * kRows);
+  hipLaunchKernelGGL(bf16_forward_kernel<DP>, dim3(tiles * p.H), dim3(256), kForwardLds<DP>, s, p, tiles);
+}
+
+template <int DP>
+void backward(const AttnArgs& p, hipStream_t s) {
+  static PerDeviceOnce once;
+  allow(bf16_dkv_kernel<DP>, kDkvLds<DP>, once);
+  const int tiles = (p.T + 4 * kRows - 1) / (4 * kRows);
+  hipLaunchKernelGGL(bf16_dq_kernel<DP>, dim3(tiles * p.H), dim3(256), kForwardLds<DP>, s, p, tiles);
+  hipLaunchKernelGGL(bf16_dkv_kernel<DP>, dim3(tiles * p.G * p.splits), dim3(256), kDkvLds<DP>, s, p, tiles);
+}
+
+}  // namespace
+
+bool attention_bf16_covers(const AttnArgs& p) {
+  uintptr_t bits = reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v) |
+                   reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.o) | reinterpret_cast<uintptr_t>(p.rest) |
+                   reinterpret_cast<uintptr_t>(p.dout) | reinterpret_cast<uintptr_t>(p.dq) | reinterpret_cast<uintptr_t>(p.dk) |
+                   reinterpret_cast<uintptr_t>(p.dv);
+  const int64_t sizes = p.D | p.q_token | p.q_head | p.k_token | p.k_head | p.v_token | p.v_head;
+  // a tile's rows lie within 32-bit offsets of its first one
+  const int64_t reach = std::max(std::max(p.q_token, p.k_token), std::max<int64_t>(p.v_token, static_cast<int64_t>(p.H) * p.D));
+  return p.D <= 128 && bits % 16 == 0 && sizes % 8 == 0 && reach < (1 << 22) &&
+         static_cast<int64_t>((p.T + 127) / 128) * p.H < (1ll << 31);
+}
+
+void attention_bf16_forward(const AttnArgs& p, hipStream_t s) {
+  if (p.D <= 64) forward<64>(p, s);
+  else forward<128>(p, s);
+}
+
+void attention_bf16_backward(const AttnArgs& p, hipStream_t s) {
+  if (p.D <= 64) backward<64>(p, s);
+  else backward<128>(p, s);
+}
+
+}  // namespace mi355

@@ -469,20 +469,20 @@ std::tuple<Tensor, Tensor> qk_norm_rotary_autograd(const Tensor& q, const Tensor
 }
 
 // ---- causal attention over packed sequences: the row statistics carry no gradient -----------------------
-using AttentionFwdSig = std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const Tensor&, double);
+using AttentionFwdSig = std::tuple<Tensor, Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const Tensor&, double, bool);
 using AttentionBwdSig = std::tuple<Tensor, Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
-                                                           const Tensor&, const Tensor&, double);
+                                                           const Tensor&, const Tensor&, const Tensor&, double);
 
 struct VarlenAttention : public torch::autograd::Function<VarlenAttention> {
   static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu, double scale) {
     at::AutoDispatchBelowADInplaceOrView below;
     static auto op = typed_op<AttentionFwdSig>("mi355_moe::varlen_attention_fwd");
-    auto r = op.call(q, k, v, cu, scale);
-    ctx->save_for_backward({q, k, v, std::get<0>(r), std::get<1>(r), cu});
+    auto r = op.call(q, k, v, cu, scale, true);
+    ctx->save_for_backward({q, k, v, std::get<0>(r), std::get<1>(r), std::get<2>(r), cu});
     ctx->saved_data["scale"] = scale;
-    ctx->mark_non_differentiable({std::get<1>(r)});
+    ctx->mark_non_differentiable({std::get<1>(r), std::get<2>(r)});
     ctx->set_materialize_grads(false);
-    return {std::get<0>(r), std::get<1>(r)};
+    return {std::get<0>(r), std::get<1>(r), std::get<2>(r)};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     variable_list out(5);
@@ -490,7 +490,7 @@ struct VarlenAttention : public torch::autograd::Function<VarlenAttention> {
     if (!grads[0].defined() || !(n0 || n1 || n2)) return out;
     const auto s = ctx->get_saved_variables();
     static auto op = typed_op<AttentionBwdSig>("mi355_moe::varlen_attention_bwd");
-    auto r = op.call(grads[0], s[0], s[1], s[2], s[3], s[4], s[5], ctx->saved_data["scale"].toDouble());
+    auto r = op.call(grads[0], s[0], s[1], s[2], s[3], s[4], s[5], s[6], ctx->saved_data["scale"].toDouble());
     out[0] = keep(std::get<0>(r), n0);
     out[1] = keep(std::get<1>(r), n1);
     out[2] = keep(std::get<2>(r), n2);
@@ -498,14 +498,15 @@ struct VarlenAttention : public torch::autograd::Function<VarlenAttention> {
   }
 };
 
-std::tuple<Tensor, Tensor> varlen_attention_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu, double scale) {
+std::tuple<Tensor, Tensor, Tensor> varlen_attention_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu,
+                                                             double scale, bool for_backward) {
   if (!torch::autograd::compute_requires_grad(q, k, v)) {
     at::AutoDispatchBelowADInplaceOrView below;
     static auto op = typed_op<AttentionFwdSig>("mi355_moe::varlen_attention_fwd");
-    return op.call(q, k, v, cu, scale);
+    return op.call(q, k, v, cu, scale, for_backward);
   }
   auto r = VarlenAttention::apply(q, k, v, cu, scale);
-  return {r[0], r[1]};
+  return {r[0], r[1], r[2]};
 }
 
 // ---- load-balance loss: out = (loss, f_E...); the gradient flows into the scores -------------------

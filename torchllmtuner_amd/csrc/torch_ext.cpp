@@ -300,32 +300,36 @@ void check_attention(const Heads& q, const Heads& k, const Heads& v, const Tenso
                     "queries, keys, values and cu_seqlens must share a device");
 }
 
-std::tuple<Tensor, Tensor> varlen_attention_fwd(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& cu_, double scale) {
+std::tuple<Tensor, Tensor, Tensor> varlen_attention_fwd(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& cu_,
+                                                        double scale, bool for_backward) {
   Launch L(q_);
   const Heads q(q_), k(k_), v(v_);
   check_attention(q, k, v, cu_);
   const Tensor cu = cu_.contiguous();
   Tensor out = at::empty(q_.sizes(), q_.options()), lse = at::empty({q.heads, q.tokens}, q_.options().dtype(at::kFloat));
+  Tensor rest = for_backward && q_.scalar_type() == at::kBFloat16 ? at::empty_like(out) : none_like(out);
   check(mi355_varlen_attention_fwd(ptr(q.t), q.token_stride, q.head_stride, ptr(k.t), k.token_stride, k.head_stride, ptr(v.t),
                                    v.token_stride, v.head_stride, dtype_code(q.t), iptr(cu), cu.numel() - 1, (float)scale, ptr(out),
-                                   static_cast<float*>(ptr(lse)), q.tokens, q.heads, k.heads, q.size, L.stream),
+                                   ptr(rest), static_cast<float*>(ptr(lse)), q.tokens, q.heads, k.heads, q.size, L.stream),
         "varlen_attention_fwd");
-  return {out, lse};
+  return {out, lse, rest};
 }
 
 std::tuple<Tensor, Tensor, Tensor> varlen_attention_bwd(const Tensor& dout_, const Tensor& q_, const Tensor& k_, const Tensor& v_,
-                                                        const Tensor& out_, const Tensor& lse_, const Tensor& cu_, double scale) {
+                                                        const Tensor& out_, const Tensor& lse_, const Tensor& rest_, const Tensor& cu_,
+                                                        double scale) {
   Launch L(q_);
   const Heads q(q_), k(k_), v(v_);
   check_attention(q, k, v, cu_);
-  const Tensor dout = heads_like(dout_, q_), out = dense(out_), lse = dense(lse_), cu = cu_.contiguous();
+  const Tensor dout = heads_like(dout_, q_), out = dense(out_), lse = dense(lse_), rest = dense(rest_), cu = cu_.contiguous();
   TORCH_CHECK_VALUE(dout.sizes() == q_.sizes() && out.sizes() == q_.sizes() && out.scalar_type() == q_.scalar_type() &&
-                        lse.numel() == q.heads * q.tokens && lse.scalar_type() == at::kFloat,
+                        lse.numel() == q.heads * q.tokens && lse.scalar_type() == at::kFloat &&
+                        (rest.numel() == 0 || (rest.numel() == out.numel() && rest.scalar_type() == out.scalar_type())),
                     "the gradient, the result and its statistics do not fit the queries");
   Tensor dq = at::empty(q_.sizes(), q_.options()), dk = at::empty(k_.sizes(), k_.options()), dv = at::empty(v_.sizes(), v_.options());
   const Tensor ws = bytes(mi355_varlen_attention_bwd_workspace_bytes(q.tokens, q.heads, k.heads, q.size), q_);
   check(mi355_varlen_attention_bwd(ptr(dout), ptr(q.t), q.token_stride, q.head_stride, ptr(k.t), k.token_stride, k.head_stride,
-                                   ptr(v.t), v.token_stride, v.head_stride, ptr(out), fptr(lse), dtype_code(q.t), iptr(cu),
+                                   ptr(v.t), v.token_stride, v.head_stride, ptr(out), ptr(rest), fptr(lse), dtype_code(q.t), iptr(cu),
                                    cu.numel() - 1, (float)scale, ptr(dq), ptr(dk), ptr(dv), ptr(ws), q.tokens, q.heads, k.heads,
                                    q.size, L.stream),
         "varlen_attention_bwd");
@@ -768,9 +772,11 @@ TORCH_LIBRARY(mi355_moe, m) {
       "qk_norm_rotary_bwd(Tensor? dq_out, Tensor? dk_out, Tensor q, Tensor k, Tensor q_weight, Tensor k_weight, "
       "Tensor positions, Tensor inv_freq, float epsilon, bool interleaved, float attention_factor, bool need_dx, "
       "bool need_dw) -> (Tensor, Tensor, Tensor, Tensor)");
-  m.def("varlen_attention_fwd(Tensor q, Tensor k, Tensor v, Tensor cu_seqlens, float scale) -> (Tensor, Tensor)");
   m.def(
-      "varlen_attention_bwd(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor out, Tensor lse, Tensor cu_seqlens, "
+      "varlen_attention_fwd(Tensor q, Tensor k, Tensor v, Tensor cu_seqlens, float scale, bool for_backward) -> "
+      "(Tensor, Tensor, Tensor)");
+  m.def(
+      "varlen_attention_bwd(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor out, Tensor lse, Tensor out_rest, Tensor cu_seqlens, "
       "float scale) -> (Tensor, Tensor, Tensor)");
   m.def("balance_loss_fwd(Tensor scores, Tensor routing_map, Tensor? padding_mask) -> Tensor");
   m.def("balance_loss_bwd(Tensor scores, Tensor f, Tensor? padding_mask, Tensor grad_loss) -> Tensor");

@@ -188,12 +188,14 @@ def _(dq_out, dk_out, q, k, q_weight, k_weight, positions, inv_freq, epsilon, in
 
 
 @_fake("varlen_attention_fwd")
-def _(q, k, v, cu_seqlens, scale):
-    return q.new_empty(q.shape), q.new_empty((q.shape[1], q.shape[0]), dtype=torch.float32)
+def _(q, k, v, cu_seqlens, scale, for_backward):
+    kept = for_backward and q.dtype == torch.bfloat16
+    return (q.new_empty(q.shape), q.new_empty((q.shape[1], q.shape[0]), dtype=torch.float32),
+            q.new_empty(q.shape) if kept else _e0(q))
 
 
 @_fake("varlen_attention_bwd")
-def _(dout, q, k, v, out, lse, cu_seqlens, scale):
+def _(dout, q, k, v, out, lse, out_rest, cu_seqlens, scale):
     return tuple(t.new_empty(t.shape) for t in (q, k, v))
 
 
@@ -554,7 +556,7 @@ def varlen_attention(q, k, v, cu_seqlens, *, scale=None):
         scale = q.shape[2] ** -0.5
     if not (math.isfinite(scale) and scale > 0):
         raise ValueError(f"varlen_attention: the scale must be finite and positive, got {scale}")
-    return _O.varlen_attention_fwd(q, k, v, cu_seqlens, float(scale))[0]
+    return _O.varlen_attention_fwd(q, k, v, cu_seqlens, float(scale), False)[0]
 
 
 def _as_bool(m):
