@@ -29,7 +29,7 @@ struct AttnArgs {
   void* rest;             // (T, H, D) dense, bf16 only: what rounding took from out (written forward, read backward); null: not kept
   // backward
   const void *o, *dout;   // (T, H, D) dense
-  float* delta;           // (H, T)
+  float* delta;           // (H, T), negated by the bf16 kernels, which put -lse / c behind it (2 H, T)
   void *dq, *dk, *dv;     // dense; (splits > 1: dk_part, dv_part instead of dk, dv)
   float *dk_part, *dv_part;  // [splits][T][G][D] fp32
   const int32_t* cu;      // [sequences + 1]
@@ -40,6 +40,14 @@ struct AttnArgs {
 };
 
 constexpr float kNegInf = -INFINITY;
+
+// A kernel's arguments (AttnArgs its first) as memory to be read from here on.  What a kernel needs behind its loop only, and the careful
+// forms at its end above all, is otherwise fetched and prepared in front of it, and held in registers that the loop has no room for.
+__device__ __forceinline__ const AttnArgs& late_arguments() {
+  uint64_t at = reinterpret_cast<uint64_t>(__builtin_amdgcn_kernarg_segment_ptr());
+  asm volatile("" : "+s"(at));
+  return *(const AttnArgs*)reinterpret_cast<const __attribute__((address_space(4))) AttnArgs*>(at);
+}
 
 // The sequence [start, end) that a row lies in, or start = end = 0.  The entries on both sides of the answer have been compared with the
 // row, so start <= row < end however the array is ordered; clamped to the rows there are.
@@ -139,9 +147,9 @@ __device__ __forceinline__ void careful_dq_row(const AttnArgs& p, int h, int row
     if (lane + 64 * i < p.D) store_from_f32<T>(dq + lane + 64 * i, acc[i] * p.scale);
 }
 
-// dk and dv of one key over the query heads [h0, h1), into the part `split` where there are parts
+// dk and dv of one key over the query heads [h0, h1), into the part `split` where there are parts; delta is kept times `sign`
 template <typename T>
-__device__ __forceinline__ void careful_dkv_row(const AttnArgs& p, int g, int key, int end, int h0, int h1, int split) {
+__device__ __forceinline__ void careful_dkv_row(const AttnArgs& p, int g, int key, int end, int h0, int h1, int split, float sign) {
   const int lane = threadIdx.x & 63;
   const T* k = row_at<T>(p.k, p.k_token, p.k_head, key, g);
   const T* v = row_at<T>(p.v, p.v_token, p.v_head, key, g);
@@ -154,7 +162,7 @@ __device__ __forceinline__ void careful_dkv_row(const AttnArgs& p, int g, int ke
         const T* dout = static_cast<const T*>(p.dout) + (static_cast<int64_t>(r) * p.H + h) * p.D;
         const int64_t at = static_cast<int64_t>(h) * p.T + r;
         w = exp2_f32(fmaf(careful_dot<T>(row_at<T>(p.q, p.q_token, p.q_head, r, h), k, p.D), p.c, -p.lse[at]));
-        ds = w * (careful_dot<T>(dout, v, p.D) - p.delta[at]);
+        ds = w * (careful_dot<T>(dout, v, p.D) - sign * p.delta[at]);
       }
       for (int n = 0; n < kWave && r0 + n < end; ++n) {
         const float wn = __shfl(w, n, kWave), dn = __shfl(ds, n, kWave);

@@ -402,7 +402,7 @@ __global__ __launch_bounds__(256) void any_dkv_kernel(const AttnArgs p, int vec)
       const int r = key0 + 16 * qw + kw * (16 / KW) + i;
       int first, last;
       sequence_of(p.cu, p.sequences, p.T, r, first, last);
-      careful_dkv_row<T>(p, g, r, last, h0, h1, split);
+      careful_dkv_row<T>(p, g, r, last, h0, h1, split, 1.0f);
     }
 }
 
@@ -546,7 +546,7 @@ extern "C" int mi355_varlen_attention_fwd(const void* q, int64_t q_token_stride,
 extern "C" int64_t mi355_varlen_attention_bwd_workspace_bytes(int64_t T, int64_t H, int64_t G, int64_t D) {
   if (T < 1 || H < 1 || G < 1 || H % G || D < 1) return 0;
   const int64_t parts = head_parts(T, H, G);
-  return 4 * ((H * T + 3) / 4 * 4 + (parts > 1 ? 2 * parts * T * G * D : 0));
+  return 4 * ((2 * H * T + 3) / 4 * 4 + (parts > 1 ? 2 * parts * T * G * D : 0));
 }
 
 extern "C" int mi355_varlen_attention_bwd(const void* dout, const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
@@ -564,7 +564,7 @@ extern "C" int mi355_varlen_attention_bwd(const void* dout, const void* q, int64
   p.dout = dout, p.lse = const_cast<float*>(lse), p.dq = dq, p.dk = dk, p.dv = dv;
   p.splits = head_parts(T, H, G);
   p.delta = static_cast<float*>(workspace);
-  p.dk_part = p.delta + (H * T + 3) / 4 * 4;
+  p.dk_part = p.delta + (2 * H * T + 3) / 4 * 4;
   p.dv_part = p.dk_part + static_cast<int64_t>(p.splits) * T * G * D;
   if (dtype == MI355_BF16 && attention_bf16_covers(p)) attention_bf16_backward(p, as_stream(stream));
   else attention_any_backward(p, dtype, as_stream(stream));

@@ -28,30 +28,29 @@ __device__ __forceinline__ int swizzle(int r) {  // (of the low four bits of r)
   return DP == 64 ? (((r >> 1) & 1) << 2) | ((r >> 2) & 3) : ((r & 3) << 2) | ((r >> 2) & 3);
 }
 
-// LDS byte offsets of a lane's reads of a tile
+// LDS byte offsets of a lane's reads of a tile: the swizzle is an exclusive or, and so are the steps over a row's pieces
 template <int DP>
 struct Reads {
-  uint32_t row[DP / 16];        // 8 elements of row lane % 32 (+ 32 b), step kk
-  uint32_t turned[DP / 32][2];  // elements 32 n + lane % 32 of rows 4 h + {0..3} and 8 + 4 h + {0..3} (+ 16 kk)
-  __device__ __forceinline__ void find(int lane) {
+  uint32_t row_, turned_;
+  __device__ __forceinline__ void find(int lane, uint32_t lds0) {
     const int h = lane >> 5, r = lane & 31;
-#pragma unroll
-    for (int kk = 0; kk < DP / 16; ++kk) row[kk] = r * DP * 2 + (((2 * kk + h) ^ swizzle<DP>(r)) << 4);
-    const int i = lane & 15, side = (lane >> 4) & 1;
-#pragma unroll
-    for (int n = 0; n < DP / 32; ++n)
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int t = 8 * half + 4 * h + (i >> 2), c = 4 * n + 2 * side + ((i & 3) >> 1);
-        turned[n][half] = t * DP * 2 + ((c ^ swizzle<DP>(t)) << 4) + 8 * (i & 1);
-      }
+    row_ = lds0 + r * DP * 2 + ((h ^ swizzle<DP>(r)) << 4);
+    const int i = lane & 15, side = (lane >> 4) & 1, t = 4 * h + (i >> 2);
+    turned_ = lds0 + t * DP * 2 + (((2 * side + ((i & 3) >> 1)) ^ swizzle<DP>(t)) << 4) + 8 * (i & 1);
   }
+  // the same, to be formed from here on: what is formed from these is otherwise held in registers over the loop
+  __device__ __forceinline__ Reads here() const { return {static_cast<uint32_t>(opaque(row_)), static_cast<uint32_t>(opaque(turned_))}; }
+  // 8 elements of row lane % 32, step kk
+  __device__ __forceinline__ uint32_t row(int kk) const { return row_ ^ (kk << 5); }
+  // elements 32 n + lane % 32 of rows 4 h + {0..3}, or 8 rows on
+  __device__ __forceinline__ uint32_t turned(int n, int half) const { return (turned_ ^ (n << 6) ^ (half << 5)) + half * 8 * DP * 2; }
 };
 
 __device__ __forceinline__ bf16x8 read_row(uint32_t at) { return lds_read16(at); }
-__device__ __forceinline__ bf16x8 read_turned(uint32_t at_lo, uint32_t at_hi) {
-  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<s16x4>(at_lo));
-  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<s16x4>(at_hi));
+template <int DP>
+__device__ __forceinline__ bf16x8 read_turned(const Reads<DP>& reads, int n, uint32_t rows) {
+  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<s16x4>(reads.turned(n, 0) + rows));
+  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<s16x4>(reads.turned(n, 1) + rows));
   const s16x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
   return __builtin_bit_cast(bf16x8, v);
 }
@@ -63,26 +62,25 @@ struct Requests {
   static constexpr int ROWS = 1024 / (DP * 2);        // rows a request
   uint64_t base;
   int64_t row_bytes;
-  uint32_t voff[EACH];
+  uint32_t voff;
   int T, D;
   __device__ __forceinline__ void find(const void* p, int64_t token, int T_, int D_, int lane, int wave) {
     base = reinterpret_cast<uint64_t>(p);
     row_bytes = token * 2;
     T = T_, D = D_;
     constexpr int CPR = DP / 8;
-#pragma unroll
-    for (int j = 0; j < EACH; ++j) {
-      const int r = ROWS * (4 * j + wave) + lane / CPR, c = (lane % CPR) ^ swizzle<DP>(r);
-      voff[j] = c * 8 < D_ ? static_cast<uint32_t>(r * row_bytes) + c * 16 : kFarOff;
-    }
+    // (a wave's requests are 4 ROWS = 16 or 32 rows apart: the same swizzle)
+    const int r = ROWS * wave + lane / CPR, c = (lane % CPR) ^ swizzle<DP>(r);
+    voff = c * 8 < D_ ? static_cast<uint32_t>(r * row_bytes) + c * 16 : kFarOff;
   }
   // rows [row0, row0 + 64) to LDS at `lds`; zeros for rows from T on
   __device__ __forceinline__ void request(int row0, uint32_t lds, int wave) const {
     const int64_t left = static_cast<int64_t>(T - 1 - row0) * row_bytes + D * 2;
     const uint32_t bytes = left < 0 ? 0 : left < kFarOff ? static_cast<uint32_t>(left) : kFarOff;
     const uint64_t at = base + static_cast<int64_t>(row0) * row_bytes;
+    const uint32_t step = 4 * ROWS * static_cast<uint32_t>(row_bytes), off = opaque(voff);
 #pragma unroll
-    for (int j = 0; j < EACH; ++j) lds_load16_within(at, bytes, voff[j], lds + (4 * j + wave) * 1024);
+    for (int j = 0; j < EACH; ++j) lds_load16_within(at, bytes, off + j * step, lds + (4 * j + wave) * 1024);
   }
 };
 
@@ -96,6 +94,27 @@ __device__ __forceinline__ void own_rows(bf16x8 (&x)[DP / 16], const uint16_t* r
     if (on && d < D) v = *reinterpret_cast<const u32x4*>(row + d);
     x[kk] = __builtin_bit_cast(bf16x8, v);
   }
+}
+// Waits for the operands here: the compiler, which does not count requests to LDS, would wait in the loop, for all that are under way.
+template <int N>
+__device__ __forceinline__ void settle(bf16x8 (&x)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(x[i]));
+}
+
+// Order of a stretch of code, N times: a matrix instruction, READS reads of LDS, VALU vector instructions
+template <int N, int READS, int VALU>
+__device__ __forceinline__ void interleave() {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    if (READS) __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+    if (VALU) __builtin_amdgcn_sched_group_barrier(0x002, VALU, 0);
+  }
+}
+template <int READS>
+__device__ __forceinline__ void reads_first() {
+  __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
 }
 
 __device__ __forceinline__ f32x16 mfma(const bf16x8& a, const bf16x8& b, const f32x16& c) {
@@ -200,7 +219,7 @@ __global__ __launch_bounds__(256, 2) void bf16_forward_kernel(const AttnArgs p, 
   range.find(on ? start : p.T, on ? row + 1 : 0, reinterpret_cast<int*>(smem), wave);
   const int latest = most(on ? start : p.T);  // keys from here to the wave's first row are seen by all its rows
   Reads<DP> reads;
-  reads.find(lane);
+  reads.find(lane, lds0);
   Requests<DP> keys, values;
   keys.find(static_cast<const uint16_t*>(p.k) + g * p.k_head, p.k_token, p.T, p.D, lane, wave);
   values.find(static_cast<const uint16_t*>(p.v) + g * p.v_head, p.v_token, p.T, p.D, lane, wave);
@@ -211,25 +230,27 @@ __global__ __launch_bounds__(256, 2) void bf16_forward_kernel(const AttnArgs p, 
   if (range.lo < range.hi) request(range.lo, 0);
   bf16x8 q[KK];
   own_rows<DP>(q, row_at<uint16_t>(p.q, p.q_token, p.q_head, min(row, p.T - 1), h), on, p.D, lane);
+  settle(q);
   f32x16 o[NB];
 #pragma unroll
   for (int n = 0; n < NB; ++n) o[n] = zeros();
   float m = kNegInf, ref = 0.0f, l = 0.0f;
   const float c = p.c, growth = kGrowth / p.c;
-  uint32_t buffer = 0;
-  for (int k0 = range.lo; k0 < range.hi; k0 += kTile, buffer ^= 1) {
+  auto tile = [&](int k0, auto which) {
+    constexpr uint32_t BUFFER = decltype(which)::value;
     lds_wait<0>();
     lds_sync<63>();  // everyone's requests of this tile have landed, and everyone has read the other buffer
-    if (k0 + kTile < range.hi) request(k0 + kTile, buffer ^ 1);
-    if (k0 >= range.last || k0 + kTile <= range.first) continue;
-    const uint32_t kt = lds0 + buffer * 2 * TILE_BYTES, vt = kt + TILE_BYTES;
-    f32x16 s[2];
+    if (k0 + kTile < range.hi) request(k0 + kTile, BUFFER ^ 1);
+    if (k0 >= range.last || k0 + kTile <= range.first) return;
+    constexpr uint32_t kt = BUFFER * 2 * TILE_BYTES, vt = kt + TILE_BYTES;
+    f32x16 s[2] = {zeros(), zeros()};
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      s[b] = zeros();
+    for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
-      for (int kk = 0; kk < KK; ++kk) s[b] = mfma(read_row(kt + reads.row[kk] + b * 32 * DP * 2), q[kk], s[b]);
-    }
+      for (int b = 0; b < 2; ++b) s[b] = mfma(read_row(reads.row(kk) + kt + b * 32 * DP * 2), q[kk], s[b]);
+    reads_first<6>();
+    interleave<2 * KK - 6, 1, 0>();
+    interleave<6, 0, 0>();
     if (k0 + kTile - 1 > row0 || k0 < latest) {
 #pragma unroll
       for (int b = 0; b < 2; ++b)
@@ -254,24 +275,32 @@ __global__ __launch_bounds__(256, 2) void bf16_forward_kernel(const AttnArgs p, 
       m = next;
       ref = next_ref;
     }
+    // 16 keys a step: the matrix instructions of one beside the exponentials of the next
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+    for (int t = 0; t < 4; ++t) {
+      float part[2] = {0.0f, 0.0f};
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[b][i] = exp2_f32(fmaf(s[b][i], c, -ref));
-        l += s[b][i];
+      for (int i = 8 * (t & 1); i < 8 * (t & 1) + 8; ++i) {
+        s[t >> 1][i] = exp2_f32(fmaf(s[t >> 1][i], c, -ref));
+        part[i & 1] += s[t >> 1][i];
       }
+      l += part[0] + part[1];
+      const bf16x8 w = operand_of(s[t >> 1], t & 1);
 #pragma unroll
-      for (int kk = 0; kk < 2; ++kk) {
-        const bf16x8 w = operand_of(s[b], kk);
-        const uint32_t rows = vt + (2 * b + kk) * 16 * DP * 2;
-#pragma unroll
-        for (int n = 0; n < NB; ++n) o[n] = mfma(read_turned(rows + reads.turned[n][0], rows + reads.turned[n][1]), w, o[n]);
-      }
+      for (int n = 0; n < NB; ++n) o[n] = mfma(read_turned(reads, n, vt + t * 16 * DP * 2), w, o[n]);
     }
+    reads_first<2 * NB>();
+    __builtin_amdgcn_sched_group_barrier(0x002, 30, 0);
+    interleave<3 * NB, 2, 32 / NB>();
+    interleave<NB, 0, 0>();
+  };
+  for (int k0 = range.lo; k0 < range.hi; k0 += 2 * kTile) {
+    tile(k0, std::integral_constant<uint32_t, 0>{});
+    if (k0 + kTile < range.hi) tile(k0 + kTile, std::integral_constant<uint32_t, 1>{});
   }
   l = halves_sum(l);
   const float inverse = 1.0f / l;
+  const AttnArgs& z = late_arguments();
   bool spoilt = false;
 #pragma unroll
   for (int n = 0; n < NB; ++n)
@@ -280,8 +309,8 @@ __global__ __launch_bounds__(256, 2) void bf16_forward_kernel(const AttnArgs p, 
       o[n][i] = on ? o[n][i] * inverse : 0.0f;
       spoilt |= o[n][i] != o[n][i];
     }
-  if (row < p.T) {
-    const int64_t dense = (static_cast<int64_t>(row) * p.H + h) * p.D;
+  if (row < z.T) {
+    const int64_t dense = (static_cast<int64_t>(row) * z.H + h) * z.D;
 #pragma unroll
     for (int n = 0; n < NB; ++n)
 #pragma unroll
@@ -289,23 +318,23 @@ __global__ __launch_bounds__(256, 2) void bf16_forward_kernel(const AttnArgs p, 
         float v[8];
         eight_of(o[n], a, v);
         const int d = 32 * n + 16 * a + 8 * half;
-        if (d >= p.D) continue;
+        if (d >= z.D) continue;
         const u32x4 packed = pack8(v);
-        *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p.out) + dense + d) = packed;
-        if (p.rest) {
+        *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(z.out) + dense + d) = packed;
+        if (z.rest) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) v[i] -= __uint_as_float(i & 1 ? packed[i / 2] & 0xffff0000u : packed[i / 2] << 16);
-          *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p.rest) + dense + d) = pack8(v);
+          *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(z.rest) + dense + d) = pack8(v);
         }
       }
-    if (half == 0 && p.lse) p.lse[static_cast<int64_t>(h) * p.T + row] = on ? ref + log2f(l) : INFINITY;
+    if (half == 0 && z.lse) z.lse[static_cast<int64_t>(h) * z.T + row] = on ? ref + log2f(l) : INFINITY;
   }
-  uint64_t again = __ballot(spoilt && row < p.T);
+  uint64_t again = __ballot(spoilt && row < z.T);
   again = (again | again >> 32) & 0xffffffffu;
   if (again) lds_wait<0>();
   for (; again; again &= again - 1) {
     const int i = __builtin_ctzll(again);
-    careful_forward_row<uint16_t>(p, h, row0 + i, __builtin_amdgcn_readlane(start, i));
+    careful_forward_row<uint16_t>(z, h, row0 + i, __builtin_amdgcn_readlane(start, i));
   }
 }
 
@@ -327,7 +356,7 @@ __global__ __launch_bounds__(256, 2) void bf16_dq_kernel(const AttnArgs p, int t
   range.find(on ? start : p.T, on ? row + 1 : 0, reinterpret_cast<int*>(smem), wave);
   const int latest = most(on ? start : p.T);
   Reads<DP> reads;
-  reads.find(lane);
+  reads.find(lane, lds0);
   Requests<DP> keys, values;
   keys.find(static_cast<const uint16_t*>(p.k) + g * p.k_head, p.k_token, p.T, p.D, lane, wave);
   values.find(static_cast<const uint16_t*>(p.v) + g * p.v_head, p.v_token, p.T, p.D, lane, wave);
@@ -356,26 +385,35 @@ __global__ __launch_bounds__(256, 2) void bf16_dq_kernel(const AttnArgs p, int t
   }
   delta = halves_sum(delta);
   const float lse = on ? p.lse[static_cast<int64_t>(h) * p.T + row] : INFINITY;
-  if (half == 0 && row < p.T) p.delta[static_cast<int64_t>(h) * p.T + row] = on ? delta : 0.0f;
+  if (half == 0 && row < p.T) {  // as the kernel behind this one starts its sums from: -lse / c and -delta
+    p.delta[static_cast<int64_t>(h) * p.T + row] = on ? -delta : 0.0f;
+    p.delta[static_cast<int64_t>(p.H + h) * p.T + row] = -lse / p.c;
+  }
+  settle(q);
+  settle(dout);
   f32x16 dq[NB];
 #pragma unroll
   for (int n = 0; n < NB; ++n) dq[n] = zeros();
   const float c = p.c;
-  uint32_t buffer = 0;
-  for (int k0 = range.lo; k0 < range.hi; k0 += kTile, buffer ^= 1) {
+  auto tile = [&](int k0, auto which) {
+    constexpr uint32_t BUFFER = decltype(which)::value;
     lds_wait<0>();
     lds_sync<63>();
-    if (k0 + kTile < range.hi) request(k0 + kTile, buffer ^ 1);
-    if (k0 >= range.last || k0 + kTile <= range.first) continue;
-    const uint32_t kt = lds0 + buffer * 2 * TILE_BYTES, vt = kt + TILE_BYTES;
+    if (k0 + kTile < range.hi) request(k0 + kTile, BUFFER ^ 1);
+    if (k0 >= range.last || k0 + kTile <= range.first) return;
+    constexpr uint32_t kt = BUFFER * 2 * TILE_BYTES, vt = kt + TILE_BYTES;
     const bool masked = k0 + kTile - 1 > row0 || k0 < latest;
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       f32x16 s = zeros(), ds = zeros();
 #pragma unroll
-      for (int kk = 0; kk < KK; ++kk) s = mfma(read_row(kt + reads.row[kk] + b * 32 * DP * 2), q[kk], s);
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk) ds = mfma(read_row(vt + reads.row[kk] + b * 32 * DP * 2), dout[kk], ds);
+      for (int kk = 0; kk < KK; ++kk) {
+        s = mfma(read_row(reads.row(kk) + kt + b * 32 * DP * 2), q[kk], s);
+        ds = mfma(read_row(reads.row(kk) + vt + b * 32 * DP * 2), dout[kk], ds);
+      }
+      reads_first<4>();
+      interleave<2 * KK - 4, 1, 0>();
+      interleave<4, 0, 0>();
 #pragma unroll
       for (int i = 0; i < 16; ++i) ds[i] = exp2_f32(fmaf(s[i], c, -lse)) * (ds[i] - delta);
       if (masked) {
@@ -386,23 +424,30 @@ __global__ __launch_bounds__(256, 2) void bf16_dq_kernel(const AttnArgs p, int t
         }
       }
 #pragma unroll
-      for (int kk = 0; kk < 2; ++kk) {
-        const bf16x8 w = operand_of(ds, kk);
-        const uint32_t rows = kt + (2 * b + kk) * 16 * DP * 2;
+      for (int t = 0; t < 2; ++t) {
+        const bf16x8 w = operand_of(ds, t);
 #pragma unroll
-        for (int n = 0; n < NB; ++n) dq[n] = mfma(read_turned(rows + reads.turned[n][0], rows + reads.turned[n][1]), w, dq[n]);
+        for (int n = 0; n < NB; ++n) dq[n] = mfma(read_turned(reads, n, kt + (2 * b + t) * 16 * DP * 2), w, dq[n]);
       }
+      reads_first<8>();
+      interleave<2 * NB - 4, 2, 0>();
+      interleave<4, 0, 0>();
     }
+  };
+  for (int k0 = range.lo; k0 < range.hi; k0 += 2 * kTile) {
+    tile(k0, std::integral_constant<uint32_t, 0>{});
+    if (k0 + kTile < range.hi) tile(k0 + kTile, std::integral_constant<uint32_t, 1>{});
   }
+  const AttnArgs& z = late_arguments();
   bool spoilt = false;
 #pragma unroll
   for (int n = 0; n < NB; ++n)
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      dq[n][i] = on ? dq[n][i] * p.scale : 0.0f;
+      dq[n][i] = on ? dq[n][i] * z.scale : 0.0f;
       spoilt |= dq[n][i] != dq[n][i];
     }
-  if (row < p.T) {
+  if (row < z.T) {
 #pragma unroll
     for (int n = 0; n < NB; ++n)
 #pragma unroll
@@ -410,15 +455,15 @@ __global__ __launch_bounds__(256, 2) void bf16_dq_kernel(const AttnArgs p, int t
         float v[8];
         eight_of(dq[n], a, v);
         const int d = 32 * n + 16 * a + 8 * half;
-        if (d < p.D) *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p.dq) + dense + d) = pack8(v);
+        if (d < z.D) *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(z.dq) + dense + d) = pack8(v);
       }
   }
-  uint64_t again = __ballot(spoilt && row < p.T);
+  uint64_t again = __ballot(spoilt && row < z.T);
   again = (again | again >> 32) & 0xffffffffu;
   if (again) lds_wait<0>();
   for (; again; again &= again - 1) {
     const int i = __builtin_ctzll(again);
-    careful_dq_row<uint16_t>(p, h, row0 + i, __builtin_amdgcn_readlane(start, i),
+    careful_dq_row<uint16_t>(z, h, row0 + i, __builtin_amdgcn_readlane(start, i),
                              __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lse), i)),
                              __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(delta), i)));
   }
@@ -426,9 +471,9 @@ __global__ __launch_bounds__(256, 2) void bf16_dq_kernel(const AttnArgs p, int t
 
 // dk and dv: a wave's 32 keys against the query heads of their group, or a part of them
 template <int DP>
-__global__ __launch_bounds__(256, 1) void bf16_dkv_kernel(const AttnArgs p, int tiles) {
+__global__ __launch_bounds__(256, 2) void bf16_dkv_kernel(const AttnArgs p, int tiles) {
   constexpr int KK = DP / 16, NB = DP / 32;
-  constexpr uint32_t TILE_BYTES = kTile * DP * 2, STAGE = 2 * TILE_BYTES + 512;  // queries, gradients, lse, delta
+  constexpr uint32_t TILE_BYTES = kTile * DP * 2, STAGE = 2 * TILE_BYTES + 512;  // queries, gradients, -lse / c, -delta
   extern __shared__ __attribute__((aligned(16))) uint16_t smem[];
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_cptr)smem));
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
@@ -443,7 +488,8 @@ __global__ __launch_bounds__(256, 1) void bf16_dkv_kernel(const AttnArgs p, int 
   range.find(on ? key : p.T, on ? end : 0, reinterpret_cast<int*>(smem), wave);
   const int earliest = least(on ? end : 0);  // rows from the wave's last key to here see all its keys
   Reads<DP> reads;
-  reads.find(lane);
+  reads.find(lane, lds0);
+  const uint32_t from_stats = lds0 + 16 * half;
   const int here = min(key, p.T - 1);
   bf16x8 k[KK], v[KK];
   own_rows<DP>(k, row_at<uint16_t>(p.k, p.k_token, p.k_head, here, g), on, p.D, lane);
@@ -462,74 +508,94 @@ __global__ __launch_bounds__(256, 1) void bf16_dkv_kernel(const AttnArgs p, int 
     grads.base = reinterpret_cast<uint64_t>(static_cast<const uint16_t*>(p.dout) + h * p.D);
     queries.request(r0, to, wave);
     grads.request(r0, to + TILE_BYTES, wave);
-    if (wave < 2) {  // lse and delta of the tile's 64 rows, one wave each
-      const float* from = (wave ? p.delta : p.lse) + static_cast<int64_t>(h) * p.T;
+    if (wave < 2) {  // -lse / c and -delta of the tile's 64 rows, one wave each
+      const float* from = p.delta + static_cast<int64_t>(wave ? h : p.H + h) * p.T;
       lds_load4_within(reinterpret_cast<uint64_t>(from + r0), static_cast<uint32_t>(min(p.T - r0, kTile)) * 4, lane * 4,
                        to + 2 * TILE_BYTES + wave * 256);
     }
   };
-  uint32_t buffer = 0;
-  if (steps) request(h0, range.lo, 0);
-  for (int h = h0; h < h1 && steps; ++h)
-    for (int t = 0; t < steps; ++t, buffer ^= 1) {
-      const int r0 = range.lo + t * kTile;
-      lds_wait<0>();
-      lds_sync<63>();
-      if (t + 1 < steps) request(h, r0 + kTile, buffer ^ 1);
-      else if (h + 1 < h1) request(h + 1, range.lo, buffer ^ 1);
-      if (r0 >= range.last || r0 + kTile <= range.first) continue;
-      const uint32_t qt = lds0 + buffer * STAGE, dt = qt + TILE_BYTES, stats = dt + TILE_BYTES;
-      const bool masked = r0 < key0 + kRows - 1 || r0 + kTile > earliest;
+  settle(k);
+  settle(v);
+  auto tile = [&](int h, int t, auto which) {
+    constexpr uint32_t BUFFER = decltype(which)::value;
+    const int r0 = range.lo + t * kTile;
+    lds_wait<0>();
+    lds_sync<63>();
+    if (t + 1 < steps) request(h, r0 + kTile, BUFFER ^ 1);
+    else if (h + 1 < h1) request(h + 1, range.lo, BUFFER ^ 1);
+    if (r0 >= range.last || r0 + kTile <= range.first) return;
+    constexpr uint32_t qt = BUFFER * STAGE, dt = qt + TILE_BYTES, stats = dt + TILE_BYTES;
+    const bool masked = r0 < key0 + kRows - 1 || r0 + kTile > earliest;
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        f32x16 s = zeros(), ds = zeros();
+    for (int b = 0; b < 2; ++b) {
+      const Reads<DP> at_tile = reads.here();
+      f32x16 s, ds;  // from -lse / c and -delta of the lane's rows
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk) s = mfma(read_row(qt + reads.row[kk] + b * 32 * DP * 2), k[kk], s);
+      for (int a = 0; a < 4; ++a) {
+        const f32x4 x = *lds_at<const f32x4>(from_stats + stats + (32 * b + 8 * a) * 4);
+        const f32x4 y = *lds_at<const f32x4>(from_stats + stats + 256 + (32 * b + 8 * a) * 4);
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk) ds = mfma(read_row(dt + reads.row[kk] + b * 32 * DP * 2), v[kk], ds);
+        for (int i = 0; i < 4; ++i) s[4 * a + i] = x[i], ds[4 * a + i] = y[i];
+      }
 #pragma unroll
-        for (int a = 0; a < 4; ++a) {
-          const f32x4 lse = *lds_at<const f32x4>(stats + (32 * b + 8 * a + 4 * half) * 4);
-          const f32x4 delta = *lds_at<const f32x4>(stats + 256 + (32 * b + 8 * a + 4 * half) * 4);
+      for (int kk = 0; kk < KK; ++kk) {
+        s = mfma(read_row(at_tile.row(kk) + qt + b * 32 * DP * 2), k[kk], s);
+        ds = mfma(read_row(at_tile.row(kk) + dt + b * 32 * DP * 2), v[kk], ds);
+      }
+      reads_first<12>();
+      interleave<2 * KK - 4, 1, 0>();
+      interleave<4, 0, 0>();
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            s[4 * a + i] = exp2_f32(fmaf(s[4 * a + i], c, -lse[i]));
-            ds[4 * a + i] = s[4 * a + i] * (ds[4 * a + i] - delta[i]);
-          }
-        }
-        if (masked) {
+      for (int i = 0; i < 16; ++i) {
+        s[i] = exp2_f32(s[i] * c);
+        ds[i] *= s[i];
+      }
+      if (masked) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int r = r0 + 32 * b + 8 * (i >> 2) + 4 * half + (i & 3);
-            const bool seen = on && r >= key && r < end;
-            s[i] = seen ? s[i] : 0.0f;
-            ds[i] = seen ? ds[i] : 0.0f;
-          }
-        }
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-          const bf16x8 w = operand_of(s, kk), dw = operand_of(ds, kk);
-          const uint32_t rows = (2 * b + kk) * 16 * DP * 2;
-#pragma unroll
-          for (int n = 0; n < NB; ++n)
-            dv[n] = mfma(read_turned(dt + rows + reads.turned[n][0], dt + rows + reads.turned[n][1]), w, dv[n]);
-#pragma unroll
-          for (int n = 0; n < NB; ++n)
-            dk[n] = mfma(read_turned(qt + rows + reads.turned[n][0], qt + rows + reads.turned[n][1]), dw, dk[n]);
+        for (int i = 0; i < 16; ++i) {
+          const int r = r0 + 32 * b + 8 * (i >> 2) + 4 * half + (i & 3);
+          const bool seen = on && r >= key && r < end;
+          s[i] = seen ? s[i] : 0.0f;
+          ds[i] = seen ? ds[i] : 0.0f;
         }
       }
+      bf16x8 w[4];
+#pragma unroll
+      for (int t2 = 0; t2 < 2; ++t2) w[t2] = operand_of(s, t2), w[2 + t2] = operand_of(ds, t2);
+#pragma unroll
+      for (int t2 = 0; t2 < 2; ++t2)
+#pragma unroll
+        for (int n = 0; n < NB; ++n) dv[n] = mfma(read_turned(at_tile, n, dt + (2 * b + t2) * 16 * DP * 2), w[t2], dv[n]);
+#pragma unroll
+      for (int t2 = 0; t2 < 2; ++t2)
+#pragma unroll
+        for (int n = 0; n < NB; ++n) dk[n] = mfma(read_turned(at_tile, n, qt + (2 * b + t2) * 16 * DP * 2), w[2 + t2], dk[n]);
+      reads_first<8>();
+      interleave<4 * NB - 4, 2, 0>();
+      interleave<4, 0, 0>();
     }
+  };
+  if (steps) request(h0, range.lo, 0);
+  const int all = steps * max(h1 - h0, 0);  // tiles, the first head's first
+  for (int n = 0, h = h0, t = 0; n < all; n += 2) {
+    tile(h, t, std::integral_constant<uint32_t, 0>{});
+    if (++t == steps) t = 0, ++h;
+    if (n + 1 == all) break;
+    tile(h, t, std::integral_constant<uint32_t, 1>{});
+    if (++t == steps) t = 0, ++h;
+  }
+  const AttnArgs& z = late_arguments();
   bool spoilt = false;
 #pragma unroll
   for (int n = 0; n < NB; ++n)
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      dk[n][i] = on ? dk[n][i] * p.scale : 0.0f;
+      dk[n][i] = on ? dk[n][i] * z.scale : 0.0f;
       dv[n][i] = on ? dv[n][i] : 0.0f;
       spoilt |= dk[n][i] != dk[n][i] || dv[n][i] != dv[n][i];
     }
-  if (key < p.T) {
-    const int64_t dense = (static_cast<int64_t>(key) * p.G + g) * p.D, part = static_cast<int64_t>(split) * p.T * p.G * p.D + dense;
+  if (key < z.T) {
+    const int64_t dense = (static_cast<int64_t>(key) * z.G + g) * z.D, part = static_cast<int64_t>(split) * z.T * z.G * z.D + dense;
 #pragma unroll
     for (int n = 0; n < NB; ++n)
 #pragma unroll
@@ -539,22 +605,22 @@ __global__ __launch_bounds__(256, 1) void bf16_dkv_kernel(const AttnArgs p, int 
           float x[8];
           eight_of(which ? dk[n] : dv[n], a, x);
           const int d = 32 * n + 16 * a + 8 * half;
-          if (d >= p.D) continue;
-          if (p.splits > 1) {
-            f32x4* to = reinterpret_cast<f32x4*>((which ? p.dk_part : p.dv_part) + part + d);
+          if (d >= z.D) continue;
+          if (z.splits > 1) {
+            f32x4* to = reinterpret_cast<f32x4*>((which ? z.dk_part : z.dv_part) + part + d);
             to[0] = f32x4{x[0], x[1], x[2], x[3]};
             to[1] = f32x4{x[4], x[5], x[6], x[7]};
           } else {
-            *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(which ? p.dk : p.dv) + dense + d) = pack8(x);
+            *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(which ? z.dk : z.dv) + dense + d) = pack8(x);
           }
         }
   }
-  uint64_t again = __ballot(spoilt && key < p.T);
+  uint64_t again = __ballot(spoilt && key < z.T);
   again = (again | again >> 32) & 0xffffffffu;
   if (again) lds_wait<0>();
   for (; again; again &= again - 1) {
     const int i = __builtin_ctzll(again);
-    careful_dkv_row<uint16_t>(p, g, key0 + i, __builtin_amdgcn_readlane(end, i), h0, h1, split);
+    careful_dkv_row<uint16_t>(z, g, key0 + i, __builtin_amdgcn_readlane(end, i), h0, h1, split, -1.0f);
   }
 }
 
