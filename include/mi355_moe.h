@@ -798,13 +798,16 @@ int mi355_qk_norm_rotary_bwd(const void* dq_out, const void* dk_out, const void*
  * out_rest: optional, bf16 only, dense like out: what rounding took from it, rounded itself; with it the backward's out . dout is as good as
  * out in fp32 (from the rounded out alone, the gradients of short rows come out twice as far from the formula).
  * lse: optional (H, T) fp32, log2 of each row's sum of exp(scale q.k), +inf for rows in no sequence; the backward reads it.
+ * workspace: mi355_varlen_attention_fwd_workspace_bytes(T, H, sequences) bytes, or NULL: then tiles of several sequences start in the order in which
+ * they lie, not the longest first.
  */
 int mi355_varlen_attention_fwd(const void* q, int64_t q_token_stride, int64_t q_head_stride,
                                const void* k, int64_t k_token_stride, int64_t k_head_stride,
                                const void* v, int64_t v_token_stride, int64_t v_head_stride,
                                int dtype, const int32_t* cu_seqlens, int64_t sequences, float scale,
-                               void* out, void* out_rest, float* lse, int64_t T, int64_t H,
-                               int64_t G, int64_t D, void* stream);
+                               void* out, void* out_rest, float* lse, void* workspace,
+                               int64_t T, int64_t H, int64_t G, int64_t D, void* stream);
+int64_t mi355_varlen_attention_fwd_workspace_bytes(int64_t T, int64_t H, int64_t sequences);
 
 /*
  * Its backward; dout, out and out_rest (the forward's; out_rest may be NULL) dense, so are dq, dk and dv.  Scores are formed again.  No atomics: dk and dv of a key

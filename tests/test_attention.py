@@ -428,7 +428,8 @@ def test_c_entry_points_refuse_before_any_launch():
     lib, p = _lib.load(), 0x1000  # (never dereferenced)
 
     def forward(T=4, H=4, G=2, D=64, dtype=1, scale=0.1, cu=p, sequences=1):
-        return lib.mi355_varlen_attention_fwd(p, H * D, D, p, G * D, D, p, G * D, D, dtype, cu, sequences, scale, p, p, p, T, H, G, D, None)
+        return lib.mi355_varlen_attention_fwd(p, H * D, D, p, G * D, D, p, G * D, D, dtype, cu, sequences, scale, p, p, p, p, T, H, G,
+                                              D, None)
 
     def backward(T=4, H=4, G=2, D=64, workspace=p):
         return lib.mi355_varlen_attention_bwd(p, p, H * D, D, p, G * D, D, p, G * D, D, p, p, p, 1, p, 1, 0.1, p, p, p, workspace, T, H,

@@ -39,17 +39,29 @@ __device__ __forceinline__ float4 four_at(const T* p, int n, bool vec) {  // the
   return v;
 }
 
-// rows [row0, row0 + ROWS) of a head into LDS as fp32, zeros behind row T and behind the head's elements
+// Rows [row0, row0 + ROWS) of a head on their way to LDS as fp32, zeros behind row T and behind the head's elements: held in registers from
+// where they are fetched, a tile ahead, to where the tile before has been read
 template <typename T, int DP, int ROWS>
-__device__ __forceinline__ void fill_tile(float* tile, const T* base, int64_t token, int row0, int T_, int D, bool vec) {
-  constexpr int P = DP + 4, QUADS = DP / 4;
-  for (int i = threadIdx.x; i < ROWS * QUADS; i += 256) {
-    const int r = i / QUADS, d = (i % QUADS) * 4;
-    float4 v = make_float4(0, 0, 0, 0);
-    if (row0 + r < T_ && d < D) v = four_at<T>(base + static_cast<int64_t>(row0 + r) * token + d, D - d, vec && d + 4 <= D);
-    *reinterpret_cast<float4*>(tile + r * P + d) = v;
+struct Staged {
+  static constexpr int P = DP + 4, QUADS = DP / 4, EACH = ROWS * QUADS / 256;
+  static_assert(ROWS * QUADS % 256 == 0, "whole rounds of the workgroup");
+  float4 x[EACH];
+  __device__ __forceinline__ void fetch(const T* base, int64_t token, int row0, int T_, int D, bool vec) {
+#pragma unroll
+    for (int n = 0; n < EACH; ++n) {
+      const int i = threadIdx.x + 256 * n, r = row0 + i / QUADS, d = (i % QUADS) * 4;
+      x[n] = make_float4(0, 0, 0, 0);
+      if (r < T_ && d < D) x[n] = four_at<T>(base + static_cast<int64_t>(r) * token + d, D - d, vec && d + 4 <= D);
+    }
   }
-}
+  __device__ __forceinline__ void put(float* tile) const {
+#pragma unroll
+    for (int n = 0; n < EACH; ++n) {
+      const int i = threadIdx.x + 256 * n;
+      *reinterpret_cast<float4*>(tile + (i / QUADS) * P + (i % QUADS) * 4) = x[n];
+    }
+  }
+};
 
 // a wave's 16 rows as an operand over the head's elements: lane's row lane % 16, elements 16 j + 4 (lane / 16) + i
 template <typename T, int DP>
@@ -131,8 +143,49 @@ __device__ __forceinline__ Range group_range(int lo, int hi, int* red) {
   return r;
 }
 
-// the last tiles first: the later rows of a long sequence have the most keys, and what starts last should be short
-__device__ __forceinline__ int tile_from_the_end(int tiles) { return tiles - 1 - static_cast<int>(blockIdx.x); }
+// what starts last should be short: the sorted order, or the last tiles, whose rows see the most keys of a long sequence, first
+__device__ __forceinline__ int query_tile(const AttnArgs& p, int tiles) {
+  return p.query_order ? p.query_order[blockIdx.x] : tiles - 1 - static_cast<int>(blockIdx.x);
+}
+
+// One workgroup: the work of every tile, then a counting sort into 256 classes of it, the largest first.  Tiles of a class come in
+// whatever order the counters give: it decides who starts when, not what is added to what.
+__global__ __launch_bounds__(1024) void sort_tiles_kernel(const AttnArgs p, int rows, int tiles, int32_t* query_order, int32_t* key_order) {
+  __shared__ int count[256], red[16], most;
+  int32_t* order = blockIdx.x ? key_order : query_order;
+  if (!order) return;
+  auto work = [&](int tile) {
+    const int first = tile * rows, last = min(first + rows, p.T) - 1;
+    int start, end, start2, end2;
+    sequence_of(p.cu, p.sequences, p.T, first, start, end);
+    sequence_of(p.cu, p.sequences, p.T, last, start2, end2);
+    if (blockIdx.x) return max(end2, last + 1) - first;
+    return last + 1 - (start < end ? start : first);
+  };
+  int top = 1;
+  for (int t = threadIdx.x; t < tiles; t += 1024) top = max(top, work(t));
+  top = wave_max_i(top);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
+  if (threadIdx.x < 256) count[threadIdx.x] = 0;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 16; ++i) top = max(top, red[i]);
+    most = top;
+  }
+  __syncthreads();
+  const float per = 255.0f / static_cast<float>(most);
+  auto class_of = [&](int tile) { return 255 - min(255, static_cast<int>(static_cast<float>(work(tile)) * per)); };
+  for (int t = threadIdx.x; t < tiles; t += 1024) atomicAdd(&count[class_of(t)], 1);
+  __syncthreads();
+  if (threadIdx.x < 64) {  // where each class begins: four classes a lane
+    int sum = 0, mine[4];
+    for (int i = 0; i < 4; ++i) mine[i] = count[4 * threadIdx.x + i], sum += mine[i];
+    int at = wave_scan(sum) - sum;
+    for (int i = 0; i < 4; ++i) count[4 * threadIdx.x + i] = at, at += mine[i];
+  }
+  __syncthreads();
+  for (int t = threadIdx.x; t < tiles; t += 1024) order[atomicAdd(&count[class_of(t)], 1)] = t;
+}
 
 template <typename T, int DP, int KW>
 __global__ __launch_bounds__(256) void any_forward_kernel(const AttnArgs p, int tiles, int vec) {
@@ -141,7 +194,7 @@ __global__ __launch_bounds__(256) void any_forward_kernel(const AttnArgs p, int 
   float *kt = lds, *vt = lds + KW * kStep * P, *stats = lds + 2 * KW * kStep * P;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int qw = wave / KW, kw = wave % KW, h = blockIdx.y, g = h / p.group;
-  const int row0 = tile_from_the_end(tiles) * 16 * QW, row = row0 + 16 * qw + (lane & 15);
+  const int row0 = query_tile(p, tiles) * 16 * QW, row = row0 + 16 * qw + (lane & 15);
   int start, end;
   sequence_of(p.cu, p.sequences, p.T, row, start, end);
   const bool on = start < end;
@@ -153,11 +206,18 @@ __global__ __launch_bounds__(256) void any_forward_kernel(const AttnArgs p, int 
 #pragma unroll
   for (int n = 0; n < NB; ++n) o[n] = f32x4{0, 0, 0, 0};
   float m = kNegInf, l = 0.0f;
+  Staged<T, DP, KW * kStep> keys, values;
+  auto fetch = [&](int k0) {
+    keys.fetch(static_cast<const T*>(p.k) + g * p.k_head, p.k_token, k0, p.T, p.D, vec);
+    values.fetch(static_cast<const T*>(p.v) + g * p.v_head, p.v_token, k0, p.T, p.D, vec);
+  };
+  if (all.lo < all.hi) fetch(all.lo);
   for (int k0 = all.lo; k0 < all.hi; k0 += KW * kStep) {
     __syncthreads();
-    fill_tile<T, DP, KW * kStep>(kt, static_cast<const T*>(p.k) + g * p.k_head, p.k_token, k0, p.T, p.D, vec);
-    fill_tile<T, DP, KW * kStep>(vt, static_cast<const T*>(p.v) + g * p.v_head, p.v_token, k0, p.T, p.D, vec);
-    __syncthreads();
+    keys.put(kt);
+    values.put(vt);
+    phase_barrier();  // (the next tile's loads stay under way across it)
+    if (k0 + KW * kStep < all.hi) fetch(k0 + KW * kStep);
     const int kb = k0 + kw * kStep;
     if (kb >= hi || kb + kStep <= lo) continue;
     f32x4 s[2];
@@ -191,6 +251,7 @@ __global__ __launch_bounds__(256) void any_forward_kernel(const AttnArgs p, int 
     columns_product<DP>(o, vt + (kw * kStep + 16) * P, s[1], lane);
   }
   l = column_sum(l);
+  const AttnArgs& z = late_arguments();
   // join the parts: [wave][16 rows][DP] of sums, [wave][16] of maxima and sums
   __syncthreads();
   float *sums = lds, *tops = stats, *lens = stats + 64;
@@ -203,33 +264,33 @@ __global__ __launch_bounds__(256) void any_forward_kernel(const AttnArgs p, int 
   // a wave writes the rows that it and its parts share: 16 / KW of them
   for (int i = 0; i < 16 / KW; ++i) {
     const int mine = kw * (16 / KW) + i, r = row0 + 16 * qw + mine;
-    if (r >= p.T) break;
+    if (r >= z.T) break;
     int first, last;
-    sequence_of(p.cu, p.sequences, p.T, r, first, last);
+    sequence_of(z.cu, z.sequences, z.T, r, first, last);
     float w[KW], best = kNegInf, len = 0.0f;
 #pragma unroll
     for (int part = 0; part < KW; ++part) best = fmaxf(best, tops[(qw * KW + part) * 16 + mine]);
-    const float ref = best == kNegInf ? 0.0f : best * p.c;
+    const float ref = best == kNegInf ? 0.0f : best * z.c;
 #pragma unroll
     for (int part = 0; part < KW; ++part) {
       const float t = tops[(qw * KW + part) * 16 + mine];
-      w[part] = t == kNegInf ? 0.0f : exp2_f32(t * p.c - ref);
+      w[part] = t == kNegInf ? 0.0f : exp2_f32(t * z.c - ref);
       len += w[part] * lens[(qw * KW + part) * 16 + mine];
       // a part without a finite score: 0 as above, unless its own sum is NaN already
       if (t == kNegInf && lens[(qw * KW + part) * 16 + mine] != 0.0f) len = NAN;
     }
     bool spoilt = false;
-    const int64_t dense = (static_cast<int64_t>(r) * p.H + h) * p.D;
-    for (int d = lane; d < p.D; d += kWave) {
+    const int64_t dense = (static_cast<int64_t>(r) * z.H + h) * z.D;
+    for (int d = lane; d < z.D; d += kWave) {
       float v = 0.0f;
 #pragma unroll
       for (int part = 0; part < KW; ++part) v += w[part] * sums[((qw * KW + part) * 16 + mine) * P + d];
       v /= len;
       spoilt |= v != v;
-      store_result<T>(p, dense + d, first < last ? v : 0.0f);
+      store_result<T>(z, dense + d, first < last ? v : 0.0f);
     }
-    if (lane == 0 && p.lse) p.lse[static_cast<int64_t>(h) * p.T + r] = first < last ? ref + log2f(len) : INFINITY;
-    if (first < last && __any(spoilt)) careful_forward_row<T>(p, h, r, first);
+    if (lane == 0 && z.lse) z.lse[static_cast<int64_t>(h) * z.T + r] = first < last ? ref + log2f(len) : INFINITY;
+    if (first < last && __any(spoilt)) careful_forward_row<T>(z, h, r, first);
   }
 }
 
@@ -241,7 +302,7 @@ __global__ __launch_bounds__(256) void any_dq_kernel(const AttnArgs p, int tiles
   float *kt = lds, *vt = lds + KW * kStep * P, *stats = lds + 2 * KW * kStep * P;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int qw = wave / KW, kw = wave % KW, h = blockIdx.y, g = h / p.group;
-  const int row0 = tile_from_the_end(tiles) * 16 * QW, row = row0 + 16 * qw + (lane & 15);
+  const int row0 = query_tile(p, tiles) * 16 * QW, row = row0 + 16 * qw + (lane & 15);
   int start, end;
   sequence_of(p.cu, p.sequences, p.T, row, start, end);
   const bool on = start < end;
@@ -268,11 +329,18 @@ __global__ __launch_bounds__(256) void any_dq_kernel(const AttnArgs p, int tiles
   f32x4 dq[NB];
 #pragma unroll
   for (int n = 0; n < NB; ++n) dq[n] = f32x4{0, 0, 0, 0};
+  Staged<T, DP, KW * kStep> keys, values;
+  auto fetch = [&](int k0) {
+    keys.fetch(static_cast<const T*>(p.k) + g * p.k_head, p.k_token, k0, p.T, p.D, vec);
+    values.fetch(static_cast<const T*>(p.v) + g * p.v_head, p.v_token, k0, p.T, p.D, vec);
+  };
+  if (all.lo < all.hi) fetch(all.lo);
   for (int k0 = all.lo; k0 < all.hi; k0 += KW * kStep) {
     __syncthreads();
-    fill_tile<T, DP, KW * kStep>(kt, static_cast<const T*>(p.k) + g * p.k_head, p.k_token, k0, p.T, p.D, vec);
-    fill_tile<T, DP, KW * kStep>(vt, static_cast<const T*>(p.v) + g * p.v_head, p.v_token, k0, p.T, p.D, vec);
-    __syncthreads();
+    keys.put(kt);
+    values.put(vt);
+    phase_barrier();  // (the next tile's loads stay under way across it)
+    if (k0 + KW * kStep < all.hi) fetch(k0 + KW * kStep);
     const int kb = k0 + kw * kStep;
     if (kb >= hi || kb + kStep <= lo) continue;
 #pragma unroll
@@ -290,6 +358,7 @@ __global__ __launch_bounds__(256) void any_dq_kernel(const AttnArgs p, int tiles
       columns_product<DP>(dq, kb_t, ds, lane);
     }
   }
+  const AttnArgs& z = late_arguments();
   __syncthreads();
   float *sums = lds, *lses = stats, *deltas = stats + 64;
 #pragma unroll
@@ -299,19 +368,19 @@ __global__ __launch_bounds__(256) void any_dq_kernel(const AttnArgs p, int tiles
   __syncthreads();
   for (int i = 0; i < 16 / KW; ++i) {
     const int mine = kw * (16 / KW) + i, r = row0 + 16 * qw + mine;
-    if (r >= p.T) break;
+    if (r >= z.T) break;
     int first, last;
-    sequence_of(p.cu, p.sequences, p.T, r, first, last);
+    sequence_of(z.cu, z.sequences, z.T, r, first, last);
     bool spoilt = false;
-    T* out = static_cast<T*>(p.dq) + (static_cast<int64_t>(r) * p.H + h) * p.D;
-    for (int d = lane; d < p.D; d += kWave) {
+    T* out = static_cast<T*>(z.dq) + (static_cast<int64_t>(r) * z.H + h) * z.D;
+    for (int d = lane; d < z.D; d += kWave) {
       float v = 0.0f;
 #pragma unroll
       for (int part = 0; part < KW; ++part) v += sums[((qw * KW + part) * 16 + mine) * P + d];
       spoilt |= v != v;
-      store_from_f32<T>(out + d, first < last ? v * p.scale : 0.0f);
+      store_from_f32<T>(out + d, first < last ? v * z.scale : 0.0f);
     }
-    if (first < last && __any(spoilt)) careful_dq_row<T>(p, h, r, first, lses[(qw * KW) * 16 + mine], deltas[(qw * KW) * 16 + mine]);
+    if (first < last && __any(spoilt)) careful_dq_row<T>(z, h, r, first, lses[(qw * KW) * 16 + mine], deltas[(qw * KW) * 16 + mine]);
   }
 }
 
@@ -325,7 +394,7 @@ __global__ __launch_bounds__(256) void any_dkv_kernel(const AttnArgs p, int vec)
   const int qw = wave / KW, kw = wave % KW;
   const int g = blockIdx.y / p.splits, split = blockIdx.y % p.splits;
   const int heads = (p.group + p.splits - 1) / p.splits, h0 = g * p.group + split * heads, h1 = min(h0 + heads, (g + 1) * p.group);
-  const int key0 = blockIdx.x * 16 * QW, key = key0 + 16 * qw + (lane & 15);
+  const int key0 = (p.key_order ? p.key_order[blockIdx.x] : static_cast<int>(blockIdx.x)) * 16 * QW, key = key0 + 16 * qw + (lane & 15);
   int start, end;
   sequence_of(p.cu, p.sequences, p.T, key, start, end);
   const bool on = start < end;
@@ -338,13 +407,21 @@ __global__ __launch_bounds__(256) void any_dkv_kernel(const AttnArgs p, int vec)
 #pragma unroll
   for (int n = 0; n < NB; ++n) dk[n] = dv[n] = f32x4{0, 0, 0, 0};
   const int64_t dense = static_cast<int64_t>(p.H) * p.D;
+  Staged<T, DP, KW * kStep> queries, grads;
+  auto fetch = [&](int h, int r0) {
+    queries.fetch(static_cast<const T*>(p.q) + h * p.q_head, p.q_token, r0, p.T, p.D, vec);
+    grads.fetch(static_cast<const T*>(p.dout) + h * p.D, dense, r0, p.T, p.D, vec);
+  };
+  if (all.lo < all.hi && h0 < h1) fetch(h0, all.lo);
   for (int h = h0; h < h1; ++h) {
     const float *lse = p.lse + static_cast<int64_t>(h) * p.T, *delta = p.delta + static_cast<int64_t>(h) * p.T;
     for (int r0 = all.lo; r0 < all.hi; r0 += KW * kStep) {
       __syncthreads();
-      fill_tile<T, DP, KW * kStep>(qt, static_cast<const T*>(p.q) + h * p.q_head, p.q_token, r0, p.T, p.D, vec);
-      fill_tile<T, DP, KW * kStep>(dt, static_cast<const T*>(p.dout) + h * p.D, dense, r0, p.T, p.D, vec);
-      __syncthreads();
+      queries.put(qt);
+      grads.put(dt);
+      phase_barrier();
+      if (r0 + KW * kStep < all.hi) fetch(h, r0 + KW * kStep);
+      else if (h + 1 < h1) fetch(h + 1, all.lo);
       const int rb = r0 + kw * kStep;
       if (rb >= hi || rb + kStep <= lo) continue;
 #pragma unroll
@@ -365,7 +442,8 @@ __global__ __launch_bounds__(256) void any_dkv_kernel(const AttnArgs p, int vec)
       }
     }
   }
-  const int64_t part0 = static_cast<int64_t>(split) * p.T * p.G * p.D;
+  const AttnArgs& z = late_arguments();
+  const int64_t part0 = static_cast<int64_t>(split) * z.T * z.G * z.D;
   bool spoilt[16 / KW];
 #pragma unroll
   for (int i = 0; i < 16 / KW; ++i) spoilt[i] = false;
@@ -379,19 +457,19 @@ __global__ __launch_bounds__(256) void any_dkv_kernel(const AttnArgs p, int vec)
 #pragma unroll
     for (int i = 0; i < 16 / KW; ++i) {
       const int mine = kw * (16 / KW) + i, r = key0 + 16 * qw + mine;
-      if (r >= p.T) continue;
+      if (r >= z.T) continue;
       int first, last;
-      sequence_of(p.cu, p.sequences, p.T, r, first, last);
-      const int64_t at = (static_cast<int64_t>(r) * p.G + g) * p.D;
+      sequence_of(z.cu, z.sequences, z.T, r, first, last);
+      const int64_t at = (static_cast<int64_t>(r) * z.G + g) * z.D;
       bool bad = false;
-      for (int d = lane; d < p.D; d += kWave) {
+      for (int d = lane; d < z.D; d += kWave) {
         float x = 0.0f;
 #pragma unroll
         for (int part = 0; part < KW; ++part) x += lds[((qw * KW + part) * 16 + mine) * P + d];
         bad |= x != x;
-        x = first < last ? (which ? x * p.scale : x) : 0.0f;
-        if (p.splits > 1) (which ? p.dk_part : p.dv_part)[part0 + at + d] = x;
-        else store_from_f32<T>(static_cast<T*>(which ? p.dk : p.dv) + at + d, x);
+        x = first < last ? (which ? x * z.scale : x) : 0.0f;
+        if (z.splits > 1) (which ? z.dk_part : z.dv_part)[part0 + at + d] = x;
+        else store_from_f32<T>(static_cast<T*>(which ? z.dk : z.dv) + at + d, x);
       }
       spoilt[i] |= first < last && __any(bad);
     }
@@ -401,30 +479,42 @@ __global__ __launch_bounds__(256) void any_dkv_kernel(const AttnArgs p, int vec)
     if (spoilt[i]) {
       const int r = key0 + 16 * qw + kw * (16 / KW) + i;
       int first, last;
-      sequence_of(p.cu, p.sequences, p.T, r, first, last);
-      careful_dkv_row<T>(p, g, r, last, h0, h1, split, 1.0f);
+      sequence_of(z.cu, z.sequences, z.T, r, first, last);
+      careful_dkv_row<T>(z, g, r, last, h0, h1, split, 1.0f);
     }
 }
 
-// dk and dv from their parts, added in order
-template <typename T>
+// dk and dv from their parts, added in order, four elements a lane (n is the number of fours, or of elements where they are no whole fours)
+template <typename T, int N>
 __global__ __launch_bounds__(256) void join_parts_kernel(const float* __restrict__ dk_part, const float* __restrict__ dv_part,
                                                          T* __restrict__ dk, T* __restrict__ dv, int splits, int64_t n) {
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (i >= n) return;
-  const float* part = blockIdx.y ? dv_part : dk_part;
-  float v = 0.0f;
-  for (int s = 0; s < splits; ++s) v += part[s * n + i];
-  store_from_f32<T>((blockIdx.y ? dv : dk) + i, v);
+  const float* part = (blockIdx.y ? dv_part : dk_part) + N * i;
+  T* out = (blockIdx.y ? dv : dk) + N * i;
+  if constexpr (N == 4) {
+    f32x4 v = {0, 0, 0, 0};
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s) v += __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(part + s * n * N));
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<f32x4*>(out) = v;
+    else *reinterpret_cast<u32x2*>(out) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+  } else {
+    float v = 0.0f;
+    for (int s = 0; s < splits; ++s) v += part[s * n];
+    store_from_f32<T>(out, v);
+  }
 }
 
+// the head's padded size and the parts of the other axis that go with it
 template <typename Fn>
 void with_head(int D, Fn f) {
-  if (D <= 64) f(std::integral_constant<int, 64>{});
-  else if (D <= 96) f(std::integral_constant<int, 96>{});
-  else if (D <= 128) f(std::integral_constant<int, 128>{});
-  else if (D <= 192) f(std::integral_constant<int, 192>{});
-  else f(std::integral_constant<int, 256>{});
+  const std::integral_constant<int, 1> one;
+  const std::integral_constant<int, 2> two;
+  if (D <= 64) f(std::integral_constant<int, 64>{}, two);
+  else if (D <= 96) f(std::integral_constant<int, 96>{}, two);
+  else if (D <= 128) f(std::integral_constant<int, 128>{}, two);
+  else if (D <= 192) f(std::integral_constant<int, 192>{}, one);  // (twice the rows a tile would take twice the registers for the next one)
+  else f(std::integral_constant<int, 256>{}, one);
 }
 
 bool in_fours(const AttnArgs& p, int item, bool backward) {
@@ -442,6 +532,10 @@ void allow_lds(K kernel, size_t bytes, PerDeviceOnce& once) {
 
 }  // namespace
 
+void attention_sort_tiles(const AttnArgs& p, int rows, int32_t* query_order, int32_t* key_order, hipStream_t s) {
+  hipLaunchKernelGGL(sort_tiles_kernel, dim3(2), dim3(1024), 0, s, p, rows, (p.T + rows - 1) / rows, query_order, key_order);
+}
+
 template <typename T, int DP, int KW>
 void any_forward(const AttnArgs& p, int vec, hipStream_t s) {
   static PerDeviceOnce once;
@@ -450,11 +544,13 @@ void any_forward(const AttnArgs& p, int vec, hipStream_t s) {
   hipLaunchKernelGGL((any_forward_kernel<T, DP, KW>), dim3(tiles, p.H), dim3(256), (kAnyLds<DP, KW>), s, p, tiles, vec);
 }
 
+int attention_any_rows(int D) { return D <= 128 ? 32 : 64; }
+
 void attention_any_forward(const AttnArgs& p, int dtype, hipStream_t s) {
   auto run = [&](auto tag) {
     using T = decltype(tag);
     const int vec = in_fours(p, sizeof(T), false);
-    with_head(p.D, [&](auto d) { any_forward<T, decltype(d)::value, 2>(p, vec, s); });
+    with_head(p.D, [&](auto d, auto parts) { any_forward<T, decltype(d)::value, decltype(parts)::value>(p, vec, s); });
   };
   if (dtype == MI355_F32) run(float{});
   else run(uint16_t{});
@@ -474,15 +570,20 @@ template <typename T>
 void join_parts(const AttnArgs& p, hipStream_t s) {
   if (p.splits <= 1) return;
   const int64_t n = static_cast<int64_t>(p.T) * p.G * p.D;
-  hipLaunchKernelGGL(join_parts_kernel<T>, dim3((unsigned)((n + 255) / 256), 2), dim3(256), 0, s, p.dk_part, p.dv_part,
-                     static_cast<T*>(p.dk), static_cast<T*>(p.dv), p.splits, n);
+  const bool fours = n % 4 == 0 && (reinterpret_cast<uintptr_t>(p.dk) | reinterpret_cast<uintptr_t>(p.dv)) % (4 * sizeof(T)) == 0;
+  auto launch = [&](auto kernel, int64_t items) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((items + 255) / 256), 2), dim3(256), 0, s, p.dk_part, p.dv_part, static_cast<T*>(p.dk),
+                       static_cast<T*>(p.dv), p.splits, items);
+  };
+  if (fours) launch(join_parts_kernel<T, 4>, n / 4);
+  else launch(join_parts_kernel<T, 1>, n);
 }
 
 void attention_any_backward(const AttnArgs& p, int dtype, hipStream_t s) {
   auto run = [&](auto tag) {
     using T = decltype(tag);
     const int vec = in_fours(p, sizeof(T), true);
-    with_head(p.D, [&](auto d) { any_backward<T, decltype(d)::value, 2>(p, vec, s); });
+    with_head(p.D, [&](auto d, auto parts) { any_backward<T, decltype(d)::value, decltype(parts)::value>(p, vec, s); });
   };
   if (dtype == MI355_F32) run(float{});
   else run(uint16_t{});
@@ -505,10 +606,12 @@ int check_attention(const char* what, int dtype, int64_t sequences, int64_t T, i
   return MI355_OK;
 }
 
-// Parts of a key head's group of query heads: as many as it takes for dk and dv to fill the card
+// Parts of a key head's group of query heads: as many as it takes to give every CU two workgroups, and up to four for shares that can be
+// evened out.  Parts cost a trip of dk and dv through memory in fp32.  Tiles of 128 keys, 32/4 heads of 128, us, dk/dv and joining the
+// parts: 8192 rows in 4 sequences 2 parts 398 + 20, 4 294 + 37, 8 322 + 89; 16384 in 11 1 1221, 2 692 + 49, 4 598 + 85.
 int head_parts(int64_t T, int64_t H, int64_t G) {
-  const int64_t group = H / G, tiles = (T + 63) / 64 * G;
-  int64_t parts = std::min<int64_t>(group, (1024 + tiles - 1) / std::max<int64_t>(tiles, 1));
+  const int64_t group = H / G, tiles = (T + 127) / 128 * G;
+  const int64_t parts = std::min(group, std::max((kHeldAtOnce + tiles - 1) / tiles, std::min<int64_t>(4, (2048 + tiles - 1) / tiles)));
   const int64_t heads = (group + parts - 1) / parts;
   return (int)((group + heads - 1) / heads);
 }
@@ -530,23 +633,34 @@ AttnArgs attention_args(const void* q, int64_t q_token, int64_t q_head, const vo
 extern "C" int mi355_varlen_attention_fwd(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
                                           int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
                                           int64_t v_head_stride, int dtype, const int32_t* cu_seqlens, int64_t sequences, float scale,
-                                          void* out, void* out_rest, float* lse, int64_t T, int64_t H, int64_t G, int64_t D,
-                                          void* stream) {
+                                          void* out, void* out_rest, float* lse, void* workspace, int64_t T, int64_t H,
+                                          int64_t G, int64_t D, void* stream) {
   if (int rc = check_attention("varlen_attention_fwd", dtype, sequences, T, H, G, D, scale)) return rc;
   if (T == 0) return MI355_OK;
   MI355_REQUIRE(q && k && v && cu_seqlens && out, "varlen_attention_fwd: null pointer");
   AttnArgs p = attention_args(q, q_token_stride, q_head_stride, k, k_token_stride, k_head_stride, v, v_token_stride, v_head_stride,
                               cu_seqlens, sequences, scale, T, H, G, D);
   p.out = out, p.lse = lse, p.rest = dtype == MI355_BF16 ? out_rest : nullptr;
-  if (dtype == MI355_BF16 && attention_bf16_covers(p)) attention_bf16_forward(p, as_stream(stream));
+  const bool matrix = dtype == MI355_BF16 && attention_bf16_covers(p);
+  const int rows = matrix ? attention_bf16_rows() : attention_any_rows(p.D);
+  if (workspace && sorted_tiles(p.sequences, T, (T + rows - 1) / rows, H)) {
+    attention_sort_tiles(p, rows, static_cast<int32_t*>(workspace), nullptr, as_stream(stream));
+    p.query_order = static_cast<int32_t*>(workspace);
+  }
+  if (matrix) attention_bf16_forward(p, as_stream(stream));
   else attention_any_forward(p, dtype, as_stream(stream));
   return check_launch("varlen_attention_fwd");
 }
 
+extern "C" int64_t mi355_varlen_attention_fwd_workspace_bytes(int64_t T, int64_t H, int64_t sequences) {
+  const int64_t tiles = (T + kLeastRows - 1) / kLeastRows;  // (the most there can be)
+  return T > 0 && sorted_tiles(sequences, T, tiles, H) ? 4 * tiles : 0;
+}
+
 extern "C" int64_t mi355_varlen_attention_bwd_workspace_bytes(int64_t T, int64_t H, int64_t G, int64_t D) {
   if (T < 1 || H < 1 || G < 1 || H % G || D < 1) return 0;
-  const int64_t parts = head_parts(T, H, G);
-  return 4 * ((2 * H * T + 3) / 4 * 4 + (parts > 1 ? 2 * parts * T * G * D : 0));
+  const int64_t parts = head_parts(T, H, G), tiles = (T + kLeastRows - 1) / kLeastRows;
+  return 4 * ((2 * H * T + 3) / 4 * 4 + (2 * tiles + 3) / 4 * 4 + (parts > 1 ? 2 * parts * T * G * D : 0));
 }
 
 extern "C" int mi355_varlen_attention_bwd(const void* dout, const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
@@ -564,9 +678,17 @@ extern "C" int mi355_varlen_attention_bwd(const void* dout, const void* q, int64
   p.dout = dout, p.lse = const_cast<float*>(lse), p.dq = dq, p.dk = dk, p.dv = dv;
   p.splits = head_parts(T, H, G);
   p.delta = static_cast<float*>(workspace);
-  p.dk_part = p.delta + (2 * H * T + 3) / 4 * 4;
+  const int64_t most_tiles = (T + kLeastRows - 1) / kLeastRows;
+  int32_t* order = reinterpret_cast<int32_t*>(p.delta + (2 * H * T + 3) / 4 * 4);
+  p.dk_part = reinterpret_cast<float*>(order + (2 * most_tiles + 3) / 4 * 4);
   p.dv_part = p.dk_part + static_cast<int64_t>(p.splits) * T * G * D;
-  if (dtype == MI355_BF16 && attention_bf16_covers(p)) attention_bf16_backward(p, as_stream(stream));
+  const bool matrix = dtype == MI355_BF16 && attention_bf16_covers(p);
+  const int rows = matrix ? attention_bf16_rows() : attention_any_rows(p.D);
+  if (sorted_tiles(p.sequences, T, (T + rows - 1) / rows, H)) {
+    attention_sort_tiles(p, rows, order, order + most_tiles, as_stream(stream));
+    p.query_order = order, p.key_order = order + most_tiles;
+  }
+  if (matrix) attention_bf16_backward(p, as_stream(stream));
   else attention_any_backward(p, dtype, as_stream(stream));
   if (dtype == MI355_F32) join_parts<float>(p, as_stream(stream));
   else join_parts<uint16_t>(p, as_stream(stream));

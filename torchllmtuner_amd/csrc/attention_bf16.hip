@@ -171,18 +171,20 @@ __device__ __forceinline__ u32x4 pack8(const float (&v)[8]) {
 struct Place {
   int head, tile;
 };
-// Workgroup b runs on XCD b % 8.  Heads that share keys go to one XCD, whose L2 then holds them once; the last tiles, which see the most
-// keys, start first, so that what starts last is short.
-__device__ __forceinline__ Place place_of(int block, int heads, int tiles) {
+// Workgroup b runs on XCD b % 8.  Heads that share keys go to one XCD, whose L2 then holds them once; tiles in their sorted order, or
+// as they lie, `last` first.
+__device__ __forceinline__ Place place_of(int block, int heads, int tiles, const int32_t* order, bool last) {
   Place w;
+  int rank;
   if (heads % 8 == 0) {
     const int each = heads / 8, j = block >> 3;
     w.head = (block & 7) * each + j % each;
-    w.tile = tiles - 1 - j / each;
+    rank = j / each;
   } else {
     w.head = block % heads;
-    w.tile = tiles - 1 - block / heads;
+    rank = block / heads;
   }
+  w.tile = order ? order[rank] : last ? tiles - 1 - rank : rank;
   return w;
 }
 
@@ -209,7 +211,7 @@ __global__ __launch_bounds__(256, 2) void bf16_forward_kernel(const AttnArgs p, 
   extern __shared__ __attribute__((aligned(16))) uint16_t smem[];
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_cptr)smem));
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-  const Place at = place_of(blockIdx.x, p.H, tiles);
+  const Place at = place_of(blockIdx.x, p.H, tiles, p.query_order, true);
   const int h = at.head, g = h / p.group;
   const int row0 = at.tile * 4 * kRows + wave * kRows, row = row0 + (lane & 31);
   int start, end;
@@ -346,7 +348,7 @@ __global__ __launch_bounds__(256, 2) void bf16_dq_kernel(const AttnArgs p, int t
   extern __shared__ __attribute__((aligned(16))) uint16_t smem[];
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_cptr)smem));
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-  const Place at = place_of(blockIdx.x, p.H, tiles);
+  const Place at = place_of(blockIdx.x, p.H, tiles, p.query_order, true);
   const int h = at.head, g = h / p.group;
   const int row0 = at.tile * 4 * kRows + wave * kRows, row = row0 + (lane & 31);
   int start, end;
@@ -477,10 +479,10 @@ __global__ __launch_bounds__(256, 2) void bf16_dkv_kernel(const AttnArgs p, int 
   extern __shared__ __attribute__((aligned(16))) uint16_t smem[];
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_cptr)smem));
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-  const Place at = place_of(blockIdx.x, p.G * p.splits, tiles);
+  const Place at = place_of(blockIdx.x, p.G * p.splits, tiles, p.key_order, false);
   const int g = at.head / p.splits, split = at.head % p.splits;
   const int heads = (p.group + p.splits - 1) / p.splits, h0 = g * p.group + split * heads, h1 = min(h0 + heads, (g + 1) * p.group);
-  const int key0 = (tiles - 1 - at.tile) * 4 * kRows + wave * kRows, key = key0 + (lane & 31);  // the first keys are seen by the most rows
+  const int key0 = at.tile * 4 * kRows + wave * kRows, key = key0 + (lane & 31);
   int start, end;
   sequence_of(p.cu, p.sequences, p.T, key, start, end);
   const bool on = start < end;
@@ -664,6 +666,8 @@ bool attention_bf16_covers(const AttnArgs& p) {
   return p.D <= 128 && bits % 16 == 0 && sizes % 8 == 0 && reach < (1 << 22) &&
          static_cast<int64_t>((p.T + 127) / 128) * p.H < (1ll << 31);
 }
+
+int attention_bf16_rows() { return 4 * kRows; }
 
 void attention_bf16_forward(const AttnArgs& p, hipStream_t s) {
   if (p.D <= 64) forward<64>(p, s);

@@ -308,9 +308,11 @@ std::tuple<Tensor, Tensor, Tensor> varlen_attention_fwd(const Tensor& q_, const 
   const Tensor cu = cu_.contiguous();
   Tensor out = at::empty(q_.sizes(), q_.options()), lse = at::empty({q.heads, q.tokens}, q_.options().dtype(at::kFloat));
   Tensor rest = for_backward && q_.scalar_type() == at::kBFloat16 ? at::empty_like(out) : none_like(out);
+  Tensor ws;
+  if (const int64_t need = mi355_varlen_attention_fwd_workspace_bytes(q.tokens, q.heads, cu.numel() - 1)) ws = bytes(need, q_);
   check(mi355_varlen_attention_fwd(ptr(q.t), q.token_stride, q.head_stride, ptr(k.t), k.token_stride, k.head_stride, ptr(v.t),
                                    v.token_stride, v.head_stride, dtype_code(q.t), iptr(cu), cu.numel() - 1, (float)scale, ptr(out),
-                                   ptr(rest), static_cast<float*>(ptr(lse)), q.tokens, q.heads, k.heads, q.size, L.stream),
+                                   ptr(rest), static_cast<float*>(ptr(lse)), ptr(ws), q.tokens, q.heads, k.heads, q.size, L.stream),
         "varlen_attention_fwd");
   return {out, lse, rest};
 }
