@@ -66,6 +66,41 @@ __device__ __forceinline__ void sequence_of(const int32_t* cu, int sequences, in
   end = min(cu[a], T);
 }
 
+// Order of a stretch of code, N times: a matrix instruction, READS reads of LDS, VALU vector instructions
+template <int N, int READS, int VALU>
+__device__ __forceinline__ void interleave() {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    if (READS) __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+    if (VALU) __builtin_amdgcn_sched_group_barrier(0x002, VALU, 0);
+  }
+}
+template <int READS>
+__device__ __forceinline__ void reads_first() {
+  __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+}
+
+struct Place {
+  int head, tile;
+};
+// Workgroup b runs on XCD b % 8.  Heads that share keys go to one XCD, whose L2 then holds them once; tiles in their sorted order, or
+// as they lie, `last` first.
+__device__ __forceinline__ Place place_of(int block, int heads, int tiles, const int32_t* order, bool last) {
+  Place w;
+  int rank;
+  if (heads % 8 == 0) {
+    const int each = heads / 8, j = block >> 3;
+    w.head = (block & 7) * each + j % each;
+    rank = j / each;
+  } else {
+    w.head = block % heads;
+    rank = block / heads;
+  }
+  w.tile = order ? order[rank] : last ? tiles - 1 - rank : rank;
+  return w;
+}
+
 __device__ __forceinline__ float exp2_f32(float x) { return __builtin_amdgcn_exp2f(x); }
 
 template <typename T>
@@ -202,7 +237,7 @@ __device__ __forceinline__ void careful_dkv_row(const AttnArgs& p, int g, int ke
 constexpr int kHeldAtOnce = 512;     // workgroups: two a CU
 constexpr int kLongOnAverage = 512;  // rows a sequence: below, a tile's work differs by less than the sorting costs
 inline bool sorted_tiles(int64_t sequences, int64_t T, int64_t tiles, int64_t heads) {
-  return sequences > 1 && T >= kLongOnAverage * sequences && tiles * heads > kHeldAtOnce;
+  return sequences > 1 && T >= kLongOnAverage * sequences && tiles * heads > kHeldAtOnce / 2;
 }
 // order[i]: the i-th tile of `rows` rows to start
 void attention_sort_tiles(const AttnArgs& p, int rows, int32_t* query_order, int32_t* key_order, hipStream_t s);

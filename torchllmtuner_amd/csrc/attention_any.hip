@@ -23,6 +23,8 @@
 namespace mi355 {
 namespace {
 
+constexpr uint32_t kFar = 1u << 30;  // an offset past every buffer: reads zeros
+
 template <typename T>
 __device__ __forceinline__ float4 four_at(const T* p, int n, bool vec) {  // the first n of p[0..3], zeros behind them
   if (vec) {
@@ -47,11 +49,29 @@ struct Staged {
   static_assert(ROWS * QUADS % 256 == 0, "whole rounds of the workgroup");
   float4 x[EACH];
   __device__ __forceinline__ void fetch(const T* base, int64_t token, int row0, int T_, int D, bool vec) {
+    if (vec) {  // from a buffer that ends with the last row: zeros behind it, and no branch a request
+      const int64_t left = (static_cast<int64_t>(T_ - 1 - row0) * token + D) * sizeof(T);
+      const uint32_t bytes = left < 0 ? 0 : left < kFar ? static_cast<uint32_t>(left) : kFar;
+      const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base) + static_cast<int64_t>(row0) * token, 0, bytes, 0x00020000);
+#pragma unroll
+      for (int n = 0; n < EACH; ++n) {
+        const int i = threadIdx.x + 256 * n, d = (i % QUADS) * 4;
+        const uint32_t at = d < D ? (static_cast<uint32_t>(i / QUADS) * static_cast<uint32_t>(token) + d) * sizeof(T) : kFar;
+        if constexpr (sizeof(T) == 4) {
+          x[n] = __builtin_bit_cast(float4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, at, 0, 0));
+        } else {
+          const auto q = __builtin_amdgcn_raw_buffer_load_b64(rsrc, at, 0, 0);
+          x[n] = make_float4(__uint_as_float(q[0] << 16), __uint_as_float(q[0] & 0xffff0000u), __uint_as_float(q[1] << 16),
+                             __uint_as_float(q[1] & 0xffff0000u));
+        }
+      }
+      return;
+    }
 #pragma unroll
     for (int n = 0; n < EACH; ++n) {
       const int i = threadIdx.x + 256 * n, r = row0 + i / QUADS, d = (i % QUADS) * 4;
       x[n] = make_float4(0, 0, 0, 0);
-      if (r < T_ && d < D) x[n] = four_at<T>(base + static_cast<int64_t>(r) * token + d, D - d, vec && d + 4 <= D);
+      if (r < T_ && d < D) x[n] = four_at<T>(base + static_cast<int64_t>(r) * token + d, D - d, false);
     }
   }
   __device__ __forceinline__ void put(float* tile) const {
@@ -89,6 +109,14 @@ __device__ __forceinline__ f32x4 rows_product(const float* tile, const float (&x
     s = __builtin_amdgcn_mfma_f32_16x16x4f32(v.z, x[4 * j + 2], s, 0, 0, 0);
     s = __builtin_amdgcn_mfma_f32_16x16x4f32(v.w, x[4 * j + 3], s, 0, 0, 0);
   }
+  // two reads of 16 bytes ahead of the matrix instructions
+  reads_first<2>();
+#pragma unroll
+  for (int j = 0; j < DP / 16 - 2; ++j) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+    reads_first<1>();
+  }
+  __builtin_amdgcn_sched_group_barrier(0x008, 8, 0);
   return s;
 }
 
@@ -101,6 +129,9 @@ __device__ __forceinline__ void columns_product(f32x4 (&acc)[DP / 16], const flo
   for (int n = 0; n < DP / 16; ++n)
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i * P + 16 * n], w[i], acc[n], 0, 0, 0);
+  reads_first<6>();  // (of 4 bytes a lane)
+  interleave<DP / 4 - 6, 1, 0>();
+  interleave<6, 0, 0>();
 }
 
 // over the four lane groups that hold a column
@@ -141,11 +172,6 @@ __device__ __forceinline__ Range group_range(int lo, int hi, int* red) {
   r.lo = __builtin_amdgcn_readfirstlane(r.lo);
   r.hi = __builtin_amdgcn_readfirstlane(r.hi);
   return r;
-}
-
-// what starts last should be short: the sorted order, or the last tiles, whose rows see the most keys of a long sequence, first
-__device__ __forceinline__ int query_tile(const AttnArgs& p, int tiles) {
-  return p.query_order ? p.query_order[blockIdx.x] : tiles - 1 - static_cast<int>(blockIdx.x);
 }
 
 // One workgroup: the work of every tile, then a counting sort into 256 classes of it, the largest first.  Tiles of a class come in
@@ -193,8 +219,9 @@ __global__ __launch_bounds__(256) void any_forward_kernel(const AttnArgs p, int 
   extern __shared__ __attribute__((aligned(16))) float lds[];
   float *kt = lds, *vt = lds + KW * kStep * P, *stats = lds + 2 * KW * kStep * P;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int qw = wave / KW, kw = wave % KW, h = blockIdx.y, g = h / p.group;
-  const int row0 = query_tile(p, tiles) * 16 * QW, row = row0 + 16 * qw + (lane & 15);
+  const Place at = place_of(blockIdx.x, p.H, tiles, p.query_order, true);
+  const int qw = wave / KW, kw = wave % KW, h = at.head, g = h / p.group;
+  const int row0 = at.tile * 16 * QW, row = row0 + 16 * qw + (lane & 15);
   int start, end;
   sequence_of(p.cu, p.sequences, p.T, row, start, end);
   const bool on = start < end;
@@ -301,8 +328,9 @@ __global__ __launch_bounds__(256) void any_dq_kernel(const AttnArgs p, int tiles
   extern __shared__ __attribute__((aligned(16))) float lds[];
   float *kt = lds, *vt = lds + KW * kStep * P, *stats = lds + 2 * KW * kStep * P;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int qw = wave / KW, kw = wave % KW, h = blockIdx.y, g = h / p.group;
-  const int row0 = query_tile(p, tiles) * 16 * QW, row = row0 + 16 * qw + (lane & 15);
+  const Place at = place_of(blockIdx.x, p.H, tiles, p.query_order, true);
+  const int qw = wave / KW, kw = wave % KW, h = at.head, g = h / p.group;
+  const int row0 = at.tile * 16 * QW, row = row0 + 16 * qw + (lane & 15);
   int start, end;
   sequence_of(p.cu, p.sequences, p.T, row, start, end);
   const bool on = start < end;
@@ -386,15 +414,16 @@ __global__ __launch_bounds__(256) void any_dq_kernel(const AttnArgs p, int tiles
 
 // dk and dv: a wave's 16 keys against the query heads of their group, or a part of them
 template <typename T, int DP, int KW>
-__global__ __launch_bounds__(256) void any_dkv_kernel(const AttnArgs p, int vec) {
+__global__ __launch_bounds__(256) void any_dkv_kernel(const AttnArgs p, int tiles, int vec) {
   constexpr int QW = 4 / KW, P = DP + 4, NB = DP / 16;
   extern __shared__ __attribute__((aligned(16))) float lds[];
   float *qt = lds, *dt = lds + KW * kStep * P, *stats = lds + 2 * KW * kStep * P;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int qw = wave / KW, kw = wave % KW;
-  const int g = blockIdx.y / p.splits, split = blockIdx.y % p.splits;
+  const Place at = place_of(blockIdx.x, p.G * p.splits, tiles, p.key_order, false);
+  const int g = at.head / p.splits, split = at.head % p.splits;
   const int heads = (p.group + p.splits - 1) / p.splits, h0 = g * p.group + split * heads, h1 = min(h0 + heads, (g + 1) * p.group);
-  const int key0 = (p.key_order ? p.key_order[blockIdx.x] : static_cast<int>(blockIdx.x)) * 16 * QW, key = key0 + 16 * qw + (lane & 15);
+  const int key0 = at.tile * 16 * QW, key = key0 + 16 * qw + (lane & 15);
   int start, end;
   sequence_of(p.cu, p.sequences, p.T, key, start, end);
   const bool on = start < end;
@@ -520,7 +549,9 @@ void with_head(int D, Fn f) {
 bool in_fours(const AttnArgs& p, int item, bool backward) {
   uintptr_t bits = reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v);
   if (backward) bits |= reinterpret_cast<uintptr_t>(p.o) | reinterpret_cast<uintptr_t>(p.rest) | reinterpret_cast<uintptr_t>(p.dout);
-  return bits % (4 * item) == 0 && (p.q_token | p.q_head | p.k_token | p.k_head | p.v_token | p.v_head | p.D) % 4 == 0;
+  // (a tile's rows lie within 32-bit offsets of its first one)
+  const int64_t reach = std::max(std::max(p.q_token, p.k_token), std::max<int64_t>(p.v_token, static_cast<int64_t>(p.H) * p.D));
+  return bits % (4 * item) == 0 && reach < (1 << 20) && (p.q_token | p.q_head | p.k_token | p.k_head | p.v_token | p.v_head | p.D) % 4 == 0;
 }
 
 template <typename K>
@@ -541,7 +572,7 @@ void any_forward(const AttnArgs& p, int vec, hipStream_t s) {
   static PerDeviceOnce once;
   allow_lds(any_forward_kernel<T, DP, KW>, kAnyLds<DP, KW>, once);
   const int rows = 64 / KW, tiles = (p.T + rows - 1) / rows;
-  hipLaunchKernelGGL((any_forward_kernel<T, DP, KW>), dim3(tiles, p.H), dim3(256), (kAnyLds<DP, KW>), s, p, tiles, vec);
+  hipLaunchKernelGGL((any_forward_kernel<T, DP, KW>), dim3(tiles * p.H), dim3(256), (kAnyLds<DP, KW>), s, p, tiles, vec);
 }
 
 int attention_any_rows(int D) { return D <= 128 ? 32 : 64; }
@@ -562,8 +593,8 @@ void any_backward(const AttnArgs& p, int vec, hipStream_t s) {
   allow_lds(any_dq_kernel<T, DP, KW>, kAnyLds<DP, KW>, once_q);
   allow_lds(any_dkv_kernel<T, DP, KW>, kAnyLds<DP, KW>, once_kv);
   const int rows = 64 / KW, tiles = (p.T + rows - 1) / rows;
-  hipLaunchKernelGGL((any_dq_kernel<T, DP, KW>), dim3(tiles, p.H), dim3(256), (kAnyLds<DP, KW>), s, p, tiles, vec);
-  hipLaunchKernelGGL((any_dkv_kernel<T, DP, KW>), dim3(tiles, p.G * p.splits), dim3(256), (kAnyLds<DP, KW>), s, p, vec);
+  hipLaunchKernelGGL((any_dq_kernel<T, DP, KW>), dim3(tiles * p.H), dim3(256), (kAnyLds<DP, KW>), s, p, tiles, vec);
+  hipLaunchKernelGGL((any_dkv_kernel<T, DP, KW>), dim3(tiles * p.G * p.splits), dim3(256), (kAnyLds<DP, KW>), s, p, tiles, vec);
 }
 
 template <typename T>
@@ -601,6 +632,8 @@ int check_attention(const char* what, int dtype, int64_t sequences, int64_t T, i
                 (long long)T, (long long)sequences);
   MI355_REQUIRE(H >= 1 && G >= 1 && H <= 65535 && H % G == 0, "%s: %lld query heads are no multiple of %lld key heads", what,
                 (long long)H, (long long)G);
+  MI355_REQUIRE((T + kLeastRows - 1) / kLeastRows * H < (1ll << 31), "%s: %lld tokens of %lld heads are too many for one launch", what, (long long)T,
+                (long long)H);
   MI355_REQUIRE(D >= 1 && D <= kHeadMax, "%s: head size %lld is not within 1 to %d", what, (long long)D, kHeadMax);
   MI355_REQUIRE(std::isfinite(scale) && scale > 0.0f, "%s: the scale must be finite and positive", what);
   return MI355_OK;

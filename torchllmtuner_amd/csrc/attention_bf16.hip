@@ -102,21 +102,6 @@ __device__ __forceinline__ void settle(bf16x8 (&x)[N]) {
   for (int i = 0; i < N; ++i) asm volatile("" : "+v"(x[i]));
 }
 
-// Order of a stretch of code, N times: a matrix instruction, READS reads of LDS, VALU vector instructions
-template <int N, int READS, int VALU>
-__device__ __forceinline__ void interleave() {
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-    if (READS) __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
-    if (VALU) __builtin_amdgcn_sched_group_barrier(0x002, VALU, 0);
-  }
-}
-template <int READS>
-__device__ __forceinline__ void reads_first() {
-  __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
-}
-
 __device__ __forceinline__ f32x16 mfma(const bf16x8& a, const bf16x8& b, const f32x16& c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
@@ -166,26 +151,6 @@ __device__ __forceinline__ void eight_of(const f32x16& o, int a, float (&v)[8]) 
 }
 __device__ __forceinline__ u32x4 pack8(const float (&v)[8]) {
   return u32x4{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
-}
-
-struct Place {
-  int head, tile;
-};
-// Workgroup b runs on XCD b % 8.  Heads that share keys go to one XCD, whose L2 then holds them once; tiles in their sorted order, or
-// as they lie, `last` first.
-__device__ __forceinline__ Place place_of(int block, int heads, int tiles, const int32_t* order, bool last) {
-  Place w;
-  int rank;
-  if (heads % 8 == 0) {
-    const int each = heads / 8, j = block >> 3;
-    w.head = (block & 7) * each + j % each;
-    rank = j / each;
-  } else {
-    w.head = block % heads;
-    rank = block / heads;
-  }
-  w.tile = order ? order[rank] : last ? tiles - 1 - rank : rank;
-  return w;
 }
 
 // the workgroup's range over the other axis and the wave's, from every lane's row's
@@ -663,8 +628,7 @@ bool attention_bf16_covers(const AttnArgs& p) {
   const int64_t sizes = p.D | p.q_token | p.q_head | p.k_token | p.k_head | p.v_token | p.v_head;
   // a tile's rows lie within 32-bit offsets of its first one
   const int64_t reach = std::max(std::max(p.q_token, p.k_token), std::max<int64_t>(p.v_token, static_cast<int64_t>(p.H) * p.D));
-  return p.D <= 128 && bits % 16 == 0 && sizes % 8 == 0 && reach < (1 << 22) &&
-         static_cast<int64_t>((p.T + 127) / 128) * p.H < (1ll << 31);
+  return p.D <= 128 && bits % 16 == 0 && sizes % 8 == 0 && reach < (1 << 22);
 }
 
 int attention_bf16_rows() { return 4 * kRows; }
