@@ -292,8 +292,7 @@ __global__ __launch_bounds__(256) void any_forward_kernel(const AttnArgs p, int 
   for (int i = 0; i < 16 / KW; ++i) {
     const int mine = kw * (16 / KW) + i, r = row0 + 16 * qw + mine;
     if (r >= z.T) break;
-    int first, last;
-    sequence_of(z.cu, z.sequences, z.T, r, first, last);
+    const int first = __builtin_amdgcn_readlane(start, mine), last = __builtin_amdgcn_readlane(end, mine);
     float w[KW], best = kNegInf, len = 0.0f;
 #pragma unroll
     for (int part = 0; part < KW; ++part) best = fmaxf(best, tops[(qw * KW + part) * 16 + mine]);
@@ -397,8 +396,7 @@ __global__ __launch_bounds__(256) void any_dq_kernel(const AttnArgs p, int tiles
   for (int i = 0; i < 16 / KW; ++i) {
     const int mine = kw * (16 / KW) + i, r = row0 + 16 * qw + mine;
     if (r >= z.T) break;
-    int first, last;
-    sequence_of(z.cu, z.sequences, z.T, r, first, last);
+    const int first = __builtin_amdgcn_readlane(start, mine), last = __builtin_amdgcn_readlane(end, mine);
     bool spoilt = false;
     T* out = static_cast<T*>(z.dq) + (static_cast<int64_t>(r) * z.H + h) * z.D;
     for (int d = lane; d < z.D; d += kWave) {
@@ -487,8 +485,7 @@ __global__ __launch_bounds__(256) void any_dkv_kernel(const AttnArgs p, int tile
     for (int i = 0; i < 16 / KW; ++i) {
       const int mine = kw * (16 / KW) + i, r = key0 + 16 * qw + mine;
       if (r >= z.T) continue;
-      int first, last;
-      sequence_of(z.cu, z.sequences, z.T, r, first, last);
+      const int first = __builtin_amdgcn_readlane(start, mine), last = __builtin_amdgcn_readlane(end, mine);
       const int64_t at = (static_cast<int64_t>(r) * z.G + g) * z.D;
       bool bad = false;
       for (int d = lane; d < z.D; d += kWave) {
@@ -506,9 +503,8 @@ __global__ __launch_bounds__(256) void any_dkv_kernel(const AttnArgs p, int tile
 #pragma unroll
   for (int i = 0; i < 16 / KW; ++i)
     if (spoilt[i]) {
-      const int r = key0 + 16 * qw + kw * (16 / KW) + i;
-      int first, last;
-      sequence_of(z.cu, z.sequences, z.T, r, first, last);
+      const int mine = kw * (16 / KW) + i, r = key0 + 16 * qw + mine;
+      const int first = __builtin_amdgcn_readlane(start, mine), last = __builtin_amdgcn_readlane(end, mine);
       careful_dkv_row<T>(z, g, r, last, h0, h1, split, 1.0f);
     }
 }
