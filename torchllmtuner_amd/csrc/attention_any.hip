@@ -129,9 +129,11 @@ __device__ __forceinline__ void columns_product(f32x4 (&acc)[DP / 16], const flo
   for (int n = 0; n < DP / 16; ++n)
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i * P + 16 * n], w[i], acc[n], 0, 0, 0);
-  reads_first<6>();  // (of 4 bytes a lane)
-  interleave<DP / 4 - 6, 1, 0>();
-  interleave<6, 0, 0>();
+  if constexpr (DP <= 192) {  // (larger heads have no registers for it)
+    reads_first<6>();  // (of 4 bytes a lane)
+    interleave<DP / 4 - 6, 1, 0>();
+    interleave<6, 0, 0>();
+  }
 }
 
 // over the four lane groups that hold a column

@@ -165,7 +165,7 @@ __device__ __forceinline__ void item_at(int i, int pairs, int& a, int& b, bool& 
 }
 
 template <typename T, int N, int ITER, bool INTER, int MODE>
-__global__ __launch_bounds__(256) void qk_rotary_kernel(const QkArgs p) {
+__global__ __launch_bounds__(256, MODE == kNormTurnBwd ? 4 : 1) void qk_rotary_kernel(const QkArgs p) {
   __shared__ float trig[4][2][kMaxPairs];
   extern __shared__ float dw_sum[];  // kNormTurnBwd: [4][2][D]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -365,30 +365,32 @@ __global__ __launch_bounds__(256) void qk_rotary_kernel(const QkArgs p) {
   }
 }
 
-// dw[d] = sum of the workgroups' partial sums: 16 columns x 16 slices a workgroup, the slices added in order
+// dw[d] = sum of the workgroups' partial sums: 16 columns x 64 slices a workgroup, the slices added in order
 template <typename T>
-__global__ __launch_bounds__(256) void qk_dw_final_kernel(const float* __restrict__ partial, T* __restrict__ dwq,
-                                                          T* __restrict__ dwk, int blocks, int D) {
-  __shared__ float part[16][17];
+__global__ __launch_bounds__(1024) void qk_dw_final_kernel(const float* __restrict__ partial, T* __restrict__ dwq,
+                                                           T* __restrict__ dwk, int blocks, int D) {
+  __shared__ float part[64][17];
   const int col = threadIdx.x & 15, slice = threadIdx.x >> 4;
   const int d = blockIdx.x * 16 + col;
   float acc = 0.0f;
   if (d < 2 * D) {
 #pragma unroll 8
-    for (int b = slice; b < blocks; b += 16) acc += partial[static_cast<int64_t>(b) * 2 * D + d];
+    for (int b = slice; b < blocks; b += 64) acc += partial[static_cast<int64_t>(b) * 2 * D + d];
   }
   part[slice][col] = acc;
   __syncthreads();
   if (slice == 0 && d < 2 * D) {
     float total = 0.0f;
 #pragma unroll
-    for (int k = 0; k < 16; ++k) total += part[k][col];
+    for (int k = 0; k < 64; ++k) total += part[k][col];
     T* out = d < D ? dwq : dwk;
     if (out) store_from_f32(out + (d < D ? d : d - D), total);
   }
 }
 
-constexpr int kBwdBlocks = 1024;  // workgroups of the backward with the norm, at most: rows of partial sums
+// Workgroups of the backward with the norm, at most: rows of partial sums, and as many as the card holds at once, four waves a SIMD (with 133 registers
+// instead of 128, three, the last quarter waited for the others: 60 us where it is 47 now, 8192 tokens x 36 heads of 128, 4.8 TB/s).
+constexpr int kBwdBlocks = 1024;
 
 // the most elements (16 bytes' worth down to 1) that every piece is a whole number of and starts on
 int piece_of(const QkArgs& p, int dtype, std::initializer_list<const void*> ptrs) {
@@ -419,9 +421,11 @@ int launch_qk(const char* what, QkArgs p, int dtype, int interleaved, int64_t bl
   p.lanes = 1, p.log_lanes = 0;
   while (p.lanes < p.items && p.lanes < kWave) p.lanes *= 2, ++p.log_lanes;
   const int heads_pass = kWave / p.lanes, passes = (p.H + p.G + heads_pass - 1) / heads_pass;
-  // a wave takes all heads of its token where there are tokens for all the card's waves; else they are shared out
-  const int64_t want = 4096;
-  int64_t chunks = p.T >= want ? 1 : std::min<int64_t>(passes, (want + p.T - 1) / p.T);
+  // A wave takes all heads of its token where there are tokens for that many waves; else they are shared out.  Each wave forms the angles again: worth it
+  // for what more waves have under way (4096 tokens, 129 heads of 64: 1 wave a token 33.5 us, 8 26.0), but not backward with the norm, whose waves
+  // stay for several tokens (8192, 36 of 128: 60 us, with 4 waves a token 71).
+  const int64_t want = MODE == kNormTurnBwd ? 4 * kBwdBlocks : 32768;
+  const int64_t chunks = p.T >= want ? 1 : std::min<int64_t>(passes, (want + p.T - 1) / p.T);
   p.passes = static_cast<int>((passes + chunks - 1) / chunks);
   p.chunks = (passes + p.passes - 1) / p.passes;
   const int64_t blocks = std::min<int64_t>((p.T * p.chunks + 3) / 4, blocks_at_most);
@@ -521,10 +525,10 @@ extern "C" int mi355_qk_norm_rotary_bwd(const void* dq_out, const void* dk_out, 
   if (!weights) return MI355_OK;
   const dim3 grid((unsigned)((2 * D + 15) / 16));  // (no tokens: the sum over nothing, zeros)
   if (dtype == MI355_F32)
-    hipLaunchKernelGGL(qk_dw_final_kernel<float>, grid, dim3(256), 0, as_stream(stream), p.partial, static_cast<float*>(dq_weight),
+    hipLaunchKernelGGL(qk_dw_final_kernel<float>, grid, dim3(1024), 0, as_stream(stream), p.partial, static_cast<float*>(dq_weight),
                        static_cast<float*>(dk_weight), used, (int)D);
   else
-    hipLaunchKernelGGL(qk_dw_final_kernel<uint16_t>, grid, dim3(256), 0, as_stream(stream), p.partial,
+    hipLaunchKernelGGL(qk_dw_final_kernel<uint16_t>, grid, dim3(1024), 0, as_stream(stream), p.partial,
                        static_cast<uint16_t*>(dq_weight), static_cast<uint16_t*>(dk_weight), used, (int)D);
   return check_launch("qk_norm_rotary_bwd");
 }

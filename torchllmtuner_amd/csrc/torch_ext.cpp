@@ -193,7 +193,6 @@ struct Heads {
   Tensor t;
   int64_t tokens, heads, size, token_stride, head_stride;
   explicit Heads(const Tensor& x) {
-    TORCH_CHECK_VALUE(x.dim() >= 3, "queries and keys are (..., heads, size), got ", x.sizes());
     t = x.dim() == 3 ? x : x.flatten(0, x.dim() - 3);
     if (t.size(2) > 1 && t.stride(2) != 1) t = t.contiguous();
     tokens = t.size(0), heads = t.size(1), size = t.size(2);
@@ -207,37 +206,50 @@ Tensor heads_like(const OptTensor& grad, const Tensor& like) {
   return dense(grad->scalar_type() == like.scalar_type() ? *grad : grad->to(like.scalar_type()));
 }
 
-void check_heads(const Heads& q, const Heads& k, const Tensor& positions, const Tensor& inv_freq) {
-  TORCH_CHECK_TYPE(q.t.scalar_type() == k.t.scalar_type(), "queries (", q.t.scalar_type(), ") and keys (", k.t.scalar_type(),
+void check_heads(const char* what, const Tensor& q, const Tensor& k, const Tensor& positions, const Tensor& inv_freq) {
+  TORCH_CHECK_VALUE(q.dim() >= 3 && k.dim() == q.dim() && q.sizes().slice(0, q.dim() - 2) == k.sizes().slice(0, q.dim() - 2) &&
+                        q.size(-1) == k.size(-1),
+                    what, ": queries ", q.sizes(), " and keys ", k.sizes(), " must be (..., heads, size) and agree in all but the heads");
+  TORCH_CHECK_TYPE(q.scalar_type() == k.scalar_type(), what, ": queries (", q.scalar_type(), ") and keys (", k.scalar_type(),
                    ") must share a dtype");
-  TORCH_CHECK_VALUE(q.tokens == k.tokens && q.size == k.size, "queries ", q.t.sizes(), " and keys ", k.t.sizes(),
-                    " must agree in tokens and head size");
-  TORCH_CHECK_VALUE(positions.numel() == q.tokens, "got ", positions.numel(), " positions for ", q.tokens, " tokens");
-  TORCH_CHECK_VALUE(k.t.device() == q.t.device() && positions.device() == q.t.device() && inv_freq.device() == q.t.device(),
-                    "queries, keys, positions and inv_freq must share a device");
+  TORCH_CHECK_TYPE(q.scalar_type() == at::kFloat || q.scalar_type() == at::kBFloat16,
+                   "MI355 MoE kernels support float32 and bfloat16, got ", q.scalar_type());
+  TORCH_CHECK_VALUE(q.size(-1) >= 2 && q.size(-1) <= 512 && q.size(-2) >= 1 && k.size(-2) >= 1, what,
+                    ": heads must have 2 to 512 elements, got ", q.sizes(), " and ", k.sizes());
+  TORCH_CHECK_TYPE(positions.scalar_type() == at::kInt || positions.scalar_type() == at::kLong, what,
+                   ": positions must be int32 or int64, got ", positions.scalar_type());
+  TORCH_CHECK_VALUE(positions.sizes() == q.sizes().slice(0, q.dim() - 2), what, ": positions ", positions.sizes(),
+                    " must match the tokens of ", q.sizes());
+  TORCH_CHECK_TYPE(inv_freq.scalar_type() == at::kFloat && inv_freq.dim() == 1, what, ": inv_freq must be a 1-D float32 tensor");
+  TORCH_CHECK_VALUE(!inv_freq.requires_grad(), what, ": there is no gradient for inv_freq");
+  TORCH_CHECK_VALUE(inv_freq.size(0) >= 1 && 2 * inv_freq.size(0) <= q.size(-1), what, ": ", inv_freq.size(0), " frequencies turn ",
+                    2 * inv_freq.size(0), " elements of heads of ", q.size(-1));
+  TORCH_CHECK(k.device() == q.device() && positions.device() == q.device() && inv_freq.device() == q.device(),
+              "tensors on different devices: queries, keys, positions and inv_freq of ", what, " must share one");
 }
-void check_weights(const Heads& q, const Tensor& qw, const Tensor& kw) {
-  TORCH_CHECK_TYPE(qw.scalar_type() == q.t.scalar_type() && kw.scalar_type() == q.t.scalar_type(),
-                   "norm weights must have the queries' dtype");
-  TORCH_CHECK_VALUE(qw.numel() == q.size && kw.numel() == q.size, "norm weights must have the head's ", q.size, " elements");
-  TORCH_CHECK_VALUE(qw.device() == q.t.device() && kw.device() == q.t.device(), "norm weights must be on the queries' device");
+void check_weights(const Tensor& q, const Tensor& qw, const Tensor& kw) {
+  for (const Tensor* w : {&qw, &kw}) {
+    TORCH_CHECK_TYPE(w->scalar_type() == q.scalar_type(), "qk_norm_rotary: heads (", q.scalar_type(), ") and norm weights (",
+                     w->scalar_type(), ") must share a dtype");
+    TORCH_CHECK_VALUE(w->dim() == 1 && w->size(0) == q.size(-1), "qk_norm_rotary: norm weights must be (", q.size(-1), ",), got ",
+                      w->sizes());
+    TORCH_CHECK(w->device() == q.device(), "tensors on different devices: norm weights must be on the heads'");
+  }
 }
 
 struct Positions {
   Tensor t;
   int wide;
-  explicit Positions(const Tensor& p) : t(p.contiguous()), wide(p.scalar_type() == at::kLong) {
-    TORCH_CHECK_TYPE(wide || p.scalar_type() == at::kInt, "positions must be int32 or int64, got ", p.scalar_type());
-  }
+  explicit Positions(const Tensor& p) : t(p.contiguous()), wide(p.scalar_type() == at::kLong) {}
 };
 
 std::tuple<Tensor, Tensor> rotary(const Tensor& q_, const Tensor& k_, const Tensor& positions_, const Tensor& inv_freq_,
                                   bool interleaved, double factor, bool transpose) {
   Launch L(q_);
+  check_heads("rotary", q_, k_, positions_, inv_freq_);
   const Heads q(q_), k(k_);
   const Positions positions(positions_);
-  const Tensor inv_freq = cf(inv_freq_);
-  check_heads(q, k, positions.t, inv_freq);
+  const Tensor inv_freq = inv_freq_.contiguous();
   Tensor q_out = at::empty(q_.sizes(), q_.options()), k_out = at::empty(k_.sizes(), k_.options());
   check(mi355_rotary(ptr(q.t), q.token_stride, q.head_stride, ptr(k.t), k.token_stride, k.head_stride, dtype_code(q.t),
                      ptr(positions.t), positions.wide, fptr(inv_freq), inv_freq.numel(), (float)factor, interleaved, transpose,
@@ -250,11 +262,11 @@ std::tuple<Tensor, Tensor> qk_norm_rotary_fwd(const Tensor& q_, const Tensor& k_
                                               const Tensor& positions_, const Tensor& inv_freq_, double eps, bool interleaved,
                                               double factor) {
   Launch L(q_);
+  check_heads("qk_norm_rotary", q_, k_, positions_, inv_freq_);
+  check_weights(q_, qw_, kw_);
   const Heads q(q_), k(k_);
-  const Tensor qw = qw_.contiguous(), kw = kw_.contiguous(), inv_freq = cf(inv_freq_);
+  const Tensor qw = qw_.contiguous(), kw = kw_.contiguous(), inv_freq = inv_freq_.contiguous();
   const Positions positions(positions_);
-  check_heads(q, k, positions.t, inv_freq);
-  check_weights(q, qw, kw);
   Tensor q_out = at::empty(q_.sizes(), q_.options()), k_out = at::empty(k_.sizes(), k_.options());
   check(mi355_qk_norm_rotary_fwd(ptr(q.t), q.token_stride, q.head_stride, ptr(k.t), k.token_stride, k.head_stride, ptr(qw), ptr(kw),
                                  dtype_code(q.t), ptr(positions.t), positions.wide, fptr(inv_freq), inv_freq.numel(), (float)factor,
@@ -268,12 +280,12 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> qk_norm_rotary_bwd(const OptTensor& d
                                                               const Tensor& positions_, const Tensor& inv_freq_, double eps,
                                                               bool interleaved, double factor, bool need_dx, bool need_dw) {
   Launch L(q_);
+  check_heads("qk_norm_rotary", q_, k_, positions_, inv_freq_);
+  check_weights(q_, qw_, kw_);
   const Heads q(q_), k(k_);
   const Tensor dq_out = heads_like(dq_out_, q_), dk_out = heads_like(dk_out_, k_);
-  const Tensor qw = qw_.contiguous(), kw = kw_.contiguous(), inv_freq = cf(inv_freq_);
+  const Tensor qw = qw_.contiguous(), kw = kw_.contiguous(), inv_freq = inv_freq_.contiguous();
   const Positions positions(positions_);
-  check_heads(q, k, positions.t, inv_freq);
-  check_weights(q, qw, kw);
   TORCH_CHECK_VALUE(dq_out.sizes() == q_.sizes() && dk_out.sizes() == k_.sizes(), "gradients must have the results' shapes");
   Tensor dq = need_dx ? at::empty(q_.sizes(), q_.options()) : none_like(q_);
   Tensor dk = need_dx ? at::empty(k_.sizes(), k_.options()) : none_like(k_);
@@ -290,21 +302,28 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> qk_norm_rotary_bwd(const OptTensor& d
   return {dq, dk, dqw, dkw};
 }
 
-void check_attention(const Heads& q, const Heads& k, const Heads& v, const Tensor& cu) {
-  TORCH_CHECK_TYPE(q.t.scalar_type() == k.t.scalar_type() && q.t.scalar_type() == v.t.scalar_type(), "queries, keys and values must share a dtype");
-  TORCH_CHECK_VALUE(k.t.sizes() == v.t.sizes() && q.tokens == k.tokens && q.size == k.size, "queries ", q.t.sizes(), ", keys ",
-                    k.t.sizes(), " and values ", v.t.sizes(), " must agree in tokens and head size");
-  TORCH_CHECK_TYPE(cu.scalar_type() == at::kInt, "cu_seqlens must be int32, got ", cu.scalar_type());
-  TORCH_CHECK_VALUE(cu.dim() == 1 && cu.numel() >= 1, "cu_seqlens must be 1-D with at least one entry");
-  TORCH_CHECK_VALUE(k.t.device() == q.t.device() && v.t.device() == q.t.device() && cu.device() == q.t.device(),
-                    "queries, keys, values and cu_seqlens must share a device");
+void check_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu) {
+  TORCH_CHECK_VALUE(q.dim() == 3 && k.dim() == 3 && k.sizes() == v.sizes() && k.size(0) == q.size(0) && k.size(2) == q.size(2),
+                    "varlen_attention: queries ", q.sizes(), ", keys ", k.sizes(), " and values ", v.sizes(),
+                    " must be (tokens, heads, size) and agree in tokens and size");
+  TORCH_CHECK_TYPE(q.scalar_type() == k.scalar_type() && q.scalar_type() == v.scalar_type(), "varlen_attention: queries (",
+                   q.scalar_type(), "), keys (", k.scalar_type(), ") and values (", v.scalar_type(), ") must share a dtype");
+  TORCH_CHECK_TYPE(q.scalar_type() == at::kFloat || q.scalar_type() == at::kBFloat16,
+                   "MI355 MoE kernels support float32 and bfloat16, got ", q.scalar_type());
+  TORCH_CHECK_VALUE(k.size(1) >= 1 && q.size(1) >= 1 && q.size(1) % k.size(1) == 0, "varlen_attention: ", q.size(1),
+                    " query heads are no multiple of ", k.size(1), " key heads");
+  TORCH_CHECK_VALUE(q.size(2) >= 1 && q.size(2) <= 256, "varlen_attention: heads must have 1 to 256 elements, got ", q.size(2));
+  TORCH_CHECK_VALUE(cu.scalar_type() == at::kInt && cu.dim() == 1 && cu.size(0) >= 1,
+                    "varlen_attention: cu_seqlens must be a 1-D int32 tensor with at least one entry, got ", cu.scalar_type(), " ", cu.sizes());
+  TORCH_CHECK(k.device() == q.device() && v.device() == q.device() && cu.device() == q.device(),
+              "tensors on different devices: queries, keys, values and cu_seqlens must share one");
 }
 
 std::tuple<Tensor, Tensor, Tensor> varlen_attention_fwd(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& cu_,
                                                         double scale, bool for_backward) {
   Launch L(q_);
+  check_attention(q_, k_, v_, cu_);
   const Heads q(q_), k(k_), v(v_);
-  check_attention(q, k, v, cu_);
   const Tensor cu = cu_.contiguous();
   Tensor out = at::empty(q_.sizes(), q_.options()), lse = at::empty({q.heads, q.tokens}, q_.options().dtype(at::kFloat));
   Tensor rest = for_backward && q_.scalar_type() == at::kBFloat16 ? at::empty_like(out) : none_like(out);
@@ -321,8 +340,8 @@ std::tuple<Tensor, Tensor, Tensor> varlen_attention_bwd(const Tensor& dout_, con
                                                         const Tensor& out_, const Tensor& lse_, const Tensor& rest_, const Tensor& cu_,
                                                         double scale) {
   Launch L(q_);
+  check_attention(q_, k_, v_, cu_);
   const Heads q(q_), k(k_), v(v_);
-  check_attention(q, k, v, cu_);
   const Tensor dout = heads_like(dout_, q_), out = dense(out_), lse = dense(lse_), rest = dense(rest_), cu = cu_.contiguous();
   TORCH_CHECK_VALUE(dout.sizes() == q_.sizes() && out.sizes() == q_.sizes() && out.scalar_type() == q_.scalar_type() &&
                         lse.numel() == q.heads * q.tokens && lse.scalar_type() == at::kFloat &&

@@ -172,11 +172,14 @@ def _(dy, x, weight, rstd, need_dx, need_dw):
 
 @_fake("rotary")
 def _(q, k, positions, inv_freq, interleaved, attention_factor, transpose):
+    _check_rotary("rotary", q, k, positions, inv_freq, attention_factor)
     return q.new_empty(q.shape), k.new_empty(k.shape)
 
 
 @_fake("qk_norm_rotary_fwd")
 def _(q, k, q_weight, k_weight, positions, inv_freq, epsilon, interleaved, attention_factor):
+    _check_rotary("qk_norm_rotary", q, k, positions, inv_freq, attention_factor)
+    _check_qk_norm(q, q_weight, k_weight, epsilon)
     return q.new_empty(q.shape), k.new_empty(k.shape)
 
 
@@ -189,6 +192,7 @@ def _(dq_out, dk_out, q, k, q_weight, k_weight, positions, inv_freq, epsilon, in
 
 @_fake("varlen_attention_fwd")
 def _(q, k, v, cu_seqlens, scale, for_backward):
+    _check_attention(q, k, v, cu_seqlens, scale)
     kept = for_backward and q.dtype == torch.bfloat16
     return (q.new_empty(q.shape), q.new_empty((q.shape[1], q.shape[0]), dtype=torch.float32),
             q.new_empty(q.shape) if kept else _e0(q))
@@ -502,21 +506,7 @@ def _check_rotary(what, q, k, positions, inv_freq, attention_factor):
         raise ValueError(f"{what}: the attention factor must be finite")
 
 
-def rotary(q, k, positions, inv_freq, *, interleaved=False, attention_factor=1.0):
-    """Queries ``(..., H, D)`` and keys ``(..., G, D)`` with their first ``2 len(inv_freq)`` elements turned by
-    ``positions * inv_freq``: pairs ``(i, i + len(inv_freq))``, or ``(2 i, 2 i + 1)`` where ``interleaved``; the turned
-    elements are scaled by ``attention_factor``, the others copied.  ``positions`` has the tokens' shape ``(...)``.
-    Heads may be views into a fused projection (their elements next to each other): they are read where they lie; the
-    results are new dense tensors.  Differentiable in both (the same kernel, turned back)."""
-    _check_rotary("rotary", q, k, positions, inv_freq, attention_factor)
-    return _O.rotary(q, k, positions, inv_freq, bool(interleaved), float(attention_factor), False)
-
-
-def qk_norm_rotary(q, k, q_weight, k_weight, positions, inv_freq, epsilon, *, interleaved=False, attention_factor=1.0):
-    """``rotary(rms_norm(q, q_weight), rms_norm(k, k_weight))`` over the heads' elements in one pass, rounded once.
-    Weights are ``(D,)`` in the dtype of the heads.  Differentiable in the heads and the weights; the
-    backward keeps nothing but the inputs."""
-    _check_rotary("qk_norm_rotary", q, k, positions, inv_freq, attention_factor)
+def _check_qk_norm(q, q_weight, k_weight, epsilon):
     _dev(q, q_weight, k_weight)
     for w in (q_weight, k_weight):
         if w.dtype != q.dtype:
@@ -525,19 +515,38 @@ def qk_norm_rotary(q, k, q_weight, k_weight, positions, inv_freq, epsilon, *, in
             raise ValueError(f"qk_norm_rotary: norm weights must be ({q.shape[-1]},), got {tuple(w.shape)}")
     if not math.isfinite(epsilon) or epsilon < 0:
         raise ValueError("qk_norm_rotary: epsilon must be finite and nonnegative")
-    return _O.qk_norm_rotary_fwd(q, k, q_weight, k_weight, positions, inv_freq, float(epsilon), bool(interleaved),
-                                 float(attention_factor))
+
+
+# A call of one token is a few microseconds: what the operators take is checked once, by themselves -- the device kernels' C++ and, for
+# tracing, the shape functions above, which call the checks here.
+_rotary = _O.rotary.default
+_qk_norm_rotary = _O.qk_norm_rotary_fwd.default
+_varlen_attention = _O.varlen_attention_fwd.default
+
+
+def rotary(q, k, positions, inv_freq, *, interleaved=False, attention_factor=1.0):
+    """Queries ``(..., H, D)`` and keys ``(..., G, D)`` with their first ``2 len(inv_freq)`` elements turned by
+    ``positions * inv_freq``: pairs ``(i, i + len(inv_freq))``, or ``(2 i, 2 i + 1)`` where ``interleaved``; the turned
+    elements are scaled by ``attention_factor``, the others copied.  ``positions`` has the tokens' shape ``(...)``.
+    Heads may be views into a fused projection (their elements next to each other): they are read where they lie; the
+    results are new dense tensors.  Differentiable in both (the same kernel, turned back)."""
+    if not q.is_cuda:
+        _dev(q)
+    return _rotary(q, k, positions, inv_freq, bool(interleaved), float(attention_factor), False)
+
+
+def qk_norm_rotary(q, k, q_weight, k_weight, positions, inv_freq, epsilon, *, interleaved=False, attention_factor=1.0):
+    """``rotary(rms_norm(q, q_weight), rms_norm(k, k_weight))`` over the heads' elements in one pass, rounded once.
+    Weights are ``(D,)`` in the dtype of the heads.  Differentiable in the heads and the weights; the
+    backward keeps nothing but the inputs."""
+    if not q.is_cuda:
+        _dev(q)
+    return _qk_norm_rotary(q, k, q_weight, k_weight, positions, inv_freq, float(epsilon), bool(interleaved),
+                           float(attention_factor))
 
 
 # ====================================================================== attention
-def varlen_attention(q, k, v, cu_seqlens, *, scale=None):
-    """Causal attention over packed sequences: queries ``(T, H, D)``, keys and values ``(T, G, D)`` with ``H`` a
-    multiple of ``G`` (query head ``h`` reads key head ``h // (H // G)``), ``1 <= D <= 256``, fp32 or bf16.
-    ``cu_seqlens`` (int32, ascending, on the device) holds where each sequence begins and where the last one ends, as
-    ``[0, n_0, n_0 + n_1, ...]``; sequences may be empty.  A row sees the rows of its own sequence up to itself; rows behind the last
-    sequence get zeros and have zero gradients.  ``scale`` defaults to ``D ** -0.5``.  Views into a fused projection are read
-    where they lie.  Nothing is read back from the device: a call can be captured, and replayed over other
-    lengths.  Differentiable in queries, keys and values; bit-identical from run to run."""
+def _check_attention(q, k, v, cu_seqlens, scale):
     _dev(q, k, v, cu_seqlens)
     if q.ndim != 3 or k.ndim != 3 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
         raise ValueError(f"varlen_attention: queries {tuple(q.shape)}, keys {tuple(k.shape)} and values {tuple(v.shape)} "
@@ -552,11 +561,21 @@ def varlen_attention(q, k, v, cu_seqlens, *, scale=None):
     if cu_seqlens.dtype != torch.int32 or cu_seqlens.ndim != 1 or cu_seqlens.shape[0] < 1:
         raise ValueError("varlen_attention: cu_seqlens must be a 1-D int32 tensor with at least one entry, got "
                          f"{cu_seqlens.dtype} {tuple(cu_seqlens.shape)}")
-    if scale is None:
-        scale = q.shape[2] ** -0.5
     if not (math.isfinite(scale) and scale > 0):
         raise ValueError(f"varlen_attention: the scale must be finite and positive, got {scale}")
-    return _O.varlen_attention_fwd(q, k, v, cu_seqlens, float(scale), False)[0]
+
+
+def varlen_attention(q, k, v, cu_seqlens, *, scale=None):
+    """Causal attention over packed sequences: queries ``(T, H, D)``, keys and values ``(T, G, D)`` with ``H`` a
+    multiple of ``G`` (query head ``h`` reads key head ``h // (H // G)``), ``1 <= D <= 256``, fp32 or bf16.
+    ``cu_seqlens`` (int32, ascending, on the device) holds where each sequence begins and where the last one ends, as
+    ``[0, n_0, n_0 + n_1, ...]``; sequences may be empty.  A row sees the rows of its own sequence up to itself; rows behind the last
+    sequence get zeros and have zero gradients.  ``scale`` defaults to ``D ** -0.5``.  Views into a fused projection are read
+    where they lie.  Nothing is read back from the device: a call can be captured, and replayed over other
+    lengths.  Differentiable in queries, keys and values; bit-identical from run to run."""
+    if not q.is_cuda:
+        _dev(q)
+    return _varlen_attention(q, k, v, cu_seqlens, q.shape[-1] ** -0.5 if scale is None else float(scale), False)[0]
 
 
 def _as_bool(m):
