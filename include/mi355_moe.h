@@ -794,12 +794,14 @@ int mi355_qk_norm_rotary_bwd(const void* dq_out, const void* dk_out, const void*
  * range give meaningless rows but never an access outside the tensors.
  * q (T, H, D), k and v (T, G, D) with the given strides in elements, a head's elements next to each other; out dense.
  * fp32 or bf16, 1 <= D <= 256, H a multiple of G, scale finite and positive, T < 2^30.  Scores, weights' statistics
- * and sums are fp32; with bf16 storage the weights are rounded to bf16 for the second product where matrix kernels serve the call.
+ * and sums are fp32; with bf16 storage the weights, and ds in the backward, are rounded to bf16 for the products that they go into.
  * out_rest: optional, bf16 only, dense like out: what rounding took from it, rounded itself; with it the backward's out . dout is as good as
  * out in fp32 (from the rounded out alone, the gradients of short rows come out twice as far from the formula).
  * lse: optional (H, T) fp32, log2 of each row's sum of exp(scale q.k), +inf for rows in no sequence; the backward reads it.
- * workspace: mi355_varlen_attention_fwd_workspace_bytes(T, H, sequences) bytes, or NULL: then tiles of several sequences start in the order in which
- * they lie, not the longest first.
+ * bf16 operands start and stride in whole pieces of 16 bytes, unless D is no whole number of them: then they are copied into padded rows in
+ * the workspace first.  Token strides below 2^22 elements for bf16.
+ * workspace: mi355_varlen_attention_fwd_workspace_bytes(T, H, G, D, sequences, dtype) bytes, on a 16-byte boundary; NULL where D is a multiple of 8
+ * or fp32: then tiles of several sequences start in the order in which they lie, not the longest first.
  */
 int mi355_varlen_attention_fwd(const void* q, int64_t q_token_stride, int64_t q_head_stride,
                                const void* k, int64_t k_token_stride, int64_t k_head_stride,
@@ -807,14 +809,16 @@ int mi355_varlen_attention_fwd(const void* q, int64_t q_token_stride, int64_t q_
                                int dtype, const int32_t* cu_seqlens, int64_t sequences, float scale,
                                void* out, void* out_rest, float* lse, void* workspace,
                                int64_t T, int64_t H, int64_t G, int64_t D, void* stream);
-int64_t mi355_varlen_attention_fwd_workspace_bytes(int64_t T, int64_t H, int64_t sequences);
+int64_t mi355_varlen_attention_fwd_workspace_bytes(int64_t T, int64_t H, int64_t G, int64_t D,
+                                                   int64_t sequences, int dtype);
 
 /*
  * Its backward; dout, out and out_rest (the forward's; out_rest may be NULL) dense, so are dq, dk and dv.  Scores are formed again.  No atomics: dk and dv of a key
  * head are sums over its query heads in a fixed order, by way of fp32 parts in the workspace where few key heads would
- * leave the card idle.  workspace: mi355_varlen_attention_bwd_workspace_bytes(T, H, G, D) bytes.
+ * leave the card idle.  workspace: mi355_varlen_attention_bwd_workspace_bytes(T, H, G, D, dtype) bytes.
  */
-int64_t mi355_varlen_attention_bwd_workspace_bytes(int64_t T, int64_t H, int64_t G, int64_t D);
+int64_t mi355_varlen_attention_bwd_workspace_bytes(int64_t T, int64_t H, int64_t G, int64_t D,
+                                                   int dtype);
 int mi355_varlen_attention_bwd(const void* dout, const void* q, int64_t q_token_stride,
                                int64_t q_head_stride, const void* k, int64_t k_token_stride,
                                int64_t k_head_stride, const void* v, int64_t v_token_stride,

@@ -130,6 +130,13 @@ CASES = [
     ([3] * 60, 4, 2, 2, 64),
     ([513], 0, 4, 4, 128),
     ([400, 380], 0, 2, 1, 128),
+    ([200, 90], 3, 4, 2, 75),    # heads that are no whole number of 16 bytes, copied into padded rows
+    ([260], 0, 3, 1, 150),
+    ([0, 301, 2], 1, 2, 2, 33),
+    ([250], 0, 2, 1, 201),
+    ([300], 5, 2, 1, 1),
+    ([600, 520], 7, 8, 8, 64),   # long on average and more tiles than the card holds at once: sorted by their work
+    ([512, 3, 1100], 0, 16, 4, 40),
 ]
 
 
@@ -189,12 +196,12 @@ def test_gradients_match_differences():
 
 @gpu
 @pytest.mark.parametrize("dtype", [BF, F32])
-@pytest.mark.parametrize("D", [64, 128, 40, 160])
+@pytest.mark.parametrize("D", [64, 128, 40, 160, 35])
 @pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
 def test_values_in_masked_places_reach_no_row(value, D, dtype):
     """A sequence whose inputs are spoilt, and the rows behind the last sequence, leave the others' results as they were bit for bit; in a
     sequence, what comes before a spoilt row is its own, too."""
-    cu, T = bounds_of([20, 30, 90], 6)
+    cu, T = bounds_of([20, 30, 90 if D > 35 else 250], 6)
     print(f"varlen_attention with {value} {D} {dtype}", flush=True)
     leaves, dout = inputs(T, 4, 2, D, dtype, seed=12)
     at = torch.tensor(cu, dtype=torch.int32, device=DEV)
@@ -427,9 +434,9 @@ def test_operator_refuses_what_does_not_fit_and_propagates_shapes():
 def test_c_entry_points_refuse_before_any_launch():
     lib, p = _lib.load(), 0x1000  # (never dereferenced)
 
-    def forward(T=4, H=4, G=2, D=64, dtype=1, scale=0.1, cu=p, sequences=1):
-        return lib.mi355_varlen_attention_fwd(p, H * D, D, p, G * D, D, p, G * D, D, dtype, cu, sequences, scale, p, p, p, p, T, H, G,
-                                              D, None)
+    def forward(T=4, H=4, G=2, D=64, dtype=1, scale=0.1, cu=p, sequences=1, k=p, k_token=None, workspace=p):
+        return lib.mi355_varlen_attention_fwd(p, H * D, D, k, k_token or G * D, D, p, G * D, D, dtype, cu, sequences, scale, p, p, p,
+                                              workspace, T, H, G, D, None)
 
     def backward(T=4, H=4, G=2, D=64, workspace=p):
         return lib.mi355_varlen_attention_bwd(p, p, H * D, D, p, G * D, D, p, G * D, D, p, p, p, 1, p, 1, 0.1, p, p, p, workspace, T, H,
@@ -448,10 +455,19 @@ def test_c_entry_points_refuse_before_any_launch():
     text(forward(scale=0.0), b"finite and positive")
     text(forward(scale=math.nan), b"finite and positive")
     text(forward(cu=None), b"null pointer")
+    text(forward(k=p + 2), b"whole pieces of 16 bytes")
+    text(forward(k_token=2 * 64 + 4), b"whole pieces of 16 bytes")
+    text(forward(k_token=1 << 22), b"whole pieces of 16 bytes")
+    text(forward(D=65, workspace=None), b"workspace required")
+    text(forward(workspace=p + 4), b"16-byte")
+    text(forward(H=65536, G=1), b"no multiple")
+    text(forward(H=32768, G=1, D=128), b"too many")
     assert forward(T=0) == 0
     text(backward(H=3), b"no multiple")
     text(backward(workspace=None), b"null pointer")
     text(backward(workspace=p + 8), b"16-byte")
     assert backward(T=0) == 0
-    assert lib.mi355_varlen_attention_bwd_workspace_bytes(100, 4, 2, 64) >= 4 * 4 * 100
-    assert lib.mi355_varlen_attention_bwd_workspace_bytes(0, 4, 2, 64) == 0
+    assert lib.mi355_varlen_attention_bwd_workspace_bytes(100, 4, 2, 64, 1) >= 4 * 4 * 100
+    assert lib.mi355_varlen_attention_bwd_workspace_bytes(0, 4, 2, 64, 1) == 0
+    assert lib.mi355_varlen_attention_fwd_workspace_bytes(100, 4, 2, 64, 1, 1) == 0
+    assert lib.mi355_varlen_attention_fwd_workspace_bytes(100, 4, 2, 65, 1, 1) >= 2 * 100 * 8 * 72

@@ -35,6 +35,7 @@ struct AttnArgs {
   const int32_t* cu;      // [sequences + 1]
   int sequences;
   int T, H, G, D, group;  // group = H / G
+  int D_out;              // elements of a head in results and their parts: D, or fewer where the operands are copies padded to D
   int splits;             // parts that a key head's group of query heads is cut into for dk and dv
   float scale, c;         // c = scale log2(e)
   // tiles of rows by descending work, for the kernels whose rows are queries and for dk and dv; null: as they lie, the last (first) tile first
@@ -151,10 +152,10 @@ __device__ __forceinline__ void careful_forward_row(const AttnArgs& p, int h, in
     }
     m = top;
   }
-  const int64_t dense = (static_cast<int64_t>(row) * p.H + h) * p.D;
+  const int64_t dense = (static_cast<int64_t>(row) * p.H + h) * p.D_out;
 #pragma unroll
   for (int i = 0; i < kLaneCols; ++i)
-    if (lane + 64 * i < p.D) store_result<T>(p, dense + lane + 64 * i, acc[i] / l);
+    if (lane + 64 * i < p.D_out) store_result<T>(p, dense + lane + 64 * i, acc[i] / l);
 }
 
 template <typename T>
@@ -178,10 +179,10 @@ __device__ __forceinline__ void careful_dq_row(const AttnArgs& p, int h, int row
         if (lane + 64 * i < p.D) acc[i] = fmaf(dn, load_as_f32<T>(k + lane + 64 * i), acc[i]);
     }
   }
-  T* dq = static_cast<T*>(p.dq) + (static_cast<int64_t>(row) * p.H + h) * p.D;
+  T* dq = static_cast<T*>(p.dq) + (static_cast<int64_t>(row) * p.H + h) * p.D_out;
 #pragma unroll
   for (int i = 0; i < kLaneCols; ++i)
-    if (lane + 64 * i < p.D) store_from_f32<T>(dq + lane + 64 * i, acc[i] * p.scale);
+    if (lane + 64 * i < p.D_out) store_from_f32<T>(dq + lane + 64 * i, acc[i] * p.scale);
 }
 
 // dk and dv of one key over the query heads [h0, h1), into the part `split` where there are parts; delta is kept times `sign`
@@ -214,11 +215,11 @@ __device__ __forceinline__ void careful_dkv_row(const AttnArgs& p, int g, int ke
       }
     }
   }
-  const int64_t at = (static_cast<int64_t>(key) * p.G + g) * p.D, part = static_cast<int64_t>(split) * p.T * p.G * p.D + at;
+  const int64_t at = (static_cast<int64_t>(key) * p.G + g) * p.D_out, part = static_cast<int64_t>(split) * p.T * p.G * p.D_out + at;
 #pragma unroll
   for (int i = 0; i < kLaneCols; ++i) {
     const int d = lane + 64 * i;
-    if (d >= p.D) continue;
+    if (d >= p.D_out) continue;
     if (p.splits > 1) {
       p.dk_part[part + d] = dk[i] * p.scale;
       p.dv_part[part + d] = dv[i];
@@ -246,8 +247,8 @@ void attention_sort_tiles(const AttnArgs& p, int rows, int32_t* query_order, int
 constexpr int kLeastRows = 32;  // rows of a tile, at least
 int attention_any_rows(int D);
 int attention_bf16_rows();
-void attention_any_forward(const AttnArgs& p, int dtype, hipStream_t s);
-void attention_any_backward(const AttnArgs& p, int dtype, hipStream_t s);
+void attention_any_forward(const AttnArgs& p, hipStream_t s);
+void attention_any_backward(const AttnArgs& p, hipStream_t s);
 bool attention_bf16_covers(const AttnArgs& p);
 void attention_bf16_forward(const AttnArgs& p, hipStream_t s);
 void attention_bf16_backward(const AttnArgs& p, hipStream_t s);

@@ -1,6 +1,5 @@
-// Causal attention over packed sequences (attention.h has the formulas), for every head size up to 256, fp32 and bf16
-// storage, on v_mfma_f32_16x16x4_f32: fp32 products throughout.  And the entry points, which choose between this and the
-// bf16 matrix kernels.
+// Causal attention over packed sequences (attention.h has the formulas) in fp32, for every head size up to 256, on
+// v_mfma_f32_16x16x4_f32: fp32 products throughout.  And the entry points of both types, the order of the tiles, and what joins parts.
 //
 // v_mfma_f32_16x16x4_f32 takes one element a lane of each operand (row or column lane % 16, k = lane / 16) and yields four
 // (column lane % 16, rows 4 (lane / 16) + i).  Products are formed turned so that one's result is the next one's operand as it lies:
@@ -25,45 +24,33 @@ namespace {
 
 constexpr uint32_t kFar = 1u << 30;  // an offset past every buffer: reads zeros
 
-template <typename T>
-__device__ __forceinline__ float4 four_at(const T* p, int n, bool vec) {  // the first n of p[0..3], zeros behind them
-  if (vec) {
-    if constexpr (sizeof(T) == 4) return *reinterpret_cast<const float4*>(p);
-    const u32x2 q = *reinterpret_cast<const u32x2*>(p);
-    return make_float4(__uint_as_float(q[0] << 16), __uint_as_float(q[0] & 0xffff0000u), __uint_as_float(q[1] << 16),
-                       __uint_as_float(q[1] & 0xffff0000u));
-  }
+__device__ __forceinline__ float4 four_at(const float* p, int n, bool vec) {  // the first n of p[0..3], zeros behind them
+  if (vec) return *reinterpret_cast<const float4*>(p);
   float4 v = make_float4(0, 0, 0, 0);
-  if (n > 0) v.x = load_as_f32<T>(p);
-  if (n > 1) v.y = load_as_f32<T>(p + 1);
-  if (n > 2) v.z = load_as_f32<T>(p + 2);
-  if (n > 3) v.w = load_as_f32<T>(p + 3);
+  if (n > 0) v.x = p[0];
+  if (n > 1) v.y = p[1];
+  if (n > 2) v.z = p[2];
+  if (n > 3) v.w = p[3];
   return v;
 }
 
 // Rows [row0, row0 + ROWS) of a head on their way to LDS as fp32, zeros behind row T and behind the head's elements: held in registers from
 // where they are fetched, a tile ahead, to where the tile before has been read
-template <typename T, int DP, int ROWS>
+template <int DP, int ROWS>
 struct Staged {
   static constexpr int P = DP + 4, QUADS = DP / 4, EACH = ROWS * QUADS / 256;
   static_assert(ROWS * QUADS % 256 == 0, "whole rounds of the workgroup");
   float4 x[EACH];
-  __device__ __forceinline__ void fetch(const T* base, int64_t token, int row0, int T_, int D, bool vec) {
+  __device__ __forceinline__ void fetch(const float* base, int64_t token, int row0, int T_, int D, bool vec) {
     if (vec) {  // from a buffer that ends with the last row: zeros behind it, and no branch a request
-      const int64_t left = (static_cast<int64_t>(T_ - 1 - row0) * token + D) * sizeof(T);
+      const int64_t left = (static_cast<int64_t>(T_ - 1 - row0) * token + D) * sizeof(float);
       const uint32_t bytes = left < 0 ? 0 : left < kFar ? static_cast<uint32_t>(left) : kFar;
-      const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base) + static_cast<int64_t>(row0) * token, 0, bytes, 0x00020000);
+      const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(base) + static_cast<int64_t>(row0) * token, 0, bytes, 0x00020000);
 #pragma unroll
       for (int n = 0; n < EACH; ++n) {
         const int i = threadIdx.x + 256 * n, d = (i % QUADS) * 4;
-        const uint32_t at = d < D ? (static_cast<uint32_t>(i / QUADS) * static_cast<uint32_t>(token) + d) * sizeof(T) : kFar;
-        if constexpr (sizeof(T) == 4) {
-          x[n] = __builtin_bit_cast(float4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, at, 0, 0));
-        } else {
-          const auto q = __builtin_amdgcn_raw_buffer_load_b64(rsrc, at, 0, 0);
-          x[n] = make_float4(__uint_as_float(q[0] << 16), __uint_as_float(q[0] & 0xffff0000u), __uint_as_float(q[1] << 16),
-                             __uint_as_float(q[1] & 0xffff0000u));
-        }
+        const uint32_t at = d < D ? (static_cast<uint32_t>(i / QUADS) * static_cast<uint32_t>(token) + d) * sizeof(float) : kFar;
+        x[n] = __builtin_bit_cast(float4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, at, 0, 0));
       }
       return;
     }
@@ -71,7 +58,7 @@ struct Staged {
     for (int n = 0; n < EACH; ++n) {
       const int i = threadIdx.x + 256 * n, r = row0 + i / QUADS, d = (i % QUADS) * 4;
       x[n] = make_float4(0, 0, 0, 0);
-      if (r < T_ && d < D) x[n] = four_at<T>(base + static_cast<int64_t>(r) * token + d, D - d, false);
+      if (r < T_ && d < D) x[n] = four_at(base + static_cast<int64_t>(r) * token + d, D - d, false);
     }
   }
   __device__ __forceinline__ void put(float* tile) const {
@@ -84,13 +71,13 @@ struct Staged {
 };
 
 // a wave's 16 rows as an operand over the head's elements: lane's row lane % 16, elements 16 j + 4 (lane / 16) + i
-template <typename T, int DP>
-__device__ __forceinline__ void own_rows(float (&x)[DP / 4], const T* base, int64_t token, int row, bool on, int D, bool vec, int lane) {
+template <int DP>
+__device__ __forceinline__ void own_rows(float (&x)[DP / 4], const float* base, int64_t token, int row, bool on, int D, bool vec, int lane) {
 #pragma unroll
   for (int j = 0; j < DP / 16; ++j) {
     const int d = 16 * j + 4 * (lane >> 4);
     float4 v = make_float4(0, 0, 0, 0);
-    if (on && d < D) v = four_at<T>(base + static_cast<int64_t>(row) * token + d, D - d, vec && d + 4 <= D);
+    if (on && d < D) v = four_at(base + static_cast<int64_t>(row) * token + d, D - d, vec && d + 4 <= D);
     x[4 * j] = v.x, x[4 * j + 1] = v.y, x[4 * j + 2] = v.z, x[4 * j + 3] = v.w;
   }
 }
@@ -215,7 +202,7 @@ __global__ __launch_bounds__(1024) void sort_tiles_kernel(const AttnArgs p, int 
   for (int t = threadIdx.x; t < tiles; t += 1024) order[atomicAdd(&count[class_of(t)], 1)] = t;
 }
 
-template <typename T, int DP, int KW>
+template <int DP, int KW>
 __global__ __launch_bounds__(256) void any_forward_kernel(const AttnArgs p, int tiles, int vec) {
   constexpr int QW = 4 / KW, P = DP + 4, NB = DP / 16;
   extern __shared__ __attribute__((aligned(16))) float lds[];
@@ -230,15 +217,15 @@ __global__ __launch_bounds__(256) void any_forward_kernel(const AttnArgs p, int 
   const int lo = wave_min_i(on ? start : p.T), hi = wave_max_i(on ? row + 1 : 0);
   const Range all = group_range(lo, hi, reinterpret_cast<int*>(stats));
   float q[DP / 4];
-  own_rows<T, DP>(q, static_cast<const T*>(p.q) + h * p.q_head, p.q_token, row, on, p.D, vec, lane);
+  own_rows<DP>(q, static_cast<const float*>(p.q) + h * p.q_head, p.q_token, row, on, p.D, vec, lane);
   f32x4 o[NB];
 #pragma unroll
   for (int n = 0; n < NB; ++n) o[n] = f32x4{0, 0, 0, 0};
   float m = kNegInf, l = 0.0f;
-  Staged<T, DP, KW * kStep> keys, values;
+  Staged<DP, KW * kStep> keys, values;
   auto fetch = [&](int k0) {
-    keys.fetch(static_cast<const T*>(p.k) + g * p.k_head, p.k_token, k0, p.T, p.D, vec);
-    values.fetch(static_cast<const T*>(p.v) + g * p.v_head, p.v_token, k0, p.T, p.D, vec);
+    keys.fetch(static_cast<const float*>(p.k) + g * p.k_head, p.k_token, k0, p.T, p.D, vec);
+    values.fetch(static_cast<const float*>(p.v) + g * p.v_head, p.v_token, k0, p.T, p.D, vec);
   };
   if (all.lo < all.hi) fetch(all.lo);
   for (int k0 = all.lo; k0 < all.hi; k0 += KW * kStep) {
@@ -315,15 +302,15 @@ __global__ __launch_bounds__(256) void any_forward_kernel(const AttnArgs p, int 
       for (int part = 0; part < KW; ++part) v += w[part] * sums[((qw * KW + part) * 16 + mine) * P + d];
       v /= len;
       spoilt |= v != v;
-      store_result<T>(z, dense + d, first < last ? v : 0.0f);
+      store_result<float>(z, dense + d, first < last ? v : 0.0f);
     }
     if (lane == 0 && z.lse) z.lse[static_cast<int64_t>(h) * z.T + r] = first < last ? ref + log2f(len) : INFINITY;
-    if (first < last && __any(spoilt)) careful_forward_row<T>(z, h, r, first);
+    if (first < last && __any(spoilt)) careful_forward_row<float>(z, h, r, first);
   }
 }
 
 // dq, and delta for the kernel behind this one
-template <typename T, int DP, int KW>
+template <int DP, int KW>
 __global__ __launch_bounds__(256) void any_dq_kernel(const AttnArgs p, int tiles, int vec) {
   constexpr int QW = 4 / KW, P = DP + 4, NB = DP / 16;
   extern __shared__ __attribute__((aligned(16))) float lds[];
@@ -339,18 +326,14 @@ __global__ __launch_bounds__(256) void any_dq_kernel(const AttnArgs p, int tiles
   const Range all = group_range(lo, hi, reinterpret_cast<int*>(stats));
   float q[DP / 4], dout[DP / 4];
   const int64_t dense = static_cast<int64_t>(p.H) * p.D;
-  own_rows<T, DP>(q, static_cast<const T*>(p.q) + h * p.q_head, p.q_token, row, on, p.D, vec, lane);
-  own_rows<T, DP>(dout, static_cast<const T*>(p.dout) + h * p.D, dense, row, on, p.D, vec, lane);
+  own_rows<DP>(q, static_cast<const float*>(p.q) + h * p.q_head, p.q_token, row, on, p.D, vec, lane);
+  own_rows<DP>(dout, static_cast<const float*>(p.dout) + h * p.D, dense, row, on, p.D, vec, lane);
   float delta = 0.0f;
   {
     float o[DP / 4];
-    auto dot = [&](const void* base) {
-      own_rows<T, DP>(o, static_cast<const T*>(base) + h * p.D, dense, row, on, p.D, vec, lane);
+    own_rows<DP>(o, static_cast<const float*>(p.o) + h * p.D, dense, row, on, p.D, vec, lane);
 #pragma unroll
-      for (int i = 0; i < DP / 4; ++i) delta = fmaf(o[i], dout[i], delta);
-    };
-    dot(p.o);
-    if (p.rest) dot(p.rest);
+    for (int i = 0; i < DP / 4; ++i) delta = fmaf(o[i], dout[i], delta);
   }
   delta = column_sum(delta);
   const float lse = on ? p.lse[static_cast<int64_t>(h) * p.T + row] : INFINITY;
@@ -358,10 +341,10 @@ __global__ __launch_bounds__(256) void any_dq_kernel(const AttnArgs p, int tiles
   f32x4 dq[NB];
 #pragma unroll
   for (int n = 0; n < NB; ++n) dq[n] = f32x4{0, 0, 0, 0};
-  Staged<T, DP, KW * kStep> keys, values;
+  Staged<DP, KW * kStep> keys, values;
   auto fetch = [&](int k0) {
-    keys.fetch(static_cast<const T*>(p.k) + g * p.k_head, p.k_token, k0, p.T, p.D, vec);
-    values.fetch(static_cast<const T*>(p.v) + g * p.v_head, p.v_token, k0, p.T, p.D, vec);
+    keys.fetch(static_cast<const float*>(p.k) + g * p.k_head, p.k_token, k0, p.T, p.D, vec);
+    values.fetch(static_cast<const float*>(p.v) + g * p.v_head, p.v_token, k0, p.T, p.D, vec);
   };
   if (all.lo < all.hi) fetch(all.lo);
   for (int k0 = all.lo; k0 < all.hi; k0 += KW * kStep) {
@@ -400,20 +383,20 @@ __global__ __launch_bounds__(256) void any_dq_kernel(const AttnArgs p, int tiles
     if (r >= z.T) break;
     const int first = __builtin_amdgcn_readlane(start, mine), last = __builtin_amdgcn_readlane(end, mine);
     bool spoilt = false;
-    T* out = static_cast<T*>(z.dq) + (static_cast<int64_t>(r) * z.H + h) * z.D;
+    float* out = static_cast<float*>(z.dq) + (static_cast<int64_t>(r) * z.H + h) * z.D;
     for (int d = lane; d < z.D; d += kWave) {
       float v = 0.0f;
 #pragma unroll
       for (int part = 0; part < KW; ++part) v += sums[((qw * KW + part) * 16 + mine) * P + d];
       spoilt |= v != v;
-      store_from_f32<T>(out + d, first < last ? v * z.scale : 0.0f);
+      store_from_f32<float>(out + d, first < last ? v * z.scale : 0.0f);
     }
-    if (first < last && __any(spoilt)) careful_dq_row<T>(z, h, r, first, lses[(qw * KW) * 16 + mine], deltas[(qw * KW) * 16 + mine]);
+    if (first < last && __any(spoilt)) careful_dq_row<float>(z, h, r, first, lses[(qw * KW) * 16 + mine], deltas[(qw * KW) * 16 + mine]);
   }
 }
 
 // dk and dv: a wave's 16 keys against the query heads of their group, or a part of them
-template <typename T, int DP, int KW>
+template <int DP, int KW>
 __global__ __launch_bounds__(256) void any_dkv_kernel(const AttnArgs p, int tiles, int vec) {
   constexpr int QW = 4 / KW, P = DP + 4, NB = DP / 16;
   extern __shared__ __attribute__((aligned(16))) float lds[];
@@ -430,16 +413,16 @@ __global__ __launch_bounds__(256) void any_dkv_kernel(const AttnArgs p, int tile
   const int lo = wave_min_i(on ? key : p.T), hi = wave_max_i(on ? end : 0);
   const Range all = group_range(lo, hi, reinterpret_cast<int*>(stats));
   float k[DP / 4], v[DP / 4];
-  own_rows<T, DP>(k, static_cast<const T*>(p.k) + g * p.k_head, p.k_token, key, on, p.D, vec, lane);
-  own_rows<T, DP>(v, static_cast<const T*>(p.v) + g * p.v_head, p.v_token, key, on, p.D, vec, lane);
+  own_rows<DP>(k, static_cast<const float*>(p.k) + g * p.k_head, p.k_token, key, on, p.D, vec, lane);
+  own_rows<DP>(v, static_cast<const float*>(p.v) + g * p.v_head, p.v_token, key, on, p.D, vec, lane);
   f32x4 dk[NB], dv[NB];
 #pragma unroll
   for (int n = 0; n < NB; ++n) dk[n] = dv[n] = f32x4{0, 0, 0, 0};
   const int64_t dense = static_cast<int64_t>(p.H) * p.D;
-  Staged<T, DP, KW * kStep> queries, grads;
+  Staged<DP, KW * kStep> queries, grads;
   auto fetch = [&](int h, int r0) {
-    queries.fetch(static_cast<const T*>(p.q) + h * p.q_head, p.q_token, r0, p.T, p.D, vec);
-    grads.fetch(static_cast<const T*>(p.dout) + h * p.D, dense, r0, p.T, p.D, vec);
+    queries.fetch(static_cast<const float*>(p.q) + h * p.q_head, p.q_token, r0, p.T, p.D, vec);
+    grads.fetch(static_cast<const float*>(p.dout) + h * p.D, dense, r0, p.T, p.D, vec);
   };
   if (all.lo < all.hi && h0 < h1) fetch(h0, all.lo);
   for (int h = h0; h < h1; ++h) {
@@ -497,7 +480,7 @@ __global__ __launch_bounds__(256) void any_dkv_kernel(const AttnArgs p, int tile
         bad |= x != x;
         x = first < last ? (which ? x * z.scale : x) : 0.0f;
         if (z.splits > 1) (which ? z.dk_part : z.dv_part)[part0 + at + d] = x;
-        else store_from_f32<T>(static_cast<T*>(which ? z.dk : z.dv) + at + d, x);
+        else store_from_f32<float>(static_cast<float*>(which ? z.dk : z.dv) + at + d, x);
       }
       spoilt[i] |= first < last && __any(bad);
     }
@@ -506,9 +489,45 @@ __global__ __launch_bounds__(256) void any_dkv_kernel(const AttnArgs p, int tile
   for (int i = 0; i < 16 / KW; ++i)
     if (spoilt[i]) {
       const int mine = kw * (16 / KW) + i, r = key0 + 16 * qw + mine;
-      const int first = __builtin_amdgcn_readlane(start, mine), last = __builtin_amdgcn_readlane(end, mine);
-      careful_dkv_row<T>(z, g, r, last, h0, h1, split, 1.0f);
+      const int last = __builtin_amdgcn_readlane(end, mine);
+      careful_dkv_row<float>(z, g, r, last, h0, h1, split, 1.0f);
     }
+}
+
+// bf16 heads of a size that is no whole number of 16 bytes, copied for the matrix kernels into rows that are: a wave a head, zeros behind its
+// elements.  8192 rows of 16/4 heads of 75, forward 140 us, forward and backward 558; in fp32 products from where they lay 1054 and 4631,
+// and of 64 rows no faster.
+struct PadArgs {
+  const uint16_t* from[6];
+  uint16_t* to[6];
+  int64_t token[6], head[6];
+  int heads[6];
+  int D, D8;
+  int64_t T;
+};
+constexpr int kPadRows = 8;  // heads a wave: their loads are under way together
+__global__ __launch_bounds__(256) void pad_heads_kernel(const PadArgs p) {
+  typedef uint32_t __attribute__((aligned(2))) two;  // two elements, wherever they begin
+  const int n = blockIdx.y, lane = threadIdx.x & 63;
+  const uint32_t heads = p.heads[n], rows = static_cast<uint32_t>(p.T) * heads;
+  const uint32_t first = (blockIdx.x * 4 + (threadIdx.x >> 6)) * kPadRows;
+  if (first >= rows) return;
+  const uint16_t* from[kPadRows];
+#pragma unroll
+  for (int i = 0; i < kPadRows; ++i) {
+    const uint32_t row = min(first + i, rows - 1), t = row / heads, h = row - t * heads;
+    from[i] = p.from[n] + t * p.token[n] + h * p.head[n];
+  }
+  uint16_t* to = p.to[n] + static_cast<int64_t>(first) * p.D8;
+  for (int d = 2 * lane; d < p.D8; d += 2 * kWave) {
+    uint32_t x[kPadRows];
+#pragma unroll
+    for (int i = 0; i < kPadRows; ++i)
+      x[i] = d + 1 < p.D ? *reinterpret_cast<const two*>(from[i] + d) : d < p.D ? from[i][d] : 0;
+#pragma unroll
+    for (int i = 0; i < kPadRows; ++i)
+      if (first + i < rows) *reinterpret_cast<uint32_t*>(to + i * p.D8 + d) = x[i];
+  }
 }
 
 // dk and dv from their parts, added in order, four elements a lane (n is the number of fours, or of elements where they are no whole fours)
@@ -544,12 +563,12 @@ void with_head(int D, Fn f) {
   else f(std::integral_constant<int, 256>{}, one);
 }
 
-bool in_fours(const AttnArgs& p, int item, bool backward) {
+bool in_fours(const AttnArgs& p, bool backward) {
   uintptr_t bits = reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v);
-  if (backward) bits |= reinterpret_cast<uintptr_t>(p.o) | reinterpret_cast<uintptr_t>(p.rest) | reinterpret_cast<uintptr_t>(p.dout);
+  if (backward) bits |= reinterpret_cast<uintptr_t>(p.o) | reinterpret_cast<uintptr_t>(p.dout);
   // (a tile's rows lie within 32-bit offsets of its first one)
   const int64_t reach = std::max(std::max(p.q_token, p.k_token), std::max<int64_t>(p.v_token, static_cast<int64_t>(p.H) * p.D));
-  return bits % (4 * item) == 0 && reach < (1 << 20) && (p.q_token | p.q_head | p.k_token | p.k_head | p.v_token | p.v_head | p.D) % 4 == 0;
+  return bits % 16 == 0 && reach < (1 << 20) && (p.q_token | p.q_head | p.k_token | p.k_head | p.v_token | p.v_head | p.D) % 4 == 0;
 }
 
 template <typename K>
@@ -565,40 +584,35 @@ void attention_sort_tiles(const AttnArgs& p, int rows, int32_t* query_order, int
   hipLaunchKernelGGL(sort_tiles_kernel, dim3(2), dim3(1024), 0, s, p, rows, (p.T + rows - 1) / rows, query_order, key_order);
 }
 
-template <typename T, int DP, int KW>
+template <int DP, int KW>
 void any_forward(const AttnArgs& p, int vec, hipStream_t s) {
   static PerDeviceOnce once;
-  allow_lds(any_forward_kernel<T, DP, KW>, kAnyLds<DP, KW>, once);
+  allow_lds(any_forward_kernel<DP, KW>, kAnyLds<DP, KW>, once);
   const int rows = 64 / KW, tiles = (p.T + rows - 1) / rows;
-  hipLaunchKernelGGL((any_forward_kernel<T, DP, KW>), dim3(tiles * p.H), dim3(256), (kAnyLds<DP, KW>), s, p, tiles, vec);
+  hipLaunchKernelGGL((any_forward_kernel<DP, KW>), dim3(tiles * p.H), dim3(256), (kAnyLds<DP, KW>), s, p, tiles, vec);
 }
 
 int attention_any_rows(int D) { return D <= 128 ? 32 : 64; }
 
-void attention_any_forward(const AttnArgs& p, int dtype, hipStream_t s) {
-  auto run = [&](auto tag) {
-    using T = decltype(tag);
-    const int vec = in_fours(p, sizeof(T), false);
-    with_head(p.D, [&](auto d, auto parts) { any_forward<T, decltype(d)::value, decltype(parts)::value>(p, vec, s); });
-  };
-  if (dtype == MI355_F32) run(float{});
-  else run(uint16_t{});
+void attention_any_forward(const AttnArgs& p, hipStream_t s) {
+  const int vec = in_fours(p, false);
+  with_head(p.D, [&](auto d, auto parts) { any_forward<decltype(d)::value, decltype(parts)::value>(p, vec, s); });
 }
 
-template <typename T, int DP, int KW>
+template <int DP, int KW>
 void any_backward(const AttnArgs& p, int vec, hipStream_t s) {
   static PerDeviceOnce once_q, once_kv;
-  allow_lds(any_dq_kernel<T, DP, KW>, kAnyLds<DP, KW>, once_q);
-  allow_lds(any_dkv_kernel<T, DP, KW>, kAnyLds<DP, KW>, once_kv);
+  allow_lds(any_dq_kernel<DP, KW>, kAnyLds<DP, KW>, once_q);
+  allow_lds(any_dkv_kernel<DP, KW>, kAnyLds<DP, KW>, once_kv);
   const int rows = 64 / KW, tiles = (p.T + rows - 1) / rows;
-  hipLaunchKernelGGL((any_dq_kernel<T, DP, KW>), dim3(tiles * p.H), dim3(256), (kAnyLds<DP, KW>), s, p, tiles, vec);
-  hipLaunchKernelGGL((any_dkv_kernel<T, DP, KW>), dim3(tiles * p.G * p.splits), dim3(256), (kAnyLds<DP, KW>), s, p, tiles, vec);
+  hipLaunchKernelGGL((any_dq_kernel<DP, KW>), dim3(tiles * p.H), dim3(256), (kAnyLds<DP, KW>), s, p, tiles, vec);
+  hipLaunchKernelGGL((any_dkv_kernel<DP, KW>), dim3(tiles * p.G * p.splits), dim3(256), (kAnyLds<DP, KW>), s, p, tiles, vec);
 }
 
 template <typename T>
 void join_parts(const AttnArgs& p, hipStream_t s) {
   if (p.splits <= 1) return;
-  const int64_t n = static_cast<int64_t>(p.T) * p.G * p.D;
+  const int64_t n = static_cast<int64_t>(p.T) * p.G * p.D_out;
   const bool fours = n % 4 == 0 && (reinterpret_cast<uintptr_t>(p.dk) | reinterpret_cast<uintptr_t>(p.dv)) % (4 * sizeof(T)) == 0;
   auto launch = [&](auto kernel, int64_t items) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)((items + 255) / 256), 2), dim3(256), 0, s, p.dk_part, p.dv_part, static_cast<T*>(p.dk),
@@ -608,14 +622,9 @@ void join_parts(const AttnArgs& p, hipStream_t s) {
   else launch(join_parts_kernel<T, 1>, n);
 }
 
-void attention_any_backward(const AttnArgs& p, int dtype, hipStream_t s) {
-  auto run = [&](auto tag) {
-    using T = decltype(tag);
-    const int vec = in_fours(p, sizeof(T), true);
-    with_head(p.D, [&](auto d, auto parts) { any_backward<T, decltype(d)::value, decltype(parts)::value>(p, vec, s); });
-  };
-  if (dtype == MI355_F32) run(float{});
-  else run(uint16_t{});
+void attention_any_backward(const AttnArgs& p, hipStream_t s) {
+  const int vec = in_fours(p, true);
+  with_head(p.D, [&](auto d, auto parts) { any_backward<decltype(d)::value, decltype(parts)::value>(p, vec, s); });
 }
 
 }  // namespace mi355
@@ -632,6 +641,7 @@ int check_attention(const char* what, int dtype, int64_t sequences, int64_t T, i
                 (long long)H, (long long)G);
   MI355_REQUIRE((T + kLeastRows - 1) / kLeastRows * H < (1ll << 31), "%s: %lld tokens of %lld heads are too many for one launch", what, (long long)T,
                 (long long)H);
+  MI355_REQUIRE(T * H < (1ll << 31) && H * ((D + 7) / 8 * 8) < (1 << 22), "%s: %lld heads of %lld are too many", what, (long long)H, (long long)D);
   MI355_REQUIRE(D >= 1 && D <= kHeadMax, "%s: head size %lld is not within 1 to %d", what, (long long)D, kHeadMax);
   MI355_REQUIRE(std::isfinite(scale) && scale > 0.0f, "%s: the scale must be finite and positive", what);
   return MI355_OK;
@@ -656,7 +666,45 @@ AttnArgs attention_args(const void* q, int64_t q_token, int64_t q_head, const vo
   p.cu = cu, p.sequences = (int)sequences;
   p.T = (int)T, p.H = (int)H, p.G = (int)G, p.D = (int)D, p.group = (int)(H / G);
   p.scale = scale, p.c = (float)(scale * 1.4426950408889634);
+  p.D_out = (int)D;
   return p;
+}
+
+// an order of the tiles, in whole pieces of 16 bytes
+int64_t order_bytes(int64_t T) { return ((T + kLeastRows - 1) / kLeastRows + 3) / 4 * 16; }
+
+bool padded_heads(int64_t D, int dtype) { return dtype == MI355_BF16 && D % 8 != 0; }
+int64_t padded_bytes(int64_t T, int64_t heads, int64_t D) { return T * heads * ((D + 7) / 8 * 8) * 2; }
+
+// Lets p's q, k and v (and dout, out and its rest) be padded copies in `space`.
+void pad_heads(AttnArgs& p, bool backward, void* space, hipStream_t s) {
+  AttnArgs q = p;
+  PadArgs a = {};
+  a.T = p.T, a.D = p.D, a.D8 = (p.D + 7) / 8 * 8;
+  uint16_t* at = static_cast<uint16_t*>(space);
+  int n = 0;
+  auto add = [&](const void*& x, int64_t token, int64_t head, int heads) {
+    a.from[n] = static_cast<const uint16_t*>(x), a.to[n] = at, a.token[n] = token, a.head[n] = head, a.heads[n] = heads;
+    x = at;
+    at += static_cast<int64_t>(p.T) * heads * a.D8;
+    ++n;
+  };
+  const int64_t dense = static_cast<int64_t>(p.H) * p.D;
+  add(q.q, p.q_token, p.q_head, p.H);
+  add(q.k, p.k_token, p.k_head, p.G);
+  add(q.v, p.v_token, p.v_head, p.G);
+  if (backward) {
+    add(q.dout, dense, p.D, p.H);
+    add(q.o, dense, p.D, p.H);
+    const void* rest = p.rest;
+    if (rest) add(rest, dense, p.D, p.H);
+    q.rest = const_cast<void*>(rest);
+  }
+  q.D = a.D8;
+  q.q_token = static_cast<int64_t>(p.H) * a.D8, q.k_token = q.v_token = static_cast<int64_t>(p.G) * a.D8;
+  q.q_head = q.k_head = q.v_head = a.D8;
+  hipLaunchKernelGGL(pad_heads_kernel, dim3((unsigned)((static_cast<int64_t>(p.T) * p.H + 4 * kPadRows - 1) / (4 * kPadRows)), n), dim3(256), 0, s, a);
+  p = q;
 }
 
 }  // namespace
@@ -672,26 +720,32 @@ extern "C" int mi355_varlen_attention_fwd(const void* q, int64_t q_token_stride,
   AttnArgs p = attention_args(q, q_token_stride, q_head_stride, k, k_token_stride, k_head_stride, v, v_token_stride, v_head_stride,
                               cu_seqlens, sequences, scale, T, H, G, D);
   p.out = out, p.lse = lse, p.rest = dtype == MI355_BF16 ? out_rest : nullptr;
-  const bool matrix = dtype == MI355_BF16 && attention_bf16_covers(p);
+  MI355_REQUIRE(aligned16(workspace), "varlen_attention_fwd: the workspace must start on a 16-byte boundary");
+  const bool matrix = dtype == MI355_BF16, padded = padded_heads(D, dtype);
+  MI355_REQUIRE(!padded || workspace, "varlen_attention_fwd: workspace required for bf16 heads of %lld elements", (long long)D);
+  if (padded) pad_heads(p, false, static_cast<char*>(workspace) + order_bytes(T), as_stream(stream));
+  MI355_REQUIRE(!matrix || attention_bf16_covers(p), "varlen_attention_fwd: bf16 operands must start and stride in whole pieces of 16 bytes");
   const int rows = matrix ? attention_bf16_rows() : attention_any_rows(p.D);
   if (workspace && sorted_tiles(p.sequences, T, (T + rows - 1) / rows, H)) {
     attention_sort_tiles(p, rows, static_cast<int32_t*>(workspace), nullptr, as_stream(stream));
     p.query_order = static_cast<int32_t*>(workspace);
   }
   if (matrix) attention_bf16_forward(p, as_stream(stream));
-  else attention_any_forward(p, dtype, as_stream(stream));
+  else attention_any_forward(p, as_stream(stream));
   return check_launch("varlen_attention_fwd");
 }
 
-extern "C" int64_t mi355_varlen_attention_fwd_workspace_bytes(int64_t T, int64_t H, int64_t sequences) {
-  const int64_t tiles = (T + kLeastRows - 1) / kLeastRows;  // (the most there can be)
-  return T > 0 && sorted_tiles(sequences, T, tiles, H) ? 4 * tiles : 0;
+extern "C" int64_t mi355_varlen_attention_fwd_workspace_bytes(int64_t T, int64_t H, int64_t G, int64_t D, int64_t sequences, int dtype) {
+  if (T < 1 || H < 1 || G < 1 || D < 1) return 0;
+  if (padded_heads(D, dtype)) return order_bytes(T) + padded_bytes(T, H + 2 * G, D);
+  return sorted_tiles(sequences, T, (T + kLeastRows - 1) / kLeastRows, H) ? order_bytes(T) : 0;  // (the most tiles there can be)
 }
 
-extern "C" int64_t mi355_varlen_attention_bwd_workspace_bytes(int64_t T, int64_t H, int64_t G, int64_t D) {
+extern "C" int64_t mi355_varlen_attention_bwd_workspace_bytes(int64_t T, int64_t H, int64_t G, int64_t D, int dtype) {
   if (T < 1 || H < 1 || G < 1 || H % G || D < 1) return 0;
-  const int64_t parts = head_parts(T, H, G), tiles = (T + kLeastRows - 1) / kLeastRows;
-  return 4 * ((2 * H * T + 3) / 4 * 4 + (2 * tiles + 3) / 4 * 4 + (parts > 1 ? 2 * parts * T * G * D : 0));
+  const int64_t parts = head_parts(T, H, G);
+  return 4 * ((2 * H * T + 3) / 4 * 4) + 2 * order_bytes(T) + (padded_heads(D, dtype) ? padded_bytes(T, 4 * H + 2 * G, D) : 0) +
+         (parts > 1 ? 8 * parts * T * G * D : 0);
 }
 
 extern "C" int mi355_varlen_attention_bwd(const void* dout, const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
@@ -709,18 +763,24 @@ extern "C" int mi355_varlen_attention_bwd(const void* dout, const void* q, int64
   p.dout = dout, p.lse = const_cast<float*>(lse), p.dq = dq, p.dk = dk, p.dv = dv;
   p.splits = head_parts(T, H, G);
   p.delta = static_cast<float*>(workspace);
-  const int64_t most_tiles = (T + kLeastRows - 1) / kLeastRows;
-  int32_t* order = reinterpret_cast<int32_t*>(p.delta + (2 * H * T + 3) / 4 * 4);
-  p.dk_part = reinterpret_cast<float*>(order + (2 * most_tiles + 3) / 4 * 4);
+  char* at = reinterpret_cast<char*>(p.delta + (2 * H * T + 3) / 4 * 4);
+  int32_t *query_order = reinterpret_cast<int32_t*>(at), *key_order = reinterpret_cast<int32_t*>(at + order_bytes(T));
+  at += 2 * order_bytes(T);
+  if (padded_heads(D, dtype)) {
+    pad_heads(p, true, at, as_stream(stream));
+    at += padded_bytes(T, 4 * H + 2 * G, D);
+  }
+  p.dk_part = reinterpret_cast<float*>(at);
   p.dv_part = p.dk_part + static_cast<int64_t>(p.splits) * T * G * D;
-  const bool matrix = dtype == MI355_BF16 && attention_bf16_covers(p);
+  const bool matrix = dtype == MI355_BF16;
+  MI355_REQUIRE(!matrix || attention_bf16_covers(p), "varlen_attention_bwd: bf16 operands must start and stride in whole pieces of 16 bytes");
   const int rows = matrix ? attention_bf16_rows() : attention_any_rows(p.D);
   if (sorted_tiles(p.sequences, T, (T + rows - 1) / rows, H)) {
-    attention_sort_tiles(p, rows, order, order + most_tiles, as_stream(stream));
-    p.query_order = order, p.key_order = order + most_tiles;
+    attention_sort_tiles(p, rows, query_order, key_order, as_stream(stream));
+    p.query_order = query_order, p.key_order = key_order;
   }
   if (matrix) attention_bf16_backward(p, as_stream(stream));
-  else attention_any_backward(p, dtype, as_stream(stream));
+  else attention_any_backward(p, as_stream(stream));
   if (dtype == MI355_F32) join_parts<float>(p, as_stream(stream));
   else join_parts<uint16_t>(p, as_stream(stream));
   return check_launch("varlen_attention_bwd");

@@ -19,13 +19,17 @@
 namespace mi355 {
 namespace {
 
+template <int DP>
+constexpr int kWaves = DP <= 128 ? 2 : 1;  // a SIMD, by the registers that sums and operands of a wave's rows take
 constexpr int kTile = 64;     // rows of the other axis a tile
 constexpr int kRows = 32;     // rows a wave
 constexpr uint32_t kFarOff = 1u << 30;  // an offset past every buffer: reads zeros
 
+// (of the low four bits of r; of three for heads beyond 128, so that rows eight apart share it: their row reads meet a bank twice)
 template <int DP>
-__device__ __forceinline__ int swizzle(int r) {  // (of the low four bits of r)
-  return DP == 64 ? (((r >> 1) & 1) << 2) | ((r >> 2) & 3) : ((r & 3) << 2) | ((r >> 2) & 3);
+__device__ __forceinline__ int swizzle(int r) {
+  if constexpr (DP == 64) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+  return ((r & 3) << 2) | ((r >> 2) & (DP == 128 ? 3 : 1));
 }
 
 // LDS byte offsets of a lane's reads of a tile: the swizzle is an exclusive or, and so are the steps over a row's pieces
@@ -43,7 +47,7 @@ struct Reads {
   // 8 elements of row lane % 32, step kk
   __device__ __forceinline__ uint32_t row(int kk) const { return row_ ^ (kk << 5); }
   // elements 32 n + lane % 32 of rows 4 h + {0..3}, or 8 rows on
-  __device__ __forceinline__ uint32_t turned(int n, int half) const { return (turned_ ^ (n << 6) ^ (half << 5)) + half * 8 * DP * 2; }
+  __device__ __forceinline__ uint32_t turned(int n, int half) const { return (turned_ ^ (n << 6) ^ (DP <= 128 ? half << 5 : 0)) + half * 8 * DP * 2; }
 };
 
 __device__ __forceinline__ bf16x8 read_row(uint32_t at) { return lds_read16(at); }
@@ -54,6 +58,9 @@ __device__ __forceinline__ bf16x8 read_turned(const Reads<DP>& reads, int n, uin
   const s16x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
   return __builtin_bit_cast(bf16x8, v);
 }
+
+// the lane, formed anew where a kernel has no register to keep it in
+__device__ __forceinline__ int lane_anew() { return opaque(__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0))); }
 
 // Requests of a workgroup's four waves for a tile of a head's rows, 1 KiB each: a wave's j-th brings rows of its own
 template <int DP>
@@ -68,17 +75,23 @@ struct Requests {
     base = reinterpret_cast<uint64_t>(p);
     row_bytes = token * 2;
     T = T_, D = D_;
+    if constexpr (DP <= 128) voff = offset(lane, wave);
+  }
+  __device__ __forceinline__ uint32_t offset(int lane, int wave) const {
     constexpr int CPR = DP / 8;
-    // (a wave's requests are 4 ROWS = 16 or 32 rows apart: the same swizzle)
+    // (a wave's requests are 4 ROWS = 32, 16 or 8 rows apart: the same swizzle)
     const int r = ROWS * wave + lane / CPR, c = (lane % CPR) ^ swizzle<DP>(r);
-    voff = c * 8 < D_ ? static_cast<uint32_t>(r * row_bytes) + c * 16 : kFarOff;
+    return c * 8 < D ? static_cast<uint32_t>(r * row_bytes) + c * 16 : kFarOff;
   }
   // rows [row0, row0 + 64) to LDS at `lds`; zeros for rows from T on
   __device__ __forceinline__ void request(int row0, uint32_t lds, int wave) const {
     const int64_t left = static_cast<int64_t>(T - 1 - row0) * row_bytes + D * 2;
     const uint32_t bytes = left < 0 ? 0 : left < kFarOff ? static_cast<uint32_t>(left) : kFarOff;
     const uint64_t at = base + static_cast<int64_t>(row0) * row_bytes;
-    const uint32_t step = 4 * ROWS * static_cast<uint32_t>(row_bytes), off = opaque(voff);
+    const uint32_t step = 4 * ROWS * static_cast<uint32_t>(row_bytes);
+    uint32_t off;
+    if constexpr (DP <= 128) off = opaque(voff);
+    else off = offset(lane_anew(), wave);
 #pragma unroll
     for (int j = 0; j < EACH; ++j) lds_load16_within(at, bytes, off + j * step, lds + (4 * j + wave) * 1024);
   }
@@ -153,6 +166,52 @@ __device__ __forceinline__ u32x4 pack8(const float (&v)[8]) {
   return u32x4{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
 }
 
+__device__ __forceinline__ void put8(uint16_t* to, const float (&v)[8]) { *reinterpret_cast<u32x4*>(to) = pack8(v); }
+__device__ __forceinline__ void put8(float* to, const float (&v)[8]) {
+  reinterpret_cast<f32x4*>(to)[0] = f32x4{v[0], v[1], v[2], v[3]};
+  reinterpret_cast<f32x4*>(to)[1] = f32x4{v[4], v[5], v[6], v[7]};
+}
+
+// The first `rows` of the wave's 32 result rows, `D` elements each, to `to` + row * pitch; eight(n, a, v) gives elements 32 n + 16 a + 8 half ..
+// + 7 of the lane's row.  Rows that are whole numbers of 16 bytes are stored from the registers.  Others, whose elements lie anywhere, pass
+// through the wave's quarter of LDS (which everyone is done with by then) and go out row by row, lanes side by side: an
+// element a lane of 32 rows at once took 104 us of a forward's 296 (8192 rows, 16 heads of 150).
+template <int DP, typename E, typename Eight>
+__device__ __forceinline__ void store_rows(E* to, int64_t pitch, int rows, int D, uint16_t* smem, int wave, int lane, Eight eight) {
+  const int half = lane >> 5, row = lane & 31;
+  constexpr int WHOLE = 16 / sizeof(E);
+  E* part = reinterpret_cast<E*>(smem) + wave * 32 * DP;
+  auto at = [&](int r, int d) { return r * DP + (((d / WHOLE) ^ (r & 7)) * WHOLE) + d % WHOLE; };
+  const bool whole = D % 8 == 0;
+#pragma unroll
+  for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      float v[8];
+      eight(n, a, v);
+      const int d = 32 * n + 16 * a + 8 * half;
+      if (whole) {
+        if (row < rows && d < D) put8(to + row * pitch + d, v);
+      } else if constexpr (sizeof(E) == 2) {
+        put8(part + at(row, d), v);
+      } else {
+        *reinterpret_cast<f32x4*>(part + at(row, d)) = f32x4{v[0], v[1], v[2], v[3]};
+        *reinterpret_cast<f32x4*>(part + at(row, d + 4)) = f32x4{v[4], v[5], v[6], v[7]};
+      }
+    }
+  if (whole) return;
+  wave_lds_sync();
+  if (sizeof(E) == 2 && D % 2 == 0) {  // two elements of 2 bytes a lane
+    for (int r = 0; r < rows; ++r)
+      for (int d = 2 * lane; d < D; d += 2 * kWave)
+        *reinterpret_cast<uint32_t*>(to + r * pitch + d) = *reinterpret_cast<const uint32_t*>(part + at(r, d));
+  } else {
+    for (int r = 0; r < rows; ++r)
+      for (int d = lane; d < D; d += kWave) to[r * pitch + d] = part[at(r, d)];
+  }
+  wave_lds_sync();  // read before the next result's rows come
+}
+
 // the workgroup's range over the other axis and the wave's, from every lane's row's
 struct Ranges {
   int lo, hi, first, last;  // workgroup: [lo, hi), wave: [first, last)
@@ -170,7 +229,7 @@ struct Ranges {
 constexpr float kGrowth = 8.0f;  // a row's weights stay below 2^8 of its reference: the reference follows its maximum in such steps
 
 template <int DP>
-__global__ __launch_bounds__(256, 2) void bf16_forward_kernel(const AttnArgs p, int tiles) {
+__global__ __launch_bounds__(256, kWaves<DP>) void bf16_forward_kernel(const AttnArgs p, int tiles) {
   constexpr int KK = DP / 16, NB = DP / 32;
   constexpr uint32_t TILE_BYTES = kTile * DP * 2;
   extern __shared__ __attribute__((aligned(16))) uint16_t smem[];
@@ -276,26 +335,20 @@ __global__ __launch_bounds__(256, 2) void bf16_forward_kernel(const AttnArgs p, 
       o[n][i] = on ? o[n][i] * inverse : 0.0f;
       spoilt |= o[n][i] != o[n][i];
     }
-  if (row < z.T) {
-    const int64_t dense = (static_cast<int64_t>(row) * z.H + h) * z.D;
+  if (z.D_out % 8) __syncthreads();
+  const int rows = min(max(z.T - row0, 0), kRows);
+  const int64_t dense = (static_cast<int64_t>(row0) * z.H + h) * z.D_out, pitch = static_cast<int64_t>(z.H) * z.D_out;
+  store_rows<DP>(static_cast<uint16_t*>(z.out) + dense, pitch, rows, z.D_out, smem, wave, lane,
+                 [&](int n, int a, float (&v)[8]) __attribute__((always_inline)) { eight_of(o[n], a, v); });
+  if (z.rest)
+    store_rows<DP>(static_cast<uint16_t*>(z.rest) + dense, pitch, rows, z.D_out, smem, wave, lane,
+                   [&](int n, int a, float (&v)[8]) __attribute__((always_inline)) {
+                     eight_of(o[n], a, v);
+                     const u32x4 packed = pack8(v);
 #pragma unroll
-    for (int n = 0; n < NB; ++n)
-#pragma unroll
-      for (int a = 0; a < 2; ++a) {
-        float v[8];
-        eight_of(o[n], a, v);
-        const int d = 32 * n + 16 * a + 8 * half;
-        if (d >= z.D) continue;
-        const u32x4 packed = pack8(v);
-        *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(z.out) + dense + d) = packed;
-        if (z.rest) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] -= __uint_as_float(i & 1 ? packed[i / 2] & 0xffff0000u : packed[i / 2] << 16);
-          *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(z.rest) + dense + d) = pack8(v);
-        }
-      }
-    if (half == 0 && z.lse) z.lse[static_cast<int64_t>(h) * z.T + row] = on ? ref + log2f(l) : INFINITY;
-  }
+                     for (int i = 0; i < 8; ++i) v[i] -= __uint_as_float(i & 1 ? packed[i / 2] & 0xffff0000u : packed[i / 2] << 16);
+                   });
+  if (half == 0 && z.lse && row < z.T) z.lse[static_cast<int64_t>(h) * z.T + row] = on ? ref + log2f(l) : INFINITY;
   uint64_t again = __ballot(spoilt && row < z.T);
   again = (again | again >> 32) & 0xffffffffu;
   if (again) lds_wait<0>();
@@ -307,7 +360,7 @@ __global__ __launch_bounds__(256, 2) void bf16_forward_kernel(const AttnArgs p, 
 
 // dq, and delta for the kernel behind this one
 template <int DP>
-__global__ __launch_bounds__(256, 2) void bf16_dq_kernel(const AttnArgs p, int tiles) {
+__global__ __launch_bounds__(256, kWaves<DP>) void bf16_dq_kernel(const AttnArgs p, int tiles) {
   constexpr int KK = DP / 16, NB = DP / 32;
   constexpr uint32_t TILE_BYTES = kTile * DP * 2;
   extern __shared__ __attribute__((aligned(16))) uint16_t smem[];
@@ -414,17 +467,10 @@ __global__ __launch_bounds__(256, 2) void bf16_dq_kernel(const AttnArgs p, int t
       dq[n][i] = on ? dq[n][i] * z.scale : 0.0f;
       spoilt |= dq[n][i] != dq[n][i];
     }
-  if (row < z.T) {
-#pragma unroll
-    for (int n = 0; n < NB; ++n)
-#pragma unroll
-      for (int a = 0; a < 2; ++a) {
-        float v[8];
-        eight_of(dq[n], a, v);
-        const int d = 32 * n + 16 * a + 8 * half;
-        if (d < z.D) *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(z.dq) + dense + d) = pack8(v);
-      }
-  }
+  if (z.D_out % 8) __syncthreads();
+  store_rows<DP>(static_cast<uint16_t*>(z.dq) + (static_cast<int64_t>(row0) * z.H + h) * z.D_out, static_cast<int64_t>(z.H) * z.D_out,
+                 min(max(z.T - row0, 0), kRows), z.D_out, smem, wave, lane,
+                 [&](int n, int a, float (&v)[8]) __attribute__((always_inline)) { eight_of(dq[n], a, v); });
   uint64_t again = __ballot(spoilt && row < z.T);
   again = (again | again >> 32) & 0xffffffffu;
   if (again) lds_wait<0>();
@@ -438,7 +484,7 @@ __global__ __launch_bounds__(256, 2) void bf16_dq_kernel(const AttnArgs p, int t
 
 // dk and dv: a wave's 32 keys against the query heads of their group, or a part of them
 template <int DP>
-__global__ __launch_bounds__(256, 2) void bf16_dkv_kernel(const AttnArgs p, int tiles) {
+__global__ __launch_bounds__(256, kWaves<DP>) void bf16_dkv_kernel(const AttnArgs p, int tiles) {
   constexpr int KK = DP / 16, NB = DP / 32;
   constexpr uint32_t TILE_BYTES = kTile * DP * 2, STAGE = 2 * TILE_BYTES + 512;  // queries, gradients, -lse / c, -delta
   extern __shared__ __attribute__((aligned(16))) uint16_t smem[];
@@ -509,9 +555,11 @@ __global__ __launch_bounds__(256, 2) void bf16_dkv_kernel(const AttnArgs p, int 
         s = mfma(read_row(at_tile.row(kk) + qt + b * 32 * DP * 2), k[kk], s);
         ds = mfma(read_row(at_tile.row(kk) + dt + b * 32 * DP * 2), v[kk], ds);
       }
-      reads_first<12>();
-      interleave<2 * KK - 4, 1, 0>();
-      interleave<4, 0, 0>();
+      if constexpr (DP <= 128) {  // (larger heads have no registers for reads ahead)
+        reads_first<12>();
+        interleave<2 * KK - 4, 1, 0>();
+        interleave<4, 0, 0>();
+      }
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         s[i] = exp2_f32(s[i] * c);
@@ -537,9 +585,11 @@ __global__ __launch_bounds__(256, 2) void bf16_dkv_kernel(const AttnArgs p, int 
       for (int t2 = 0; t2 < 2; ++t2)
 #pragma unroll
         for (int n = 0; n < NB; ++n) dk[n] = mfma(read_turned(at_tile, n, qt + (2 * b + t2) * 16 * DP * 2), w[2 + t2], dk[n]);
-      reads_first<8>();
-      interleave<4 * NB - 4, 2, 0>();
-      interleave<4, 0, 0>();
+      if constexpr (DP <= 128) {
+        reads_first<8>();
+        interleave<4 * NB - 4, 2, 0>();
+        interleave<4, 0, 0>();
+      }
     }
   };
   if (steps) request(h0, range.lo, 0);
@@ -561,28 +611,20 @@ __global__ __launch_bounds__(256, 2) void bf16_dkv_kernel(const AttnArgs p, int 
       dv[n][i] = on ? dv[n][i] : 0.0f;
       spoilt |= dk[n][i] != dk[n][i] || dv[n][i] != dv[n][i];
     }
-  if (key < z.T) {
-    const int64_t dense = (static_cast<int64_t>(key) * z.G + g) * z.D, part = static_cast<int64_t>(split) * z.T * z.G * z.D + dense;
-#pragma unroll
-    for (int n = 0; n < NB; ++n)
-#pragma unroll
-      for (int a = 0; a < 2; ++a)
-#pragma unroll
-        for (int which = 0; which < 2; ++which) {
-          float x[8];
-          eight_of(which ? dk[n] : dv[n], a, x);
-          const int d = 32 * n + 16 * a + 8 * half;
-          if (d >= z.D) continue;
-          if (z.splits > 1) {
-            f32x4* to = reinterpret_cast<f32x4*>((which ? z.dk_part : z.dv_part) + part + d);
-            to[0] = f32x4{x[0], x[1], x[2], x[3]};
-            to[1] = f32x4{x[4], x[5], x[6], x[7]};
-          } else {
-            *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(which ? z.dk : z.dv) + dense + d) = pack8(x);
-          }
-        }
-  }
-  uint64_t again = __ballot(spoilt && key < z.T);
+  if (z.D_out % 8) __syncthreads();
+  const int lane_now = DP <= 128 ? lane : lane_anew();
+  const int rows = min(max(z.T - key0, 0), kRows);
+  const int64_t dense = (static_cast<int64_t>(key0) * z.G + g) * z.D_out, pitch = static_cast<int64_t>(z.G) * z.D_out;
+  auto store = [&](void* to, float* parts, const f32x16 (&x)[NB]) __attribute__((always_inline)) {
+    auto eight = [&](int n, int a, float (&v)[8]) __attribute__((always_inline)) { eight_of(x[n], a, v); };
+    if (z.splits > 1)
+      store_rows<DP>(parts + static_cast<int64_t>(split) * z.T * z.G * z.D_out + dense, pitch, rows, z.D_out, smem, wave, lane_now, eight);
+    else
+      store_rows<DP>(static_cast<uint16_t*>(to) + dense, pitch, rows, z.D_out, smem, wave, lane_now, eight);
+  };
+  store(z.dk, z.dk_part, dk);
+  store(z.dv, z.dv_part, dv);
+  uint64_t again = __ballot(spoilt && key0 + (lane_now & 31) < z.T);
   again = (again | again >> 32) & 0xffffffffu;
   if (again) lds_wait<0>();
   for (; again; again &= again - 1) {
@@ -605,14 +647,17 @@ void allow(K kernel, size_t bytes, PerDeviceOnce& once) {
 
 template <int DP>
 void forward(const AttnArgs& p, hipStream_t s) {
+  static PerDeviceOnce once;
+  allow(bf16_forward_kernel<DP>, kForwardLds<DP>, once);
   const int tiles = (p.T + 4 * kRows - 1) / (4 * kRows);
   hipLaunchKernelGGL(bf16_forward_kernel<DP>, dim3(tiles * p.H), dim3(256), kForwardLds<DP>, s, p, tiles);
 }
 
 template <int DP>
 void backward(const AttnArgs& p, hipStream_t s) {
-  static PerDeviceOnce once;
-  allow(bf16_dkv_kernel<DP>, kDkvLds<DP>, once);
+  static PerDeviceOnce once_q, once_kv;
+  allow(bf16_dq_kernel<DP>, kForwardLds<DP>, once_q);
+  allow(bf16_dkv_kernel<DP>, kDkvLds<DP>, once_kv);
   const int tiles = (p.T + 4 * kRows - 1) / (4 * kRows);
   hipLaunchKernelGGL(bf16_dq_kernel<DP>, dim3(tiles * p.H), dim3(256), kForwardLds<DP>, s, p, tiles);
   hipLaunchKernelGGL(bf16_dkv_kernel<DP>, dim3(tiles * p.G * p.splits), dim3(256), kDkvLds<DP>, s, p, tiles);
@@ -622,25 +667,29 @@ void backward(const AttnArgs& p, hipStream_t s) {
 
 bool attention_bf16_covers(const AttnArgs& p) {
   uintptr_t bits = reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v) |
-                   reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.o) | reinterpret_cast<uintptr_t>(p.rest) |
-                   reinterpret_cast<uintptr_t>(p.dout) | reinterpret_cast<uintptr_t>(p.dq) | reinterpret_cast<uintptr_t>(p.dk) |
-                   reinterpret_cast<uintptr_t>(p.dv);
+                   reinterpret_cast<uintptr_t>(p.o) | reinterpret_cast<uintptr_t>(p.dout);
+  if (p.o) bits |= reinterpret_cast<uintptr_t>(p.rest);
+  if (p.D_out % 8 == 0)  // (else results go out element by element)
+    bits |= reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.rest) | reinterpret_cast<uintptr_t>(p.dq) |
+            reinterpret_cast<uintptr_t>(p.dk) | reinterpret_cast<uintptr_t>(p.dv);
   const int64_t sizes = p.D | p.q_token | p.q_head | p.k_token | p.k_head | p.v_token | p.v_head;
   // a tile's rows lie within 32-bit offsets of its first one
   const int64_t reach = std::max(std::max(p.q_token, p.k_token), std::max<int64_t>(p.v_token, static_cast<int64_t>(p.H) * p.D));
-  return p.D <= 128 && bits % 16 == 0 && sizes % 8 == 0 && reach < (1 << 22);
+  return bits % 16 == 0 && sizes % 8 == 0 && reach < (1 << 22);
 }
 
 int attention_bf16_rows() { return 4 * kRows; }
 
 void attention_bf16_forward(const AttnArgs& p, hipStream_t s) {
   if (p.D <= 64) forward<64>(p, s);
-  else forward<128>(p, s);
+  else if (p.D <= 128) forward<128>(p, s);
+  else forward<256>(p, s);
 }
 
 void attention_bf16_backward(const AttnArgs& p, hipStream_t s) {
   if (p.D <= 64) backward<64>(p, s);
-  else backward<128>(p, s);
+  else if (p.D <= 128) backward<128>(p, s);
+  else backward<256>(p, s);
 }
 
 }  // namespace mi355

@@ -319,16 +319,28 @@ void check_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Te
               "tensors on different devices: queries, keys, values and cu_seqlens must share one");
 }
 
+// The same where the kernels want 16-byte pieces: heads that are whole numbers of them but start or stride elsewhere, or too far apart for
+// 32-bit offsets, are copied.
+Heads aligned_heads(const Tensor& x) {
+  Heads h(x);
+  const int64_t whole = 16 / x.element_size();
+  if (h.size % whole == 0 && (h.token_stride % whole || h.head_stride % whole || h.token_stride >= (1 << 22) ||
+                              reinterpret_cast<uintptr_t>(ptr(h.t)) % 16))
+    h = Heads(h.t.clone(at::MemoryFormat::Contiguous));
+  return h;
+}
+
 std::tuple<Tensor, Tensor, Tensor> varlen_attention_fwd(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& cu_,
                                                         double scale, bool for_backward) {
   Launch L(q_);
   check_attention(q_, k_, v_, cu_);
-  const Heads q(q_), k(k_), v(v_);
+  const Heads q = aligned_heads(q_), k = aligned_heads(k_), v = aligned_heads(v_);
   const Tensor cu = cu_.contiguous();
   Tensor out = at::empty(q_.sizes(), q_.options()), lse = at::empty({q.heads, q.tokens}, q_.options().dtype(at::kFloat));
   Tensor rest = for_backward && q_.scalar_type() == at::kBFloat16 ? at::empty_like(out) : none_like(out);
   Tensor ws;
-  if (const int64_t need = mi355_varlen_attention_fwd_workspace_bytes(q.tokens, q.heads, cu.numel() - 1)) ws = bytes(need, q_);
+  if (const int64_t need = mi355_varlen_attention_fwd_workspace_bytes(q.tokens, q.heads, k.heads, q.size, cu.numel() - 1,
+                                                                           dtype_code(q.t))) ws = bytes(need, q_);
   check(mi355_varlen_attention_fwd(ptr(q.t), q.token_stride, q.head_stride, ptr(k.t), k.token_stride, k.head_stride, ptr(v.t),
                                    v.token_stride, v.head_stride, dtype_code(q.t), iptr(cu), cu.numel() - 1, (float)scale, ptr(out),
                                    ptr(rest), static_cast<float*>(ptr(lse)), ptr(ws), q.tokens, q.heads, k.heads, q.size, L.stream),
@@ -341,14 +353,14 @@ std::tuple<Tensor, Tensor, Tensor> varlen_attention_bwd(const Tensor& dout_, con
                                                         double scale) {
   Launch L(q_);
   check_attention(q_, k_, v_, cu_);
-  const Heads q(q_), k(k_), v(v_);
+  const Heads q = aligned_heads(q_), k = aligned_heads(k_), v = aligned_heads(v_);
   const Tensor dout = heads_like(dout_, q_), out = dense(out_), lse = dense(lse_), rest = dense(rest_), cu = cu_.contiguous();
   TORCH_CHECK_VALUE(dout.sizes() == q_.sizes() && out.sizes() == q_.sizes() && out.scalar_type() == q_.scalar_type() &&
                         lse.numel() == q.heads * q.tokens && lse.scalar_type() == at::kFloat &&
                         (rest.numel() == 0 || (rest.numel() == out.numel() && rest.scalar_type() == out.scalar_type())),
                     "the gradient, the result and its statistics do not fit the queries");
   Tensor dq = at::empty(q_.sizes(), q_.options()), dk = at::empty(k_.sizes(), k_.options()), dv = at::empty(v_.sizes(), v_.options());
-  const Tensor ws = bytes(mi355_varlen_attention_bwd_workspace_bytes(q.tokens, q.heads, k.heads, q.size), q_);
+  const Tensor ws = bytes(mi355_varlen_attention_bwd_workspace_bytes(q.tokens, q.heads, k.heads, q.size, dtype_code(q.t)), q_);
   check(mi355_varlen_attention_bwd(ptr(dout), ptr(q.t), q.token_stride, q.head_stride, ptr(k.t), k.token_stride, k.head_stride,
                                    ptr(v.t), v.token_stride, v.head_stride, ptr(out), ptr(rest), fptr(lse), dtype_code(q.t), iptr(cu),
                                    cu.numel() - 1, (float)scale, ptr(dq), ptr(dk), ptr(dv), ptr(ws), q.tokens, q.heads, k.heads,
