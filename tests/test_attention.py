@@ -31,13 +31,14 @@ HALF_STEP = {BF: 2.0**-8, F32: 2.0**-24}
 gpu = pytest.mark.gpu
 
 
-def reference(q, k, v, dout, cu, scale, dtype):
+def reference(q, k, v, dout, cu, scale, dtype, ds_rounding=None):
     """fp64 values and bounds of out, dq, dk, dv (before the storage rounding), on the CPU."""
     q, k, v, dout = (t.detach().cpu().double() for t in (q, k, v, dout))
     T, H, D = q.shape
     group = H // k.shape[1]
     h = 2.0**-8 if dtype == BF else 0.0
     store = HALF_STEP[dtype]
+    h_ds = h if ds_rounding is None else ds_rounding
     val = [torch.zeros_like(t) for t in (q, q, k, v)]
     off = [torch.zeros_like(t) for t in (q, q, k, v)]
     for a, b in zip(cu, cu[1:]):
@@ -67,7 +68,7 @@ def reference(q, k, v, dout, cu, scale, dtype):
             e_delta = e_delta + 2 * D * U * (G.abs() * out.abs()).sum(1, keepdim=True)
             e_dp = D * U * (G.abs() @ V.abs().T)
             ds = p * (dp - delta)
-            e_ds = TINY * seen * (1 + dp.abs() + delta.abs()) + p * ((dp.abs() + delta.abs() + e_dp + e_delta) * (e + h + 4 * U) + e_dp + e_delta) * (1 + h)
+            e_ds = TINY * seen * (1 + dp.abs() + delta.abs()) + p * ((dp.abs() + delta.abs() + e_dp + e_delta) * (e + h_ds + 4 * U) + e_dp + e_delta) * (1 + h_ds)
             val[1][a:b, head] = scale * (ds @ K)
             off[1][a:b, head] = scale * ((e_ds + (n + 4) * U * ds.abs()) @ K.abs())
             val[2][a:b, g] += scale * (ds.T @ Q)
@@ -154,6 +155,31 @@ def test_attention_matches_the_formula_in_both_directions(lengths, behind, H, G,
     check(got, val, off, dtype)
     if behind:  # rows in no sequence: zeros, not merely small
         assert not any(x[cu[-1]:].any() for x in got)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("D", [64, 96, 75, 200])
+def test_rows_that_see_one_key_or_two(D, dtype):
+    """A row that sees one key has the weight 1: its result is the value, its gradients through the score exactly zero.  Sequences of two rows: what
+    rounding takes from ds weighs most there, and the bound on it (h of ds) is u for the kernels of short sequences up to 128
+    elements, which hold ds in two pieces: h^2 below u."""
+    print(f"varlen_attention of one and two rows {D} {dtype}", flush=True)
+    T, H, G = 150, 4, 2
+    leaves, dout = inputs(T, H, G, D, dtype, seed=17)
+    got = step(leaves, dout, torch.arange(T + 1, dtype=torch.int32, device=DEV))
+    v, g = (t.detach().cpu().double() for t in (leaves[2], dout))
+    # (its weight w = exp2 of what rounding left of score and maximum is not quite 1: w v / w, three roundings of v, of which none is left in bf16)
+    v = v.repeat_interleave(2, 1)
+    assert ((got[0].cpu().double() - v).abs() <= (0.0 if dtype == BF else 3 * U) * v.abs()).all()
+    assert not got[1].any() and not got[2].any()
+    want = g.unflatten(1, (G, H // G)).sum(2)
+    close = (got[3].cpu().double() - want).abs() - (4 * U * g.abs().unflatten(1, (G, H // G)).sum(2) + HALF_STEP[dtype] * want.abs())
+    assert close.max() <= 2.0**-30
+    cu = list(range(0, T + 1, 2))
+    got = step(leaves, dout, torch.tensor(cu, dtype=torch.int32, device=DEV))
+    val, off = reference(*leaves, dout, cu, D**-0.5, dtype, ds_rounding=None if D > 128 or dtype == F32 else 2.0**-16)
+    check(got, val, off, dtype)
 
 
 @gpu

@@ -167,7 +167,7 @@ __device__ __forceinline__ void careful_dq_row(const AttnArgs& p, int h, int row
   for (int j0 = start; j0 <= row; j0 += kWave) {
     const int j = j0 + lane;
     float ds = 0.0f;
-    if (j <= row) {
+    if (j <= row && start < row) {
       const float w = exp2_f32(fmaf(careful_dot<T>(q, row_at<T>(p.k, p.k_token, p.k_head, j, h / p.group), p.D), p.c, -lse));
       ds = w * (careful_dot<T>(dout, row_at<T>(p.v, p.v_token, p.v_head, j, h / p.group), p.D) - delta);
     }
@@ -187,7 +187,7 @@ __device__ __forceinline__ void careful_dq_row(const AttnArgs& p, int h, int row
 
 // dk and dv of one key over the query heads [h0, h1), into the part `split` where there are parts; delta is kept times `sign`
 template <typename T>
-__device__ __forceinline__ void careful_dkv_row(const AttnArgs& p, int g, int key, int end, int h0, int h1, int split, float sign) {
+__device__ __forceinline__ void careful_dkv_row(const AttnArgs& p, int g, int key, int start, int end, int h0, int h1, int split, float sign) {
   const int lane = threadIdx.x & 63;
   const T* k = row_at<T>(p.k, p.k_token, p.k_head, key, g);
   const T* v = row_at<T>(p.v, p.v_token, p.v_head, key, g);
@@ -200,7 +200,7 @@ __device__ __forceinline__ void careful_dkv_row(const AttnArgs& p, int g, int ke
         const T* dout = static_cast<const T*>(p.dout) + (static_cast<int64_t>(r) * p.H + h) * p.D;
         const int64_t at = static_cast<int64_t>(h) * p.T + r;
         w = exp2_f32(fmaf(careful_dot<T>(row_at<T>(p.q, p.q_token, p.q_head, r, h), k, p.D), p.c, -p.lse[at]));
-        ds = w * (careful_dot<T>(dout, v, p.D) - sign * p.delta[at]);
+        ds = start < r ? w * (careful_dot<T>(dout, v, p.D) - sign * p.delta[at]) : 0.0f;
       }
       for (int n = 0; n < kWave && r0 + n < end; ++n) {
         const float wn = __shfl(w, n, kWave), dn = __shfl(ds, n, kWave);

@@ -364,7 +364,7 @@ __global__ __launch_bounds__(256) void any_dq_kernel(const AttnArgs p, int tiles
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int key = kb + 16 * b + 4 * (lane >> 4) + i;
-        const bool seen = on && key >= start && key <= row;
+        const bool seen = on && key >= start && key <= row && start < row;  // (a row's only weight is 1, whatever its score)
         ds[i] = seen ? exp2_f32(fmaf(s[i], p.c, -lse)) * (dp[i] - delta) : 0.0f;
       }
       columns_product<DP>(dq, kb_t, ds, lane);
@@ -447,7 +447,7 @@ __global__ __launch_bounds__(256) void any_dkv_kernel(const AttnArgs p, int tile
           const int r = rb + 16 * b + 4 * (lane >> 4) + i;
           const bool seen = on && r >= key && r < end;
           w[i] = seen ? exp2_f32(fmaf(s[i], p.c, -lse[min(r, p.T - 1)])) : 0.0f;
-          ds[i] = seen ? w[i] * (dp[i] - delta[min(r, p.T - 1)]) : 0.0f;
+          ds[i] = seen && start < r ? w[i] * (dp[i] - delta[min(r, p.T - 1)]) : 0.0f;  // (a row's only weight is 1, whatever its score)
         }
         columns_product<DP>(dv, d_t, w, lane);
         columns_product<DP>(dk, q_t, ds, lane);
@@ -489,8 +489,8 @@ __global__ __launch_bounds__(256) void any_dkv_kernel(const AttnArgs p, int tile
   for (int i = 0; i < 16 / KW; ++i)
     if (spoilt[i]) {
       const int mine = kw * (16 / KW) + i, r = key0 + 16 * qw + mine;
-      const int last = __builtin_amdgcn_readlane(end, mine);
-      careful_dkv_row<float>(z, g, r, last, h0, h1, split, 1.0f);
+      const int first = __builtin_amdgcn_readlane(start, mine), last = __builtin_amdgcn_readlane(end, mine);
+      careful_dkv_row<float>(z, g, r, first, last, h0, h1, split, 1.0f);
     }
 }
 

@@ -153,6 +153,14 @@ __device__ __forceinline__ bf16x8 operand_of(const f32x16& s, int kk) {
   return __builtin_bit_cast(bf16x8, v);
 }
 
+// what rounding took from the operand above, as an operand of its own
+__device__ __forceinline__ bf16x8 rest_of(const f32x16& s, int kk, const bf16x8& rounded) {
+  f32x16 left;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) left[8 * kk + i] = s[8 * kk + i] - static_cast<float>(rounded[i]);
+  return operand_of(left, kk);
+}
+
 // elements 32 n + 8 (2 a + h) .. + 7 of the lane's row from a turned result's block: lane half h's pieces of 4 exchanged for whole ones of 8
 __device__ __forceinline__ void eight_of(const f32x16& o, int a, float (&v)[8]) {
 #pragma unroll
@@ -359,7 +367,7 @@ __global__ __launch_bounds__(256, kWaves<DP>) void bf16_forward_kernel(const Att
 }
 
 // dq, and delta for the kernel behind this one
-template <int DP>
+template <int DP, bool FINE>
 __global__ __launch_bounds__(256, kWaves<DP>) void bf16_dq_kernel(const AttnArgs p, int tiles) {
   constexpr int KK = DP / 16, NB = DP / 32;
   constexpr uint32_t TILE_BYTES = kTile * DP * 2;
@@ -371,7 +379,7 @@ __global__ __launch_bounds__(256, kWaves<DP>) void bf16_dq_kernel(const AttnArgs
   const int row0 = at.tile * 4 * kRows + wave * kRows, row = row0 + (lane & 31);
   int start, end;
   sequence_of(p.cu, p.sequences, p.T, row, start, end);
-  const bool on = start < end;
+  const bool on = start < end, several = on && start < row;  // (a row that sees one key: its weight is 1, whatever its score)
   Ranges range;
   range.find(on ? start : p.T, on ? row + 1 : 0, reinterpret_cast<int*>(smem), wave);
   const int latest = most(on ? start : p.T);
@@ -440,7 +448,7 @@ __global__ __launch_bounds__(256, kWaves<DP>) void bf16_dq_kernel(const AttnArgs
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int key = k0 + 32 * b + 8 * (i >> 2) + 4 * half + (i & 3);
-          ds[i] = on && key >= start && key <= row ? ds[i] : 0.0f;
+          ds[i] = several && key >= start && key <= row ? ds[i] : 0.0f;
         }
       }
 #pragma unroll
@@ -448,10 +456,17 @@ __global__ __launch_bounds__(256, kWaves<DP>) void bf16_dq_kernel(const AttnArgs
         const bf16x8 w = operand_of(ds, t);
 #pragma unroll
         for (int n = 0; n < NB; ++n) dq[n] = mfma(read_turned(reads, n, kt + (2 * b + t) * 16 * DP * 2), w, dq[n]);
+        if constexpr (FINE) {
+          const bf16x8 left = rest_of(ds, t, w);
+#pragma unroll
+          for (int n = 0; n < NB; ++n) dq[n] = mfma(read_turned(reads, n, kt + (2 * b + t) * 16 * DP * 2), left, dq[n]);
+        }
       }
-      reads_first<8>();
-      interleave<2 * NB - 4, 2, 0>();
-      interleave<4, 0, 0>();
+      if constexpr (!FINE) {
+        reads_first<8>();
+        interleave<2 * NB - 4, 2, 0>();
+        interleave<4, 0, 0>();
+      }
     }
   };
   for (int k0 = range.lo; k0 < range.hi; k0 += 2 * kTile) {
@@ -483,8 +498,8 @@ __global__ __launch_bounds__(256, kWaves<DP>) void bf16_dq_kernel(const AttnArgs
 }
 
 // dk and dv: a wave's 32 keys against the query heads of their group, or a part of them
-template <int DP>
-__global__ __launch_bounds__(256, kWaves<DP>) void bf16_dkv_kernel(const AttnArgs p, int tiles) {
+template <int DP, bool FINE>
+__global__ __launch_bounds__(256, FINE ? 1 : kWaves<DP>) void bf16_dkv_kernel(const AttnArgs p, int tiles) {
   constexpr int KK = DP / 16, NB = DP / 32;
   constexpr uint32_t TILE_BYTES = kTile * DP * 2, STAGE = 2 * TILE_BYTES + 512;  // queries, gradients, -lse / c, -delta
   extern __shared__ __attribute__((aligned(16))) uint16_t smem[];
@@ -497,6 +512,7 @@ __global__ __launch_bounds__(256, kWaves<DP>) void bf16_dkv_kernel(const AttnArg
   int start, end;
   sequence_of(p.cu, p.sequences, p.T, key, start, end);
   const bool on = start < end;
+  const int alone = key == start;  // the first row of a sequence sees this key only: its weight is 1, whatever its score
   Ranges range;
   range.find(on ? key : p.T, on ? end : 0, reinterpret_cast<int*>(smem), wave);
   const int earliest = least(on ? end : 0);  // rows from the wave's last key to here see all its keys
@@ -571,7 +587,7 @@ __global__ __launch_bounds__(256, kWaves<DP>) void bf16_dkv_kernel(const AttnArg
           const int r = r0 + 32 * b + 8 * (i >> 2) + 4 * half + (i & 3);
           const bool seen = on && r >= key && r < end;
           s[i] = seen ? s[i] : 0.0f;
-          ds[i] = seen ? ds[i] : 0.0f;
+          ds[i] = seen && r >= key + alone ? ds[i] : 0.0f;
         }
       }
       bf16x8 w[4];
@@ -585,7 +601,15 @@ __global__ __launch_bounds__(256, kWaves<DP>) void bf16_dkv_kernel(const AttnArg
       for (int t2 = 0; t2 < 2; ++t2)
 #pragma unroll
         for (int n = 0; n < NB; ++n) dk[n] = mfma(read_turned(at_tile, n, qt + (2 * b + t2) * 16 * DP * 2), w[2 + t2], dk[n]);
-      if constexpr (DP <= 128) {
+      if constexpr (FINE) {
+#pragma unroll
+        for (int t2 = 0; t2 < 2; ++t2) {
+          const bf16x8 left = rest_of(ds, t2, w[2 + t2]);
+#pragma unroll
+          for (int n = 0; n < NB; ++n) dk[n] = mfma(read_turned(at_tile, n, qt + (2 * b + t2) * 16 * DP * 2), left, dk[n]);
+        }
+      }
+      if constexpr (DP <= 128 && !FINE) {
         reads_first<8>();
         interleave<4 * NB - 4, 2, 0>();
         interleave<4, 0, 0>();
@@ -612,7 +636,7 @@ __global__ __launch_bounds__(256, kWaves<DP>) void bf16_dkv_kernel(const AttnArg
       spoilt |= dk[n][i] != dk[n][i] || dv[n][i] != dv[n][i];
     }
   if (z.D_out % 8) __syncthreads();
-  const int lane_now = DP <= 128 ? lane : lane_anew();
+  const int lane_now = lane_anew();
   const int rows = min(max(z.T - key0, 0), kRows);
   const int64_t dense = (static_cast<int64_t>(key0) * z.G + g) * z.D_out, pitch = static_cast<int64_t>(z.G) * z.D_out;
   auto store = [&](void* to, float* parts, const f32x16 (&x)[NB]) __attribute__((always_inline)) {
@@ -629,7 +653,9 @@ __global__ __launch_bounds__(256, kWaves<DP>) void bf16_dkv_kernel(const AttnArg
   if (again) lds_wait<0>();
   for (; again; again &= again - 1) {
     const int i = __builtin_ctzll(again);
-    careful_dkv_row<uint16_t>(z, g, key0 + i, __builtin_amdgcn_readlane(end, i), h0, h1, split, -1.0f);
+    int first, last;
+    sequence_of(z.cu, z.sequences, z.T, key0 + i, first, last);
+    careful_dkv_row<uint16_t>(z, g, key0 + i, first, last, h0, h1, split, -1.0f);
   }
 }
 
@@ -653,14 +679,26 @@ void forward(const AttnArgs& p, hipStream_t s) {
   hipLaunchKernelGGL(bf16_forward_kernel<DP>, dim3(tiles * p.H), dim3(256), kForwardLds<DP>, s, p, tiles);
 }
 
-template <int DP>
+// ds in two bf16 pieces instead of one, for short sequences: the ds of a row add up to nothing, and of a few keys what rounding takes
+// weighs as much as what is left.  Of sequences of two rows dq and dk are 1.7 and 1.8 times as far from the formula as rounding the results
+// would take them, from three or four on 1.4 times; so short ones cost little either way.
+constexpr int kShortOnAverage = 32;  // rows a sequence
+
+template <int DP, bool FINE>
 void backward(const AttnArgs& p, hipStream_t s) {
   static PerDeviceOnce once_q, once_kv;
-  allow(bf16_dq_kernel<DP>, kForwardLds<DP>, once_q);
-  allow(bf16_dkv_kernel<DP>, kDkvLds<DP>, once_kv);
+  allow(bf16_dq_kernel<DP, FINE>, kForwardLds<DP>, once_q);
+  allow(bf16_dkv_kernel<DP, FINE>, kDkvLds<DP>, once_kv);
   const int tiles = (p.T + 4 * kRows - 1) / (4 * kRows);
-  hipLaunchKernelGGL(bf16_dq_kernel<DP>, dim3(tiles * p.H), dim3(256), kForwardLds<DP>, s, p, tiles);
-  hipLaunchKernelGGL(bf16_dkv_kernel<DP>, dim3(tiles * p.G * p.splits), dim3(256), kDkvLds<DP>, s, p, tiles);
+  hipLaunchKernelGGL((bf16_dq_kernel<DP, FINE>), dim3(tiles * p.H), dim3(256), kForwardLds<DP>, s, p, tiles);
+  hipLaunchKernelGGL((bf16_dkv_kernel<DP, FINE>), dim3(tiles * p.G * p.splits), dim3(256), kDkvLds<DP>, s, p, tiles);
+}
+template <int DP>
+void backward(const AttnArgs& p, hipStream_t s) {
+  if constexpr (DP <= 128) {  // (larger heads have no registers for it)
+    if (p.T < static_cast<int64_t>(kShortOnAverage) * p.sequences) return backward<DP, true>(p, s);
+  }
+  backward<DP, false>(p, s);
 }
 
 }  // namespace
