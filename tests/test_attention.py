@@ -136,6 +136,9 @@ CASES = [
     ([0, 301, 2], 1, 2, 2, 33),
     ([250], 0, 2, 1, 201),
     ([300], 5, 2, 1, 1),
+    ([2, 0, 3] * 50, 1, 2, 1, 64),        # more boundaries than a wave has lanes ...
+    ([0] * 200 + [40] + [0] * 100 + [9] * 30, 0, 2, 2, 64),
+    ([1, 0, 2] * 1400, 3, 1, 1, 32),      # ... and than lanes times lanes
     ([600, 520], 7, 8, 8, 64),   # long on average and more tiles than the card holds at once: sorted by their work
     ([512, 3, 1100], 0, 16, 4, 40),
 ]
