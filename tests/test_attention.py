@@ -331,6 +331,59 @@ def test_streams_and_graphs_over_other_lengths_give_the_same_bits():
 
 
 @gpu
+@pytest.mark.parametrize("dtype,D", [(BF, 64), (BF, 33), (F32, 64)])
+def test_rows_beyond_32_bit_offsets(dtype, D):
+    """Heads that are views of rows so long that the last ones begin past 4 GiB: the same bits as of dense copies."""
+    T = 700_000
+    print(f"varlen_attention of rows 8 KiB apart, {T} of them, {dtype} {D}", flush=True)
+    wide = torch.empty(T, 4096 if dtype == BF else 2048, dtype=dtype, device=DEV)
+    assert wide.numel() * wide.element_size() > 5 << 30
+    wide[:, -4 * D:].normal_(generator=torch.Generator(device=DEV).manual_seed(3))
+    heads = [wide[:, -4 * D:-2 * D].view(T, 2, D), wide[:, -2 * D:-D].view(T, 1, D), wide[:, -D:].view(T, 1, D)]
+    cu = torch.arange(0, T + 1, 100, dtype=torch.int32, device=DEV)
+    dout = torch.randn(T, 2, D, dtype=dtype, device=DEV)
+    far = step([t.detach().requires_grad_() for t in heads], dout, cu)
+    near = step([t.detach().contiguous().requires_grad_() for t in heads], dout, cu)
+    assert all(torch.equal(a, b) for a, b in zip(far, near))
+    last = slice(T - 100, T)  # and the last sequence against the formula
+    val, off = reference(*(t[last] for t in heads), dout[last], [0, 100], D**-0.5, dtype)
+    check([t[last] for t in far], val, off, dtype)
+
+
+@gpu
+def test_two_calls_at_once_and_a_traced_one_give_the_same_bits():
+    cu = torch.tensor([0, 700, 1500], dtype=torch.int32, device=DEV)
+    inv_freq = ops.rotary_frequencies(64, device=DEV)[0]
+    positions = torch.arange(1500, device=DEV)
+    weight = torch.ones(64, dtype=BF, device=DEV)
+
+    def layer(q, k, v):
+        q, k = ops.qk_norm_rotary(q, k, weight, weight, positions, inv_freq, 1e-6)
+        q, k = ops.rotary(q, k, positions, inv_freq, interleaved=True)
+        return ops.varlen_attention(q, k, v, cu)
+
+    sets = [inputs(1500, 8, 2, 64, BF, seed=s) for s in (1, 2)]
+
+    def whole(leaves, dout, f=layer):
+        out = f(*leaves)
+        return [out.detach(), *torch.autograd.grad(out, leaves, dout)]
+
+    want = [whole(*s) for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = []
+    for s, (leaves, dout) in zip(streams, sets):
+        with torch.cuda.stream(s):
+            got.append([whole(leaves, dout) for _ in range(3)])
+    torch.cuda.synchronize()
+    for runs, w in zip(got, want):
+        assert all(torch.equal(a, b) for run in runs for a, b in zip(run, w))
+    traced = torch.compile(layer, backend="aot_eager", fullgraph=True)
+    assert all(torch.equal(a, b) for a, b in zip(whole(*sets[0], traced), want[0]))
+
+
+@gpu
 def test_bounds_out_of_order_stay_inside_the_tensors():
     """Entries that no caller should pass: results mean nothing, but every look-up stays inside (the sequence of a row always contains
     it) and rows keep to what a call with sound bounds writes."""
@@ -362,6 +415,30 @@ def test_no_tokens_and_only_some_gradients():
     assert torch.equal(torch.ops.mi355_moe.varlen_attention_bwd(
         dout.float(), *(t.detach() for t in leaves), *torch.ops.mi355_moe.varlen_attention_fwd(
             *(t.detach() for t in leaves), cu, 64**-0.5, True), cu, 64**-0.5)[0], want[1])
+
+
+@gpu
+def test_a_derivative_of_the_backward_is_refused():
+    (q, k, v), dout = inputs(40, 4, 2, 64, BF, seed=5)
+    cu = torch.tensor([0, 40], dtype=torch.int32, device=DEV)
+    weights = [torch.ones(64, dtype=BF, device=DEV, requires_grad=True) for _ in "qk"]
+    positions, inv_freq = torch.arange(40, device=DEV), ops.rotary_frequencies(64, device=DEV)[0]
+    runs = {
+        "varlen_attention_bwd": (lambda: ops.varlen_attention(q, k, v, cu), dout, (q, k, v)),
+        "qk_norm_rotary_bwd": (lambda: ops.qk_norm_rotary(q, k, *weights, positions, inv_freq, 1e-6)[0], torch.ones_like(q), (q, weights[0])),
+    }
+    for name, (run, grad, leaves) in runs.items():
+        plain = torch.autograd.grad(run(), leaves, grad)
+        assert not any(g.requires_grad for g in plain)
+        kept = torch.autograd.grad(run(), leaves, grad, create_graph=True)  # by itself no error
+        assert all(torch.equal(a, b) for a, b in zip(plain, kept))
+        with pytest.raises(RuntimeError, match=f"{name} is not implemented"):
+            torch.autograd.grad(kept[0], leaves[0], torch.ones_like(kept[0]))
+    # a rotation is linear: its backward has one
+    g = torch.ones_like(q, requires_grad=True)
+    dq, = torch.autograd.grad(ops.rotary(q, k, positions, inv_freq)[0], q, g, create_graph=True)
+    again, = torch.autograd.grad(dq, g, dout)
+    assert torch.equal(again, ops.rotary(dout, k.detach(), positions, inv_freq)[0])
 
 
 @gpu
@@ -491,6 +568,7 @@ def test_c_entry_points_refuse_before_any_launch():
     text(forward(workspace=p + 4), b"16-byte")
     text(forward(H=65536, G=1), b"no multiple")
     text(forward(H=32768, G=1, D=128), b"too many")
+    text(forward(T=1 << 25, H=64, G=1, D=8, sequences=0), b"too many")
     assert forward(T=0) == 0
     text(backward(H=3), b"no multiple")
     text(backward(workspace=None), b"null pointer")

@@ -9,11 +9,16 @@
 // 4 g + i of each 16 too, so that a lane reads 16 bytes of a row for four steps.
 //
 // Rows of the other operand pass through LDS in tiles of 32 a wave column, at a pitch of 4 floats beyond the head: the row reads
-// (16 rows, 16 bytes) and the column reads (four rows 4 apart, 16 floats) both meet every bank once.  Bound by the fp32 matrix
-// rate, 256 flops a cycle and CU; a wave's softmax is a twentieth of its products.
+// (16 rows, 16 bytes) and the column reads (four rows 4 apart, 16 floats) both meet every bank once.  The next tile is on its way to registers
+// while this one is read.
 //
-// A workgroup is four waves: QW groups of 16 rows by KW parts of the other axis, each with its own running
-// maximum and sum, joined through LDS at the end.  Four parts where the rows alone would not fill the card.
+// A workgroup is four waves: two groups of 16 rows by two parts of the other axis, each with its own running maximum and sum, joined
+// through LDS at the end; four groups and one part for heads beyond 128, whose tiles would take too many registers.  Four parts of one group, and
+// one of four, were no faster for heads of 64 either.
+//
+// Measured: 2048 rows in 3 uneven sequences, 8/2 heads of 64: forward 47 us, dq 60, dk/dv 90, where the seven products of the formulas (5.8 GFLOP) take
+// 43 at the rate of a large fp32 product (137 TFLOP/s) and the kernels form nine.  512 workgroups are two waves a SIMD, and the last rows
+// of a sequence see dozens of times what its first ones do: the longest workgroup sets the time, waiting for its products and LDS reads in turn.
 #include <algorithm>
 #include <cmath>
 
@@ -510,23 +515,24 @@ __global__ __launch_bounds__(256) void pad_heads_kernel(const PadArgs p) {
   typedef uint32_t __attribute__((aligned(2))) two;  // two elements, wherever they begin
   const int n = blockIdx.y, lane = threadIdx.x & 63;
   const uint32_t heads = p.heads[n], rows = static_cast<uint32_t>(p.T) * heads;
-  const uint32_t first = (blockIdx.x * 4 + (threadIdx.x >> 6)) * kPadRows;
-  if (first >= rows) return;
-  const uint16_t* from[kPadRows];
+  // (T x heads is under 2^31)
+  for (uint32_t first = (blockIdx.x * 4 + (threadIdx.x >> 6)) * kPadRows; first < rows; first += gridDim.x * 4 * kPadRows) {
+    const uint16_t* from[kPadRows];
 #pragma unroll
-  for (int i = 0; i < kPadRows; ++i) {
-    const uint32_t row = min(first + i, rows - 1), t = row / heads, h = row - t * heads;
-    from[i] = p.from[n] + t * p.token[n] + h * p.head[n];
-  }
-  uint16_t* to = p.to[n] + static_cast<int64_t>(first) * p.D8;
-  for (int d = 2 * lane; d < p.D8; d += 2 * kWave) {
-    uint32_t x[kPadRows];
+    for (int i = 0; i < kPadRows; ++i) {
+      const uint32_t row = min(first + i, rows - 1), t = row / heads, h = row - t * heads;
+      from[i] = p.from[n] + t * p.token[n] + h * p.head[n];
+    }
+    uint16_t* to = p.to[n] + static_cast<int64_t>(first) * p.D8;
+    for (int d = 2 * lane; d < p.D8; d += 2 * kWave) {
+      uint32_t x[kPadRows];
 #pragma unroll
-    for (int i = 0; i < kPadRows; ++i)
-      x[i] = d + 1 < p.D ? *reinterpret_cast<const two*>(from[i] + d) : d < p.D ? from[i][d] : 0;
+      for (int i = 0; i < kPadRows; ++i)
+        x[i] = d + 1 < p.D ? *reinterpret_cast<const two*>(from[i] + d) : d < p.D ? from[i][d] : 0;
 #pragma unroll
-    for (int i = 0; i < kPadRows; ++i)
-      if (first + i < rows) *reinterpret_cast<uint32_t*>(to + i * p.D8 + d) = x[i];
+      for (int i = 0; i < kPadRows; ++i)
+        if (first + i < rows) *reinterpret_cast<uint32_t*>(to + i * p.D8 + d) = x[i];
+    }
   }
 }
 
@@ -534,20 +540,20 @@ __global__ __launch_bounds__(256) void pad_heads_kernel(const PadArgs p) {
 template <typename T, int N>
 __global__ __launch_bounds__(256) void join_parts_kernel(const float* __restrict__ dk_part, const float* __restrict__ dv_part,
                                                          T* __restrict__ dk, T* __restrict__ dv, int splits, int64_t n) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= n) return;
-  const float* part = (blockIdx.y ? dv_part : dk_part) + N * i;
-  T* out = (blockIdx.y ? dv : dk) + N * i;
-  if constexpr (N == 4) {
-    f32x4 v = {0, 0, 0, 0};
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
+    const float* part = (blockIdx.y ? dv_part : dk_part) + N * i;
+    T* out = (blockIdx.y ? dv : dk) + N * i;
+    if constexpr (N == 4) {
+      f32x4 v = {0, 0, 0, 0};
 #pragma unroll 4
-    for (int s = 0; s < splits; ++s) v += __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(part + s * n * N));
-    if constexpr (sizeof(T) == 4) *reinterpret_cast<f32x4*>(out) = v;
-    else *reinterpret_cast<u32x2*>(out) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
-  } else {
-    float v = 0.0f;
-    for (int s = 0; s < splits; ++s) v += part[s * n];
-    store_from_f32<T>(out, v);
+      for (int s = 0; s < splits; ++s) v += __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(part + s * n * N));
+      if constexpr (sizeof(T) == 4) *reinterpret_cast<f32x4*>(out) = v;
+      else *reinterpret_cast<u32x2*>(out) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+    } else {
+      float v = 0.0f;
+      for (int s = 0; s < splits; ++s) v += part[s * n];
+      store_from_f32<T>(out, v);
+    }
   }
 }
 
@@ -615,8 +621,9 @@ void join_parts(const AttnArgs& p, hipStream_t s) {
   const int64_t n = static_cast<int64_t>(p.T) * p.G * p.D_out;
   const bool fours = n % 4 == 0 && (reinterpret_cast<uintptr_t>(p.dk) | reinterpret_cast<uintptr_t>(p.dv)) % (4 * sizeof(T)) == 0;
   auto launch = [&](auto kernel, int64_t items) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((items + 255) / 256), 2), dim3(256), 0, s, p.dk_part, p.dv_part, static_cast<T*>(p.dk),
-                       static_cast<T*>(p.dv), p.splits, items);
+    const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((items + 255) / 256, 1 << 20));
+    hipLaunchKernelGGL(kernel, dim3(blocks, 2), dim3(256), 0, s, p.dk_part, p.dv_part, static_cast<T*>(p.dk), static_cast<T*>(p.dv), p.splits,
+                       items);
   };
   if (fours) launch(join_parts_kernel<T, 4>, n / 4);
   else launch(join_parts_kernel<T, 1>, n);
@@ -639,9 +646,10 @@ int check_attention(const char* what, int dtype, int64_t sequences, int64_t T, i
                 (long long)T, (long long)sequences);
   MI355_REQUIRE(H >= 1 && G >= 1 && H <= 65535 && H % G == 0, "%s: %lld query heads are no multiple of %lld key heads", what,
                 (long long)H, (long long)G);
-  MI355_REQUIRE((T + kLeastRows - 1) / kLeastRows * H < (1ll << 31), "%s: %lld tokens of %lld heads are too many for one launch", what, (long long)T,
-                (long long)H);
-  MI355_REQUIRE(T * H < (1ll << 31) && H * ((D + 7) / 8 * 8) < (1 << 22), "%s: %lld heads of %lld are too many", what, (long long)H, (long long)D);
+  // (2^24 workgroups of 256 lanes a launch)
+  MI355_REQUIRE((T + 127) / 128 * H < (1ll << (dtype == MI355_BF16 ? 24 : 22)), "%s: %lld tokens of %lld heads are too many for one launch", what,
+                (long long)T, (long long)H);
+  MI355_REQUIRE(H * ((D + 7) / 8 * 8) < (1 << 22), "%s: %lld heads of %lld are too many", what, (long long)H, (long long)D);
   MI355_REQUIRE(D >= 1 && D <= kHeadMax, "%s: head size %lld is not within 1 to %d", what, (long long)D, kHeadMax);
   MI355_REQUIRE(std::isfinite(scale) && scale > 0.0f, "%s: the scale must be finite and positive", what);
   return MI355_OK;
@@ -703,7 +711,8 @@ void pad_heads(AttnArgs& p, bool backward, void* space, hipStream_t s) {
   q.D = a.D8;
   q.q_token = static_cast<int64_t>(p.H) * a.D8, q.k_token = q.v_token = static_cast<int64_t>(p.G) * a.D8;
   q.q_head = q.k_head = q.v_head = a.D8;
-  hipLaunchKernelGGL(pad_heads_kernel, dim3((unsigned)((static_cast<int64_t>(p.T) * p.H + 4 * kPadRows - 1) / (4 * kPadRows)), n), dim3(256), 0, s, a);
+  const int64_t blocks = std::min<int64_t>((static_cast<int64_t>(p.T) * p.H + 4 * kPadRows - 1) / (4 * kPadRows), 1 << 22);
+  hipLaunchKernelGGL(pad_heads_kernel, dim3((unsigned)blocks, n), dim3(256), 0, s, a);
   p = q;
 }
 

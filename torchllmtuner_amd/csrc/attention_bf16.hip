@@ -1,5 +1,5 @@
 // Causal attention over packed sequences (attention.h has the formulas) on v_mfma_f32_32x32x16_bf16: bf16 storage, head sizes in whole
-// 16-byte pieces up to 128, fp32 sums and statistics.
+// 16-byte pieces up to 256, fp32 sums and statistics.
 //
 // The matrix instruction takes per lane 8 elements of a row (column) lane % 32 at k = 8 (lane / 32) .. + 7 and yields 16 fp32 of column
 // lane % 32, rows 8 (i / 4) + 4 (lane / 32) + i % 4.  Products are formed turned so that a result is the next product's right operand where
@@ -12,6 +12,11 @@
 // A wave holds 32 rows (queries, or keys), a workgroup four waves.  The other axis passes through LDS in tiles of 64 rows, requested
 // straight into LDS a tile ahead, two buffers, one barrier a tile.  A row's 16-byte pieces are swizzled by a key of its
 // number that spreads both the row reads (16 rows, one piece) and the transposing reads (4 rows, 64 bytes) over all banks.
+//
+// Bound by the matrix pipes and the vector work beside them, which add up at two waves a SIMD rather than hide each other; a third wave, and
+// priorities around the products, did not help.  32/4 heads of 128, where a large library product reaches 1200 TFLOP/s: forward of one sequence of 8192
+// rows 0.50-0.53 ms, 1040-1100 TFLOP/s; forward, dq and dk/dv of 8192 rows in 4 sequences 172, 242 and 296 us, 800, 850 and 930
+// (two, three and four products); of 16384 in 11 uneven ones 351, 497 and 624, 760, 810 and 860.
 #include <algorithm>
 
 #include "attention.h"

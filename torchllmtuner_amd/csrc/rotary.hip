@@ -392,6 +392,8 @@ __global__ __launch_bounds__(1024) void qk_dw_final_kernel(const float* __restri
 // instead of 128, three, the last quarter waited for the others: 60 us where it is 47 now, 8192 tokens x 36 heads of 128, 4.8 TB/s).
 constexpr int kBwdBlocks = 1024;
 
+constexpr int kMostBlocks = 1 << 22;  // of a launch; waves go on to further tokens
+
 // the most elements (16 bytes' worth down to 1) that every piece is a whole number of and starts on
 int piece_of(const QkArgs& p, int dtype, std::initializer_list<const void*> ptrs) {
   uintptr_t bits = 0;
@@ -482,7 +484,7 @@ extern "C" int mi355_rotary(const void* q, int64_t q_token_stride, int64_t q_hea
   MI355_REQUIRE(q && k && positions && inv_freq && q_out && k_out, "rotary: null pointer");
   p.sign = transpose ? -1.0f : 1.0f;
   p.oq = q_out, p.ok = k_out;
-  return launch_qk<kTurn>("rotary", p, dtype, interleaved, INT32_MAX, stream, nullptr);
+  return launch_qk<kTurn>("rotary", p, dtype, interleaved, kMostBlocks, stream, nullptr);
 }
 
 extern "C" int mi355_qk_norm_rotary_fwd(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
@@ -497,7 +499,7 @@ extern "C" int mi355_qk_norm_rotary_fwd(const void* q, int64_t q_token_stride, i
   if (T == 0) return MI355_OK;
   MI355_REQUIRE(q && k && q_weight && k_weight && positions && inv_freq && q_out && k_out, "qk_norm_rotary_fwd: null pointer");
   p.wq = q_weight, p.wk = k_weight, p.eps = epsilon, p.oq = q_out, p.ok = k_out;
-  return launch_qk<kNormTurn>("qk_norm_rotary_fwd", p, dtype, interleaved, INT32_MAX, stream, nullptr);
+  return launch_qk<kNormTurn>("qk_norm_rotary_fwd", p, dtype, interleaved, kMostBlocks, stream, nullptr);
 }
 
 extern "C" int64_t mi355_qk_norm_rotary_bwd_workspace_bytes(int64_t D) {

@@ -10,10 +10,12 @@
 // Conventions shared with ops.py: an output that was not asked for is an empty (0,) tensor; a
 // gradient that is not needed is returned undefined; incoming gradients are not materialised, so
 // an output nobody differentiated arrives undefined.
+#include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/library.h>
 
+#include <optional>
 #include <tuple>
 
 #include "torch_common.h"
@@ -28,6 +30,15 @@ using torch::autograd::variable_list;
 
 OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
 Tensor keep(const Tensor& t, bool wanted) { return wanted ? t : Tensor(); }
+
+// A backward operator without a derivative: a pass that is itself differentiated (create_graph) reaches it through its Autograd key, whose
+// fallback leaves the gradients with a node that raises; any other pass goes straight to the kernel.
+struct BelowUnlessDifferentiated {
+  std::optional<at::AutoDispatchBelowADInplaceOrView> below;
+  BelowUnlessDifferentiated() {
+    if (!at::GradMode::is_enabled()) below.emplace();
+  }
+};
 
 // ---- router gate: dX in the input dtype, dW in the weight dtype --------------------------------
 using GateFwdSig = Tensor(const Tensor&, const Tensor&, const OptTensor&);
@@ -445,6 +456,7 @@ struct QkNormRotary : public torch::autograd::Function<QkNormRotary> {
     const bool dx = need[0] || need[1], dw = need[2] || need[3];
     if (!(dx || dw)) return out;
     const auto s = ctx->get_saved_variables();
+    const BelowUnlessDifferentiated guard;
     static auto op = typed_op<QkNormBwdSig>("mi355_moe::qk_norm_rotary_bwd");
     auto r = op.call(opt(grads[0]), opt(grads[1]), s[0], s[1], s[2], s[3], s[4], s[5], ctx->saved_data["eps"].toDouble(),
                      ctx->saved_data["interleaved"].toBool(), ctx->saved_data["factor"].toDouble(), dx, dw);
@@ -489,6 +501,7 @@ struct VarlenAttention : public torch::autograd::Function<VarlenAttention> {
     const bool n0 = ctx->needs_input_grad(0), n1 = ctx->needs_input_grad(1), n2 = ctx->needs_input_grad(2);
     if (!grads[0].defined() || !(n0 || n1 || n2)) return out;
     const auto s = ctx->get_saved_variables();
+    const BelowUnlessDifferentiated guard;
     static auto op = typed_op<AttentionBwdSig>("mi355_moe::varlen_attention_bwd");
     auto r = op.call(grads[0], s[0], s[1], s[2], s[3], s[4], s[5], s[6], ctx->saved_data["scale"].toDouble());
     out[0] = keep(std::get<0>(r), n0);
@@ -664,7 +677,9 @@ TORCH_LIBRARY_IMPL(mi355_moe, Autograd, m) {
   m.impl("rms_norm_fwd", rms_norm_autograd);
   m.impl("rotary", rotary_autograd);
   m.impl("qk_norm_rotary_fwd", qk_norm_rotary_autograd);
+  m.impl("qk_norm_rotary_bwd", torch::autograd::autogradNotImplementedFallback());
   m.impl("varlen_attention_fwd", varlen_attention_autograd);
+  m.impl("varlen_attention_bwd", torch::autograd::autogradNotImplementedFallback());
   m.impl("balance_loss_fwd", balance_loss_autograd);
   m.impl("permute_rows_fwd", permute_rows_autograd);
   m.impl("combine_fwd", combine_autograd);

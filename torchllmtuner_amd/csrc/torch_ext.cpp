@@ -287,6 +287,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> qk_norm_rotary_bwd(const OptTensor& d
   const Tensor qw = qw_.contiguous(), kw = kw_.contiguous(), inv_freq = inv_freq_.contiguous();
   const Positions positions(positions_);
   TORCH_CHECK_VALUE(dq_out.sizes() == q_.sizes() && dk_out.sizes() == k_.sizes(), "gradients must have the results' shapes");
+  TORCH_CHECK(dq_out.device() == q_.device() && dk_out.device() == q_.device(), "tensors on different devices: gradients must be on the heads'");
   Tensor dq = need_dx ? at::empty(q_.sizes(), q_.options()) : none_like(q_);
   Tensor dk = need_dx ? at::empty(k_.sizes(), k_.options()) : none_like(k_);
   Tensor dqw = need_dw ? at::empty(qw_.sizes(), qw_.options()) : none_like(qw_);
@@ -358,7 +359,9 @@ std::tuple<Tensor, Tensor, Tensor> varlen_attention_bwd(const Tensor& dout_, con
   TORCH_CHECK_VALUE(dout.sizes() == q_.sizes() && out.sizes() == q_.sizes() && out.scalar_type() == q_.scalar_type() &&
                         lse.numel() == q.heads * q.tokens && lse.scalar_type() == at::kFloat &&
                         (rest.numel() == 0 || (rest.numel() == out.numel() && rest.scalar_type() == out.scalar_type())),
-                    "the gradient, the result and its statistics do not fit the queries");
+                    "varlen_attention: the gradient, the result and its statistics do not fit the queries");
+  for (const Tensor* t : {&dout, &out, &lse, &rest})
+    TORCH_CHECK(t->device() == q_.device(), "tensors on different devices: the gradient, the result and its statistics must be on the queries'");
   Tensor dq = at::empty(q_.sizes(), q_.options()), dk = at::empty(k_.sizes(), k_.options()), dv = at::empty(v_.sizes(), v_.options());
   const Tensor ws = bytes(mi355_varlen_attention_bwd_workspace_bytes(q.tokens, q.heads, k.heads, q.size, dtype_code(q.t)), q_);
   check(mi355_varlen_attention_bwd(ptr(dout), ptr(q.t), q.token_stride, q.head_stride, ptr(k.t), k.token_stride, k.head_stride,

@@ -1,4 +1,4 @@
-"""Kernel-registry seam: ``moe_token_permute`` and ``rms_norm`` served by the MI355X kernels.
+"""Kernel-registry seam: ``moe_token_permute``, ``rms_norm`` and the attention half of a decoder layer served by the MI355X kernels.
 
 The reference routes a handful of operators through a name -> {device type -> callable}
 registry (``llmtuner/kernel/registry.py:22-103``) and exposes the MoE row gather as
@@ -17,7 +17,8 @@ reference's own registry::
     register_kernel("rms_norm", "cuda")(rms_norm_mi355)
 
 ``rms_norm`` (``llmtuner/kernel/ops/rms_norm.py:10-31``) is the norm the decoder layer applies
-right before the MoE block; it gets a ``"cuda"`` backend the same way.
+right before the MoE block; it gets a ``"cuda"`` backend the same way.  So do ``rotary``, ``qk_norm_rotary`` and
+``varlen_attention``, what the layer computes between its projections in front of that norm.
 
 There is no torch-math backend here: asking for one (``use_eager=True``, a CPU tensor,
 ``fallback_to_cpu=True`` with nothing registered for ``"cpu"``) raises.

@@ -575,7 +575,7 @@ def varlen_attention(q, k, v, cu_seqlens, *, scale=None):
     lengths.  Differentiable in queries, keys and values; bit-identical from run to run."""
     if not q.is_cuda:
         _dev(q)
-    return _varlen_attention(q, k, v, cu_seqlens, q.shape[-1] ** -0.5 if scale is None else float(scale), False)[0]
+    return _varlen_attention(q, k, v, cu_seqlens, max(q.shape[-1], 1) ** -0.5 if scale is None else float(scale), False)[0]
 
 
 def _as_bool(m):
