@@ -162,6 +162,43 @@ def test_attention_matches_the_formula_in_both_directions(lengths, behind, H, G,
 
 @gpu
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("lengths,behind,H,G,D", [
+    ([520], 0, 2, 1, 64),          # long on average and few tiles: their keys (queries) dealt over two, four, eight workgroups
+    ([1030], 5, 1, 1, 128),
+    ([2100], 0, 1, 1, 40),
+    ([2048], 0, 2, 2, 33),
+    ([1, 2200], 0, 4, 2, 64),      # rows that not every share has a key of
+    ([1500, 0, 1700, 40], 3, 1, 1, 96),
+    ([2300], 0, 3, 1, 200),
+    ([2, 1040], 0, 1, 1, 75),
+])
+def test_keys_dealt_over_workgroups(lengths, behind, H, G, D, dtype):
+    test_attention_matches_the_formula_in_both_directions(lengths, behind, H, G, D, dtype)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("value", [math.nan, -math.inf])
+def test_values_in_masked_places_with_keys_dealt_over_workgroups(value, dtype):
+    T, at = 1100, 700
+    cu = torch.tensor([0, T], dtype=torch.int32, device=DEV)
+    print(f"varlen_attention with {value} at {at} of {T} {dtype}", flush=True)
+    leaves, dout = inputs(T, 2, 1, 64, dtype, seed=21)
+    val, off = reference(*leaves, dout, [0, T], 64**-0.5, dtype)
+    for which in range(4):
+        spoilt = [t.detach().clone() for t in (*leaves, dout)]
+        spoilt[which][at, 0, :3] = value
+        got = step([t.requires_grad_() for t in spoilt[:3]], spoilt[3], cu)
+        above, below = slice(0, at), slice(at + 1, T)
+        check([got[0][above]], [val[0][above]], [off[0][above]], dtype)  # rows that do not see it
+        if which in (0, 3):  # and the gradients of keys that it does not see
+            check([x[below] for x in got], [w[below] for w in val], [o[below] for o in off], dtype)
+        else:
+            check([got[1][above]], [val[1][above]], [off[1][above]], dtype)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("D", [64, 96, 75, 200])
 def test_rows_that_see_one_key_or_two(D, dtype):
     """A row that sees one key has the weight 1: its result is the value, its gradients through the score exactly zero.  Sequences of two rows: what

@@ -32,11 +32,14 @@ struct AttnArgs {
   float* delta;           // (H, T), negated by the bf16 kernels, which put -lse / c behind it (2 H, T)
   void *dq, *dk, *dv;     // dense; (splits > 1: dk_part, dv_part instead of dk, dv)
   float *dk_part, *dv_part;  // [splits][T][G][D] fp32
+  // tiles whose other axis is dealt over 1 << share_bits workgroups (queries) or 1 << key_share_bits (keys): parts in fp32, joined behind them
+  int share_bits, key_share_bits;
+  float *out_part, *lse_part, *dq_part;  // [shares][T][H][D], [shares][H][T], [shares][T][H][D]
   const int32_t* cu;      // [sequences + 1]
   int sequences;
   int T, H, G, D, group;  // group = H / G
   int D_out;              // elements of a head in results and their parts: D, or fewer where the operands are copies padded to D
-  int splits;             // parts that a key head's group of query heads is cut into for dk and dv
+  int splits;             // parts of dk and dv: those a key head's group of query heads is cut into, times 1 << key_share_bits
   float scale, c;         // c = scale log2(e)
   // tiles of rows by descending work, for the kernels whose rows are queries and for dk and dv; null: as they lie, the last (first) tile first
   const int32_t *query_order, *key_order;
@@ -65,6 +68,13 @@ __device__ __forceinline__ void sequence_of(const int32_t* cu, int sequences, in
   if (a == 0 || a > sequences || row >= T) return;
   start = max(cu[a - 1], 0);
   end = min(cu[a], T);
+}
+
+// Narrows [lo, hi) to the steps that fall to one of 1 << bits workgroups.
+__device__ __forceinline__ void take_share(int& lo, int& hi, int step, int share, int bits) {
+  const int from = lo, steps = lo < hi ? (hi - lo + step - 1) / step : 0;
+  lo = from + ((steps * share) >> bits) * step;
+  hi = min(hi, from + ((steps * (share + 1)) >> bits) * step);
 }
 
 // Order of a stretch of code, N times: a matrix instruction, READS reads of LDS, VALU vector instructions
@@ -158,20 +168,22 @@ __device__ __forceinline__ void careful_forward_row(const AttnArgs& p, int h, in
     if (lane + 64 * i < p.D_out) store_result<T>(p, dense + lane + 64 * i, acc[i] / l);
 }
 
+// dq of one row over the keys of [from, to), into the part `share` where there are parts
 template <typename T>
-__device__ __forceinline__ void careful_dq_row(const AttnArgs& p, int h, int row, int start, float lse, float delta) {
+__device__ __forceinline__ void careful_dq_row(const AttnArgs& p, int h, int row, int start, float lse, float delta, int from, int to, int share) {
   const int lane = threadIdx.x & 63;
   const T* q = row_at<T>(p.q, p.q_token, p.q_head, row, h);
   const T* dout = static_cast<const T*>(p.dout) + (static_cast<int64_t>(row) * p.H + h) * p.D;
   float acc[kLaneCols] = {};
-  for (int j0 = start; j0 <= row; j0 += kWave) {
+  to = min(to, row + 1);
+  for (int j0 = max(start, from); j0 < to; j0 += kWave) {
     const int j = j0 + lane;
     float ds = 0.0f;
-    if (j <= row && start < row) {
+    if (j < to && start < row) {
       const float w = exp2_f32(fmaf(careful_dot<T>(q, row_at<T>(p.k, p.k_token, p.k_head, j, h / p.group), p.D), p.c, -lse));
       ds = w * (careful_dot<T>(dout, row_at<T>(p.v, p.v_token, p.v_head, j, h / p.group), p.D) - delta);
     }
-    for (int n = 0; n < kWave && j0 + n <= row; ++n) {
+    for (int n = 0; n < kWave && j0 + n < to; ++n) {
       const float dn = __shfl(ds, n, kWave);
       const T* k = row_at<T>(p.k, p.k_token, p.k_head, j0 + n, h / p.group);
 #pragma unroll
@@ -179,21 +191,28 @@ __device__ __forceinline__ void careful_dq_row(const AttnArgs& p, int h, int row
         if (lane + 64 * i < p.D) acc[i] = fmaf(dn, load_as_f32<T>(k + lane + 64 * i), acc[i]);
     }
   }
-  T* dq = static_cast<T*>(p.dq) + (static_cast<int64_t>(row) * p.H + h) * p.D_out;
+  const int64_t at = (static_cast<int64_t>(row) * p.H + h) * p.D_out, part = static_cast<int64_t>(share) * p.T * p.H * p.D_out + at;
 #pragma unroll
-  for (int i = 0; i < kLaneCols; ++i)
-    if (lane + 64 * i < p.D_out) store_from_f32<T>(dq + lane + 64 * i, acc[i] * p.scale);
+  for (int i = 0; i < kLaneCols; ++i) {
+    const int d = lane + 64 * i;
+    if (d >= p.D_out) continue;
+    if (p.share_bits) p.dq_part[part + d] = acc[i] * p.scale;
+    else store_from_f32<T>(static_cast<T*>(p.dq) + at + d, acc[i] * p.scale);
+  }
 }
 
-// dk and dv of one key over the query heads [h0, h1), into the part `split` where there are parts; delta is kept times `sign`
+// dk and dv of one key over the rows of [from, to) of the query heads [h0, h1), into the part `split` where there are parts; delta is kept
+// times `sign`
 template <typename T>
-__device__ __forceinline__ void careful_dkv_row(const AttnArgs& p, int g, int key, int start, int end, int h0, int h1, int split, float sign) {
+__device__ __forceinline__ void careful_dkv_row(const AttnArgs& p, int g, int key, int start, int end, int h0, int h1, int from, int to, int split,
+                                                float sign) {
   const int lane = threadIdx.x & 63;
   const T* k = row_at<T>(p.k, p.k_token, p.k_head, key, g);
   const T* v = row_at<T>(p.v, p.v_token, p.v_head, key, g);
   float dk[kLaneCols] = {}, dv[kLaneCols] = {};
+  end = min(end, to);
   for (int h = h0; h < h1; ++h) {
-    for (int r0 = key; r0 < end; r0 += kWave) {
+    for (int r0 = max(key, from); r0 < end; r0 += kWave) {
       const int r = r0 + lane;
       float w = 0.0f, ds = 0.0f;
       if (r < end) {

@@ -16,9 +16,10 @@
 // through LDS at the end; four groups and one part for heads beyond 128, whose tiles would take too many registers.  Four parts of one group, and
 // one of four, were no faster for heads of 64 either.
 //
-// Measured: 2048 rows in 3 uneven sequences, 8/2 heads of 64: forward 47 us, dq 60, dk/dv 90, where the seven products of the formulas (5.8 GFLOP) take
+// Measured: 2048 rows in 3 uneven sequences, 8/2 heads of 64: forward 48 us, dq 57, dk/dv 77, where the seven products of the formulas (5.8 GFLOP) take
 // 43 at the rate of a large fp32 product (137 TFLOP/s) and the kernels form nine.  512 workgroups are two waves a SIMD, and the last rows
 // of a sequence see dozens of times what its first ones do: the longest workgroup sets the time, waiting for its products and LDS reads in turn.
+// Backward each is dealt over two (share_bits), dq 60 -> 57 and dk/dv 90 -> 77.
 #include <algorithm>
 #include <cmath>
 
@@ -213,14 +214,15 @@ __global__ __launch_bounds__(256) void any_forward_kernel(const AttnArgs p, int 
   extern __shared__ __attribute__((aligned(16))) float lds[];
   float *kt = lds, *vt = lds + KW * kStep * P, *stats = lds + 2 * KW * kStep * P;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Place at = place_of(blockIdx.x, p.H, tiles, p.query_order, true);
-  const int qw = wave / KW, kw = wave % KW, h = at.head, g = h / p.group;
+  const Place at = place_of(blockIdx.x, p.H << p.share_bits, tiles, p.query_order, true);
+  const int qw = wave / KW, kw = wave % KW, h = at.head >> p.share_bits, share = at.head - (h << p.share_bits), g = h / p.group;
   const int row0 = at.tile * 16 * QW, row = row0 + 16 * qw + (lane & 15);
   int start, end;
   sequence_of(p.cu, p.sequences, p.T, row, start, end);
   const bool on = start < end;
   const int lo = wave_min_i(on ? start : p.T), hi = wave_max_i(on ? row + 1 : 0);
-  const Range all = group_range(lo, hi, reinterpret_cast<int*>(stats));
+  Range all = group_range(lo, hi, reinterpret_cast<int*>(stats));
+  take_share(all.lo, all.hi, KW * kStep, share, p.share_bits);
   float q[DP / 4];
   own_rows<DP>(q, static_cast<const float*>(p.q) + h * p.q_head, p.q_token, row, on, p.D, vec, lane);
   f32x4 o[NB];
@@ -301,13 +303,19 @@ __global__ __launch_bounds__(256) void any_forward_kernel(const AttnArgs p, int 
     }
     bool spoilt = false;
     const int64_t dense = (static_cast<int64_t>(r) * z.H + h) * z.D;
+    const bool nothing = z.share_bits && len == 0.0f;  // a share without a key of the row's
     for (int d = lane; d < z.D; d += kWave) {
       float v = 0.0f;
 #pragma unroll
       for (int part = 0; part < KW; ++part) v += w[part] * sums[((qw * KW + part) * 16 + mine) * P + d];
-      v /= len;
+      v = nothing ? 0.0f : v / len;
       spoilt |= v != v;
-      store_result<float>(z, dense + d, first < last ? v : 0.0f);
+      if (z.share_bits) z.out_part[static_cast<int64_t>(share) * z.T * z.H * z.D + dense + d] = first < last ? v : 0.0f;
+      else store_result<float>(z, dense + d, first < last ? v : 0.0f);
+    }
+    if (z.share_bits) {  // (the kernel that joins the parts looks for spoilt rows)
+      if (lane == 0) z.lse_part[(static_cast<int64_t>(share) * z.H + h) * z.T + r] = first >= last ? INFINITY : nothing ? kNegInf : ref + log2f(len);
+      continue;
     }
     if (lane == 0 && z.lse) z.lse[static_cast<int64_t>(h) * z.T + r] = first < last ? ref + log2f(len) : INFINITY;
     if (first < last && __any(spoilt)) careful_forward_row<float>(z, h, r, first);
@@ -321,14 +329,15 @@ __global__ __launch_bounds__(256) void any_dq_kernel(const AttnArgs p, int tiles
   extern __shared__ __attribute__((aligned(16))) float lds[];
   float *kt = lds, *vt = lds + KW * kStep * P, *stats = lds + 2 * KW * kStep * P;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Place at = place_of(blockIdx.x, p.H, tiles, p.query_order, true);
-  const int qw = wave / KW, kw = wave % KW, h = at.head, g = h / p.group;
+  const Place at = place_of(blockIdx.x, p.H << p.share_bits, tiles, p.query_order, true);
+  const int qw = wave / KW, kw = wave % KW, h = at.head >> p.share_bits, share = at.head - (h << p.share_bits), g = h / p.group;
   const int row0 = at.tile * 16 * QW, row = row0 + 16 * qw + (lane & 15);
   int start, end;
   sequence_of(p.cu, p.sequences, p.T, row, start, end);
   const bool on = start < end;
   const int lo = wave_min_i(on ? start : p.T), hi = wave_max_i(on ? row + 1 : 0);
-  const Range all = group_range(lo, hi, reinterpret_cast<int*>(stats));
+  Range all = group_range(lo, hi, reinterpret_cast<int*>(stats));
+  take_share(all.lo, all.hi, KW * kStep, share, p.share_bits);
   float q[DP / 4], dout[DP / 4];
   const int64_t dense = static_cast<int64_t>(p.H) * p.D;
   own_rows<DP>(q, static_cast<const float*>(p.q) + h * p.q_head, p.q_token, row, on, p.D, vec, lane);
@@ -342,7 +351,7 @@ __global__ __launch_bounds__(256) void any_dq_kernel(const AttnArgs p, int tiles
   }
   delta = column_sum(delta);
   const float lse = on ? p.lse[static_cast<int64_t>(h) * p.T + row] : INFINITY;
-  if (kw == 0 && lane < 16 && row < p.T) p.delta[static_cast<int64_t>(h) * p.T + row] = on ? delta : 0.0f;
+  if (kw == 0 && lane < 16 && row < p.T && share == 0) p.delta[static_cast<int64_t>(h) * p.T + row] = on ? delta : 0.0f;
   f32x4 dq[NB];
 #pragma unroll
   for (int n = 0; n < NB; ++n) dq[n] = f32x4{0, 0, 0, 0};
@@ -388,7 +397,8 @@ __global__ __launch_bounds__(256) void any_dq_kernel(const AttnArgs p, int tiles
     if (r >= z.T) break;
     const int first = __builtin_amdgcn_readlane(start, mine), last = __builtin_amdgcn_readlane(end, mine);
     bool spoilt = false;
-    float* out = static_cast<float*>(z.dq) + (static_cast<int64_t>(r) * z.H + h) * z.D;
+    float* out = (z.share_bits ? z.dq_part + static_cast<int64_t>(share) * z.T * z.H * z.D : static_cast<float*>(z.dq)) +
+                 (static_cast<int64_t>(r) * z.H + h) * z.D;
     for (int d = lane; d < z.D; d += kWave) {
       float v = 0.0f;
 #pragma unroll
@@ -396,7 +406,8 @@ __global__ __launch_bounds__(256) void any_dq_kernel(const AttnArgs p, int tiles
       spoilt |= v != v;
       store_from_f32<float>(out + d, first < last ? v * z.scale : 0.0f);
     }
-    if (first < last && __any(spoilt)) careful_dq_row<float>(z, h, r, first, lses[(qw * KW) * 16 + mine], deltas[(qw * KW) * 16 + mine]);
+    if (first < last && __any(spoilt))
+      careful_dq_row<float>(z, h, r, first, lses[(qw * KW) * 16 + mine], deltas[(qw * KW) * 16 + mine], all.lo, all.hi, share);
   }
 }
 
@@ -410,13 +421,15 @@ __global__ __launch_bounds__(256) void any_dkv_kernel(const AttnArgs p, int tile
   const int qw = wave / KW, kw = wave % KW;
   const Place at = place_of(blockIdx.x, p.G * p.splits, tiles, p.key_order, false);
   const int g = at.head / p.splits, split = at.head % p.splits;
-  const int heads = (p.group + p.splits - 1) / p.splits, h0 = g * p.group + split * heads, h1 = min(h0 + heads, (g + 1) * p.group);
+  const int parts = p.splits >> p.key_share_bits, heads = (p.group + parts - 1) / parts;
+  const int h0 = g * p.group + (split >> p.key_share_bits) * heads, h1 = min(h0 + heads, (g + 1) * p.group);
   const int key0 = at.tile * 16 * QW, key = key0 + 16 * qw + (lane & 15);
   int start, end;
   sequence_of(p.cu, p.sequences, p.T, key, start, end);
   const bool on = start < end;
   const int lo = wave_min_i(on ? key : p.T), hi = wave_max_i(on ? end : 0);
-  const Range all = group_range(lo, hi, reinterpret_cast<int*>(stats));
+  Range all = group_range(lo, hi, reinterpret_cast<int*>(stats));
+  take_share(all.lo, all.hi, KW * kStep, split & ((1 << p.key_share_bits) - 1), p.key_share_bits);
   float k[DP / 4], v[DP / 4];
   own_rows<DP>(k, static_cast<const float*>(p.k) + g * p.k_head, p.k_token, key, on, p.D, vec, lane);
   own_rows<DP>(v, static_cast<const float*>(p.v) + g * p.v_head, p.v_token, key, on, p.D, vec, lane);
@@ -495,7 +508,7 @@ __global__ __launch_bounds__(256) void any_dkv_kernel(const AttnArgs p, int tile
     if (spoilt[i]) {
       const int mine = kw * (16 / KW) + i, r = key0 + 16 * qw + mine;
       const int first = __builtin_amdgcn_readlane(start, mine), last = __builtin_amdgcn_readlane(end, mine);
-      careful_dkv_row<float>(z, g, r, first, last, h0, h1, split, 1.0f);
+      careful_dkv_row<float>(z, g, r, first, last, h0, h1, all.lo, all.hi, split, 1.0f);
     }
 }
 
@@ -536,7 +549,68 @@ __global__ __launch_bounds__(256) void pad_heads_kernel(const PadArgs p) {
   }
 }
 
-// dk and dv from their parts, added in order, four elements a lane (n is the number of fours, or of elements where they are no whole fours)
+// Results of rows from the shares of their keys: each share's own softmax, weighted by what it holds of the whole.  Lanes hold N elements of a
+// row, as few lanes a row as that takes.
+template <typename T, int N, int BITS>
+__global__ __launch_bounds__(256) void join_forward_kernel(const AttnArgs p, int log_lanes) {
+  constexpr int SHARES = 1 << BITS, ITER = N == 4 ? 1 : kLaneCols;
+  const int lane = threadIdx.x & 63, lanes = 1 << log_lanes, each = kWave >> log_lanes;
+  const int64_t items = static_cast<int64_t>(p.T) * p.H;
+  const int64_t first = (static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * each;
+  const int64_t item = min(first + (lane >> log_lanes), items - 1);
+  const int row = static_cast<int>(item / p.H), h = static_cast<int>(item - static_cast<int64_t>(row) * p.H);
+  const float* from = p.lse_part + static_cast<int64_t>(h) * p.T + row;
+  float lse[SHARES], top = kNegInf, sum = 0.0f, acc[ITER][N] = {};
+#pragma unroll
+  for (int s = 0; s < SHARES; ++s) lse[s] = from[s * items];
+#pragma unroll
+  for (int s = 0; s < SHARES; ++s) top = fmaxf(top, lse[s]);
+#pragma unroll
+  for (int s = 0; s < SHARES; ++s) {
+    const float w = exp2_f32(lse[s] - top);  // (no share with a finite sum: NaN, and the row is formed again)
+    sum += w;
+    const float* part = p.out_part + (s * items + item) * p.D_out;
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+      const int d = N * (lane & (lanes - 1)) + 64 * i;
+      if (d >= p.D_out) continue;
+      if constexpr (N == 4) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(part + d);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[0][j] = fmaf(w, x[j], acc[0][j]);
+      } else {
+        acc[i][0] = fmaf(w, part[d], acc[i][0]);
+      }
+    }
+  }
+  int start = 0, end = p.T;
+  if (top == INFINITY) sequence_of(p.cu, p.sequences, p.T, row, start, end);  // (of rows in no sequence, and of infinite scores)
+  const bool on = start < end, mine = first + (lane >> log_lanes) < items;
+  bool spoilt = false;
+#pragma unroll
+  for (int i = 0; i < ITER; ++i) {
+    const int d = N * (lane & (lanes - 1)) + 64 * i;
+    if (d >= p.D_out || !mine) continue;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const float v = on ? acc[i][j] / sum : 0.0f;
+      spoilt |= v != v;
+      store_result<T>(p, item * p.D_out + d + j, v);
+    }
+  }
+  if (mine && (lane & (lanes - 1)) == 0 && p.lse) p.lse[static_cast<int64_t>(h) * p.T + row] = on ? top + log2f(sum) : INFINITY;
+  for (uint64_t again = __ballot(spoilt); again;) {
+    const int at = __builtin_ctzll(again) >> log_lanes;
+    const int64_t it = first + at;
+    const int r = static_cast<int>(it / p.H);
+    sequence_of(p.cu, p.sequences, p.T, r, start, end);
+    careful_forward_row<T>(p, static_cast<int>(it - static_cast<int64_t>(r) * p.H), r, start);
+    const int done = (at + 1) << log_lanes;
+    again = done < 64 ? again & ~0ull << done : 0;
+  }
+}
+
+// dq, or dk and dv, from their parts, added in order, four elements a lane (n is the number of fours, or of elements where they are no whole fours)
 template <typename T, int N>
 __global__ __launch_bounds__(256) void join_parts_kernel(const float* __restrict__ dk_part, const float* __restrict__ dv_part,
                                                          T* __restrict__ dk, T* __restrict__ dv, int splits, int64_t n) {
@@ -595,7 +669,7 @@ void any_forward(const AttnArgs& p, int vec, hipStream_t s) {
   static PerDeviceOnce once;
   allow_lds(any_forward_kernel<DP, KW>, kAnyLds<DP, KW>, once);
   const int rows = 64 / KW, tiles = (p.T + rows - 1) / rows;
-  hipLaunchKernelGGL((any_forward_kernel<DP, KW>), dim3(tiles * p.H), dim3(256), (kAnyLds<DP, KW>), s, p, tiles, vec);
+  hipLaunchKernelGGL((any_forward_kernel<DP, KW>), dim3((tiles * p.H) << p.share_bits), dim3(256), (kAnyLds<DP, KW>), s, p, tiles, vec);
 }
 
 int attention_any_rows(int D) { return D <= 128 ? 32 : 64; }
@@ -611,22 +685,39 @@ void any_backward(const AttnArgs& p, int vec, hipStream_t s) {
   allow_lds(any_dq_kernel<DP, KW>, kAnyLds<DP, KW>, once_q);
   allow_lds(any_dkv_kernel<DP, KW>, kAnyLds<DP, KW>, once_kv);
   const int rows = 64 / KW, tiles = (p.T + rows - 1) / rows;
-  hipLaunchKernelGGL((any_dq_kernel<DP, KW>), dim3(tiles * p.H), dim3(256), (kAnyLds<DP, KW>), s, p, tiles, vec);
+  hipLaunchKernelGGL((any_dq_kernel<DP, KW>), dim3((tiles * p.H) << p.share_bits), dim3(256), (kAnyLds<DP, KW>), s, p, tiles, vec);
   hipLaunchKernelGGL((any_dkv_kernel<DP, KW>), dim3(tiles * p.G * p.splits), dim3(256), (kAnyLds<DP, KW>), s, p, tiles, vec);
 }
 
 template <typename T>
 void join_parts(const AttnArgs& p, hipStream_t s) {
-  if (p.splits <= 1) return;
-  const int64_t n = static_cast<int64_t>(p.T) * p.G * p.D_out;
-  const bool fours = n % 4 == 0 && (reinterpret_cast<uintptr_t>(p.dk) | reinterpret_cast<uintptr_t>(p.dv)) % (4 * sizeof(T)) == 0;
-  auto launch = [&](auto kernel, int64_t items) {
-    const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((items + 255) / 256, 1 << 20));
-    hipLaunchKernelGGL(kernel, dim3(blocks, 2), dim3(256), 0, s, p.dk_part, p.dv_part, static_cast<T*>(p.dk), static_cast<T*>(p.dv), p.splits,
-                       items);
+  auto join = [&](const float* a_part, const float* b_part, void* a, void* b, int heads, int parts) {
+    if (parts <= 1) return;
+    const int64_t n = static_cast<int64_t>(p.T) * heads * p.D_out;
+    const bool fours = n % 4 == 0 && (reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) % (4 * sizeof(T)) == 0;
+    const int64_t items = fours ? n / 4 : n;
+    const dim3 grid(static_cast<unsigned>(std::min<int64_t>((items + 255) / 256, 1 << 20)), b ? 2 : 1);
+    if (fours) hipLaunchKernelGGL((join_parts_kernel<T, 4>), grid, dim3(256), 0, s, a_part, b_part, static_cast<T*>(a), static_cast<T*>(b), parts, items);
+    else hipLaunchKernelGGL((join_parts_kernel<T, 1>), grid, dim3(256), 0, s, a_part, b_part, static_cast<T*>(a), static_cast<T*>(b), parts, items);
   };
-  if (fours) launch(join_parts_kernel<T, 4>, n / 4);
-  else launch(join_parts_kernel<T, 1>, n);
+  join(p.dq_part, nullptr, p.dq, nullptr, p.H, 1 << p.share_bits);
+  join(p.dk_part, p.dv_part, p.dk, p.dv, p.G, p.splits);
+}
+
+template <typename T, int N>
+void join_forward(const AttnArgs& p, hipStream_t s) {
+  int log_lanes = 0;
+  while (N << log_lanes < p.D_out && log_lanes < 6) ++log_lanes;
+  const int64_t each = 4 * (kWave >> log_lanes), items = static_cast<int64_t>(p.T) * p.H;
+  const dim3 grid(static_cast<unsigned>((items + each - 1) / each));  // (at most 1024 x 128 rows, or there are no shares)
+  if (p.share_bits == 1) hipLaunchKernelGGL((join_forward_kernel<T, N, 1>), grid, dim3(256), 0, s, p, log_lanes);
+  else if (p.share_bits == 2) hipLaunchKernelGGL((join_forward_kernel<T, N, 2>), grid, dim3(256), 0, s, p, log_lanes);
+  else hipLaunchKernelGGL((join_forward_kernel<T, N, 3>), grid, dim3(256), 0, s, p, log_lanes);
+}
+template <typename T>
+void join_forward(const AttnArgs& p, hipStream_t s) {
+  if (p.D_out % 4 == 0) join_forward<T, 4>(p, s);
+  else join_forward<T, 1>(p, s);
 }
 
 void attention_any_backward(const AttnArgs& p, hipStream_t s) {
@@ -664,6 +755,45 @@ int head_parts(int64_t T, int64_t H, int64_t G) {
   const int64_t heads = (group + parts - 1) / parts;
   return (int)((group + heads - 1) / heads);
 }
+
+// Where tiles are too few to fill the card, each one's other axis is dealt over workgroups (1 << bits of them, up to eight), whose parts are joined
+// through memory in fp32.  Whether that pays is a matter of what a workgroup of its own takes against the trip: of `products` per key, a
+// workgroup alone reaches two thirds of the matrix rate of its CU, and the card no more than the whole of it; a launch that joins 3 us; memory 5 TB/s.
+// One sequence, bf16 heads of 128, us, whole / dealt: forward of 16384 rows of one head 287 / 101, 4096 of 4 77 / 42, 1024 of 4 24 / 19 (of 16 25 / 30: not
+// dealt); backward 1060 / 305, 292 / 126, 90 / 54 (of 16 99 / 74); fp32, 4096 of one 223 / 85 and 664 / 238.
+int tile_rows(int64_t D, int dtype) { return dtype == MI355_BF16 ? attention_bf16_rows() : attention_any_rows((int)D); }
+int64_t tiles_of(int64_t T, int64_t D, int dtype) { return (T + tile_rows(D, dtype) - 1) / tile_rows(D, dtype); }
+constexpr int kMostShares = 3;  // a power of two
+// as many as there can be, of sequences of any length
+int most_share_bits(int64_t workgroups, int64_t T) {
+  int bits = 0;
+  while (bits < kMostShares && workgroups << (bits + 1) <= 2 * kHeldAtOnce && T >= 64 << (bits + 1)) ++bits;
+  return bits;
+}
+// `part`: elements that a share writes and its joining reads; `parts`: those of other cuts, joined in any case if there are several
+int share_bits(int64_t workgroups, int products, int64_t T, int64_t sequences, int64_t D, int dtype, int64_t part, int64_t parts) {
+  const double rate = dtype == MI355_BF16 ? 1200e6 / 256 : 137e6 / 256;  // flops a us and CU
+  const double keys = static_cast<double>(T) / std::max<int64_t>(sequences, 1), whole = keys * products * 2.0 * tile_rows(D, dtype) * D / rate;
+  auto time = [&](int bits) {
+    const double rounds = static_cast<double>(workgroups) / kHeldAtOnce;  // (a tile's rows see half of the keys on average, and two are held by a CU)
+    return whole * std::max(1.5 / (1 << bits), rounds) + (bits && parts == 1 ? 3.0 : 0.0) + ((parts << bits) > 1 ? 8e-6 / 5 * part * (parts << bits) : 0.0);
+  };
+  int best = 0;
+  for (int bits = 1; bits <= most_share_bits(workgroups, T); ++bits) {
+    // fp32 workgroups hold a CU's registers, those of heads beyond 96 all of them: more than 512 end later (4096 rows of a head of 128 in 1024 109 us, in
+    // 512 85; of 4 heads 268 and 242), but smaller heads' 512 end sooner as halves (4 of 64: backward 518 -> 366)
+    if (dtype == MI355_F32 && (bits > 1 || D > 96) && workgroups << bits > kHeldAtOnce) break;
+    if (time(bits) < 0.95 * time(best)) best = bits;
+  }
+  return best;
+}
+int forward_bits(int64_t T, int64_t H, int64_t D, int64_t sequences, int dtype) {
+  return share_bits(tiles_of(T, D, dtype) * H, 2, T, sequences, D, dtype, T * H * D, 1);
+}
+int64_t out_part_bytes(int64_t T, int64_t H, int64_t D, int bits) {
+  return bits ? ((4 * T * H * D << bits) + 15) / 16 * 16 : 0;
+}
+int64_t lse_part_bytes(int64_t T, int64_t H, int bits) { return bits ? ((4 * T * H << bits) + 15) / 16 * 16 : 0; }
 
 AttnArgs attention_args(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token, int64_t k_head, const void* v,
                         int64_t v_token, int64_t v_head, const int32_t* cu, int64_t sequences, float scale, int64_t T, int64_t H,
@@ -734,27 +864,38 @@ extern "C" int mi355_varlen_attention_fwd(const void* q, int64_t q_token_stride,
   MI355_REQUIRE(!padded || workspace, "varlen_attention_fwd: workspace required for bf16 heads of %lld elements", (long long)D);
   if (padded) pad_heads(p, false, static_cast<char*>(workspace) + order_bytes(T), as_stream(stream));
   MI355_REQUIRE(!matrix || attention_bf16_covers(p), "varlen_attention_fwd: bf16 operands must start and stride in whole pieces of 16 bytes");
-  const int rows = matrix ? attention_bf16_rows() : attention_any_rows(p.D);
-  if (workspace && sorted_tiles(p.sequences, T, (T + rows - 1) / rows, H)) {
-    attention_sort_tiles(p, rows, static_cast<int32_t*>(workspace), nullptr, as_stream(stream));
+  if (workspace && sorted_tiles(p.sequences, T, tiles_of(T, D, dtype), H)) {
+    attention_sort_tiles(p, matrix ? attention_bf16_rows() : attention_any_rows((int)D), static_cast<int32_t*>(workspace), nullptr, as_stream(stream));
     p.query_order = static_cast<int32_t*>(workspace);
+  }
+  if (workspace) p.share_bits = forward_bits(T, H, D, sequences, dtype);
+  if (p.share_bits) {
+    char* at = static_cast<char*>(workspace) + order_bytes(T) + (padded ? padded_bytes(T, H + 2 * G, D) : 0);
+    p.out_part = reinterpret_cast<float*>(at);
+    p.lse_part = reinterpret_cast<float*>(at + out_part_bytes(T, H, D, p.share_bits));
   }
   if (matrix) attention_bf16_forward(p, as_stream(stream));
   else attention_any_forward(p, as_stream(stream));
+  if (p.share_bits) matrix ? join_forward<uint16_t>(p, as_stream(stream)) : join_forward<float>(p, as_stream(stream));
   return check_launch("varlen_attention_fwd");
 }
 
 extern "C" int64_t mi355_varlen_attention_fwd_workspace_bytes(int64_t T, int64_t H, int64_t G, int64_t D, int64_t sequences, int dtype) {
   if (T < 1 || H < 1 || G < 1 || D < 1) return 0;
-  if (padded_heads(D, dtype)) return order_bytes(T) + padded_bytes(T, H + 2 * G, D);
-  return sorted_tiles(sequences, T, (T + kLeastRows - 1) / kLeastRows, H) ? order_bytes(T) : 0;  // (the most tiles there can be)
+  const int64_t tiles = tiles_of(T, D, dtype);
+  const int bits = forward_bits(T, H, D, sequences, dtype);
+  const int64_t copies = padded_heads(D, dtype) ? padded_bytes(T, H + 2 * G, D) : 0;
+  if (!copies && !bits && !sorted_tiles(sequences, T, tiles, H)) return 0;
+  return order_bytes(T) + copies + out_part_bytes(T, H, D, bits) + lse_part_bytes(T, H, bits);
 }
 
 extern "C" int64_t mi355_varlen_attention_bwd_workspace_bytes(int64_t T, int64_t H, int64_t G, int64_t D, int dtype) {
   if (T < 1 || H < 1 || G < 1 || H % G || D < 1) return 0;
-  const int64_t parts = head_parts(T, H, G);
+  const int64_t parts = head_parts(T, H, G), tiles = tiles_of(T, D, dtype);
+  const int bits = most_share_bits(tiles * H, T);
+  const int64_t key_parts = parts << most_share_bits(tiles * G * parts, T);
   return 4 * ((2 * H * T + 3) / 4 * 4) + 2 * order_bytes(T) + (padded_heads(D, dtype) ? padded_bytes(T, 4 * H + 2 * G, D) : 0) +
-         (parts > 1 ? 8 * parts * T * G * D : 0);
+         out_part_bytes(T, H, D, bits) + (key_parts > 1 ? 8 * key_parts * T * G * D : 0);
 }
 
 extern "C" int mi355_varlen_attention_bwd(const void* dout, const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
@@ -770,7 +911,11 @@ extern "C" int mi355_varlen_attention_bwd(const void* dout, const void* q, int64
                               cu_seqlens, sequences, scale, T, H, G, D);
   p.o = out, p.rest = dtype == MI355_BF16 ? const_cast<void*>(out_rest) : nullptr;
   p.dout = dout, p.lse = const_cast<float*>(lse), p.dq = dq, p.dk = dk, p.dv = dv;
+  const int64_t tiles = tiles_of(T, D, dtype);
   p.splits = head_parts(T, H, G);
+  p.share_bits = share_bits(tiles * H, 3, T, sequences, D, dtype, T * H * D, 1);
+  p.key_share_bits = share_bits(tiles * G * p.splits, 4, T, sequences, D, dtype, 2 * T * G * D, p.splits);
+  p.splits <<= p.key_share_bits;
   p.delta = static_cast<float*>(workspace);
   char* at = reinterpret_cast<char*>(p.delta + (2 * H * T + 3) / 4 * 4);
   int32_t *query_order = reinterpret_cast<int32_t*>(at), *key_order = reinterpret_cast<int32_t*>(at + order_bytes(T));
@@ -779,13 +924,14 @@ extern "C" int mi355_varlen_attention_bwd(const void* dout, const void* q, int64
     pad_heads(p, true, at, as_stream(stream));
     at += padded_bytes(T, 4 * H + 2 * G, D);
   }
+  p.dq_part = reinterpret_cast<float*>(at);
+  at += out_part_bytes(T, H, D, p.share_bits);
   p.dk_part = reinterpret_cast<float*>(at);
   p.dv_part = p.dk_part + static_cast<int64_t>(p.splits) * T * G * D;
   const bool matrix = dtype == MI355_BF16;
   MI355_REQUIRE(!matrix || attention_bf16_covers(p), "varlen_attention_bwd: bf16 operands must start and stride in whole pieces of 16 bytes");
-  const int rows = matrix ? attention_bf16_rows() : attention_any_rows(p.D);
-  if (sorted_tiles(p.sequences, T, (T + rows - 1) / rows, H)) {
-    attention_sort_tiles(p, rows, query_order, key_order, as_stream(stream));
+  if (sorted_tiles(p.sequences, T, tiles, H)) {
+    attention_sort_tiles(p, matrix ? attention_bf16_rows() : attention_any_rows((int)D), query_order, key_order, as_stream(stream));
     p.query_order = query_order, p.key_order = key_order;
   }
   if (matrix) attention_bf16_backward(p, as_stream(stream));

@@ -248,14 +248,15 @@ __global__ __launch_bounds__(256, kWaves<DP>) void bf16_forward_kernel(const Att
   extern __shared__ __attribute__((aligned(16))) uint16_t smem[];
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_cptr)smem));
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-  const Place at = place_of(blockIdx.x, p.H, tiles, p.query_order, true);
-  const int h = at.head, g = h / p.group;
+  const Place at = place_of(blockIdx.x, p.H << p.share_bits, tiles, p.query_order, true);
+  const int h = at.head >> p.share_bits, share = at.head - (h << p.share_bits), g = h / p.group;
   const int row0 = at.tile * 4 * kRows + wave * kRows, row = row0 + (lane & 31);
   int start, end;
   sequence_of(p.cu, p.sequences, p.T, row, start, end);
   const bool on = start < end;
   Ranges range;
   range.find(on ? start : p.T, on ? row + 1 : 0, reinterpret_cast<int*>(smem), wave);
+  take_share(range.lo, range.hi, kTile, share, p.share_bits);
   const int latest = most(on ? start : p.T);  // keys from here to the wave's first row are seen by all its rows
   Reads<DP> reads;
   reads.find(lane, lds0);
@@ -338,8 +339,9 @@ __global__ __launch_bounds__(256, kWaves<DP>) void bf16_forward_kernel(const Att
     if (k0 + kTile < range.hi) tile(k0 + kTile, std::integral_constant<uint32_t, 1>{});
   }
   l = halves_sum(l);
-  const float inverse = 1.0f / l;
   const AttnArgs& z = late_arguments();
+  // (a share without a key of the row's: nothing to add)
+  const float inverse = z.share_bits && l == 0.0f ? 0.0f : 1.0f / l;
   bool spoilt = false;
 #pragma unroll
   for (int n = 0; n < NB; ++n)
@@ -351,6 +353,13 @@ __global__ __launch_bounds__(256, kWaves<DP>) void bf16_forward_kernel(const Att
   if (z.D_out % 8) __syncthreads();
   const int rows = min(max(z.T - row0, 0), kRows);
   const int64_t dense = (static_cast<int64_t>(row0) * z.H + h) * z.D_out, pitch = static_cast<int64_t>(z.H) * z.D_out;
+  if (z.share_bits) {
+    store_rows<DP>(z.out_part + static_cast<int64_t>(share) * z.T * pitch + dense, pitch, rows, z.D_out, smem, wave, lane,
+                   [&](int n, int a, float (&v)[8]) __attribute__((always_inline)) { eight_of(o[n], a, v); });
+    if (half == 0 && row < z.T)
+      z.lse_part[(static_cast<int64_t>(share) * z.H + h) * z.T + row] = !on ? INFINITY : l == 0.0f ? kNegInf : ref + log2f(l);
+    return;
+  }
   store_rows<DP>(static_cast<uint16_t*>(z.out) + dense, pitch, rows, z.D_out, smem, wave, lane,
                  [&](int n, int a, float (&v)[8]) __attribute__((always_inline)) { eight_of(o[n], a, v); });
   if (z.rest)
@@ -379,14 +388,15 @@ __global__ __launch_bounds__(256, kWaves<DP>) void bf16_dq_kernel(const AttnArgs
   extern __shared__ __attribute__((aligned(16))) uint16_t smem[];
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_cptr)smem));
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-  const Place at = place_of(blockIdx.x, p.H, tiles, p.query_order, true);
-  const int h = at.head, g = h / p.group;
+  const Place at = place_of(blockIdx.x, p.H << p.share_bits, tiles, p.query_order, true);
+  const int h = at.head >> p.share_bits, share = at.head - (h << p.share_bits), g = h / p.group;
   const int row0 = at.tile * 4 * kRows + wave * kRows, row = row0 + (lane & 31);
   int start, end;
   sequence_of(p.cu, p.sequences, p.T, row, start, end);
   const bool on = start < end, several = on && start < row;  // (a row that sees one key: its weight is 1, whatever its score)
   Ranges range;
   range.find(on ? start : p.T, on ? row + 1 : 0, reinterpret_cast<int*>(smem), wave);
+  take_share(range.lo, range.hi, kTile, share, p.share_bits);
   const int latest = most(on ? start : p.T);
   Reads<DP> reads;
   reads.find(lane, lds0);
@@ -418,7 +428,7 @@ __global__ __launch_bounds__(256, kWaves<DP>) void bf16_dq_kernel(const AttnArgs
   }
   delta = halves_sum(delta);
   const float lse = on ? p.lse[static_cast<int64_t>(h) * p.T + row] : INFINITY;
-  if (half == 0 && row < p.T) {  // as the kernel behind this one starts its sums from: -lse / c and -delta
+  if (half == 0 && row < p.T && share == 0) {  // as the kernel behind this one starts its sums from: -lse / c and -delta
     p.delta[static_cast<int64_t>(h) * p.T + row] = on ? -delta : 0.0f;
     p.delta[static_cast<int64_t>(p.H + h) * p.T + row] = -lse / p.c;
   }
@@ -488,9 +498,13 @@ __global__ __launch_bounds__(256, kWaves<DP>) void bf16_dq_kernel(const AttnArgs
       spoilt |= dq[n][i] != dq[n][i];
     }
   if (z.D_out % 8) __syncthreads();
-  store_rows<DP>(static_cast<uint16_t*>(z.dq) + (static_cast<int64_t>(row0) * z.H + h) * z.D_out, static_cast<int64_t>(z.H) * z.D_out,
-                 min(max(z.T - row0, 0), kRows), z.D_out, smem, wave, lane,
-                 [&](int n, int a, float (&v)[8]) __attribute__((always_inline)) { eight_of(dq[n], a, v); });
+  const int rows = min(max(z.T - row0, 0), kRows);
+  const int64_t dense_dq = (static_cast<int64_t>(row0) * z.H + h) * z.D_out, pitch = static_cast<int64_t>(z.H) * z.D_out;
+  auto eight = [&](int n, int a, float (&v)[8]) __attribute__((always_inline)) { eight_of(dq[n], a, v); };
+  if (z.share_bits)
+    store_rows<DP>(z.dq_part + static_cast<int64_t>(share) * z.T * pitch + dense_dq, pitch, rows, z.D_out, smem, wave, lane, eight);
+  else
+    store_rows<DP>(static_cast<uint16_t*>(z.dq) + dense_dq, pitch, rows, z.D_out, smem, wave, lane, eight);
   uint64_t again = __ballot(spoilt && row < z.T);
   again = (again | again >> 32) & 0xffffffffu;
   if (again) lds_wait<0>();
@@ -498,7 +512,7 @@ __global__ __launch_bounds__(256, kWaves<DP>) void bf16_dq_kernel(const AttnArgs
     const int i = __builtin_ctzll(again);
     careful_dq_row<uint16_t>(z, h, row0 + i, __builtin_amdgcn_readlane(start, i),
                              __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lse), i)),
-                             __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(delta), i)));
+                             __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(delta), i)), range.lo, range.hi, share);
   }
 }
 
@@ -512,7 +526,8 @@ __global__ __launch_bounds__(256, FINE ? 1 : kWaves<DP>) void bf16_dkv_kernel(co
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
   const Place at = place_of(blockIdx.x, p.G * p.splits, tiles, p.key_order, false);
   const int g = at.head / p.splits, split = at.head % p.splits;
-  const int heads = (p.group + p.splits - 1) / p.splits, h0 = g * p.group + split * heads, h1 = min(h0 + heads, (g + 1) * p.group);
+  const int parts = p.splits >> p.key_share_bits, heads = (p.group + parts - 1) / parts;
+  const int h0 = g * p.group + (split >> p.key_share_bits) * heads, h1 = min(h0 + heads, (g + 1) * p.group);
   const int key0 = at.tile * 4 * kRows + wave * kRows, key = key0 + (lane & 31);
   int start, end;
   sequence_of(p.cu, p.sequences, p.T, key, start, end);
@@ -520,6 +535,7 @@ __global__ __launch_bounds__(256, FINE ? 1 : kWaves<DP>) void bf16_dkv_kernel(co
   const int alone = key == start;  // the first row of a sequence sees this key only: its weight is 1, whatever its score
   Ranges range;
   range.find(on ? key : p.T, on ? end : 0, reinterpret_cast<int*>(smem), wave);
+  take_share(range.lo, range.hi, kTile, split & ((1 << p.key_share_bits) - 1), p.key_share_bits);
   const int earliest = least(on ? end : 0);  // rows from the wave's last key to here see all its keys
   Reads<DP> reads;
   reads.find(lane, lds0);
@@ -660,7 +676,7 @@ __global__ __launch_bounds__(256, FINE ? 1 : kWaves<DP>) void bf16_dkv_kernel(co
     const int i = __builtin_ctzll(again);
     int first, last;
     sequence_of(z.cu, z.sequences, z.T, key0 + i, first, last);
-    careful_dkv_row<uint16_t>(z, g, key0 + i, first, last, h0, h1, split, -1.0f);
+    careful_dkv_row<uint16_t>(z, g, key0 + i, first, last, h0, h1, range.lo, range.hi, split, -1.0f);
   }
 }
 
@@ -681,7 +697,7 @@ void forward(const AttnArgs& p, hipStream_t s) {
   static PerDeviceOnce once;
   allow(bf16_forward_kernel<DP>, kForwardLds<DP>, once);
   const int tiles = (p.T + 4 * kRows - 1) / (4 * kRows);
-  hipLaunchKernelGGL(bf16_forward_kernel<DP>, dim3(tiles * p.H), dim3(256), kForwardLds<DP>, s, p, tiles);
+  hipLaunchKernelGGL(bf16_forward_kernel<DP>, dim3((tiles * p.H) << p.share_bits), dim3(256), kForwardLds<DP>, s, p, tiles);
 }
 
 // ds in two bf16 pieces instead of one, for short sequences: the ds of a row add up to nothing, and of a few keys what rounding takes
@@ -695,7 +711,7 @@ void backward(const AttnArgs& p, hipStream_t s) {
   allow(bf16_dq_kernel<DP, FINE>, kForwardLds<DP>, once_q);
   allow(bf16_dkv_kernel<DP, FINE>, kDkvLds<DP>, once_kv);
   const int tiles = (p.T + 4 * kRows - 1) / (4 * kRows);
-  hipLaunchKernelGGL((bf16_dq_kernel<DP, FINE>), dim3(tiles * p.H), dim3(256), kForwardLds<DP>, s, p, tiles);
+  hipLaunchKernelGGL((bf16_dq_kernel<DP, FINE>), dim3((tiles * p.H) << p.share_bits), dim3(256), kForwardLds<DP>, s, p, tiles);
   hipLaunchKernelGGL((bf16_dkv_kernel<DP, FINE>), dim3(tiles * p.G * p.splits), dim3(256), kDkvLds<DP>, s, p, tiles);
 }
 template <int DP>
