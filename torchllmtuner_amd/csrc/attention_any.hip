@@ -52,10 +52,15 @@ struct Staged {
       const int64_t left = (static_cast<int64_t>(T_ - 1 - row0) * token + D) * sizeof(float);
       const uint32_t bytes = left < 0 ? 0 : left < kFar ? static_cast<uint32_t>(left) : kFar;
       const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(base) + static_cast<int64_t>(row0) * token, 0, bytes, 0x00020000);
+      auto offset = [&](int i) {
+        const uint32_t d = (i % QUADS) * 4, at = (static_cast<uint32_t>(i / QUADS) * static_cast<uint32_t>(token) + d) * sizeof(float);
+        return at | (d < static_cast<uint32_t>(D) ? 0u : kFar);  // (a tile's offsets stay below kFar)
+      };
+      const uint32_t first = offset(threadIdx.x);
 #pragma unroll
       for (int n = 0; n < EACH; ++n) {
-        const int i = threadIdx.x + 256 * n, d = (i % QUADS) * 4;
-        const uint32_t at = d < D ? (static_cast<uint32_t>(i / QUADS) * static_cast<uint32_t>(token) + d) * sizeof(float) : kFar;
+        // where a round of the workgroup is whole rows, the next one is as far on for every lane
+        const uint32_t at = 256 % QUADS == 0 ? first + n * (256 / QUADS) * sizeof(float) * static_cast<uint32_t>(token) : offset(threadIdx.x + 256 * n);
         x[n] = __builtin_bit_cast(float4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, at, 0, 0));
       }
       return;
@@ -221,6 +226,7 @@ __global__ __launch_bounds__(256) void any_forward_kernel(const AttnArgs p, int 
   sequence_of(p.cu, p.sequences, p.T, row, start, end);
   const bool on = start < end;
   const int lo = wave_min_i(on ? start : p.T), hi = wave_max_i(on ? row + 1 : 0);
+  const int latest = wave_max_i(on ? start : p.T), first_row = row0 + 16 * qw;  // keys between them are seen by all the wave's rows
   Range all = group_range(lo, hi, reinterpret_cast<int*>(stats));
   take_share(all.lo, all.hi, KW * kStep, share, p.share_bits);
   float q[DP / 4];
@@ -248,12 +254,15 @@ __global__ __launch_bounds__(256) void any_forward_kernel(const AttnArgs p, int 
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       s[b] = rows_product<DP>(kt + (kw * kStep + 16 * b) * P, q, lane);
+      if (kb + kStep - 1 > first_row || kb < latest) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int key = kb + 16 * b + 4 * (lane >> 4) + i;
-        s[b][i] = on && key >= start && key <= row ? s[b][i] : kNegInf;
-        top = fmaxf(top, s[b][i]);
+        for (int i = 0; i < 4; ++i) {
+          const int key = kb + 16 * b + 4 * (lane >> 4) + i;
+          s[b][i] = on && key >= start && key <= row ? s[b][i] : kNegInf;
+        }
       }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top = fmaxf(top, s[b][i]);
     }
     top = column_max(top);
     const float ref = top == kNegInf ? 0.0f : top * p.c;  // (nothing seen yet: every weight is 0, not NaN)
@@ -336,6 +345,7 @@ __global__ __launch_bounds__(256) void any_dq_kernel(const AttnArgs p, int tiles
   sequence_of(p.cu, p.sequences, p.T, row, start, end);
   const bool on = start < end;
   const int lo = wave_min_i(on ? start : p.T), hi = wave_max_i(on ? row + 1 : 0);
+  const int latest = wave_max_i(on ? start : p.T), first_row = row0 + 16 * qw;  // keys between them are seen by all the wave's rows
   Range all = group_range(lo, hi, reinterpret_cast<int*>(stats));
   take_share(all.lo, all.hi, KW * kStep, share, p.share_bits);
   float q[DP / 4], dout[DP / 4];
@@ -376,10 +386,14 @@ __global__ __launch_bounds__(256) void any_dq_kernel(const AttnArgs p, int tiles
       const f32x4 dp = rows_product<DP>(vt + (kw * kStep + 16 * b) * P, dout, lane);
       f32x4 ds;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int key = kb + 16 * b + 4 * (lane >> 4) + i;
-        const bool seen = on && key >= start && key <= row && start < row;  // (a row's only weight is 1, whatever its score)
-        ds[i] = seen ? exp2_f32(fmaf(s[i], p.c, -lse)) * (dp[i] - delta) : 0.0f;
+      for (int i = 0; i < 4; ++i) ds[i] = exp2_f32(fmaf(s[i], p.c, -lse)) * (dp[i] - delta);
+      if (kb + kStep - 1 > first_row || kb < latest) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = kb + 16 * b + 4 * (lane >> 4) + i;
+          const bool seen = on && key >= start && key <= row && start < row;  // (a row's only weight is 1, whatever its score)
+          ds[i] = seen ? ds[i] : 0.0f;
+        }
       }
       columns_product<DP>(dq, kb_t, ds, lane);
     }
@@ -428,6 +442,7 @@ __global__ __launch_bounds__(256) void any_dkv_kernel(const AttnArgs p, int tile
   sequence_of(p.cu, p.sequences, p.T, key, start, end);
   const bool on = start < end;
   const int lo = wave_min_i(on ? key : p.T), hi = wave_max_i(on ? end : 0);
+  const int earliest = wave_min_i(on ? end : 0), last_key = key0 + 16 * qw + 15;  // rows between them see all the wave's keys
   Range all = group_range(lo, hi, reinterpret_cast<int*>(stats));
   take_share(all.lo, all.hi, KW * kStep, split & ((1 << p.key_share_bits) - 1), p.key_share_bits);
   float k[DP / 4], v[DP / 4];
@@ -462,10 +477,18 @@ __global__ __launch_bounds__(256) void any_dkv_kernel(const AttnArgs p, int tile
         f32x4 w, ds;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int r = rb + 16 * b + 4 * (lane >> 4) + i;
-          const bool seen = on && r >= key && r < end;
-          w[i] = seen ? exp2_f32(fmaf(s[i], p.c, -lse[min(r, p.T - 1)])) : 0.0f;
-          ds[i] = seen && start < r ? w[i] * (dp[i] - delta[min(r, p.T - 1)]) : 0.0f;  // (a row's only weight is 1, whatever its score)
+          const int r = min(rb + 16 * b + 4 * (lane >> 4) + i, p.T - 1);
+          w[i] = exp2_f32(fmaf(s[i], p.c, -lse[r]));
+          ds[i] = w[i] * (dp[i] - delta[r]);
+        }
+        if (rb <= last_key || rb + kStep > earliest) {  // (the row of the key itself is masked too: a row's only weight is 1, whatever its score)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = rb + 16 * b + 4 * (lane >> 4) + i;
+            const bool seen = on && r >= key && r < end;
+            w[i] = seen ? w[i] : 0.0f;
+            ds[i] = seen && start < r ? ds[i] : 0.0f;
+          }
         }
         columns_product<DP>(dv, d_t, w, lane);
         columns_product<DP>(dk, q_t, ds, lane);
