@@ -234,7 +234,8 @@ __global__ __launch_bounds__(256) void any_forward_kernel(const AttnArgs p, int 
   f32x4 o[NB];
 #pragma unroll
   for (int n = 0; n < NB; ++n) o[n] = f32x4{0, 0, 0, 0};
-  float m = kNegInf, l = 0.0f;
+  float m = kNegInf, ref = 0.0f, l = 0.0f;
+  const float growth = 8.0f / p.c;
   Staged<DP, KW * kStep> keys, values;
   auto fetch = [&](int k0) {
     keys.fetch(static_cast<const float*>(p.k) + g * p.k_head, p.k_token, k0, p.T, p.D, vec);
@@ -250,7 +251,7 @@ __global__ __launch_bounds__(256) void any_forward_kernel(const AttnArgs p, int 
     const int kb = k0 + kw * kStep;
     if (kb >= hi || kb + kStep <= lo) continue;
     f32x4 s[2];
-    float top = m;
+    float top = kNegInf;
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       s[b] = rows_product<DP>(kt + (kw * kStep + 16 * b) * P, q, lane);
@@ -265,8 +266,15 @@ __global__ __launch_bounds__(256) void any_forward_kernel(const AttnArgs p, int 
       for (int i = 0; i < 4; ++i) top = fmaxf(top, s[b][i]);
     }
     top = column_max(top);
-    const float ref = top == kNegInf ? 0.0f : top * p.c;  // (nothing seen yet: every weight is 0, not NaN)
-    const float keep = m == kNegInf ? 0.0f : exp2_f32(m * p.c - ref);
+    if (__any(!(top <= m + growth))) {  // the reference follows the maximum in steps of 2^8
+      const float next = fmaxf(m, top), next_ref = next == kNegInf ? 0.0f : next * p.c;  // (nothing seen yet: every weight is 0, not NaN)
+      const float keep = m == kNegInf ? 0.0f : exp2_f32(ref - next_ref);
+      l *= keep;
+#pragma unroll
+      for (int n = 0; n < NB; ++n) o[n] *= keep;
+      m = next;
+      ref = next_ref;
+    }
     float sum = 0.0f;
 #pragma unroll
     for (int b = 0; b < 2; ++b)
@@ -275,10 +283,7 @@ __global__ __launch_bounds__(256) void any_forward_kernel(const AttnArgs p, int 
         s[b][i] = exp2_f32(fmaf(s[b][i], p.c, -ref));
         sum += s[b][i];
       }
-    l = l * keep + sum;  // the lane group's share; the four are added at the end
-    m = top;
-#pragma unroll
-    for (int n = 0; n < NB; ++n) o[n] *= keep;
+    l += sum;  // the lane group's share; the four are added at the end
     columns_product<DP>(o, vt + (kw * kStep) * P, s[0], lane);
     columns_product<DP>(o, vt + (kw * kStep + 16) * P, s[1], lane);
   }
