@@ -801,7 +801,8 @@ int mi355_qk_norm_rotary_bwd(const void* dq_out, const void* dk_out, const void*
  * bf16 operands start and stride in whole pieces of 16 bytes, unless D is no whole number of them: then they are copied into padded rows in
  * the workspace first.  Token strides below 2^22 elements for bf16.
  * workspace: mi355_varlen_attention_fwd_workspace_bytes(T, H, G, D, sequences, dtype) bytes, on a 16-byte boundary; NULL where D is a multiple of 8
- * or fp32: then tiles of several sequences start in the order in which they lie, not the longest first.
+ * or fp32: then tiles of several sequences start in the order in which they lie, not the longest first, and the keys of tiles too few to fill the
+ * card are not dealt over workgroups (whose parts lie in the workspace).
  */
 int mi355_varlen_attention_fwd(const void* q, int64_t q_token_stride, int64_t q_head_stride,
                                const void* k, int64_t k_token_stride, int64_t k_head_stride,
@@ -814,8 +815,8 @@ int64_t mi355_varlen_attention_fwd_workspace_bytes(int64_t T, int64_t H, int64_t
 
 /*
  * Its backward; dout, out and out_rest (the forward's; out_rest may be NULL) dense, so are dq, dk and dv.  Scores are formed again.  No atomics: dk and dv of a key
- * head are sums over its query heads in a fixed order, by way of fp32 parts in the workspace where few key heads would
- * leave the card idle.  workspace: mi355_varlen_attention_bwd_workspace_bytes(T, H, G, D, dtype) bytes.
+ * head are sums over its query heads in a fixed order, by way of fp32 parts in the workspace where few key heads (for dq and all: few tiles)
+ * would leave the card idle.  workspace: mi355_varlen_attention_bwd_workspace_bytes(T, H, G, D, dtype) bytes.
  */
 int64_t mi355_varlen_attention_bwd_workspace_bytes(int64_t T, int64_t H, int64_t G, int64_t D,
                                                    int dtype);

@@ -331,11 +331,13 @@ def test_layouts_give_the_same_bits(dtype):
 
 
 @gpu
-def test_streams_and_graphs_over_other_lengths_give_the_same_bits():
-    T, H, G, D = 200, 4, 2, 128
-    leaves, dout = inputs(T, H, G, D, BF, seed=4)
+@pytest.mark.parametrize("times,dtype", [(1, BF), (12, BF), (12, F32)])  # (12: keys dealt over workgroups)
+def test_streams_and_graphs_over_other_lengths_give_the_same_bits(times, dtype):
+    T, H, G, D = 200 * times, 4, 2, 128
+    print(f"varlen_attention captured, {T} rows {dtype}", flush=True)
+    leaves, dout = inputs(T, H, G, D, dtype, seed=4)
     lengths = [[0, 120, 190], [0, 3, 200], [0, 0, 64], [0, 200, 200], [0, 77, 78]]
-    cus = [torch.tensor(c, dtype=torch.int32, device=DEV) for c in lengths]
+    cus = [torch.tensor([times * n for n in c], dtype=torch.int32, device=DEV) for c in lengths]
     want = [step(leaves, dout, c) for c in cus]
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
