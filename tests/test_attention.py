@@ -171,6 +171,8 @@ def test_attention_matches_the_formula_in_both_directions(lengths, behind, H, G,
     ([1500, 0, 1700, 40], 3, 1, 1, 96),
     ([2300], 0, 3, 1, 200),
     ([2, 1040], 0, 1, 1, 75),
+    ([1100, 960], 2, 8, 2, 64),    # in fp32 sorted by their work as well
+    ([3000, 1100], 0, 10, 2, 128),  # and in bf16
 ])
 def test_keys_dealt_over_workgroups(lengths, behind, H, G, D, dtype):
     test_attention_matches_the_formula_in_both_directions(lengths, behind, H, G, D, dtype)
