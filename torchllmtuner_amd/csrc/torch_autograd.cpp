@@ -18,10 +18,12 @@
 #include <optional>
 #include <tuple>
 
+#include "torch_autograd.h"
 #include "torch_common.h"
 
 namespace {
 
+using mi355_torch::differentiated;
 using mi355_torch::OptTensor;
 using mi355_torch::Tensor;
 using mi355_torch::typed_op;
@@ -74,7 +76,7 @@ struct RouterGate : public torch::autograd::Function<RouterGate> {
 };
 
 Tensor router_gate_autograd(const Tensor& x, const Tensor& w, const OptTensor& bias) {
-  if (!torch::autograd::compute_requires_grad(x, w, bias)) {
+  if (!differentiated("router_gate_fwd", x, w, bias)) {
     at::AutoDispatchBelowADInplaceOrView below;
     static auto op = typed_op<GateFwdSig>("mi355_moe::router_gate_fwd");
     return op.call(x, w, bias);
@@ -124,7 +126,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> router_select_autograd(const Tensor& 
                                                                   double route_scale, int64_t num_groups,
                                                                   int64_t num_limited, int64_t mode, bool want_scores,
                                                                   bool want_map) {
-  if (!torch::autograd::compute_requires_grad(logits)) {
+  if (!differentiated("router_select_fwd", logits)) {
     at::AutoDispatchBelowADInplaceOrView below;
     static auto op = typed_op<SelectFwdSig>("mi355_moe::router_select_fwd");
     return op.call(logits, bias, K, score_func, route_norm, route_scale, num_groups, num_limited, mode, want_scores,
@@ -185,7 +187,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> grouped_swiglu_autograd(const Tensor&
                                                                    const Tensor& so, const Tensor& sc, const Tensor& te,
                                                                    const Tensor& tr, const Tensor& nt, int64_t cap,
                                                                    bool zero_fill) {
-  if (!torch::autograd::compute_requires_grad(rows, w1, w3, w2)) {
+  if (!differentiated("grouped_swiglu_fwd", rows, w1, w3, w2)) {
     at::AutoDispatchBelowADInplaceOrView below;
     static auto op = typed_op<SwigluFwdSig>("mi355_moe::grouped_swiglu_fwd");
     return op.call(rows, tok, w1, w3, w2, so, sc, te, tr, nt, cap, zero_fill);
@@ -242,7 +244,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> rows_experts_combine_
     const Tensor& x, const Tensor& weights, const Tensor& w1, const Tensor& w3, const Tensor& w2, const Tensor& ros,
     const OptTensor& sor, const Tensor& total, const Tensor& so, const Tensor& sc, const Tensor& te, const Tensor& tr,
     const Tensor& nt, int64_t K, int64_t cap, bool round_terms) {
-  if (!torch::autograd::compute_requires_grad(x, weights, w1, w3, w2)) {
+  if (!differentiated("rows_experts_combine_fwd", x, weights, w1, w3, w2)) {
     at::AutoDispatchBelowADInplaceOrView below;
     static auto op = typed_op<RecFwdSig>("mi355_moe::rows_experts_combine_fwd");
     return op.call(x, weights, w1, w3, w2, ros, sor, total, so, sc, te, tr, nt, K, cap, round_terms);
@@ -299,7 +301,7 @@ std::tuple<Tensor, Tensor, Tensor> gather_experts_combine_autograd(
     const Tensor& x, const Tensor& weights, const Tensor& w1, const Tensor& w3, const Tensor& w2, const Tensor& tok,
     const Tensor& sor, const Tensor& ros, const Tensor& so, const Tensor& sc, const Tensor& te, const Tensor& tr,
     const Tensor& nt, int64_t K, int64_t cap, bool round_terms, bool save_gate_up) {
-  if (!torch::autograd::compute_requires_grad(x, weights, w1, w3, w2)) {
+  if (!differentiated("gather_experts_combine_fwd", x, weights, w1, w3, w2)) {
     at::AutoDispatchBelowADInplaceOrView below;
     static auto op = typed_op<GecFwdSig>("mi355_moe::gather_experts_combine_fwd");
     return op.call(x, weights, w1, w3, w2, tok, sor, ros, so, sc, te, tr, nt, K, cap, round_terms, save_gate_up);
@@ -343,7 +345,7 @@ struct RouterSelectCutoff : public torch::autograd::Function<RouterSelectCutoff>
 std::tuple<Tensor, Tensor, Tensor, Tensor> router_select_cutoff_autograd(const Tensor& logits, const OptTensor& bias,
                                                                          int64_t K, int64_t score_func, bool route_norm,
                                                                          double route_scale) {
-  if (!torch::autograd::compute_requires_grad(logits)) {
+  if (!differentiated("router_select_cutoff_fwd", logits)) {
     at::AutoDispatchBelowADInplaceOrView below;
     static auto op = typed_op<CutoffFwdSig>("mi355_moe::router_select_cutoff_fwd");
     return op.call(logits, bias, K, score_func, route_norm, route_scale);
@@ -379,7 +381,7 @@ struct RmsNorm : public torch::autograd::Function<RmsNorm> {
 };
 
 std::tuple<Tensor, Tensor> rms_norm_autograd(const Tensor& x, const Tensor& weight, double eps) {
-  if (!torch::autograd::compute_requires_grad(x, weight)) {
+  if (!differentiated("rms_norm_fwd", x, weight)) {
     at::AutoDispatchBelowADInplaceOrView below;
     static auto op = typed_op<RmsFwdSig>("mi355_moe::rms_norm_fwd");
     return op.call(x, weight, eps);
@@ -420,7 +422,7 @@ struct Rotary : public torch::autograd::Function<Rotary> {
 
 std::tuple<Tensor, Tensor> rotary_autograd(const Tensor& q, const Tensor& k, const Tensor& positions, const Tensor& inv_freq,
                                            bool interleaved, double factor, bool transpose) {
-  if (!torch::autograd::compute_requires_grad(q, k)) {
+  if (!differentiated("rotary", q, k, inv_freq)) {
     at::AutoDispatchBelowADInplaceOrView below;
     static auto op = typed_op<RotarySig>("mi355_moe::rotary");
     return op.call(q, k, positions, inv_freq, interleaved, factor, transpose);
@@ -471,7 +473,7 @@ struct QkNormRotary : public torch::autograd::Function<QkNormRotary> {
 std::tuple<Tensor, Tensor> qk_norm_rotary_autograd(const Tensor& q, const Tensor& k, const Tensor& qw, const Tensor& kw,
                                                    const Tensor& positions, const Tensor& inv_freq, double eps, bool interleaved,
                                                    double factor) {
-  if (!torch::autograd::compute_requires_grad(q, k, qw, kw)) {
+  if (!differentiated("qk_norm_rotary_fwd", q, k, qw, kw, inv_freq)) {
     at::AutoDispatchBelowADInplaceOrView below;
     static auto op = typed_op<QkNormFwdSig>("mi355_moe::qk_norm_rotary_fwd");
     return op.call(q, k, qw, kw, positions, inv_freq, eps, interleaved, factor);
@@ -513,7 +515,7 @@ struct VarlenAttention : public torch::autograd::Function<VarlenAttention> {
 
 std::tuple<Tensor, Tensor, Tensor> varlen_attention_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu,
                                                              double scale, bool for_backward) {
-  if (!torch::autograd::compute_requires_grad(q, k, v)) {
+  if (!differentiated("varlen_attention_fwd", q, k, v)) {
     at::AutoDispatchBelowADInplaceOrView below;
     static auto op = typed_op<AttentionFwdSig>("mi355_moe::varlen_attention_fwd");
     return op.call(q, k, v, cu, scale, for_backward);
@@ -545,7 +547,7 @@ struct BalanceLoss : public torch::autograd::Function<BalanceLoss> {
 };
 
 Tensor balance_loss_autograd(const Tensor& scores, const Tensor& map, const OptTensor& pad) {
-  if (!torch::autograd::compute_requires_grad(scores)) {
+  if (!differentiated("balance_loss_fwd", scores)) {
     at::AutoDispatchBelowADInplaceOrView below;
     static auto op = typed_op<BalanceFwdSig>("mi355_moe::balance_loss_fwd");
     return op.call(scores, map, pad);
@@ -580,7 +582,7 @@ struct PermuteRows : public torch::autograd::Function<PermuteRows> {
 
 Tensor permute_rows_autograd(const Tensor& x, const Tensor& ros, const OptTensor& sor, const Tensor& total, int64_t K,
                              int64_t cap) {
-  if (!torch::autograd::compute_requires_grad(x)) {
+  if (!differentiated("permute_rows_fwd", x)) {
     at::AutoDispatchBelowADInplaceOrView below;
     static auto op = typed_op<PermuteFwdSig>("mi355_moe::permute_rows_fwd");
     return op.call(x, ros, sor, total, K, cap);
@@ -619,7 +621,7 @@ struct Combine : public torch::autograd::Function<Combine> {
 
 Tensor combine_autograd(const Tensor& y, const Tensor& weights, const Tensor& ros, const OptTensor& sor,
                         const OptTensor& total, int64_t T, int64_t K, bool round_terms) {
-  if (!torch::autograd::compute_requires_grad(y, weights)) {
+  if (!differentiated("combine_fwd", y, weights)) {
     at::AutoDispatchBelowADInplaceOrView below;
     static auto op = typed_op<CombineFwdSig>("mi355_moe::combine_fwd");
     return op.call(y, weights, ros, sor, total, T, K, round_terms);
@@ -660,7 +662,7 @@ struct GroupedLinear : public torch::autograd::Function<GroupedLinear> {
 
 Tensor grouped_linear_autograd(const Tensor& x, const Tensor& w, const Tensor& so, const Tensor& sc, const Tensor& te,
                                const Tensor& tr, const Tensor& nt, bool zero_fill) {
-  if (!torch::autograd::compute_requires_grad(x, w)) {
+  if (!differentiated("grouped_linear_fwd", x, w)) {
     at::AutoDispatchBelowADInplaceOrView below;
     static auto op = typed_op<LinearFwdSig>("mi355_moe::grouped_linear_fwd");
     return op.call(x, w, so, sc, te, tr, nt, zero_fill);

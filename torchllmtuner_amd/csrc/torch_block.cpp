@@ -39,6 +39,7 @@
 #include <utility>
 #include <vector>
 
+#include "torch_autograd.h"
 #include "torch_common.h"
 
 namespace {
@@ -814,7 +815,7 @@ std::tuple<Tensor, Tensor, Tensor> moe_block_fwd_writing(BLOCK_PARAMS) {
 }
 
 std::tuple<Tensor, Tensor> moe_block_autograd(BLOCK_PARAMS) {
-  if (torch::autograd::compute_requires_grad(x, gate_w, gate_b, w1, w3, w2, sg, su, sd)) {
+  if (mi355_torch::differentiated("moe_block", x, gate_w, gate_b, w1, w3, w2, sg, su, sd)) {
     auto r = MoeBlock::apply(BLOCK_ARGS);
     return {r[0], r[1]};
   }
