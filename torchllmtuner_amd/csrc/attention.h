@@ -12,9 +12,15 @@
 // up its own sequence; the look-up's answer holds start <= row < end whatever the array holds, so no index leaves the tensors.
 //
 // Rows whose mask leaves nothing (in no sequence) get zeros.  A matrix product cannot leave out an element:
-// 0 x NaN, of a value in a masked place of the same tile, is NaN in the sum.  Such a sum shows at the end
-// as NaN, and only then the row is formed again by the functions here, key by key, without the masked ones.  Where no input is
-// NaN or infinite that costs one comparison an element of the result.
+// 0 x NaN, of a value in a masked place of the same tile, is NaN in the sum.  Rows of the other axis outside [lo, hi), which no row of the
+// workgroup sees, are therefore never fetched; what is left are the tiles in which a wave's rows see different things: around the diagonal
+// and where sequences meet.  Such a sum shows at the end as NaN, and the row is formed again by the functions here, key by key,
+// without the masked ones.  So does the sum of a row that sees the NaN itself, of which there may be as many as rows: not formed
+// again are rows whose statistics are NaN, and rows whose masked places, searched once a wave, hold nothing that is not finite; the others
+// begin with the nearest keys and end as soon as every spoilt element is NaN by itself.  Where no input is NaN or
+// infinite that costs one comparison an element of the result.  A training step of 4096 rows in two sequences and 96 behind, 8/2 heads of 128,
+// bf16 (fp32): 0.25 ms (1.2); all NaN 0.9 (2.0), rows behind NaN 0.25 (1.2), one query NaN 1.0 (2.0), the second sequence NaN, next to
+// whose first rows the last 56 of the first one lie in tiles with masked places only: 2.9 (3.9), which grows with the length of theirs.
 #pragma once
 #include "bf16_tiles.h"
 #include "common.h"
@@ -128,123 +134,308 @@ __device__ __forceinline__ void store_result(const AttnArgs& p, int64_t at, floa
     if (p.rest) static_cast<uint16_t*>(p.rest)[at] = f32_to_bf16(v - round_bf16(v));
 }
 
-// ---- one row by one wave: lanes over keys (or queries) for the products, over the head's elements for the sums -------------------
+// ---- rows formed again ---------------------------------------------------------------------------------
 constexpr int kHeadMax = 256;          // elements of a head
 constexpr int kLaneCols = kHeadMax / 64;
 
-// sum_d a[d] b[d], a wave's lanes each with rows of their own
+struct Span {
+  int lo, hi;
+};
+// Of the tiles of `step` rows from lo on up to hi: those within [from, to), which have no masked place.  Empty, at lo, where there are none.
+__device__ __forceinline__ Span whole_tiles(int lo, int hi, int step, int from, int to) {
+  const Span s = {lo + (max(from - lo, 0) + step - 1) / step * step, lo + max(min(to, hi) - lo, 0) / step * step};
+  return s.lo < s.hi ? s : Span{lo, lo};
+}
+
+// the lane, formed anew where a kernel has no register to keep it in
+__device__ __forceinline__ int lane_anew() { return opaque(__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0))); }
+
+// Widens `at` to the first and last of a head's rows [from, to) that hold something NaN or infinite
 template <typename T>
-__device__ float careful_dot(const T* a, const T* b, int D) {
-  float s = 0.0f;
-  for (int d = 0; d < D; ++d) s = fmaf(load_as_f32<T>(a + d), load_as_f32<T>(b + d), s);
+__device__ __forceinline__ void find_not_finite(const T* base, int64_t token, int from, int to, int D, Span& at) {
+  const int lane = lane_anew();
+  for (int r0 = from; r0 < to; r0 += 8) {  // (eight rows' loads under way together)
+    bool bad[8] = {};
+    for (int d = lane; d < D; d += kWave)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float x = load_as_f32<T>(base + min(r0 + i, to - 1) * token + d);
+        bad[i] |= x - x != 0.0f;
+      }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (__any(bad[i])) at.lo = min(at.lo, r0 + i), at.hi = max(at.hi, min(r0 + i, to - 1));
+  }
+}
+// ... of [lo, hi) but for the whole tiles
+template <typename T>
+__device__ __forceinline__ void find_beside(const T* base, int64_t token, const Span& whole, int lo, int hi, int D, Span& at) {
+  find_not_finite<T>(base, token, lo, whole.lo, D, at);
+  find_not_finite<T>(base, token, whole.hi, hi, D, at);
+}
+constexpr Span kNowhere = {INT32_MAX, -1};
+
+// Rows are formed again four at a time by matrix instructions of 4 x 4 in 16 blocks, fp32 sums, whose blocks do not mix: a score is of one row and one key
+// alone, and what four rows of a sum take from a row of the other axis is left out, or added row by row, where not all of them see it.
+constexpr int kAgain = 4;
+
+// ---- of four rows: lanes hold elements lane + 64 c of their sums, and which of them are NaN where they are stored
+struct Sums {
+  f32x4 sum[kLaneCols];
+  int lane, spoilt;  // bit 4 c + u
+  template <typename E>
+  __device__ __forceinline__ void find(int u, const E* stored, int D) {
+#pragma unroll
+    for (int c = 0; c < kLaneCols; ++c) {
+      const float x = lane + 64 * c < D ? load_as_f32<E>(stored + lane + 64 * c) : 0.0f;
+      spoilt |= x != x ? 1 << (4 * c + u) : 0;
+    }
+    spoilt = opaque(spoilt);
+  }
+  __device__ __forceinline__ void clear(int lane_) {
+    lane = lane_, spoilt = 0;
+#pragma unroll
+    for (int c = 0; c < kLaneCols; ++c) sum[c] = f32x4{0, 0, 0, 0};
+  }
+  // an element that may still come out as a number
+  __device__ __forceinline__ bool open() const {
+    bool any = false;
+#pragma unroll
+    for (int c = 0; c < kLaneCols; ++c)
+#pragma unroll
+      for (int u = 0; u < kAgain; ++u) any |= (spoilt >> (4 * c + u) & 1) && sum[c][u] == sum[c][u];
+    return __any(any);
+  }
+  template <typename Store>
+  __device__ __forceinline__ void put(int u, Store store) const {
+#pragma unroll
+    for (int c = 0; c < kLaneCols; ++c)
+      if (spoilt >> (4 * c + u) & 1) store(lane + 64 * c, sum[c][u]);
+  }
+};
+
+// The next four of a wave's rows to be formed again: `at` says where values that are not finite lie in its masked tiles, and rows that see all of those
+// keep what they have.  Lane i holds [from, to), what row row0 + i sees.
+struct Four {
+  int row0, lane[kAgain];
+  int lo[kAgain], hi[kAgain];  // what each sees
+  int first, last;             // what any of them sees
+  int kept;                    // a bit each
+  int i;                       // lane % 4
+  __device__ __forceinline__ void take(uint32_t& again, int lane_, int row0_, int from, int to, int all_lo, int all_hi, const Span& at) {
+    i = lane_ & 3, row0 = row0_;
+    first = INT32_MAX, last = 0, kept = 0;
+#pragma unroll
+    for (int u = 0; u < kAgain; ++u) {
+      const bool have = again != 0;
+      lane[u] = have ? __builtin_ctz(again) : lane[0];
+      again &= again - 1;
+      const int a = __builtin_amdgcn_readlane(from, lane[u]), b = __builtin_amdgcn_readlane(to, lane[u]);
+      const bool keeps = !have || (at.lo >= a && at.hi < b);
+      kept |= keeps ? 1 << u : 0;
+      lo[u] = max(a, all_lo), hi[u] = keeps ? lo[u] : min(b, all_hi);  // (nothing, for a row whose keys lie in other shares)
+      if (lo[u] < hi[u]) first = min(first, lo[u]), last = max(last, hi[u]);
+    }
+  }
+  __device__ __forceinline__ int row(int u) const { return row0 + lane[u]; }
+  __device__ __forceinline__ bool keeps(int u) const { return kept >> u & 1; }
+  __device__ __forceinline__ bool sees(int u, int r) const { return lo[u] <= r && r < hi[u]; }
+  // of a value per row, that of row lane % 4
+  template <typename V>
+  __device__ __forceinline__ V mine(V v0, V v1, V v2, V v3) const {
+    return i == 0 ? v0 : i == 1 ? v1 : i == 2 ? v2 : v3;
+  }
+  __device__ __forceinline__ int my_lane() const { return mine(lane[0], lane[1], lane[2], lane[3]); }
+  __device__ __forceinline__ int my_row() const { return row0 + my_lane(); }
+  __device__ __forceinline__ float of_my_row(float v) const { return __shfl(v, my_lane(), kWave); }
+};
+
+// s[i] = a . b of the row a of lane 4 (lane / 4) + i and the lane's own row b, which lanes lane % 4 share
+template <typename T>
+__device__ __forceinline__ f32x4 four_dots(const T* a, const T* b, int D) {
+  f32x4 s = {0, 0, 0, 0};
+  if constexpr (sizeof(T) == 2) {  // (rows of whole 16 bytes that start there)
+    auto eight = [&](const u32x4& x, const u32x4& y) {
+      s = __builtin_amdgcn_mfma_f32_4x4x4bf16_1k(__builtin_bit_cast(s16x4, u32x2{x[0], x[1]}), __builtin_bit_cast(s16x4, u32x2{y[0], y[1]}), s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_4x4x4bf16_1k(__builtin_bit_cast(s16x4, u32x2{x[2], x[3]}), __builtin_bit_cast(s16x4, u32x2{y[2], y[3]}), s, 0, 0, 0);
+    };
+    const u32x4 *x = reinterpret_cast<const u32x4*>(a), *y = reinterpret_cast<const u32x4*>(b);
+    int n = D / 8;
+    for (; n >= 4; n -= 4, x += 4, y += 4) {
+      const u32x4 x0 = x[0], x1 = x[1], x2 = x[2], x3 = x[3], y0 = y[0], y1 = y[1], y2 = y[2], y3 = y[3];
+      eight(x0, y0), eight(x1, y1), eight(x2, y2), eight(x3, y3);
+    }
+    for (; n > 0; --n) eight(*x++, *y++);
+  } else {
+    int d = 0;
+    for (; d + 8 <= D; d += 8)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s = __builtin_amdgcn_mfma_f32_4x4x1f32(a[d + i], b[d + i], s, 0, 0, 0);
+    for (; d < D; ++d) s = __builtin_amdgcn_mfma_f32_4x4x1f32(a[d], b[d], s, 0, 0, 0);
+  }
   return s;
 }
 
-template <typename T>
-__device__ __forceinline__ void careful_forward_row(const AttnArgs& p, int h, int row, int start) {
-  const int lane = threadIdx.x & 63;
-  const T* q = row_at<T>(p.q, p.q_token, p.q_head, row, h);
-  float acc[kLaneCols] = {}, m = kNegInf, l = 0.0f;
-  for (int j0 = start; j0 <= row; j0 += kWave) {
-    const int j = j0 + lane;
-    const float s = j <= row ? careful_dot<T>(q, row_at<T>(p.k, p.k_token, p.k_head, j, h / p.group), p.D) : kNegInf;
-    const float top = fmaxf(m, wave_max(s)), ref = top == kNegInf ? 0.0f : top * p.c;
-    const float w = j <= row ? exp2_f32(fmaf(s, p.c, -ref)) : 0.0f, keep = m == kNegInf ? 0.0f : exp2_f32(m * p.c - ref);
-    l = l * keep + wave_sum(w);
+// Adds w a of 16 rows a from `first` on that lie `token` apart: lane 4 b + u holds in w[i] the weight of row 4 b + i of 64 for the sum u; these are rows 16 PART on
+template <typename T, int PART>
+__device__ __forceinline__ void add_16(Sums& x, const f32x4& w, const Four& rows, const T* a, int64_t token, int first, int n, int D) {
+  if (n <= 0) return;
+  bool all = n >= 16;
 #pragma unroll
-    for (int i = 0; i < kLaneCols; ++i) acc[i] *= keep;
-    for (int n = 0; n < kWave && j0 + n <= row; ++n) {
-      const float wn = __shfl(w, n, kWave);
-      const T* v = row_at<T>(p.v, p.v_token, p.v_head, j0 + n, h / p.group);
+  for (int u = 0; u < kAgain; ++u) all &= rows.sees(u, first) && rows.sees(u, first + 15);
 #pragma unroll
-      for (int i = 0; i < kLaneCols; ++i)
-        if (lane + 64 * i < p.D) acc[i] = fmaf(wn, load_as_f32<T>(v + lane + 64 * i), acc[i]);
-    }
-    m = top;
-  }
-  const int64_t dense = (static_cast<int64_t>(row) * p.H + h) * p.D_out;
+  for (int c = 0; c < kLaneCols; ++c) {
+    if (64 * c >= D) break;
+    const T* at = a + min(x.lane + 64 * c, D - 1);
+    if (all) {
+      T v[16];
 #pragma unroll
-  for (int i = 0; i < kLaneCols; ++i)
-    if (lane + 64 * i < p.D_out) store_result<T>(p, dense + lane + 64 * i, acc[i] / l);
-}
-
-// dq of one row over the keys of [from, to), into the part `share` where there are parts
-template <typename T>
-__device__ __forceinline__ void careful_dq_row(const AttnArgs& p, int h, int row, int start, float lse, float delta, int from, int to, int share) {
-  const int lane = threadIdx.x & 63;
-  const T* q = row_at<T>(p.q, p.q_token, p.q_head, row, h);
-  const T* dout = static_cast<const T*>(p.dout) + (static_cast<int64_t>(row) * p.H + h) * p.D;
-  float acc[kLaneCols] = {};
-  to = min(to, row + 1);
-  for (int j0 = max(start, from); j0 < to; j0 += kWave) {
-    const int j = j0 + lane;
-    float ds = 0.0f;
-    if (j < to && start < row) {
-      const float w = exp2_f32(fmaf(careful_dot<T>(q, row_at<T>(p.k, p.k_token, p.k_head, j, h / p.group), p.D), p.c, -lse));
-      ds = w * (careful_dot<T>(dout, row_at<T>(p.v, p.v_token, p.v_head, j, h / p.group), p.D) - delta);
-    }
-    for (int n = 0; n < kWave && j0 + n < to; ++n) {
-      const float dn = __shfl(ds, n, kWave);
-      const T* k = row_at<T>(p.k, p.k_token, p.k_head, j0 + n, h / p.group);
+      for (int i = 0; i < 16; ++i) v[i] = at[i * token];
+      auto block = [&](auto which) {
+        constexpr int B = decltype(which)::value;
 #pragma unroll
-      for (int i = 0; i < kLaneCols; ++i)
-        if (lane + 64 * i < p.D) acc[i] = fmaf(dn, load_as_f32<T>(k + lane + 64 * i), acc[i]);
-    }
-  }
-  const int64_t at = (static_cast<int64_t>(row) * p.H + h) * p.D_out, part = static_cast<int64_t>(share) * p.T * p.H * p.D_out + at;
-#pragma unroll
-  for (int i = 0; i < kLaneCols; ++i) {
-    const int d = lane + 64 * i;
-    if (d >= p.D_out) continue;
-    if (p.share_bits) p.dq_part[part + d] = acc[i] * p.scale;
-    else store_from_f32<T>(static_cast<T*>(p.dq) + at + d, acc[i] * p.scale);
-  }
-}
-
-// dk and dv of one key over the rows of [from, to) of the query heads [h0, h1), into the part `split` where there are parts; delta is kept
-// times `sign`
-template <typename T>
-__device__ __forceinline__ void careful_dkv_row(const AttnArgs& p, int g, int key, int start, int end, int h0, int h1, int from, int to, int split,
-                                                float sign) {
-  const int lane = threadIdx.x & 63;
-  const T* k = row_at<T>(p.k, p.k_token, p.k_head, key, g);
-  const T* v = row_at<T>(p.v, p.v_token, p.v_head, key, g);
-  float dk[kLaneCols] = {}, dv[kLaneCols] = {};
-  end = min(end, to);
-  for (int h = h0; h < h1; ++h) {
-    for (int r0 = max(key, from); r0 < end; r0 += kWave) {
-      const int r = r0 + lane;
-      float w = 0.0f, ds = 0.0f;
-      if (r < end) {
-        const T* dout = static_cast<const T*>(p.dout) + (static_cast<int64_t>(r) * p.H + h) * p.D;
-        const int64_t at = static_cast<int64_t>(h) * p.T + r;
-        w = exp2_f32(fmaf(careful_dot<T>(row_at<T>(p.q, p.q_token, p.q_head, r, h), k, p.D), p.c, -p.lse[at]));
-        ds = start < r ? w * (careful_dot<T>(dout, v, p.D) - sign * p.delta[at]) : 0.0f;
-      }
-      for (int n = 0; n < kWave && r0 + n < end; ++n) {
-        const float wn = __shfl(w, n, kWave), dn = __shfl(ds, n, kWave);
-        const T* q = row_at<T>(p.q, p.q_token, p.q_head, r0 + n, h);
-        const T* dout = static_cast<const T*>(p.dout) + (static_cast<int64_t>(r0 + n) * p.H + h) * p.D;
-#pragma unroll
-        for (int i = 0; i < kLaneCols; ++i)
-          if (lane + 64 * i < p.D) {
-            dv[i] = fmaf(wn, load_as_f32<T>(dout + lane + 64 * i), dv[i]);
-            dk[i] = fmaf(dn, load_as_f32<T>(q + lane + 64 * i), dk[i]);
-          }
-      }
-    }
-  }
-  const int64_t at = (static_cast<int64_t>(key) * p.G + g) * p.D_out, part = static_cast<int64_t>(split) * p.T * p.G * p.D_out + at;
-#pragma unroll
-  for (int i = 0; i < kLaneCols; ++i) {
-    const int d = lane + 64 * i;
-    if (d >= p.D_out) continue;
-    if (p.splits > 1) {
-      p.dk_part[part + d] = dk[i] * p.scale;
-      p.dv_part[part + d] = dv[i];
+        for (int i = 0; i < 4; ++i)  // (block 4 PART + B of the weights to all of them)
+          x.sum[c] = __builtin_amdgcn_mfma_f32_4x4x1f32(w[i], load_as_f32<T>(&v[4 * B + i]), x.sum[c], 4, 4 * PART + B, 0);
+      };
+      block(std::integral_constant<int, 0>{});
+      block(std::integral_constant<int, 1>{});
+      block(std::integral_constant<int, 2>{});
+      block(std::integral_constant<int, 3>{});
     } else {
-      store_from_f32<T>(static_cast<T*>(p.dk) + at + d, dk[i] * p.scale);
-      store_from_f32<T>(static_cast<T*>(p.dv) + at + d, dv[i]);
+      for (int i = 0; i < min(n, 16); ++i) {
+        const float v = load_as_f32<T>(at + i * token), wi = (i & 2) ? ((i & 1) ? w[3] : w[2]) : ((i & 1) ? w[1] : w[0]);
+#pragma unroll
+        for (int u = 0; u < kAgain; ++u)
+          if (rows.sees(u, first + i))
+            x.sum[c][u] = fmaf(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(wi), 16 * PART + (i & 12) + u)), v, x.sum[c][u]);
+      }
+    }
+  }
+}
+// ... of n rows, up to 64
+template <typename T>
+__device__ __forceinline__ void add_rows(Sums& x, const f32x4& w, const Four& rows, const T* a, int64_t token, int first, int n, int D) {
+  add_16<T, 0>(x, w, rows, a, token, first, n, D);
+  add_16<T, 1>(x, w, rows, a + 16 * token, token, first + 16, n - 16, D);
+  add_16<T, 2>(x, w, rows, a + 32 * token, token, first + 32, n - 32, D);
+  add_16<T, 3>(x, w, rows, a + 48 * token, token, first + 48, n - 48, D);
+}
+
+// A wave's spoilt results over the keys of [all_lo, all_hi), by the rows' statistics, the last keys first; or with DQ its dq.  Lane i: of row row0 + i
+template <typename T, bool DQ>
+__device__ __forceinline__ void rows_again(const AttnArgs& p0, int h, int row0, uint32_t again, int start, float lse, float delta, int all_lo, int all_hi,
+                                           const Span& whole, int share) {
+  const int lane = lane_anew(), g = h / p0.group;
+  Span at = kNowhere;
+  if constexpr (DQ) find_beside(row_at<T>(p0.k, p0.k_token, p0.k_head, 0, g), p0.k_token, whole, all_lo, all_hi, p0.D, at);
+  else find_beside(row_at<T>(p0.v, p0.v_token, p0.v_head, 0, g), p0.v_token, whole, all_lo, all_hi, p0.D, at);
+  while (again) {
+    const AttnArgs& p = late_arguments();  // (anew, rather than held in scalar registers over the loops)
+    Four rows;
+    rows.take(again, lane, row0, start, row0 + lane + 1, all_lo, all_hi, at);
+    float* parts = (DQ ? p.dq_part : p.out_part) + static_cast<int64_t>(share) * p.T * p.H * p.D_out;
+    T* stored = static_cast<T*>(DQ ? p.dq : p.out);
+    Sums x;
+    x.clear(lane);
+#pragma unroll
+    for (int u = 0; u < kAgain; ++u) {
+      const int64_t dense = (static_cast<int64_t>(rows.row(u)) * p.H + h) * p.D_out;
+      if (p.share_bits) x.find(u, parts + dense, rows.keeps(u) ? 0 : p.D_out);
+      else x.find(u, stored + dense, rows.keeps(u) ? 0 : p.D_out);
+    }
+    const int64_t my_row = rows.my_row();
+    const T *q = row_at<T>(p.q, p.q_token, p.q_head, my_row, h), *dout = DQ ? static_cast<const T*>(p.dout) + (my_row * p.H + h) * p.D : nullptr;
+    const float my_lse = rows.of_my_row(lse), my_delta = DQ ? rows.of_my_row(delta) : 0.0f;
+    // (a row that sees one key: its weight is 1, whatever its score)
+    const bool several = __shfl(start, rows.my_lane(), kWave) < my_row;
+    for (int to = rows.last; rows.first < to && x.open(); to -= kWave) {
+      const int j0 = max(to - kWave, rows.first), j = min(j0 + lane, to - 1);
+      const T *k = row_at<T>(p.k, p.k_token, p.k_head, j, g), *v = row_at<T>(p.v, p.v_token, p.v_head, j, g);
+      f32x4 w = four_dots<T>(k, q, p.D);
+      if constexpr (DQ) {
+        const f32x4 dp = four_dots<T>(v, dout, p.D);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = several ? exp2_f32(fmaf(w[i], p.c, -my_lse)) * (dp[i] - my_delta) : 0.0f;
+        add_rows<T>(x, w, rows, row_at<T>(p.k, p.k_token, p.k_head, j0, g), p.k_token, j0, to - j0, p.D);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = exp2_f32(fmaf(w[i], p.c, -my_lse));
+        add_rows<T>(x, w, rows, row_at<T>(p.v, p.v_token, p.v_head, j0, g), p.v_token, j0, to - j0, p.D);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kAgain; ++u) {
+      const int64_t dense = (static_cast<int64_t>(rows.row(u)) * p.H + h) * p.D_out;
+      x.put(u, [&](int d, float sum) {
+        if (DQ) sum *= p.scale;
+        if (p.share_bits) parts[dense + d] = sum;
+        else if (DQ) store_from_f32<T>(stored + dense + d, sum);
+        else store_result<T>(p, dense + d, sum);
+      });
+    }
+  }
+}
+
+// ... and dk and dv of a wave's keys over the rows of [all_lo, all_hi) of the query heads [h0, h1), into the part `split` where there are parts, the
+// first rows first; delta is kept times `sign`
+template <typename T>
+__device__ __forceinline__ void keys_again(const AttnArgs& p0, int g, int key0, uint32_t again, int start, int end, int h0, int h1, int all_lo, int all_hi,
+                                           const Span& whole, int split, float sign) {
+  const int lane = lane_anew();
+  const int64_t dense_token = static_cast<int64_t>(p0.H) * p0.D;
+  Span at = kNowhere;
+#pragma clang loop unroll(disable)
+  for (int i = 2 * h0; i < 2 * h1; ++i) {
+    const AttnArgs& p = late_arguments();
+    if (i & 1) find_beside(static_cast<const T*>(p.dout) + (i >> 1) * p.D, dense_token, whole, all_lo, all_hi, p.D, at);
+    else find_beside(row_at<T>(p.q, p.q_token, p.q_head, 0, i >> 1), p.q_token, whole, all_lo, all_hi, p.D, at);
+  }
+#pragma clang loop unroll(disable)
+  for (int to_dk = 0; to_dk < 2; ++to_dk) {
+    for (uint32_t left = again; left;) {
+      const AttnArgs& p = late_arguments();
+      Four keys;
+      keys.take(left, lane, key0, key0 + lane, end, all_lo, all_hi, at);
+      // where the gradient of key u lies, as a part or in the storage type
+      auto with_stored = [&](int u, auto f) {
+        const AttnArgs& p = late_arguments();
+        const int64_t dense = (static_cast<int64_t>(keys.row(u)) * p.G + g) * p.D_out;
+        if (p.splits > 1) f((to_dk ? p.dk_part : p.dv_part) + static_cast<int64_t>(split) * p.T * p.G * p.D_out + dense, p);
+        else f(static_cast<T*>(to_dk ? p.dk : p.dv) + dense, p);
+      };
+      Sums x;
+      x.clear(lane);
+#pragma unroll
+      for (int u = 0; u < kAgain; ++u) with_stored(u, [&](auto* stored, const AttnArgs& p) { x.find(u, stored, keys.keeps(u) ? 0 : p.D_out); });
+      const int64_t my_key = keys.my_row();
+      const T *k = row_at<T>(p.k, p.k_token, p.k_head, my_key, g), *v = row_at<T>(p.v, p.v_token, p.v_head, my_key, g);
+      const int my_start = __shfl(start, keys.my_lane(), kWave);
+      for (int h = h0; h < h1; ++h) {
+        const T *q = row_at<T>(p.q, p.q_token, p.q_head, 0, h), *dout = static_cast<const T*>(p.dout) + h * p.D;
+        const float *lse = p.lse + static_cast<int64_t>(h) * p.T, *delta = p.delta + static_cast<int64_t>(h) * p.T;
+        for (int r0 = keys.first; r0 < keys.last && x.open(); r0 += kWave) {
+          const int n = min(keys.last - r0, kWave);
+          const int64_t r = r0 + min(lane, n - 1);
+          f32x4 w = four_dots<T>(q + r * p.q_token, k, p.D);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i] = exp2_f32(fmaf(w[i], p.c, -lse[r0 + min((lane & ~3) + i, n - 1)]));
+          if (to_dk) {
+            const f32x4 dp = four_dots<T>(dout + r * dense_token, v, p.D);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int ri = r0 + min((lane & ~3) + i, n - 1);
+              w[i] = my_start < ri ? w[i] * (dp[i] - sign * delta[ri]) : 0.0f;
+            }
+          }
+          const int64_t token = to_dk ? p.q_token : dense_token;
+          add_rows<T>(x, w, keys, (to_dk ? q : dout) + r0 * token, token, r0, n, p.D);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kAgain; ++u)
+        with_stored(u, [&](auto* stored, const AttnArgs& p) {
+          x.put(u, [&](int d, float sum) { store_from_f32(stored + d, to_dk ? sum * p.scale : sum); });
+        });
     }
   }
 }

@@ -41,16 +41,16 @@ __device__ __forceinline__ float4 four_at(const float* p, int n, bool vec) {  //
   return v;
 }
 
-// Rows [row0, row0 + ROWS) of a head on their way to LDS as fp32, zeros behind row T and behind the head's elements: held in registers from
+// Rows [row0, row0 + ROWS) of a head on their way to LDS as fp32, zeros from row `end` on and behind the head's elements: held in registers from
 // where they are fetched, a tile ahead, to where the tile before has been read
 template <int DP, int ROWS>
 struct Staged {
   static constexpr int P = DP + 4, QUADS = DP / 4, EACH = ROWS * QUADS / 256;
   static_assert(ROWS * QUADS % 256 == 0, "whole rounds of the workgroup");
   float4 x[EACH];
-  __device__ __forceinline__ void fetch(const float* base, int64_t token, int row0, int T_, int D, bool vec) {
+  __device__ __forceinline__ void fetch(const float* base, int64_t token, int row0, int end, int D, bool vec) {
     if (vec) {  // from a buffer that ends with the last row: zeros behind it, and no branch a request
-      const int64_t left = (static_cast<int64_t>(T_ - 1 - row0) * token + D) * sizeof(float);
+      const int64_t left = (static_cast<int64_t>(end - 1 - row0) * token + D) * sizeof(float);
       const uint32_t bytes = left < 0 ? 0 : left < kFar ? static_cast<uint32_t>(left) : kFar;
       const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(base) + static_cast<int64_t>(row0) * token, 0, bytes, 0x00020000);
       auto offset = [&](int i) {
@@ -70,7 +70,7 @@ struct Staged {
     for (int n = 0; n < EACH; ++n) {
       const int i = threadIdx.x + 256 * n, r = row0 + i / QUADS, d = (i % QUADS) * 4;
       x[n] = make_float4(0, 0, 0, 0);
-      if (r < T_ && d < D) x[n] = four_at(base + static_cast<int64_t>(r) * token + d, D - d, false);
+      if (r < end && d < D) x[n] = four_at(base + static_cast<int64_t>(r) * token + d, D - d, false);
     }
   }
   __device__ __forceinline__ void put(float* tile) const {
@@ -155,20 +155,20 @@ __device__ __forceinline__ int wave_max_i(int v) {
   return __builtin_amdgcn_readfirstlane(v);
 }
 
+template <int DP>
+constexpr int kAnyWaves = DP <= 64 ? 3 : 1;  // of forward and dq a SIMD, at least
+
 constexpr int kStep = 32;  // rows of the other axis that a wave takes at a time
 
 template <int DP, int KW>
 constexpr size_t kAnyLds = sizeof(float) * (KW * kStep * 2 * (DP + 4) + 128);
 
-struct Range {
-  int lo, hi;
-};
 // the range of the workgroup from those of its waves
-__device__ __forceinline__ Range group_range(int lo, int hi, int* red) {
+__device__ __forceinline__ Span group_range(int lo, int hi, int* red) {
   const int wave = threadIdx.x >> 6;
   if ((threadIdx.x & 63) == 0) red[2 * wave] = lo, red[2 * wave + 1] = hi;
   __syncthreads();
-  Range r = {min(min(red[0], red[2]), min(red[4], red[6])), max(max(red[1], red[3]), max(red[5], red[7]))};
+  Span r = {min(min(red[0], red[2]), min(red[4], red[6])), max(max(red[1], red[3]), max(red[5], red[7]))};
   __syncthreads();
   r.lo = __builtin_amdgcn_readfirstlane(r.lo);
   r.hi = __builtin_amdgcn_readfirstlane(r.hi);
@@ -215,7 +215,7 @@ __global__ __launch_bounds__(1024) void sort_tiles_kernel(const AttnArgs p, int 
 }
 
 template <int DP, int KW>
-__global__ __launch_bounds__(256) void any_forward_kernel(const AttnArgs p, int tiles, int vec) {
+__global__ __launch_bounds__(256, kAnyWaves<DP>) void any_forward_kernel(const AttnArgs p, int tiles, int vec) {
   constexpr int QW = 4 / KW, P = DP + 4, NB = DP / 16;
   extern __shared__ __attribute__((aligned(16))) float lds[];
   float *kt = lds, *vt = lds + KW * kStep * P, *stats = lds + 2 * KW * kStep * P;
@@ -228,7 +228,7 @@ __global__ __launch_bounds__(256) void any_forward_kernel(const AttnArgs p, int 
   const bool on = start < end;
   const int lo = wave_min_i(on ? start : p.T), hi = wave_max_i(on ? row + 1 : 0);
   const int latest = wave_max_i(on ? start : p.T), first_row = row0 + 16 * qw;  // keys between them are seen by all the wave's rows
-  Range all = group_range(lo, hi, reinterpret_cast<int*>(stats));
+  Span all = group_range(lo, hi, reinterpret_cast<int*>(stats));
   take_share(all.lo, all.hi, KW * kStep, share, p.share_bits);
   float q[DP / 4];
   own_rows<DP>(q, static_cast<const float*>(p.q) + h * p.q_head, p.q_token, row, on, p.D, vec, lane);
@@ -239,8 +239,8 @@ __global__ __launch_bounds__(256) void any_forward_kernel(const AttnArgs p, int 
   const float growth = 8.0f / p.c;
   Staged<DP, KW * kStep> keys, values;
   auto fetch = [&](int k0) {
-    keys.fetch(static_cast<const float*>(p.k) + g * p.k_head, p.k_token, k0, p.T, p.D, vec);
-    values.fetch(static_cast<const float*>(p.v) + g * p.v_head, p.v_token, k0, p.T, p.D, vec);
+    keys.fetch(static_cast<const float*>(p.k) + g * p.k_head, p.k_token, k0, all.hi, p.D, vec);
+    values.fetch(static_cast<const float*>(p.v) + g * p.v_head, p.v_token, k0, all.hi, p.D, vec);
   };
   if (all.lo < all.hi) fetch(all.lo);
   for (int k0 = all.lo; k0 < all.hi; k0 += KW * kStep) {
@@ -300,6 +300,8 @@ __global__ __launch_bounds__(256) void any_forward_kernel(const AttnArgs p, int 
   if (lane < 16) tops[wave * 16 + lane] = m, lens[wave * 16 + lane] = l;
   __syncthreads();
   // a wave writes the rows that it and its parts share: 16 / KW of them
+  uint32_t again = 0;
+  float row_lse = 0.0f;  // lane i: of row i of the 16
   for (int i = 0; i < 16 / KW; ++i) {
     const int mine = kw * (16 / KW) + i, r = row0 + 16 * qw + mine;
     if (r >= z.T) break;
@@ -328,18 +330,20 @@ __global__ __launch_bounds__(256) void any_forward_kernel(const AttnArgs p, int 
       if (z.share_bits) z.out_part[static_cast<int64_t>(share) * z.T * z.H * z.D + dense + d] = first < last ? v : 0.0f;
       else store_result<float>(z, dense + d, first < last ? v : 0.0f);
     }
-    if (z.share_bits) {  // (the kernel that joins the parts looks for spoilt rows)
-      if (lane == 0) z.lse_part[(static_cast<int64_t>(share) * z.H + h) * z.T + r] = first >= last ? INFINITY : nothing ? kNegInf : ref + log2f(len);
-      continue;
-    }
-    if (lane == 0 && z.lse) z.lse[static_cast<int64_t>(h) * z.T + r] = first < last ? ref + log2f(len) : INFINITY;
-    if (first < last && __any(spoilt)) careful_forward_row<float>(z, h, r, first);
+    const float lse = first >= last ? INFINITY : nothing ? kNegInf : ref + log2f(len);
+    if (lane == 0 && z.share_bits) z.lse_part[(static_cast<int64_t>(share) * z.H + h) * z.T + r] = lse;
+    if (lane == 0 && !z.share_bits && z.lse) z.lse[static_cast<int64_t>(h) * z.T + r] = lse;
+    // (a sum that is NaN, or zero: every element is NaN by the row's own scores)
+    if (first < last && len == len && len != 0.0f && __any(spoilt)) again |= 1u << mine, row_lse = lane == mine ? lse : row_lse;
   }
+  if (again)
+    rows_again<float, false>(z, h, row0 + 16 * qw, again, start, row_lse, 0.0f, all.lo, all.hi,
+                         whole_tiles(all.lo, all.hi, kStep, latest, first_row + 1), share);
 }
 
 // dq, and delta for the kernel behind this one
 template <int DP, int KW>
-__global__ __launch_bounds__(256) void any_dq_kernel(const AttnArgs p, int tiles, int vec) {
+__global__ __launch_bounds__(256, kAnyWaves<DP>) void any_dq_kernel(const AttnArgs p, int tiles, int vec) {
   constexpr int QW = 4 / KW, P = DP + 4, NB = DP / 16;
   extern __shared__ __attribute__((aligned(16))) float lds[];
   float *kt = lds, *vt = lds + KW * kStep * P, *stats = lds + 2 * KW * kStep * P;
@@ -352,7 +356,7 @@ __global__ __launch_bounds__(256) void any_dq_kernel(const AttnArgs p, int tiles
   const bool on = start < end;
   const int lo = wave_min_i(on ? start : p.T), hi = wave_max_i(on ? row + 1 : 0);
   const int latest = wave_max_i(on ? start : p.T), first_row = row0 + 16 * qw;  // keys between them are seen by all the wave's rows
-  Range all = group_range(lo, hi, reinterpret_cast<int*>(stats));
+  Span all = group_range(lo, hi, reinterpret_cast<int*>(stats));
   take_share(all.lo, all.hi, KW * kStep, share, p.share_bits);
   float q[DP / 4], dout[DP / 4];
   const int64_t dense = static_cast<int64_t>(p.H) * p.D;
@@ -373,8 +377,8 @@ __global__ __launch_bounds__(256) void any_dq_kernel(const AttnArgs p, int tiles
   for (int n = 0; n < NB; ++n) dq[n] = f32x4{0, 0, 0, 0};
   Staged<DP, KW * kStep> keys, values;
   auto fetch = [&](int k0) {
-    keys.fetch(static_cast<const float*>(p.k) + g * p.k_head, p.k_token, k0, p.T, p.D, vec);
-    values.fetch(static_cast<const float*>(p.v) + g * p.v_head, p.v_token, k0, p.T, p.D, vec);
+    keys.fetch(static_cast<const float*>(p.k) + g * p.k_head, p.k_token, k0, all.hi, p.D, vec);
+    values.fetch(static_cast<const float*>(p.v) + g * p.v_head, p.v_token, k0, all.hi, p.D, vec);
   };
   if (all.lo < all.hi) fetch(all.lo);
   for (int k0 = all.lo; k0 < all.hi; k0 += KW * kStep) {
@@ -412,6 +416,7 @@ __global__ __launch_bounds__(256) void any_dq_kernel(const AttnArgs p, int tiles
     *reinterpret_cast<f32x4*>(sums + (wave * 16 + (lane & 15)) * P + 16 * n + 4 * (lane >> 4)) = dq[n];
   if (lane < 16) lses[wave * 16 + lane] = lse, deltas[wave * 16 + lane] = delta;
   __syncthreads();
+  uint32_t again = 0;
   for (int i = 0; i < 16 / KW; ++i) {
     const int mine = kw * (16 / KW) + i, r = row0 + 16 * qw + mine;
     if (r >= z.T) break;
@@ -426,9 +431,13 @@ __global__ __launch_bounds__(256) void any_dq_kernel(const AttnArgs p, int tiles
       spoilt |= v != v;
       store_from_f32<float>(out + d, first < last ? v * z.scale : 0.0f);
     }
-    if (first < last && __any(spoilt))
-      careful_dq_row<float>(z, h, r, first, lses[(qw * KW) * 16 + mine], deltas[(qw * KW) * 16 + mine], all.lo, all.hi, share);
+    // (NaN statistics: every element is NaN by the row's own keys; but for a row that sees one, which has no gradient at all)
+    const float row_lse = lses[(qw * KW) * 16 + mine], row_delta = deltas[(qw * KW) * 16 + mine];
+    const bool own = first < r && (row_lse != row_lse || row_delta != row_delta);
+    if (first < last && !own && __any(spoilt)) again |= 1u << mine;
   }
+  if (again)
+    rows_again<float, true>(z, h, row0 + 16 * qw, again, start, lse, delta, all.lo, all.hi, whole_tiles(all.lo, all.hi, kStep, latest, first_row + 1), share);
 }
 
 // dk and dv: a wave's 16 keys against the query heads of their group, or a part of them
@@ -449,7 +458,7 @@ __global__ __launch_bounds__(256) void any_dkv_kernel(const AttnArgs p, int tile
   const bool on = start < end;
   const int lo = wave_min_i(on ? key : p.T), hi = wave_max_i(on ? end : 0);
   const int earliest = wave_min_i(on ? end : 0), last_key = key0 + 16 * qw + 15;  // rows between them see all the wave's keys
-  Range all = group_range(lo, hi, reinterpret_cast<int*>(stats));
+  Span all = group_range(lo, hi, reinterpret_cast<int*>(stats));
   take_share(all.lo, all.hi, KW * kStep, split & ((1 << p.key_share_bits) - 1), p.key_share_bits);
   float k[DP / 4], v[DP / 4];
   own_rows<DP>(k, static_cast<const float*>(p.k) + g * p.k_head, p.k_token, key, on, p.D, vec, lane);
@@ -460,8 +469,8 @@ __global__ __launch_bounds__(256) void any_dkv_kernel(const AttnArgs p, int tile
   const int64_t dense = static_cast<int64_t>(p.H) * p.D;
   Staged<DP, KW * kStep> queries, grads;
   auto fetch = [&](int h, int r0) {
-    queries.fetch(static_cast<const float*>(p.q) + h * p.q_head, p.q_token, r0, p.T, p.D, vec);
-    grads.fetch(static_cast<const float*>(p.dout) + h * p.D, dense, r0, p.T, p.D, vec);
+    queries.fetch(static_cast<const float*>(p.q) + h * p.q_head, p.q_token, r0, all.hi, p.D, vec);
+    grads.fetch(static_cast<const float*>(p.dout) + h * p.D, dense, r0, all.hi, p.D, vec);
   };
   if (all.lo < all.hi && h0 < h1) fetch(h0, all.lo);
   for (int h = h0; h < h1; ++h) {
@@ -532,13 +541,13 @@ __global__ __launch_bounds__(256) void any_dkv_kernel(const AttnArgs p, int tile
       spoilt[i] |= first < last && __any(bad);
     }
   }
+  uint32_t again = 0;
 #pragma unroll
   for (int i = 0; i < 16 / KW; ++i)
-    if (spoilt[i]) {
-      const int mine = kw * (16 / KW) + i, r = key0 + 16 * qw + mine;
-      const int first = __builtin_amdgcn_readlane(start, mine), last = __builtin_amdgcn_readlane(end, mine);
-      careful_dkv_row<float>(z, g, r, first, last, h0, h1, all.lo, all.hi, split, 1.0f);
-    }
+    if (spoilt[i]) again |= 1u << (kw * (16 / KW) + i);
+  if (again)
+    keys_again<float>(z, g, key0 + 16 * qw, again, start, end, h0, h1, all.lo, all.hi, whole_tiles(all.lo, all.hi, kStep, last_key + 1, earliest), split,
+                     1.0f);
 }
 
 // bf16 heads of a size that is no whole number of 16 bytes, copied for the matrix kernels into rows that are: a wave a head, zeros behind its
@@ -596,7 +605,7 @@ __global__ __launch_bounds__(256) void join_forward_kernel(const AttnArgs p, int
   for (int s = 0; s < SHARES; ++s) top = fmaxf(top, lse[s]);
 #pragma unroll
   for (int s = 0; s < SHARES; ++s) {
-    const float w = exp2_f32(lse[s] - top);  // (no share with a finite sum: NaN, and the row is formed again)
+    const float w = exp2_f32(lse[s] - top);  // (no share with a finite sum: NaN)
     sum += w;
     const float* part = p.out_part + (s * items + item) * p.D_out;
 #pragma unroll
@@ -612,31 +621,15 @@ __global__ __launch_bounds__(256) void join_forward_kernel(const AttnArgs p, int
       }
     }
   }
-  int start = 0, end = p.T;
-  if (top == INFINITY) sequence_of(p.cu, p.sequences, p.T, row, start, end);  // (of rows in no sequence, and of infinite scores)
-  const bool on = start < end, mine = first + (lane >> log_lanes) < items;
-  bool spoilt = false;
+  const bool on = top != INFINITY, mine = first + (lane >> log_lanes) < items;  // (infinite: of rows in no sequence, and of no others)
 #pragma unroll
   for (int i = 0; i < ITER; ++i) {
     const int d = N * (lane & (lanes - 1)) + 64 * i;
     if (d >= p.D_out || !mine) continue;
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const float v = on ? acc[i][j] / sum : 0.0f;
-      spoilt |= v != v;
-      store_result<T>(p, item * p.D_out + d + j, v);
-    }
+    for (int j = 0; j < N; ++j) store_result<T>(p, item * p.D_out + d + j, on ? acc[i][j] / sum : 0.0f);
   }
   if (mine && (lane & (lanes - 1)) == 0 && p.lse) p.lse[static_cast<int64_t>(h) * p.T + row] = on ? top + log2f(sum) : INFINITY;
-  for (uint64_t again = __ballot(spoilt); again;) {
-    const int at = __builtin_ctzll(again) >> log_lanes;
-    const int64_t it = first + at;
-    const int r = static_cast<int>(it / p.H);
-    sequence_of(p.cu, p.sequences, p.T, r, start, end);
-    careful_forward_row<T>(p, static_cast<int>(it - static_cast<int64_t>(r) * p.H), r, start);
-    const int done = (at + 1) << log_lanes;
-    again = done < 64 ? again & ~0ull << done : 0;
-  }
 }
 
 // dq, or dk and dv, from their parts, added in order, four elements a lane (n is the number of fours, or of elements where they are no whole fours)

@@ -26,6 +26,9 @@ namespace {
 
 template <int DP>
 constexpr int kWaves = DP <= 128 ? 2 : 1;  // a SIMD, by the registers that sums and operands of a wave's rows take
+// ... and at most, where LDS holds no more: a schedule for a third wave's registers takes the reads ahead away (forward of 8192 rows 504 -> 544 us)
+template <int DP>
+constexpr int kMostWaves = DP <= 64 ? 8 : kWaves<DP>;
 constexpr int kTile = 64;     // rows of the other axis a tile
 constexpr int kRows = 32;     // rows a wave
 constexpr uint32_t kFarOff = 1u << 30;  // an offset past every buffer: reads zeros
@@ -64,9 +67,6 @@ __device__ __forceinline__ bf16x8 read_turned(const Reads<DP>& reads, int n, uin
   return __builtin_bit_cast(bf16x8, v);
 }
 
-// the lane, formed anew where a kernel has no register to keep it in
-__device__ __forceinline__ int lane_anew() { return opaque(__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0))); }
-
 // Requests of a workgroup's four waves for a tile of a head's rows, 1 KiB each: a wave's j-th brings rows of its own
 template <int DP>
 struct Requests {
@@ -75,11 +75,11 @@ struct Requests {
   uint64_t base;
   int64_t row_bytes;
   uint32_t voff;
-  int T, D;
-  __device__ __forceinline__ void find(const void* p, int64_t token, int T_, int D_, int lane, int wave) {
+  int end, D;
+  __device__ __forceinline__ void find(const void* p, int64_t token, int end_, int D_, int lane, int wave) {
     base = reinterpret_cast<uint64_t>(p);
     row_bytes = token * 2;
-    T = T_, D = D_;
+    end = end_, D = D_;
     if constexpr (DP <= 128) voff = offset(lane, wave);
   }
   __device__ __forceinline__ uint32_t offset(int lane, int wave) const {
@@ -88,9 +88,9 @@ struct Requests {
     const int r = ROWS * wave + lane / CPR, c = (lane % CPR) ^ swizzle<DP>(r);
     return c * 8 < D ? static_cast<uint32_t>(r * row_bytes) + c * 16 : kFarOff;
   }
-  // rows [row0, row0 + 64) to LDS at `lds`; zeros for rows from T on
+  // rows [row0, row0 + 64) to LDS at `lds`; zeros for rows from `end` on
   __device__ __forceinline__ void request(int row0, uint32_t lds, int wave) const {
-    const int64_t left = static_cast<int64_t>(T - 1 - row0) * row_bytes + D * 2;
+    const int64_t left = static_cast<int64_t>(end - 1 - row0) * row_bytes + D * 2;
     const uint32_t bytes = left < 0 ? 0 : left < kFarOff ? static_cast<uint32_t>(left) : kFarOff;
     const uint64_t at = base + static_cast<int64_t>(row0) * row_bytes;
     const uint32_t step = 4 * ROWS * static_cast<uint32_t>(row_bytes);
@@ -242,7 +242,7 @@ struct Ranges {
 constexpr float kGrowth = 8.0f;  // a row's weights stay below 2^8 of its reference: the reference follows its maximum in such steps
 
 template <int DP>
-__global__ __launch_bounds__(256, kWaves<DP>) void bf16_forward_kernel(const AttnArgs p, int tiles) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kWaves<DP>, kMostWaves<DP>))) void bf16_forward_kernel(const AttnArgs p, int tiles) {
   constexpr int KK = DP / 16, NB = DP / 32;
   constexpr uint32_t TILE_BYTES = kTile * DP * 2;
   extern __shared__ __attribute__((aligned(16))) uint16_t smem[];
@@ -261,8 +261,8 @@ __global__ __launch_bounds__(256, kWaves<DP>) void bf16_forward_kernel(const Att
   Reads<DP> reads;
   reads.find(lane, lds0);
   Requests<DP> keys, values;
-  keys.find(static_cast<const uint16_t*>(p.k) + g * p.k_head, p.k_token, p.T, p.D, lane, wave);
-  values.find(static_cast<const uint16_t*>(p.v) + g * p.v_head, p.v_token, p.T, p.D, lane, wave);
+  keys.find(static_cast<const uint16_t*>(p.k) + g * p.k_head, p.k_token, range.hi, p.D, lane, wave);
+  values.find(static_cast<const uint16_t*>(p.v) + g * p.v_head, p.v_token, range.hi, p.D, lane, wave);
   auto request = [&](int k0, uint32_t buffer) {
     keys.request(k0, lds0 + buffer * 2 * TILE_BYTES, wave);
     values.request(k0, lds0 + buffer * 2 * TILE_BYTES + TILE_BYTES, wave);
@@ -340,49 +340,46 @@ __global__ __launch_bounds__(256, kWaves<DP>) void bf16_forward_kernel(const Att
   }
   l = halves_sum(l);
   const AttnArgs& z = late_arguments();
-  // (a share without a key of the row's: nothing to add)
-  const float inverse = z.share_bits && l == 0.0f ? 0.0f : 1.0f / l;
+  const bool nothing = z.share_bits && l == 0.0f;  // a share without a key of the row's: nothing to add
+  const float inverse = 1.0f / l, lse = !on ? INFINITY : nothing ? kNegInf : ref + log2f(l);
   bool spoilt = false;
 #pragma unroll
   for (int n = 0; n < NB; ++n)
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      o[n][i] = on ? o[n][i] * inverse : 0.0f;
+      o[n][i] = on && !nothing ? o[n][i] * inverse : 0.0f;
       spoilt |= o[n][i] != o[n][i];
     }
   if (z.D_out % 8) __syncthreads();
   const int rows = min(max(z.T - row0, 0), kRows);
   const int64_t dense = (static_cast<int64_t>(row0) * z.H + h) * z.D_out, pitch = static_cast<int64_t>(z.H) * z.D_out;
+  auto eight = [&](int n, int a, float (&v)[8]) __attribute__((always_inline)) { eight_of(o[n], a, v); };
   if (z.share_bits) {
-    store_rows<DP>(z.out_part + static_cast<int64_t>(share) * z.T * pitch + dense, pitch, rows, z.D_out, smem, wave, lane,
-                   [&](int n, int a, float (&v)[8]) __attribute__((always_inline)) { eight_of(o[n], a, v); });
-    if (half == 0 && row < z.T)
-      z.lse_part[(static_cast<int64_t>(share) * z.H + h) * z.T + row] = !on ? INFINITY : l == 0.0f ? kNegInf : ref + log2f(l);
-    return;
-  }
-  store_rows<DP>(static_cast<uint16_t*>(z.out) + dense, pitch, rows, z.D_out, smem, wave, lane,
-                 [&](int n, int a, float (&v)[8]) __attribute__((always_inline)) { eight_of(o[n], a, v); });
-  if (z.rest)
-    store_rows<DP>(static_cast<uint16_t*>(z.rest) + dense, pitch, rows, z.D_out, smem, wave, lane,
-                   [&](int n, int a, float (&v)[8]) __attribute__((always_inline)) {
-                     eight_of(o[n], a, v);
-                     const u32x4 packed = pack8(v);
+    store_rows<DP>(z.out_part + static_cast<int64_t>(share) * z.T * pitch + dense, pitch, rows, z.D_out, smem, wave, lane, eight);
+    if (half == 0 && row < z.T) z.lse_part[(static_cast<int64_t>(share) * z.H + h) * z.T + row] = lse;
+  } else {
+    store_rows<DP>(static_cast<uint16_t*>(z.out) + dense, pitch, rows, z.D_out, smem, wave, lane, eight);
+    if (z.rest)
+      store_rows<DP>(static_cast<uint16_t*>(z.rest) + dense, pitch, rows, z.D_out, smem, wave, lane,
+                     [&](int n, int a, float (&v)[8]) __attribute__((always_inline)) {
+                       eight_of(o[n], a, v);
+                       const u32x4 packed = pack8(v);
 #pragma unroll
-                     for (int i = 0; i < 8; ++i) v[i] -= __uint_as_float(i & 1 ? packed[i / 2] & 0xffff0000u : packed[i / 2] << 16);
-                   });
-  if (half == 0 && z.lse && row < z.T) z.lse[static_cast<int64_t>(h) * z.T + row] = on ? ref + log2f(l) : INFINITY;
-  uint64_t again = __ballot(spoilt && row < z.T);
-  again = (again | again >> 32) & 0xffffffffu;
-  if (again) lds_wait<0>();
-  for (; again; again &= again - 1) {
-    const int i = __builtin_ctzll(again);
-    careful_forward_row<uint16_t>(z, h, row0 + i, __builtin_amdgcn_readlane(start, i));
+                       for (int i = 0; i < 8; ++i) v[i] -= __uint_as_float(i & 1 ? packed[i / 2] & 0xffff0000u : packed[i / 2] << 16);
+                     });
+    if (half == 0 && z.lse && row < z.T) z.lse[static_cast<int64_t>(h) * z.T + row] = lse;
   }
+  // (a sum that is NaN, or zero: every element is NaN by the row's own scores)
+  const uint64_t again = __ballot(spoilt && l == l && l != 0.0f && row < z.T);
+  if (!again) return;
+  lds_wait<0>();
+  rows_again<uint16_t, false>(z, h, row0, static_cast<uint32_t>(again | again >> 32), start, lse, 0.0f, range.lo, range.hi,
+                          whole_tiles(range.lo, range.hi, kTile, latest, row0 + 1), share);
 }
 
 // dq, and delta for the kernel behind this one
 template <int DP, bool FINE>
-__global__ __launch_bounds__(256, kWaves<DP>) void bf16_dq_kernel(const AttnArgs p, int tiles) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kWaves<DP>, kMostWaves<DP>))) void bf16_dq_kernel(const AttnArgs p, int tiles) {
   constexpr int KK = DP / 16, NB = DP / 32;
   constexpr uint32_t TILE_BYTES = kTile * DP * 2;
   extern __shared__ __attribute__((aligned(16))) uint16_t smem[];
@@ -401,8 +398,8 @@ __global__ __launch_bounds__(256, kWaves<DP>) void bf16_dq_kernel(const AttnArgs
   Reads<DP> reads;
   reads.find(lane, lds0);
   Requests<DP> keys, values;
-  keys.find(static_cast<const uint16_t*>(p.k) + g * p.k_head, p.k_token, p.T, p.D, lane, wave);
-  values.find(static_cast<const uint16_t*>(p.v) + g * p.v_head, p.v_token, p.T, p.D, lane, wave);
+  keys.find(static_cast<const uint16_t*>(p.k) + g * p.k_head, p.k_token, range.hi, p.D, lane, wave);
+  values.find(static_cast<const uint16_t*>(p.v) + g * p.v_head, p.v_token, range.hi, p.D, lane, wave);
   auto request = [&](int k0, uint32_t buffer) {
     keys.request(k0, lds0 + buffer * 2 * TILE_BYTES, wave);
     values.request(k0, lds0 + buffer * 2 * TILE_BYTES + TILE_BYTES, wave);
@@ -505,15 +502,12 @@ __global__ __launch_bounds__(256, kWaves<DP>) void bf16_dq_kernel(const AttnArgs
     store_rows<DP>(z.dq_part + static_cast<int64_t>(share) * z.T * pitch + dense_dq, pitch, rows, z.D_out, smem, wave, lane, eight);
   else
     store_rows<DP>(static_cast<uint16_t*>(z.dq) + dense_dq, pitch, rows, z.D_out, smem, wave, lane, eight);
-  uint64_t again = __ballot(spoilt && row < z.T);
-  again = (again | again >> 32) & 0xffffffffu;
-  if (again) lds_wait<0>();
-  for (; again; again &= again - 1) {
-    const int i = __builtin_ctzll(again);
-    careful_dq_row<uint16_t>(z, h, row0 + i, __builtin_amdgcn_readlane(start, i),
-                             __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lse), i)),
-                             __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(delta), i)), range.lo, range.hi, share);
-  }
+  // (NaN statistics: every element is NaN by the row's own keys; but for a row that sees one, which has no gradient at all)
+  const uint64_t again = __ballot(spoilt && !(several && (lse != lse || delta != delta)) && row < z.T);
+  if (!again) return;
+  lds_wait<0>();
+  rows_again<uint16_t, true>(z, h, row0, static_cast<uint32_t>(again | again >> 32), start, lse, delta, range.lo, range.hi,
+                     whole_tiles(range.lo, range.hi, kTile, latest, row0 + 1), share);
 }
 
 // dk and dv: a wave's 32 keys against the query heads of their group, or a part of them
@@ -549,8 +543,8 @@ __global__ __launch_bounds__(256, FINE ? 1 : kWaves<DP>) void bf16_dkv_kernel(co
   for (int n = 0; n < NB; ++n) dk[n] = zeros(), dv[n] = zeros();
   const float c = p.c;
   Requests<DP> queries, grads;
-  queries.find(p.q, p.q_token, p.T, p.D, lane, wave);
-  grads.find(p.dout, static_cast<int64_t>(p.H) * p.D, p.T, p.D, lane, wave);
+  queries.find(p.q, p.q_token, range.hi, p.D, lane, wave);
+  grads.find(p.dout, static_cast<int64_t>(p.H) * p.D, range.hi, p.D, lane, wave);
   const int steps = range.lo < range.hi ? (range.hi - range.lo + kTile - 1) / kTile : 0;
   auto request = [&](int h, int r0, uint32_t buffer) {
     const uint32_t to = lds0 + buffer * STAGE;
@@ -669,15 +663,13 @@ __global__ __launch_bounds__(256, FINE ? 1 : kWaves<DP>) void bf16_dkv_kernel(co
   };
   store(z.dk, z.dk_part, dk);
   store(z.dv, z.dv_part, dv);
-  uint64_t again = __ballot(spoilt && key0 + (lane_now & 31) < z.T);
-  again = (again | again >> 32) & 0xffffffffu;
-  if (again) lds_wait<0>();
-  for (; again; again &= again - 1) {
-    const int i = __builtin_ctzll(again);
-    int first, last;
-    sequence_of(z.cu, z.sequences, z.T, key0 + i, first, last);
-    careful_dkv_row<uint16_t>(z, g, key0 + i, first, last, h0, h1, range.lo, range.hi, split, -1.0f);
-  }
+  const uint64_t again = __ballot(spoilt && key0 + (lane_now & 31) < z.T);
+  if (!again) return;
+  lds_wait<0>();
+  int first, last;
+  sequence_of(z.cu, z.sequences, z.T, key0 + (lane_now & 31), first, last);
+  keys_again<uint16_t>(z, g, key0, static_cast<uint32_t>(again | again >> 32), first, last, h0, h1, range.lo, range.hi,
+                      whole_tiles(range.lo, range.hi, kTile, key0 + kRows - 1, earliest), split, -1.0f);
 }
 
 template <int DP>
