@@ -217,37 +217,35 @@ struct Sums {
 // The next four of a wave's rows to be formed again: `at` says where values that are not finite lie in its masked tiles, and rows that see all of those
 // keep what they have.  Lane i holds [from, to), what row row0 + i sees.
 struct Four {
-  int row0, lane[kAgain];
-  int lo[kAgain], hi[kAgain];  // what each sees
-  int first, last;             // what any of them sees
-  int kept;                    // a bit each
-  int i;                       // lane % 4
+  int row0, lanes;     // the rows' lanes, six bits each from bit 8 u on, and a bit for those that keep what they have
+  int lo, hi;          // lane i: what row i sees of [all_lo, all_hi) (held by the lanes: there are not as many scalar registers)
+  int first, last;     // what any of them sees
+  int i;               // lane % 4
   __device__ __forceinline__ void take(uint32_t& again, int lane_, int row0_, int from, int to, int all_lo, int all_hi, const Span& at) {
-    i = lane_ & 3, row0 = row0_;
-    first = INT32_MAX, last = 0, kept = 0;
+    i = lane_ & 3, row0 = row0_, lo = max(from, all_lo), hi = min(to, all_hi);
+    lanes = 0, first = INT32_MAX, last = 0;
 #pragma unroll
     for (int u = 0; u < kAgain; ++u) {
       const bool have = again != 0;
-      lane[u] = have ? __builtin_ctz(again) : lane[0];
+      const int l = have ? __builtin_ctz(again) : lanes & 63;
       again &= again - 1;
-      const int a = __builtin_amdgcn_readlane(from, lane[u]), b = __builtin_amdgcn_readlane(to, lane[u]);
-      const bool keeps = !have || (at.lo >= a && at.hi < b);
-      kept |= keeps ? 1 << u : 0;
-      lo[u] = max(a, all_lo), hi[u] = keeps ? lo[u] : min(b, all_hi);  // (nothing, for a row whose keys lie in other shares)
-      if (lo[u] < hi[u]) first = min(first, lo[u]), last = max(last, hi[u]);
+      const bool keeps = !have || (at.lo >= __builtin_amdgcn_readlane(from, l) && at.hi < __builtin_amdgcn_readlane(to, l));
+      lanes |= (l | (keeps ? 64 : 0)) << 8 * u;
+      const int a = __builtin_amdgcn_readlane(lo, l), b = __builtin_amdgcn_readlane(hi, l);
+      if (!keeps && a < b) first = min(first, a), last = max(last, b);  // (a row whose keys all lie in other shares sees nothing here: its sum is 0)
     }
   }
-  __device__ __forceinline__ int row(int u) const { return row0 + lane[u]; }
-  __device__ __forceinline__ bool keeps(int u) const { return kept >> u & 1; }
-  __device__ __forceinline__ bool sees(int u, int r) const { return lo[u] <= r && r < hi[u]; }
-  // of a value per row, that of row lane % 4
-  template <typename V>
-  __device__ __forceinline__ V mine(V v0, V v1, V v2, V v3) const {
-    return i == 0 ? v0 : i == 1 ? v1 : i == 2 ? v2 : v3;
+  __device__ __forceinline__ int lane(int u) const { return lanes >> 8 * u & 63; }
+  __device__ __forceinline__ int row(int u) const { return row0 + lane(u); }
+  __device__ __forceinline__ bool keeps(int u) const { return lanes >> (8 * u + 6) & 1; }
+  __device__ __forceinline__ bool sees(int u, int r) const {
+    return !keeps(u) && __builtin_amdgcn_readlane(lo, lane(u)) <= r && r < __builtin_amdgcn_readlane(hi, lane(u));
   }
-  __device__ __forceinline__ int my_lane() const { return mine(lane[0], lane[1], lane[2], lane[3]); }
+  // what lanes hold per row: that of row lane % 4
+  __device__ __forceinline__ int my_lane() const { return lanes >> 8 * i & 63; }
   __device__ __forceinline__ int my_row() const { return row0 + my_lane(); }
   __device__ __forceinline__ float of_my_row(float v) const { return __shfl(v, my_lane(), kWave); }
+  __device__ __forceinline__ int of_my_row(int v) const { return __shfl(v, my_lane(), kWave); }
 };
 
 // s[i] = a . b of the row a of lane 4 (lane / 4) + i and the lane's own row b, which lanes lane % 4 share
@@ -282,7 +280,7 @@ __device__ __forceinline__ void add_16(Sums& x, const f32x4& w, const Four& rows
   if (n <= 0) return;
   bool all = n >= 16;
 #pragma unroll
-  for (int u = 0; u < kAgain; ++u) all &= rows.sees(u, first) && rows.sees(u, first + 15);
+  for (int u = 0; u < kAgain; ++u) all &= rows.keeps(u) || (rows.sees(u, first) && rows.sees(u, first + 15));  // (a sum that is not kept may take anything)
 #pragma unroll
   for (int c = 0; c < kLaneCols; ++c) {
     if (64 * c >= D) break;
@@ -347,7 +345,7 @@ __device__ __forceinline__ void rows_again(const AttnArgs& p0, int h, int row0, 
     const T *q = row_at<T>(p.q, p.q_token, p.q_head, my_row, h), *dout = DQ ? static_cast<const T*>(p.dout) + (my_row * p.H + h) * p.D : nullptr;
     const float my_lse = rows.of_my_row(lse), my_delta = DQ ? rows.of_my_row(delta) : 0.0f;
     // (a row that sees one key: its weight is 1, whatever its score)
-    const bool several = __shfl(start, rows.my_lane(), kWave) < my_row;
+    const bool several = rows.of_my_row(start) < my_row;
     for (int to = rows.last; rows.first < to && x.open(); to -= kWave) {
       const int j0 = max(to - kWave, rows.first), j = min(j0 + lane, to - 1);
       const T *k = row_at<T>(p.k, p.k_token, p.k_head, j, g), *v = row_at<T>(p.v, p.v_token, p.v_head, j, g);
@@ -409,7 +407,7 @@ __device__ __forceinline__ void keys_again(const AttnArgs& p0, int g, int key0, 
       for (int u = 0; u < kAgain; ++u) with_stored(u, [&](auto* stored, const AttnArgs& p) { x.find(u, stored, keys.keeps(u) ? 0 : p.D_out); });
       const int64_t my_key = keys.my_row();
       const T *k = row_at<T>(p.k, p.k_token, p.k_head, my_key, g), *v = row_at<T>(p.v, p.v_token, p.v_head, my_key, g);
-      const int my_start = __shfl(start, keys.my_lane(), kWave);
+      const int my_start = keys.of_my_row(start);
       for (int h = h0; h < h1; ++h) {
         const T *q = row_at<T>(p.q, p.q_token, p.q_head, 0, h), *dout = static_cast<const T*>(p.dout) + h * p.D;
         const float *lse = p.lse + static_cast<int64_t>(h) * p.T, *delta = p.delta + static_cast<int64_t>(h) * p.T;

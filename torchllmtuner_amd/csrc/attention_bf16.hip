@@ -239,6 +239,12 @@ struct Ranges {
   }
 };
 
+// ds in two bf16 pieces instead of one where a wave has rows (keys) of a sequence shorter than this: the ds of a row add up to nothing, and of a few
+// keys what rounding takes weighs as much as what is left.  Of sequences of two rows dq and dk were 1.7 and 1.8 times as far from the
+// formula as rounding the results would take them, from three or four on 1.4 times.  Such sequences lie in masked tiles only, where
+// the second piece's products stand: the others' code is the same with it and without.
+constexpr int kShort = 32;
+
 constexpr float kGrowth = 8.0f;  // a row's weights stay below 2^8 of its reference: the reference follows its maximum in such steps
 
 template <int DP>
@@ -378,7 +384,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kWaves<DP>,
 }
 
 // dq, and delta for the kernel behind this one
-template <int DP, bool FINE>
+template <int DP>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kWaves<DP>, kMostWaves<DP>))) void bf16_dq_kernel(const AttnArgs p, int tiles) {
   constexpr int KK = DP / 16, NB = DP / 32;
   constexpr uint32_t TILE_BYTES = kTile * DP * 2;
@@ -395,6 +401,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kWaves<DP>,
   range.find(on ? start : p.T, on ? row + 1 : 0, reinterpret_cast<int*>(smem), wave);
   take_share(range.lo, range.hi, kTile, share, p.share_bits);
   const int latest = most(on ? start : p.T);
+  const bool fine = __any(on && end - start < kShort);
   Reads<DP> reads;
   reads.find(lane, lds0);
   Requests<DP> keys, values;
@@ -462,23 +469,24 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kWaves<DP>,
           const int key = k0 + 32 * b + 8 * (i >> 2) + 4 * half + (i & 3);
           ds[i] = several && key >= start && key <= row ? ds[i] : 0.0f;
         }
+        if (fine) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const bf16x8 left = rest_of(ds, t, operand_of(ds, t));
+#pragma unroll
+            for (int n = 0; n < NB; ++n) dq[n] = mfma(read_turned(reads, n, kt + (2 * b + t) * 16 * DP * 2), left, dq[n]);
+          }
+        }
       }
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const bf16x8 w = operand_of(ds, t);
 #pragma unroll
         for (int n = 0; n < NB; ++n) dq[n] = mfma(read_turned(reads, n, kt + (2 * b + t) * 16 * DP * 2), w, dq[n]);
-        if constexpr (FINE) {
-          const bf16x8 left = rest_of(ds, t, w);
-#pragma unroll
-          for (int n = 0; n < NB; ++n) dq[n] = mfma(read_turned(reads, n, kt + (2 * b + t) * 16 * DP * 2), left, dq[n]);
-        }
       }
-      if constexpr (!FINE) {
-        reads_first<8>();
-        interleave<2 * NB - 4, 2, 0>();
-        interleave<4, 0, 0>();
-      }
+      reads_first<8>();
+      interleave<2 * NB - 4, 2, 0>();
+      interleave<4, 0, 0>();
     }
   };
   for (int k0 = range.lo; k0 < range.hi; k0 += 2 * kTile) {
@@ -511,8 +519,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kWaves<DP>,
 }
 
 // dk and dv: a wave's 32 keys against the query heads of their group, or a part of them
-template <int DP, bool FINE>
-__global__ __launch_bounds__(256, FINE ? 1 : kWaves<DP>) void bf16_dkv_kernel(const AttnArgs p, int tiles) {
+template <int DP>
+__global__ __launch_bounds__(256, kWaves<DP>) void bf16_dkv_kernel(const AttnArgs p, int tiles) {
   constexpr int KK = DP / 16, NB = DP / 32;
   constexpr uint32_t TILE_BYTES = kTile * DP * 2, STAGE = 2 * TILE_BYTES + 512;  // queries, gradients, -lse / c, -delta
   extern __shared__ __attribute__((aligned(16))) uint16_t smem[];
@@ -526,14 +534,14 @@ __global__ __launch_bounds__(256, FINE ? 1 : kWaves<DP>) void bf16_dkv_kernel(co
   int start, end;
   sequence_of(p.cu, p.sequences, p.T, key, start, end);
   const bool on = start < end;
-  const int alone = key == start;  // the first row of a sequence sees this key only: its weight is 1, whatever its score
+  // bit 0: the first row of a sequence sees this key only: its weight is 1, whatever its score; bit 1: of a short sequence
+  const int alone = (key == start) | (on && end - start < kShort) << 1;
   Ranges range;
   range.find(on ? key : p.T, on ? end : 0, reinterpret_cast<int*>(smem), wave);
   take_share(range.lo, range.hi, kTile, split & ((1 << p.key_share_bits) - 1), p.key_share_bits);
   const int earliest = least(on ? end : 0);  // rows from the wave's last key to here see all its keys
   Reads<DP> reads;
   reads.find(lane, lds0);
-  const uint32_t from_stats = lds0 + 16 * half;
   const int here = min(key, p.T - 1);
   bf16x8 k[KK], v[KK];
   own_rows<DP>(k, row_at<uint16_t>(p.k, p.k_token, p.k_head, here, g), on, p.D, lane);
@@ -573,6 +581,7 @@ __global__ __launch_bounds__(256, FINE ? 1 : kWaves<DP>) void bf16_dkv_kernel(co
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       const Reads<DP> at_tile = reads.here();
+      const uint32_t from_stats = lds0 + 16 * (lane_anew() >> 5);
       f32x16 s, ds;  // from -lse / c and -delta of the lane's rows
 #pragma unroll
       for (int a = 0; a < 4; ++a) {
@@ -602,7 +611,15 @@ __global__ __launch_bounds__(256, FINE ? 1 : kWaves<DP>) void bf16_dkv_kernel(co
           const int r = r0 + 32 * b + 8 * (i >> 2) + 4 * half + (i & 3);
           const bool seen = on && r >= key && r < end;
           s[i] = seen ? s[i] : 0.0f;
-          ds[i] = seen && r >= key + alone ? ds[i] : 0.0f;
+          ds[i] = seen && r >= key + (alone & 1) ? ds[i] : 0.0f;
+        }
+        if (__any(alone & 2)) {
+#pragma unroll
+          for (int t2 = 0; t2 < 2; ++t2) {
+            const bf16x8 left = rest_of(ds, t2, operand_of(ds, t2));
+#pragma unroll
+            for (int n = 0; n < NB; ++n) dk[n] = mfma(read_turned(at_tile, n, qt + (2 * b + t2) * 16 * DP * 2), left, dk[n]);
+          }
         }
       }
       bf16x8 w[4];
@@ -616,15 +633,7 @@ __global__ __launch_bounds__(256, FINE ? 1 : kWaves<DP>) void bf16_dkv_kernel(co
       for (int t2 = 0; t2 < 2; ++t2)
 #pragma unroll
         for (int n = 0; n < NB; ++n) dk[n] = mfma(read_turned(at_tile, n, qt + (2 * b + t2) * 16 * DP * 2), w[2 + t2], dk[n]);
-      if constexpr (FINE) {
-#pragma unroll
-        for (int t2 = 0; t2 < 2; ++t2) {
-          const bf16x8 left = rest_of(ds, t2, w[2 + t2]);
-#pragma unroll
-          for (int n = 0; n < NB; ++n) dk[n] = mfma(read_turned(at_tile, n, qt + (2 * b + t2) * 16 * DP * 2), left, dk[n]);
-        }
-      }
-      if constexpr (DP <= 128 && !FINE) {
+      if constexpr (DP <= 128) {
         reads_first<8>();
         interleave<4 * NB - 4, 2, 0>();
         interleave<4, 0, 0>();
@@ -692,26 +701,14 @@ void forward(const AttnArgs& p, hipStream_t s) {
   hipLaunchKernelGGL(bf16_forward_kernel<DP>, dim3((tiles * p.H) << p.share_bits), dim3(256), kForwardLds<DP>, s, p, tiles);
 }
 
-// ds in two bf16 pieces instead of one, for short sequences: the ds of a row add up to nothing, and of a few keys what rounding takes
-// weighs as much as what is left.  Of sequences of two rows dq and dk are 1.7 and 1.8 times as far from the formula as rounding the results
-// would take them, from three or four on 1.4 times; so short ones cost little either way.
-constexpr int kShortOnAverage = 32;  // rows a sequence
-
-template <int DP, bool FINE>
-void backward(const AttnArgs& p, hipStream_t s) {
-  static PerDeviceOnce once_q, once_kv;
-  allow(bf16_dq_kernel<DP, FINE>, kForwardLds<DP>, once_q);
-  allow(bf16_dkv_kernel<DP, FINE>, kDkvLds<DP>, once_kv);
-  const int tiles = (p.T + 4 * kRows - 1) / (4 * kRows);
-  hipLaunchKernelGGL((bf16_dq_kernel<DP, FINE>), dim3((tiles * p.H) << p.share_bits), dim3(256), kForwardLds<DP>, s, p, tiles);
-  hipLaunchKernelGGL((bf16_dkv_kernel<DP, FINE>), dim3(tiles * p.G * p.splits), dim3(256), kDkvLds<DP>, s, p, tiles);
-}
 template <int DP>
 void backward(const AttnArgs& p, hipStream_t s) {
-  if constexpr (DP <= 128) {  // (larger heads have no registers for it)
-    if (p.T < static_cast<int64_t>(kShortOnAverage) * p.sequences) return backward<DP, true>(p, s);
-  }
-  backward<DP, false>(p, s);
+  static PerDeviceOnce once_q, once_kv;
+  allow(bf16_dq_kernel<DP>, kForwardLds<DP>, once_q);
+  allow(bf16_dkv_kernel<DP>, kDkvLds<DP>, once_kv);
+  const int tiles = (p.T + 4 * kRows - 1) / (4 * kRows);
+  hipLaunchKernelGGL(bf16_dq_kernel<DP>, dim3((tiles * p.H) << p.share_bits), dim3(256), kForwardLds<DP>, s, p, tiles);
+  hipLaunchKernelGGL(bf16_dkv_kernel<DP>, dim3(tiles * p.G * p.splits), dim3(256), kDkvLds<DP>, s, p, tiles);
 }
 
 }  // namespace
