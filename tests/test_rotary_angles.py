@@ -1,0 +1,35 @@
+"""The sines and cosines of the rotary kernels, seen through pairs (1, 0), which come out as (cos a, sin a) exactly."""
+
+import pytest
+import torch
+
+from torchllmtuner_amd import ops
+
+DEV = "cuda:0"
+U = 2.0**-24
+
+
+def turned(positions, base, interleaved):
+    """(kernel's, fp64's) cosines and sines of positions times frequencies; the angles, of positions below 2^29 and 24 bits, are exact in fp64."""
+    T, pairs = positions.numel(), 64
+    inv_freq = ops.rotary_frequencies(2 * pairs, base)[0]
+    x = torch.zeros(T, 1, 2 * pairs, device=DEV)
+    if interleaved:
+        x[..., ::2] = 1.0
+    else:
+        x[..., :pairs] = 1.0
+    y = ops.rotary(x, x, positions.to(DEV), inv_freq.to(DEV), interleaved=interleaved)[0][:, 0].cpu().double()
+    c, s = (y[:, ::2], y[:, 1::2]) if interleaved else (y[:, :pairs], y[:, pairs:])
+    angle = positions.double()[:, None] * inv_freq.double()
+    return ("cosine", c, angle.cos()), ("sine", s, angle.sin())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("start", [2**29 - 10000, 10 - 2**29])
+def test_far_positions_keep_their_angle(start):
+    """An angle is off by the rounding of its turn to fp32 at most, half of 2^-25 turns or 2 pi 2^-26, near and far; fp32's sine and cosine by 4 u and the
+    product with the factor by u of themselves; the fp64 turn by 2^-53."""
+    print(f"rotary angles from position {start}", flush=True)
+    for name, got, want in turned(torch.arange(4096) + start, 10000.0, False):
+        over = (got - want).abs() - 6 * U * want.abs() - 6.2832 * 2.0**-26 - 2.0**-44
+        assert over.max() <= 0, f"{name}: {over.max():.3g} beyond the bound, {(over > 0).sum()} of {over.numel()}"

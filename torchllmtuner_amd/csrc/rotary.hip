@@ -147,9 +147,10 @@ __device__ __forceinline__ float lanes_sum(float v, int lanes) {
 __device__ __forceinline__ void turn_of(double position, float inv_freq, float factor, float& c, float& s) {
   constexpr double kHi = 0.15915494309189535, kLo = -9.839338337591243e-18;  // 1/(2 pi) = kHi + kLo
   const double a = position * static_cast<double>(inv_freq);
-  const double hi = a * kHi;
-  const double lo = fma(a, kHi, -hi) + a * kLo;
-  const float part = static_cast<float>((hi - rint(hi)) + lo);  // turns in [-1/2, 1/2]
+  // (one fused operation: a product of its own less the whole turns is one that the compiler may fuse as well, and what it then keeps of the product must
+  // not be added a second time)
+  const double turns = fma(a, kHi, -rint(a * kHi)) + a * kLo;  // in [-1/2, 1/2]
+  const float part = static_cast<float>(turns);
   float sn, cs;
   sincospif(2.0f * part, &sn, &cs);
   c = cs * factor;
