@@ -33,3 +33,16 @@ def test_far_positions_keep_their_angle(start):
     for name, got, want in turned(torch.arange(4096) + start, 10000.0, False):
         over = (got - want).abs() - 6 * U * want.abs() - 6.2832 * 2.0**-26 - 2.0**-44
         assert over.max() <= 0, f"{name}: {over.max():.3g} beyond the bound, {(over > 0).sum()} of {over.numel()}"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("base,start,step", [(10000.0, 0, 1), (500000.0, -4096, 1), (1000000.0, 10**6, 7), (10000.0, 2**29 - 10000, 1)])
+def test_sines_near_zero_are_good_relative_to_themselves(base, start, step, interleaved):
+    """fp32's sine and cosine of the rounded turn are good to 4 u of themselves (two units in the last place); what the rounding took, r <= 2 pi 2^-26
+    radians, turns them on by one fused multiply-add, rounded to u of the result; r and its product are good to 3 u of r < 2^-23, its square, left out, is
+    below 2^-46, and the fp64 turn is good to 2^-53: 6 u of the value and 2^-44."""
+    print(f"rotary sines from {start} by {step}, base {base}", flush=True)
+    for name, got, want in turned(torch.arange(4096) * step + start, base, interleaved):
+        over = (got - want).abs() - 6 * U * want.abs() - 2.0**-44
+        assert over.max() <= 0, f"{name}: {over.max():.3g} beyond the bound, {(over > 0).sum()} of {over.numel()}"

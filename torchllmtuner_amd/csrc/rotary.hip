@@ -11,8 +11,9 @@
 // and r is formed again from x, which is read anyway: the forward keeps nothing.
 //
 // Angles: the product of a position and an fp32 frequency has at most 53 bits up to positions of 2^29 and is exact in fp64;
-// it is taken to turns with 1/(2 pi) in two fp64 pieces, whole turns go away exactly, and what is left, at most
-// half a turn, is what fp32 sees: an angle of a million radians is as good as one of one.
+// it is taken to turns with 1/(2 pi) in two fp64 pieces, whole turns go away exactly, and sine and cosine of what is left, at most
+// half a turn, are fp32's of its rounded value, turned on by what the rounding took: an angle of a million radians is as good as one of one, and a sine
+// near zero as good, relative to itself, as any other.
 //
 // Bound by HBM: every element is read and written once.  A wave takes one token: its lanes form the token's sines
 // and cosines once, a pair a lane, and share them through LDS; then a lane holds the two pieces (16 bytes each where sizes
@@ -150,11 +151,11 @@ __device__ __forceinline__ void turn_of(double position, float inv_freq, float f
   // (one fused operation: a product of its own less the whole turns is one that the compiler may fuse as well, and what it then keeps of the product must
   // not be added a second time)
   const double turns = fma(a, kHi, -rint(a * kHi)) + a * kLo;  // in [-1/2, 1/2]
-  const float part = static_cast<float>(turns);
+  const float part = static_cast<float>(turns), rest = static_cast<float>(turns - part) * 6.2831853f;  // (radians, below 2^-23: their square is nothing)
   float sn, cs;
   sincospif(2.0f * part, &sn, &cs);
-  c = cs * factor;
-  s = sn * factor;
+  c = fmaf(-sn, rest, cs) * factor;
+  s = fmaf(cs, rest, sn) * factor;
 }
 
 // where the two pieces of item i of a head begin; the second may lie behind the head's end
