@@ -793,7 +793,7 @@ int mi355_qk_norm_rotary_bwd(const void* dq_out, const void* dk_out, const void*
  * it.  Rows in no sequence (behind the last entry) get zeros, and have zero gradients.  Entries out of order or out of
  * range give meaningless rows but never an access outside the tensors.
  * q (T, H, D), k and v (T, G, D) with the given strides in elements, a head's elements next to each other; out dense.
- * fp32 or bf16, 1 <= D <= 256, H a multiple of G, scale finite and positive, T < 2^30.  Scores, weights' statistics
+ * fp32 or bf16, 1 <= D <= 256, H a multiple of G, scale from 2^-100 to 2^100, T < 2^30.  Scores, weights' statistics
  * and sums are fp32; with bf16 storage the weights, and ds in the backward, are rounded to bf16 for the products that they go into.
  * out_rest: optional, bf16 only, dense like out: what rounding took from it, rounded itself; with it the backward's out . dout is as good as
  * out in fp32 (from the rounded out alone, the gradients of short rows come out twice as far from the formula).

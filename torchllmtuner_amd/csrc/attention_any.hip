@@ -764,7 +764,8 @@ int check_attention(const char* what, int dtype, int64_t sequences, int64_t T, i
                 (long long)T, (long long)H);
   MI355_REQUIRE(H * ((D + 7) / 8 * 8) < (1 << 22), "%s: %lld heads of %lld are too many", what, (long long)H, (long long)D);
   MI355_REQUIRE(D >= 1 && D <= kHeadMax, "%s: head size %lld is not within 1 to %d", what, (long long)D, kHeadMax);
-  MI355_REQUIRE(std::isfinite(scale) && scale > 0.0f, "%s: the scale must be finite and positive", what);
+  // (lse over scale log2(e), which the backward starts its sums from, stays a number)
+  MI355_REQUIRE(scale >= 0x1p-100f && scale <= 0x1p100f, "%s: the scale must be finite and positive, from 2^-100 to 2^100", what);
   return MI355_OK;
 }
 

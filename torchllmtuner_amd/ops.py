@@ -561,8 +561,8 @@ def _check_attention(q, k, v, cu_seqlens, scale):
     if cu_seqlens.dtype != torch.int32 or cu_seqlens.ndim != 1 or cu_seqlens.shape[0] < 1:
         raise ValueError("varlen_attention: cu_seqlens must be a 1-D int32 tensor with at least one entry, got "
                          f"{cu_seqlens.dtype} {tuple(cu_seqlens.shape)}")
-    if not (math.isfinite(scale) and scale > 0):
-        raise ValueError(f"varlen_attention: the scale must be finite and positive, got {scale}")
+    if not 2.0**-100 <= scale <= 2.0**100:
+        raise ValueError(f"varlen_attention: the scale must be finite and positive, from 2^-100 to 2^100, got {scale}")
 
 
 def varlen_attention(q, k, v, cu_seqlens, *, scale=None):
@@ -570,7 +570,7 @@ def varlen_attention(q, k, v, cu_seqlens, *, scale=None):
     multiple of ``G`` (query head ``h`` reads key head ``h // (H // G)``), ``1 <= D <= 256``, fp32 or bf16.
     ``cu_seqlens`` (int32, ascending, on the device) holds where each sequence begins and where the last one ends, as
     ``[0, n_0, n_0 + n_1, ...]``; sequences may be empty.  A row sees the rows of its own sequence up to itself; rows behind the last
-    sequence get zeros and have zero gradients.  ``scale`` defaults to ``D ** -0.5``.  Views into a fused projection are read
+    sequence get zeros and have zero gradients.  ``scale``, from 2^-100 to 2^100, defaults to ``D ** -0.5``.  Views into a fused projection are read
     where they lie.  Nothing is read back from the device: a call can be captured, and replayed over other
     lengths.  Differentiable in queries, keys and values; bit-identical from run to run."""
     if not q.is_cuda:
