@@ -813,6 +813,12 @@ int mi355_varlen_attention_fwd(const void* q, int64_t q_token_stride, int64_t q_
 int64_t mi355_varlen_attention_fwd_workspace_bytes(int64_t T, int64_t H, int64_t G, int64_t D,
                                                    int64_t sequences, int dtype);
 
+/* Which launches a call of these sizes makes, for tests and measurements: tiles sorted by their work, and as powers of two over how many workgroups a
+ * tile's keys are dealt in the forward (bits 4 and 5) and for dq (8, 9) and its queries for dk and dv (12, 13); bits 16 on: parts of a key head's group
+ * of query heads.  0 where the sizes are refused. */
+enum { MI355_ATTENTION_SORTED = 1 };
+int mi355_varlen_attention_paths(int64_t T, int64_t H, int64_t G, int64_t D, int64_t sequences, int dtype);
+
 /*
  * Its backward; dout, out and out_rest (the forward's; out_rest may be NULL) dense, so are dq, dk and dv.  Scores are formed again.  No atomics: dk and dv of a key
  * head are sums over its query heads in a fixed order, by way of fp32 parts in the workspace where few key heads (for dq and all: few tiles)

@@ -50,6 +50,7 @@ SIGNATURES = {
         [P, P, P, L, L, P, L, L, P, P, I, P, I, P, L, F, I, F, P, P, P, P, P, L, L, L, L, P],
     ),
     "mi355_varlen_attention_fwd": (I, [P, L, L, P, L, L, P, L, L, I, P, L, F, P, P, P, P, L, L, L, L, P]),
+    "mi355_varlen_attention_paths": (I, [L, L, L, L, L, I]),
     "mi355_varlen_attention_fwd_workspace_bytes": (L, [L, L, L, L, L, I]),
     "mi355_varlen_attention_bwd_workspace_bytes": (L, [L, L, L, L, I]),
     "mi355_varlen_attention_bwd": (

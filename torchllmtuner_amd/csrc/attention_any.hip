@@ -813,6 +813,22 @@ int share_bits(int64_t workgroups, int products, int64_t T, int64_t sequences, i
 int forward_bits(int64_t T, int64_t H, int64_t D, int64_t sequences, int dtype) {
   return share_bits(tiles_of(T, D, dtype) * H, 2, T, sequences, D, dtype, T * H * D, 1);
 }
+// What a call's launches are, by its sizes alone
+struct AttnPaths {
+  bool sorted;            // tiles in the order of their work
+  int bits, dq_bits;      // shares of the keys: 1 << bits in the forward, 1 << dq_bits for dq
+  int parts, key_bits;    // of dk and dv: parts of the group of query heads, times 1 << key_bits shares of the queries
+};
+AttnPaths paths_of(int64_t T, int64_t H, int64_t G, int64_t D, int64_t sequences, int dtype) {
+  const int64_t tiles = tiles_of(T, D, dtype);
+  AttnPaths x;
+  x.sorted = sorted_tiles(sequences, T, tiles, H);
+  x.bits = forward_bits(T, H, D, sequences, dtype);
+  x.dq_bits = share_bits(tiles * H, 3, T, sequences, D, dtype, T * H * D, 1);
+  x.parts = head_parts(T, H, G);
+  x.key_bits = share_bits(tiles * G * x.parts, 4, T, sequences, D, dtype, 2 * T * G * D, x.parts);
+  return x;
+}
 int64_t out_part_bytes(int64_t T, int64_t H, int64_t D, int bits) {
   return bits ? ((4 * T * H * D << bits) + 15) / 16 * 16 : 0;
 }
@@ -887,11 +903,12 @@ extern "C" int mi355_varlen_attention_fwd(const void* q, int64_t q_token_stride,
   MI355_REQUIRE(!padded || workspace, "varlen_attention_fwd: workspace required for bf16 heads of %lld elements", (long long)D);
   if (padded) pad_heads(p, false, static_cast<char*>(workspace) + order_bytes(T), as_stream(stream));
   MI355_REQUIRE(!matrix || attention_bf16_covers(p), "varlen_attention_fwd: bf16 operands must start and stride in whole pieces of 16 bytes");
-  if (workspace && sorted_tiles(p.sequences, T, tiles_of(T, D, dtype), H)) {
+  const AttnPaths paths = paths_of(T, H, G, D, sequences, dtype);
+  if (workspace && paths.sorted) {
     attention_sort_tiles(p, matrix ? attention_bf16_rows() : attention_any_rows((int)D), static_cast<int32_t*>(workspace), nullptr, as_stream(stream));
     p.query_order = static_cast<int32_t*>(workspace);
   }
-  if (workspace) p.share_bits = forward_bits(T, H, D, sequences, dtype);
+  if (workspace) p.share_bits = paths.bits;
   if (p.share_bits) {
     char* at = static_cast<char*>(workspace) + order_bytes(T) + (padded ? padded_bytes(T, H + 2 * G, D) : 0);
     p.out_part = reinterpret_cast<float*>(at);
@@ -903,12 +920,17 @@ extern "C" int mi355_varlen_attention_fwd(const void* q, int64_t q_token_stride,
   return check_launch("varlen_attention_fwd");
 }
 
+extern "C" int mi355_varlen_attention_paths(int64_t T, int64_t H, int64_t G, int64_t D, int64_t sequences, int dtype) {
+  if (T < 1 || check_attention("varlen_attention_paths", dtype, sequences, T, H, G, D, 1.0f)) return 0;
+  const AttnPaths x = paths_of(T, H, G, D, sequences, dtype);
+  return (x.sorted ? MI355_ATTENTION_SORTED : 0) | x.bits << 4 | x.dq_bits << 8 | x.key_bits << 12 | x.parts << 16;
+}
+
 extern "C" int64_t mi355_varlen_attention_fwd_workspace_bytes(int64_t T, int64_t H, int64_t G, int64_t D, int64_t sequences, int dtype) {
   if (T < 1 || H < 1 || G < 1 || D < 1) return 0;
-  const int64_t tiles = tiles_of(T, D, dtype);
   const int bits = forward_bits(T, H, D, sequences, dtype);
   const int64_t copies = padded_heads(D, dtype) ? padded_bytes(T, H + 2 * G, D) : 0;
-  if (!copies && !bits && !sorted_tiles(sequences, T, tiles, H)) return 0;
+  if (!copies && !bits && !sorted_tiles(sequences, T, tiles_of(T, D, dtype), H)) return 0;
   return order_bytes(T) + copies + out_part_bytes(T, H, D, bits) + lse_part_bytes(T, H, bits);
 }
 
@@ -934,11 +956,8 @@ extern "C" int mi355_varlen_attention_bwd(const void* dout, const void* q, int64
                               cu_seqlens, sequences, scale, T, H, G, D);
   p.o = out, p.rest = dtype == MI355_BF16 ? const_cast<void*>(out_rest) : nullptr;
   p.dout = dout, p.lse = const_cast<float*>(lse), p.dq = dq, p.dk = dk, p.dv = dv;
-  const int64_t tiles = tiles_of(T, D, dtype);
-  p.splits = head_parts(T, H, G);
-  p.share_bits = share_bits(tiles * H, 3, T, sequences, D, dtype, T * H * D, 1);
-  p.key_share_bits = share_bits(tiles * G * p.splits, 4, T, sequences, D, dtype, 2 * T * G * D, p.splits);
-  p.splits <<= p.key_share_bits;
+  const AttnPaths paths = paths_of(T, H, G, D, sequences, dtype);
+  p.share_bits = paths.dq_bits, p.key_share_bits = paths.key_bits, p.splits = paths.parts << paths.key_bits;
   p.delta = static_cast<float*>(workspace);
   char* at = reinterpret_cast<char*>(p.delta + (2 * H * T + 3) / 4 * 4);
   int32_t *query_order = reinterpret_cast<int32_t*>(at), *key_order = reinterpret_cast<int32_t*>(at + order_bytes(T));
@@ -953,7 +972,7 @@ extern "C" int mi355_varlen_attention_bwd(const void* dout, const void* q, int64
   p.dv_part = p.dk_part + static_cast<int64_t>(p.splits) * T * G * D;
   const bool matrix = dtype == MI355_BF16;
   MI355_REQUIRE(!matrix || attention_bf16_covers(p), "varlen_attention_bwd: bf16 operands must start and stride in whole pieces of 16 bytes");
-  if (sorted_tiles(p.sequences, T, tiles, H)) {
+  if (paths.sorted) {
     attention_sort_tiles(p, matrix ? attention_bf16_rows() : attention_any_rows((int)D), query_order, key_order, as_stream(stream));
     p.query_order = query_order, p.key_order = key_order;
   }
