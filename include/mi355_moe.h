@@ -816,7 +816,7 @@ int64_t mi355_varlen_attention_fwd_workspace_bytes(int64_t T, int64_t H, int64_t
 /* Which launches a call of these sizes makes, for tests and measurements: tiles sorted by their work, and as powers of two over how many workgroups a
  * tile's keys are dealt in the forward (bits 4 and 5) and for dq (8, 9) and its queries for dk and dv (12, 13); bits 16 on: parts of a key head's group
  * of query heads.  0 where the sizes are refused. */
-enum { MI355_ATTENTION_SORTED = 1 };
+enum { MI355_ATTENTION_FWD_SORTED = 1, MI355_ATTENTION_BWD_SORTED = 2 };
 int mi355_varlen_attention_paths(int64_t T, int64_t H, int64_t G, int64_t D, int64_t sequences, int dtype);
 
 /*

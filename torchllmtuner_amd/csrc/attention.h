@@ -441,12 +441,19 @@ __device__ __forceinline__ void keys_again(const AttnArgs& p0, int g, int key0, 
 // ---- order of the tiles ---------------------------------------------------------------------------------
 // A tile's work is as long as the other axis that its rows see.  Of one sequence the last rows see the most; of several nothing about
 // it is known without cu_seqlens, and a heavy tile that starts last ends long after the others.  Where there are more
-// workgroups than the card holds at once and sequences are long on average, one small kernel (5 us) sorts the tiles by their work
-// first: forward and dq of 8192 rows in 4 sequences, 32 heads of 128, 178 -> 164 and 260 -> 239 us, of 16384 in 11 345 -> 318 and 502 -> 462.
-constexpr int kHeldAtOnce = 512;     // workgroups: two a CU
-constexpr int kLongOnAverage = 512;  // rows a sequence: below, a tile's work differs by less than the sorting costs
-inline bool sorted_tiles(int64_t sequences, int64_t T, int64_t tiles, int64_t heads) {
-  return sequences > 1 && T >= kLongOnAverage * sequences && tiles * heads > kHeldAtOnce / 2;
+// workgroups than the card holds at once and sequences are long on average (entries of cu_seqlens, empty ones among them), one small kernel (5 us) sorts
+// the tiles by their work first: the backward from 512 rows a sequence on, the forward, whose tiles take a third of the time, from 1024.  us not sorted -> sorted,
+// even lengths; uneven ones (split at random), on one box:
+//   forward   8192 rows, 32/4 heads of 128   2048 a sequence 185 -> 184; 205 -> 206   1024 99 -> 101; 134 -> 133    512 69 -> 76; 112 -> 113
+//             8192, 16/16 of 64                         73 -> 57; 99 -> 107           42 -> 37; 59 -> 60            28 -> 29; 50 -> 55
+//             fp32 4096, 8/2 of 64                      113 -> 112; 112 -> 117        80 -> 74; 92 -> 93            56 -> 54; 64 -> 63
+//   forward   8192 rows, 32/4 heads of 128   2048 781 -> 716; 1043 -> 1056            512 359 -> 364; 587 -> 560    256 290 -> 320; 457 -> 444
+//   and       8192, 16/16 of 64                   257 -> 229; 383 -> 395                  122 -> 119; 215 -> 202         96 -> 105; 169 -> 165
+//   backward  fp32 4096, 8/2 of 64                465 -> 456; 473 -> 476                  217 -> 194; 261 -> 234         156 -> 146; 227 -> 213
+constexpr int kHeldAtOnce = 512;             // workgroups: two a CU
+constexpr int kLongForward = 1024, kLongBackward = 512;  // rows a sequence: below, a tile's work differs by less than the sorting costs
+inline bool sorted_tiles(int64_t sequences, int64_t T, int64_t tiles, int64_t heads, int rows_each) {
+  return sequences > 1 && T >= rows_each * sequences && tiles * heads > kHeldAtOnce / 2;
 }
 // order[i]: the i-th tile of `rows` rows to start
 void attention_sort_tiles(const AttnArgs& p, int rows, int32_t* query_order, int32_t* key_order, hipStream_t s);

@@ -815,14 +815,14 @@ int forward_bits(int64_t T, int64_t H, int64_t D, int64_t sequences, int dtype) 
 }
 // What a call's launches are, by its sizes alone
 struct AttnPaths {
-  bool sorted;            // tiles in the order of their work
+  bool sorted, bwd_sorted;  // tiles in the order of their work: in the forward, in the backward
   int bits, dq_bits;      // shares of the keys: 1 << bits in the forward, 1 << dq_bits for dq
   int parts, key_bits;    // of dk and dv: parts of the group of query heads, times 1 << key_bits shares of the queries
 };
 AttnPaths paths_of(int64_t T, int64_t H, int64_t G, int64_t D, int64_t sequences, int dtype) {
   const int64_t tiles = tiles_of(T, D, dtype);
   AttnPaths x;
-  x.sorted = sorted_tiles(sequences, T, tiles, H);
+  x.sorted = sorted_tiles(sequences, T, tiles, H, kLongForward), x.bwd_sorted = sorted_tiles(sequences, T, tiles, H, kLongBackward);
   x.bits = forward_bits(T, H, D, sequences, dtype);
   x.dq_bits = share_bits(tiles * H, 3, T, sequences, D, dtype, T * H * D, 1);
   x.parts = head_parts(T, H, G);
@@ -923,14 +923,14 @@ extern "C" int mi355_varlen_attention_fwd(const void* q, int64_t q_token_stride,
 extern "C" int mi355_varlen_attention_paths(int64_t T, int64_t H, int64_t G, int64_t D, int64_t sequences, int dtype) {
   if (T < 1 || check_attention("varlen_attention_paths", dtype, sequences, T, H, G, D, 1.0f)) return 0;
   const AttnPaths x = paths_of(T, H, G, D, sequences, dtype);
-  return (x.sorted ? MI355_ATTENTION_SORTED : 0) | x.bits << 4 | x.dq_bits << 8 | x.key_bits << 12 | x.parts << 16;
+  return (x.sorted ? MI355_ATTENTION_FWD_SORTED : 0) | (x.bwd_sorted ? MI355_ATTENTION_BWD_SORTED : 0) | x.bits << 4 | x.dq_bits << 8 | x.key_bits << 12 | x.parts << 16;
 }
 
 extern "C" int64_t mi355_varlen_attention_fwd_workspace_bytes(int64_t T, int64_t H, int64_t G, int64_t D, int64_t sequences, int dtype) {
   if (T < 1 || H < 1 || G < 1 || D < 1) return 0;
   const int bits = forward_bits(T, H, D, sequences, dtype);
   const int64_t copies = padded_heads(D, dtype) ? padded_bytes(T, H + 2 * G, D) : 0;
-  if (!copies && !bits && !sorted_tiles(sequences, T, tiles_of(T, D, dtype), H)) return 0;
+  if (!copies && !bits && !sorted_tiles(sequences, T, tiles_of(T, D, dtype), H, kLongForward)) return 0;
   return order_bytes(T) + copies + out_part_bytes(T, H, D, bits) + lse_part_bytes(T, H, bits);
 }
 
@@ -972,7 +972,7 @@ extern "C" int mi355_varlen_attention_bwd(const void* dout, const void* q, int64
   p.dv_part = p.dk_part + static_cast<int64_t>(p.splits) * T * G * D;
   const bool matrix = dtype == MI355_BF16;
   MI355_REQUIRE(!matrix || attention_bf16_covers(p), "varlen_attention_bwd: bf16 operands must start and stride in whole pieces of 16 bytes");
-  if (paths.sorted) {
+  if (paths.bwd_sorted) {
     attention_sort_tiles(p, matrix ? attention_bf16_rows() : attention_any_rows((int)D), query_order, key_order, as_stream(stream));
     p.query_order = query_order, p.key_order = key_order;
   }
