@@ -744,12 +744,14 @@ int mi355_rms_norm_bwd(const void* dy, const void* x, const void* weight, const 
                        int64_t D, void* stream);
 
 /*
- * Rotary positions of the queries and keys (the `rotary` entry of the reference's kernel registry,
- * llmtuner/kernel/ops/rotary.py), in one launch for both.
+ * Rotary positions of the queries and keys, in one launch for both: what the `rotary` entry of the reference's kernel registry is for
+ * (llmtuner/kernel/ops/rotary.py); the signature, positions and frequencies rather than tables of sines, is this library's own, and no outputs of that file were there to
+ * hold this against (parity unpinned).
  *   a = positions[t] * inv_freq[i];  c = attention_factor cos a;  s = attention_factor sin a
  *   u' = u c - v s,  v' = v c + u s   over the pairs (i, i + pairs) of a head, or (2i, 2i + 1) where `interleaved`
  * Elements from 2 * pairs on are copied.  `transpose` turns the other way, which is the backward pass.
- * Angles are formed in fp64 and reduced there, the rest is fp32 with one rounding to `dtype` (fp32 or bf16).
+ * Angles are formed in fp64 and reduced there, for sines and cosines good to a few units in the last place of themselves; the rest is fp32 with one rounding to `dtype`
+ * (fp32 or bf16).
  * q is (T, H, D) and k (T, G, D) with the given strides in elements, the elements of a head next to each
  * other; the results are dense.  2 <= D <= 512, 2 * pairs <= D.  positions: int32, or int64 where positions_i64.
  * Operands need be aligned to their element only (16-byte pieces where sizes, strides and bases allow).
@@ -786,17 +788,22 @@ int mi355_qk_norm_rotary_bwd(const void* dq_out, const void* dk_out, const void*
                              int64_t H, int64_t G, int64_t D, void* stream);
 
 /*
- * Causal attention over packed sequences with grouped heads (the `varlen_attention` entry of the reference's kernel
- * registry, llmtuner/kernel/ops/varlen_attention.py).  Query head h of row r in sequence [start, end), key head g = h / (H / G):
+ * Causal attention over packed sequences with grouped heads: what the `varlen_attention` entry of the reference's kernel
+ * registry is for (llmtuner/kernel/ops/varlen_attention.py), with a signature of this library's own (parity unpinned).  Query head h of row r in sequence [start, end), key head g = h / (H / G):
  *   out[r][h] = sum_{start <= j <= r} softmax_j(scale q[r][h] . k[j][g]) v[j][g]
  * cu_seqlens (sequences + 1, int32, ascending): where the sequences begin and the last one ends.  It stays on the device: no size depends on
  * it.  Rows in no sequence (behind the last entry) get zeros, and have zero gradients.  Entries out of order or out of
  * range give meaningless rows but never an access outside the tensors.
  * q (T, H, D), k and v (T, G, D) with the given strides in elements, a head's elements next to each other; out dense.
  * fp32 or bf16, 1 <= D <= 256, H a multiple of G, scale from 2^-100 to 2^100, T < 2^30.  Scores, weights' statistics
- * and sums are fp32; with bf16 storage the weights, and ds in the backward, are rounded to bf16 for the products that they go into.
+ * and sums are fp32; with bf16 storage the weights, and ds in the backward, are rounded to bf16 for the products that they go into, as the matrix instructions take them
+ * (ds of sequences shorter than 32 rows in two pieces): results are then 1.06 to 1.35 and gradients 1.35 to 1.45 times as far from the formula as rounding the
+ * exact ones to bf16 takes them (relative L2), gradients of sequences shorter than 32 rows 1.07 to 1.35.
+ * Visible values that are not finite make not finite what they enter, masked ones nothing; values beyond 2^118 may overflow in the sums.
  * out_rest: optional, bf16 only, dense like out: what rounding took from it, rounded itself; with it the backward's out . dout is as good as
  * out in fp32 (from the rounded out alone, the gradients of short rows come out twice as far from the formula).
+ * How tiles are dealt and sorted goes by the number of entries of cu_seqlens: a call padded with empty slots gets the same results, up to the
+ * order in which dealt parts are summed, and may take longer.
  * lse: optional (H, T) fp32, log2 of each row's sum of exp(scale q.k), +inf for rows in no sequence; the backward reads it.
  * bf16 operands start and stride in whole pieces of 16 bytes, unless D is no whole number of them: then they are copied into padded rows in
  * the workspace first.  Token strides below 2^22 elements for bf16.

@@ -16,7 +16,7 @@
 // through LDS at the end; four groups and one part for heads beyond 128, whose tiles would take too many registers.  Four parts of one group, and
 // one of four, were no faster for heads of 64 either.
 //
-// Measured: 2048 rows in 3 uneven sequences, 8/2 heads of 64: forward 48 us, dq 53, dk/dv 64, where the seven products of the formulas (5.8 GFLOP) take
+// Measured: 2048 rows in 3 uneven sequences, 8/2 heads of 64: forward 46 us, dq 52, dk/dv 64, where the seven products of the formulas (5.8 GFLOP) take
 // 43 at the rate of a large fp32 product (137 TFLOP/s) and the kernels form nine.  512 workgroups are two waves a SIMD, and the last rows
 // of a sequence see dozens of times what its first ones do.  The matrix pipes are busy a third of the time that a CU is: a wave waits as long for its turn
 // to issue as for LDS, memory and barriers.  Masks only where a tile has any and offsets formed once took a ninth off the backward; backward tiles
@@ -551,7 +551,7 @@ __global__ __launch_bounds__(256) void any_dkv_kernel(const AttnArgs p, int tile
 }
 
 // bf16 heads of a size that is no whole number of 16 bytes, copied for the matrix kernels into rows that are: a wave a head, zeros behind its
-// elements.  8192 rows of 16/4 heads of 75, forward 140 us, forward and backward 558; in fp32 products from where they lay 1054 and 4631,
+// elements.  8192 rows in 4 sequences of 16/4 heads of 75, forward 113 us, forward and backward 467; in fp32 products from where they lay 1054 and 4631,
 // and of 64 rows no faster.
 struct PadArgs {
   const uint16_t* from[6];
@@ -783,7 +783,8 @@ int head_parts(int64_t T, int64_t H, int64_t G) {
 // through memory in fp32.  Whether that pays is a matter of what a workgroup of its own takes against the trip: of `products` per key, a
 // workgroup alone reaches two thirds of the matrix rate of its CU, and the card no more than the whole of it; a launch that joins 3 us; memory 5 TB/s.
 // One sequence, bf16 heads of 128, us, whole / dealt: forward of 16384 rows of one head 287 / 101, 4096 of 4 77 / 42, 1024 of 4 24 / 19 (of 16 25 / 30: not
-// dealt); backward 1060 / 305, 292 / 126, 90 / 54 (of 16 99 / 74); fp32, 4096 of one 223 / 80 and 664 / 216.
+// dealt); backward 1060 / 305, 292 / 126, 90 / 54 (of 16 99 / 74); fp32, 4096 of one 223 / 80 and 664 / 216.  (Drawn with earlier kernels; dealt, these are
+// 97, 40, 19, 298, 124, 54 and 77, 82 and 219 now.)
 int tile_rows(int64_t D, int dtype) { return dtype == MI355_BF16 ? attention_bf16_rows() : attention_any_rows((int)D); }
 int64_t tiles_of(int64_t T, int64_t D, int dtype) { return (T + tile_rows(D, dtype) - 1) / tile_rows(D, dtype); }
 constexpr int kMostShares = 3;  // a power of two

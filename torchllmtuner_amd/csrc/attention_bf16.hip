@@ -15,8 +15,14 @@
 //
 // Bound by the matrix pipes and the vector work beside them, which add up at two waves a SIMD rather than hide each other; a third wave, and
 // priorities around the products, did not help.  32/4 heads of 128, where a large library product reaches 1200 TFLOP/s: forward of one sequence of 8192
-// rows 0.50-0.53 ms, 1040-1100 TFLOP/s; forward, dq and dk/dv of 8192 rows in 4 sequences 172, 242 and 296 us, 800, 850 and 930
-// (two, three and four products); of 16384 in 11 uneven ones 351, 497 and 624, 760, 810 and 860.
+// rows 522 us, 1050 TFLOP/s; forward, dq and dk/dv of 8192 rows in 4 sequences 162, 230 and 277 us, 850, 900 and 990
+// (two, three and four products); of 16384 in 11 uneven ones 347, 497 and 628, 770, 810 and 850.  Boxes differ by 5 %.  Heads between the forms' sizes take
+// the next one's products: 8192 rows in 4, 16/4 heads, forward us (TFLOP/s of the heads' own products) of 64 55 (620), 80 82 (520), 96 84 (620), 128 88 (780),
+// 136 196 (370), 160 197 (430), 192 199 (520), 256 204 (670).
+//
+// Weights and ds are rounded to bf16 in front of their products, because the matrix instruction takes them so; in two pieces each they would be half as many
+// products again.  Relative L2 distance from the formula in fp64 of results and gradients as they are stored (rounding the exact ones alone: 0.0016):
+// one sequence of 8192 0.0021; 4 of 2048 0.0021, dq and dk 0.0024, dv 0.0023.
 #include <algorithm>
 
 #include "attention.h"

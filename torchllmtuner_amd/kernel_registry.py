@@ -17,8 +17,10 @@ reference's own registry::
     register_kernel("rms_norm", "cuda")(rms_norm_mi355)
 
 ``rms_norm`` (``llmtuner/kernel/ops/rms_norm.py:10-31``) is the norm the decoder layer applies
-right before the MoE block; it gets a ``"cuda"`` backend the same way.  So do ``rotary``, ``qk_norm_rotary`` and
-``varlen_attention``, what the layer computes between its projections in front of that norm.
+right before the MoE block; it gets a ``"cuda"`` backend the same way.  ``rotary``, ``qk_norm_rotary`` and
+``varlen_attention``, what the layer computes between its projections in front of that norm, are registered the same way under
+signatures of this package's own (``rotary`` takes positions and frequencies, not tables of sines); the reference's registry has
+entries for the same purposes (``llmtuner/kernel/ops/{rotary,varlen_attention}.py``) that they are not drop-in backends of.
 
 There is no torch-math backend here: asking for one (``use_eager=True``, a CPU tensor,
 ``fallback_to_cpu=True`` with nothing registered for ``"cpu"``) raises.
