@@ -443,7 +443,7 @@ __device__ __forceinline__ void keys_again(const AttnArgs& p0, int g, int key0, 
 // it is known without cu_seqlens, and a heavy tile that starts last ends long after the others.  Where there are more
 // workgroups than the card holds at once and sequences are long on average (entries of cu_seqlens, empty ones among them), one small kernel (5 us) sorts
 // the tiles by their work first: the backward from 512 rows a sequence on, the forward, whose tiles take a third of the time, from 1024.  us not sorted -> sorted,
-// even lengths; uneven ones (split at random), on one box:
+// even lengths; uneven ones (split at random), on one machine:
 //   forward   8192 rows, 32/4 heads of 128   2048 a sequence 185 -> 184; 205 -> 206   1024 99 -> 101; 134 -> 133    512 69 -> 76; 112 -> 113
 //             8192, 16/16 of 64                         73 -> 57; 99 -> 107           42 -> 37; 59 -> 60            28 -> 29; 50 -> 55
 //             fp32 4096, 8/2 of 64                      113 -> 112; 112 -> 117        80 -> 74; 92 -> 93            56 -> 54; 64 -> 63

@@ -16,7 +16,7 @@
 // Bound by the matrix pipes and the vector work beside them, which add up at two waves a SIMD rather than hide each other; a third wave, and
 // priorities around the products, did not help.  32/4 heads of 128, where a large library product reaches 1200 TFLOP/s: forward of one sequence of 8192
 // rows 522 us, 1050 TFLOP/s; forward, dq and dk/dv of 8192 rows in 4 sequences 162, 230 and 277 us, 850, 900 and 990
-// (two, three and four products); of 16384 in 11 uneven ones 347, 497 and 628, 770, 810 and 850.  Boxes differ by 5 %.  Heads between the forms' sizes take
+// (two, three and four products); of 16384 in 11 uneven ones 347, 497 and 628, 770, 810 and 850.  Machines differ by 5 %.  Heads between the forms' sizes take
 // the next one's products: 8192 rows in 4, 16/4 heads, forward us (TFLOP/s of the heads' own products) of 64 55 (620), 80 82 (520), 96 84 (620), 128 88 (780),
 // 136 196 (370), 160 197 (430), 192 199 (520), 256 204 (670).
 //
